@@ -1,0 +1,312 @@
+// Matrix products on the fifth-generation tensor cores (sm_100a) for the vocabulary head.
+//
+//   acc[m, n] = sum over k of A[m, k] * B[n, k]      (16-bit operands, fp32 accumulators)
+//
+// One persistent CTA per SM walks a list of output tiles; what happens to a finished tile
+// is the job's epilogue, which reads the accumulators from tensor memory and reduces or
+// stores them, so no product has to be written out to be used.  Warp roles:
+//   warp 0     TMA producer: one lane streams the operands of every 64-deep step through a
+//              ring of shared-memory stages
+//   warp 1     MMA issuer: one lane issues four 16-deep tcgen05.mma per stage
+//   warp 2     owns the tensor memory (two accumulators of 128 x 256, so that the products
+//              of a tile run while the epilogue drains the one before)
+//   warps 4-7  epilogue: thread i owns accumulator row i (tensor-memory lane i)
+// An operand is either K-major (rows of A or B contiguous along k) or MN-major (contiguous
+// along m or n); both are read in place with 128-byte swizzled boxes, so no transposed copy
+// is ever made.
+//
+// Every wait is bounded.  A role whose wait runs out raises the CTA's fault flag and winds
+// down after its copies and products in flight have landed; the epilogue then sees NaN
+// accumulators for that and all later tiles of the CTA, so the results show it.
+//
+// A job type provides
+//   Walk walk() const            per-thread view of this CTA's tile list
+//   Walk::get(i, Tile&)          the i-th tile of this CTA, false past the end
+//   Epi  epi(...)                per-thread epilogue state, called once per tile with the
+//                                accumulators (Acc)
+#pragma once
+#include "common.cuh"
+
+#include <cuda.h>
+
+namespace gsp {
+namespace mm {
+
+constexpr int kBM = 128;                 // rows of A per tile
+constexpr int kBN = 256;                 // most rows of B per tile
+constexpr int kBK = 64;                  // depth of one stage: 128 bytes of a 16-bit operand
+constexpr int kStages = 4;
+constexpr int kThreads = 256;
+constexpr int kEpiWarp0 = 4;             // first epilogue warp (a multiple of 4: warp % 4 is
+                                         // the tensor-memory quarter it may read)
+constexpr int kABytes = kBM * kBK * 2;
+constexpr int kBBytes = kBN * kBK * 2;
+constexpr int kStageBytes = kABytes + kBBytes;
+constexpr int kScratch = 4 * 32 * 33 * 4 + 2 * 4 * kBN * 4;   // epilogue scratch
+constexpr int kOffScratch = kStages * kStageBytes;
+constexpr int kOffBar = kOffScratch + kScratch;
+constexpr int kSmem = kOffBar + 256 + 1024;   // + alignment slack
+static_assert(kSmem <= 232448, "stages exceed shared memory");
+constexpr int kTmemCols = 2 * kBN;
+
+// One output tile.  a/b select the operand maps; a0/b0 are the tile's first row (m or n) of
+// each operand, ak/bk the first k of it.
+struct Tile {
+  int32_t a, b;          // operand map indices
+  int32_t a0, b0;
+  int32_t ak, bk;
+  int32_t nk;            // 64-deep steps; 0: the product is zero
+  bool a_mn, b_mn;       // operand is MN-major
+  int32_t bn;            // rows of B of this tile (the map's box for a K-major B)
+  int32_t x, y, flags;   // the job's own coordinates
+};
+
+// ---- PTX ---------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t su32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n));
+}
+__device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(su32(b)) : "memory");
+}
+__device__ __forceinline__ bool bar_test(uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+               : "=r"(ok)
+               : "r"(su32(b)), "r"(parity)
+               : "memory");
+  return ok != 0;
+}
+// false if `limit` polls ran out or the CTA has faulted
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, int32_t limit, volatile int32_t* fault) {
+  for (int32_t i = 0; i <= limit; ++i) {
+    if (bar_test(b, parity)) return true;
+    if ((i & 63) == 63 && *fault) return false;
+  }
+  return false;
+}
+// copies and products already issued land before the CTA gives up its memory (a bound of its
+// own: the caller's limit may be 0)
+__device__ __forceinline__ void bar_land(uint64_t* b, uint32_t parity) {
+  for (int32_t i = 0; i < (1 << 24); ++i) {
+    if (bar_test(b, parity)) return;
+    __nanosleep(32);
+  }
+}
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+          su32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(su32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
+}
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a),
+      "l"(b), "r"(idesc), "r"(acc));
+}
+// thread i of the warp gets columns c .. c+31 of tensor-memory lane (quarter base + i)
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+}
+
+// Shared-memory matrix descriptors (128-byte swizzle, offsets in 16-byte units, version bit
+// 46).  K-major: a box is rows of 64 k (128 bytes), 8-row groups 1024 bytes apart; a 16-deep
+// step advances 32 bytes.  MN-major: a box is 64 k-rows of 64 m/n (128 bytes), boxes of 64
+// m/n 8192 bytes apart (leading offset), 8-k groups 1024 bytes apart (stride offset); a
+// 16-deep step advances 2048 bytes.
+__device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn) {
+  const uint64_t lead = mn ? (8192 >> 4) : 1;
+  return uint64_t((addr >> 4) & 0x3FFF) | (lead << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// fp32 accumulators, A and B both bf16 or both fp16
+__device__ __forceinline__ uint32_t inst_desc(bool bf16, bool a_mn, bool b_mn, int32_t bn) {
+  const uint32_t ty = bf16 ? 1u : 0u;
+  return (1u << 4) | (ty << 7) | (ty << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) |
+         (uint32_t(bn >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
+}
+
+// Accumulators of a finished tile as an epilogue warp sees them.
+struct Acc {
+  uint32_t taddr;        // this warp's quarter of the tile's tensor-memory columns
+  bool zero, bad;        // nk == 0; a wait ran out
+  float* stage;          // 32 x 33 floats of this warp
+  float* cols;           // [4 warps][kBN] floats of this tile (alternating buffers)
+  int warp, lane;        // epilogue warp 0..3
+  __device__ __forceinline__ void ld32(int32_t c, float (&v)[32]) const {
+    if (bad || zero) {
+      const float f = bad ? __uint_as_float(0x7FC00000u) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = f;
+    } else {
+      __syncwarp();          // the load is a warp's: lanes may have parted since the last one
+      tmem_ld32(taddr + uint32_t(c), v);
+    }
+  }
+  // the four epilogue warps
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+};
+
+template <class Job>
+__global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Job job) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* smem =
+      reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBar);   // [kStages]
+  uint64_t* empty = full + kStages;                               // [kStages]
+  uint64_t* acc_full = empty + kStages;                           // [2]
+  uint64_t* acc_empty = acc_full + 2;                             // [2]
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int32_t* fault = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
+  const int wid = threadIdx.x >> 5, lane = lane_id();
+  const int32_t limit = job.wait_limit;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      bar_init(full + i, 1);
+      bar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(acc_full + i, 1);
+      bar_init(acc_empty + i, 4);
+    }
+    bar_init(drain, 1);
+    *fault = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (wid == 2) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)),
+                 "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+
+  if (wid == 0) {
+    if (lane == 0) {
+      auto walk = job.walk();
+      Tile t;
+      uint32_t it = 0;
+      bool ok = true;
+      for (int32_t i = 0; ok && walk.get(i, t); ++i) {
+        const CUtensorMap* ma = &job.maps[t.a];
+        const CUtensorMap* mb = &job.maps[t.b];
+        const uint32_t bytes = uint32_t(kABytes + t.bn * kBK * 2);
+        for (int32_t k = 0; k < t.nk; ++k, ++it) {
+          const uint32_t s = it % kStages, n = it / kStages;
+          if (n > 0) ok = bar_wait(empty + s, (n - 1) & 1, limit, fault);
+          if (!ok) break;
+          unsigned char* as = smem + s * kStageBytes;
+          unsigned char* bs = as + kABytes;
+          bar_expect(full + s, bytes);
+          if (!t.a_mn) {
+            tma_2d(as, ma, t.ak + k * kBK, t.a0, full + s);
+          } else {
+            for (int32_t j = 0; j < kBM / 64; ++j) tma_2d(as + j * 8192, ma, t.a0 + j * 64, t.ak + k * kBK, full + s);
+          }
+          if (!t.b_mn) {
+            tma_2d(bs, mb, t.bk + k * kBK, t.b0, full + s);
+          } else {
+            for (int32_t j = 0; j < t.bn / 64; ++j) tma_2d(bs + j * 8192, mb, t.b0 + j * 64, t.bk + k * kBK, full + s);
+          }
+        }
+      }
+      if (!ok) *fault = 1;
+      for (uint32_t i = 0; i < kStages && i < it; ++i) {
+        const uint32_t j = it - 1 - i;
+        bar_land(full + j % kStages, (j / kStages) & 1);
+      }
+    }
+  } else if (wid == 1) {
+    if (lane == 0) {
+      auto walk = job.walk();
+      Tile t;
+      uint32_t it = 0;
+      bool ok = true;
+      for (int32_t i = 0; ok && walk.get(i, t); ++i) {
+        const int32_t buf = i & 1, use = i >> 1;
+        if (use > 0) ok = bar_wait(acc_empty + buf, (use - 1) & 1, limit, fault);
+        if (!ok) break;
+        fence_after();
+        const uint32_t d = tmem + uint32_t(buf * kBN);
+        const uint32_t id = inst_desc(job.bf16 != 0, t.a_mn, t.b_mn, t.bn);
+        const uint64_t step_a = t.a_mn ? (2048 >> 4) : (32 >> 4), step_b = t.b_mn ? (2048 >> 4) : (32 >> 4);
+        for (int32_t k = 0; k < t.nk; ++k, ++it) {
+          const uint32_t s = it % kStages, n = it / kStages;
+          ok = bar_wait(full + s, n & 1, limit, fault);
+          if (!ok) break;
+          fence_after();
+          const uint32_t as = su32(smem + s * kStageBytes);
+          const uint64_t da = desc(as, t.a_mn), db = desc(as + kABytes, t.b_mn);
+#pragma unroll
+          for (int q = 0; q < kBK / 16; ++q) mma_f16(d, da + q * step_a, db + q * step_b, id, (k > 0 || q > 0) ? 1u : 0u);
+          commit(empty + s);
+        }
+        if (!ok) break;
+        commit(acc_full + buf);
+      }
+      if (!ok) *fault = 1;
+      commit(drain);          // every product issued has finished before the memory is given back
+      bar_land(drain, 0);
+    }
+  } else if (wid >= kEpiWarp0) {
+    auto walk = job.walk();
+    auto epi = job.epi();
+    Tile t;
+    Acc acc;
+    acc.warp = wid - kEpiWarp0;
+    acc.lane = lane;
+    acc.stage = reinterpret_cast<float*>(smem + kOffScratch) + acc.warp * 32 * 33;
+    float* cols = reinterpret_cast<float*>(smem + kOffScratch + 4 * 32 * 33 * 4);
+    bool ok = true;
+    for (int32_t i = 0; walk.get(i, t); ++i) {
+      const int32_t buf = i & 1, use = i >> 1;
+      if (ok) {
+        ok = bar_wait(acc_full + buf, use & 1, limit, fault);
+        if (!ok) *fault = 1;
+        ok = __all_sync(FULL, ok);
+      }
+      fence_after();
+      acc.taddr = tmem + (uint32_t(32 * acc.warp) << 16) + uint32_t(buf * kBN);
+      acc.zero = t.nk == 0;
+      acc.bad = !ok;
+      acc.cols = cols + buf * 4 * kBN;
+      epi.tile(job, t, acc);
+      fence_before();
+      __syncwarp();
+      if (lane == 0) bar_arrive(acc_empty + buf);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (wid == 2) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+}  // namespace mm
+}  // namespace gsp

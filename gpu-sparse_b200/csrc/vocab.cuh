@@ -1,0 +1,150 @@
+// Shared parts of the vocabulary head's operators (vocab_loss.cu, sparse_head.cu): tokens
+// packed to the valid ones, operand maps, and the two products every backward pass ends in.
+//
+// Notation: H [T, D] hidden states, W [V, D] vocabulary projection (both bf16 or both fp16),
+// s = H W^T + bias the logits, of which no more than a tile ever exists.
+#pragma once
+#include "mma.cuh"
+
+namespace gsp {
+namespace vocab {
+
+constexpr int kRowPad = 256;     // packed rows and vocabulary columns are allocated in these
+inline int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+inline int64_t up256(int64_t x) { return up(x, 256); }
+inline int64_t pad_rows(int64_t T) { return T > 0 ? up(T, kRowPad) : kRowPad; }
+
+// Carves a caller's buffer; with a null base it only counts.
+struct Carver {
+  char* base;
+  int64_t off = 0;
+  template <typename T>
+  T* take(int64_t n) {
+    T* p = base ? reinterpret_cast<T*>(base + off) : nullptr;
+    off = up256(off + n * int64_t(sizeof(T)));
+    return p;
+  }
+};
+
+// What the forward pass leaves for the backward pass, in a buffer of the caller's.
+struct State {
+  int32_t* head;      // [0] packed rows, [1] ticket of the reducing kernels
+  int32_t* map;       // [Tp] original row of every packed row, ascending
+  uint16_t* h;        // [Tp, Dp] packed hidden states
+  float* bias2;       // [Vp] bias in units of the exponent's base 2, -inf past V (losses)
+  float* lse2;        // [Tp] log2 of the softmax's denominator (losses)
+  int32_t* tgt;       // [Tp] target of every packed row (cross entropy)
+  int32_t* cnt;       // [T] teacher entries of every row (distillation)
+  float* ent;         // [T] sum p log p (distillation)
+  int32_t* ids;       // [T, K] ascending, distinct (distillation)
+  float* p;           // [T, K] (distillation)
+  uint8_t* flag;      // [T] row takes part (distillation)
+  int64_t Tp, Dp, Vp, bytes;
+};
+State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool loss);
+
+int check_view(const gsp_vocab_view* vw, const char* what);
+inline bool is_bf16(const gsp_vocab_view* vw) { return vw->dtype == GSP_W_BF16; }
+// bytes of the copy of W that a projection whose rows a TMA map cannot describe needs (else 0)
+int64_t weight_copy_bytes(const gsp_vocab_view* vw);
+// W as a TMA map can describe it: the caller's, or a copy in `scratch`
+int weight_rows(const gsp_vocab_view* vw, void* scratch, const uint16_t** w, int64_t* ld, cudaStream_t st);
+
+// 2D map of a row-major 16-bit matrix: boxes of 64 columns x box_rows rows, 128-byte swizzle,
+// zeros outside
+int make_map(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows);
+
+// Packs the rows that take part (targets: id in [0, V) and != ignore; else flag != 0) to the
+// front of st.h, keeping their order, and writes st.map, st.head[0]; bias2 when scale != 0.
+int pack_rows(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore, const uint8_t* flag, float bias_scale,
+              const State& s, int32_t* counts, cudaStream_t st);
+inline int64_t pack_counts(int64_t T) { return (T + 255) / 256 + 1; }
+
+// Backward products over a piece of the vocabulary [v0, v0 + cols): P [Tp, pitch] is the
+// gradient of the piece's logits,
+//   dH (+)= P W[v0 : v0 + cols],   dW[v0 : v0 + cols] = P^T H,
+// in one launch.  dh_acc [Tp, up(D, 32)] carries dH in fp32 between pieces.
+struct GradPiece {
+  const uint16_t* P;
+  int64_t pitch, v0, cols;
+  bool first, last;
+};
+int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, int64_t ldw, const GradPiece& pc,
+                  float* dh_acc, const float* scale, void* d_hidden, void* d_weight, cudaStream_t st);
+// columns of one piece: P takes at most kPieceBytes
+constexpr int64_t kPieceBytes = int64_t(512) << 20;
+int64_t piece_cols(int64_t Tp, int64_t V);
+// Zeroes the packed rows past the n taking part that the products' last 64-deep step reads:
+// their P is 0, and 0 times whatever was there must be 0.  All threads of one CTA.
+__device__ __forceinline__ void zero_tail_rows(uint16_t* h, int64_t Dp, int32_t n) {
+  const int64_t end = (int64_t(n) + 63) / 64 * 64;
+  uint4* p = reinterpret_cast<uint4*>(h + int64_t(n) * Dp);
+  for (int64_t i = threadIdx.x; i < (end - n) * Dp / 8; i += blockDim.x) p[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---- device helpers ----------------------------------------------------------------------
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float neg_inf() { return __uint_as_float(0xFF800000u); }
+// two floats rounded to nearest even into one 32-bit word, `lo` in the low half
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
+  uint32_t r;
+  if (bf16) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  } else {
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  }
+  return r;
+}
+// 32-byte accesses of global memory (sm_100a), p a multiple of 32 bytes
+__device__ __forceinline__ void st256(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ void ld256(const void* p, uint32_t* r) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "l"(p)
+               : "memory");
+}
+// 32 accumulators of one row -> 16-bit, columns c0 .. min(c0 + 32, D); vec: row starts on a
+// 32-byte boundary and D is a multiple of 16
+__device__ __forceinline__ void store_row16(uint16_t* row, int32_t c0, int32_t D, const float (&v)[32], bool bf16, bool vec) {
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
+  if (vec) {
+    if (c0 < D) st256(row + c0, w);
+    if (c0 + 16 < D) st256(row + c0 + 16, w + 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      if (c0 + j < D) row[c0 + j] = uint16_t(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+// Lane l receives the sum over the warp's lanes of v[l] (a butterfly that halves the columns
+// it carries at every step; the order of the additions is fixed).
+__device__ __forceinline__ float warp_col_sums(float (&v)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool upper = (lane & o) != 0;
+#pragma unroll
+    for (int j = 0; j < o; ++j) {
+      const float keep = upper ? v[j + o] : v[j], give = upper ? v[j] : v[j + o];
+      v[j] = keep + __shfl_xor_sync(FULL, give, o);
+    }
+  }
+  return v[0];
+}
+
+// CTA c's share [lo, hi) of `tot` tiles in a row, and the CTA that owns tile x
+__host__ __device__ __forceinline__ int64_t share_lo(int64_t tot, int64_t ctas, int64_t c) { return c * tot / ctas; }
+__host__ __device__ __forceinline__ int64_t share_of(int64_t tot, int64_t ctas, int64_t x) { return ((x + 1) * ctas - 1) / tot; }
+
+}  // namespace vocab
+}  // namespace gsp

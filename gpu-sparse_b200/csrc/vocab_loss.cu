@@ -1,0 +1,717 @@
+// Softmax losses over the vocabulary without its logits: cross entropy and distillation from
+// a teacher's top scores.
+//
+// For a row t with logits s[v] and target distribution q (one entry for cross entropy, the
+// teacher's entries for distillation), with c = log2(e) / tau and z = c s:
+//   lse2 = log2 sum_v 2^z[v],   loss = tau^2 (sum_j q_j log q_j + ln 2 (lse2 - sum_j q_j z_j))
+//   dloss/ds[v] = tau (2^(z[v] - lse2) - q[v])
+//
+// Forward.  The tiles (128 rows x 256 vocabulary rows) of all rows are one long list, row
+// block by row block, cut into equal shares, one per CTA, so every SM has the same work
+// whatever the sizes.  The epilogue thread that owns a row carries its running maximum, sum
+// and target dot product in registers along the share and writes them once per row block; a
+// second kernel joins the partial results (in share order) and sums the losses.
+//
+// Backward.  Per piece of the vocabulary: the logits' tiles again, whose epilogue turns them
+// into P = gradient of the logits, rounded once to 16 bits, then the two products of
+// vocab.cu.  A piece is as large as 512 MiB of P allow, since the products' tile lists want
+// to be long; P makes one trip through memory, which the products' arithmetic hides.
+//   d_bias sums the unrounded P (a butterfly over the warp's rows, then over row blocks).
+//   P is scaled so that the largest row coefficient is 1 in bf16, where a target's softmax - 1
+//   is then -1 or close and rounds to next to nothing, and 2^14 in fp16, whose range would lose
+//   gradients of 1e-8; the products' epilogue takes the scale out in fp32.
+#include "vocab.cuh"
+
+namespace gsp {
+namespace vocab {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kFirst = 1, kLast = 2;
+
+struct Lists {             // target entries
+  const int32_t* tgt;      // cross entropy: one per packed row
+  const int32_t* cnt;      // distillation: by original row
+  const int32_t* ids;
+  const float* p;
+  int64_t K;
+};
+
+// ---- distillation: a teacher row's probabilities, sorted by id, duplicates joined --------
+constexpr int kSortThreads = 128;
+__global__ void __launch_bounds__(kSortThreads)
+teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_ids, int32_t K, int32_t pow2, int64_t V,
+               float inv_tau, State s) {
+  extern __shared__ uint64_t key[];              // [pow2] (id << 32 | entry), then p [pow2]
+  float* p = reinterpret_cast<float*>(key + pow2);
+  __shared__ float red[kSortThreads / 32];
+  __shared__ int32_t wcount[kSortThreads / 32];
+  const int64_t t = blockIdx.x;
+  const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  auto reduce = [&](float v, bool is_max) {
+    for (int o = 16; o > 0; o >>= 1) {
+      const float u = __shfl_xor_sync(FULL, v, o);
+      v = is_max ? fmaxf(v, u) : v + u;
+    }
+    __syncthreads();
+    if (lane == 0) red[wid] = v;
+    __syncthreads();
+    v = red[0];
+    for (int i = 1; i < kSortThreads / 32; ++i) v = is_max ? fmaxf(v, red[i]) : v + red[i];
+    return v;
+  };
+  float mx = neg_inf();
+  for (int32_t j = tid; j < pow2; j += kSortThreads) {
+    uint64_t k = ~0ull;
+    float x = neg_inf();
+    if (j < K) {
+      const int64_t id = in_ids[t * K + j];
+      x = scores[t * K + j];
+      if (id >= 0 && id < V && x != neg_inf()) k = (uint64_t(id) << 32) | uint32_t(j);
+      else x = neg_inf();
+    }
+    key[j] = k;
+    p[j] = x;
+    mx = fmaxf(mx, x);
+  }
+  mx = reduce(mx, true);
+  float sum = 0.0f;
+  for (int32_t j = tid; j < pow2; j += kSortThreads) {
+    const float e = key[j] == ~0ull ? 0.0f : expf((p[j] - mx) * inv_tau);
+    p[j] = e;
+    sum += e;
+  }
+  sum = reduce(sum, false);
+  // ascending (id, entry)
+  for (int32_t size = 2; size <= pow2; size <<= 1) {
+    for (int32_t step = size >> 1; step > 0; step >>= 1) {
+      __syncthreads();
+      for (int32_t i = tid; i < pow2 / 2; i += kSortThreads) {
+        const int32_t a = 2 * i - (i & (step - 1)), b = a + step;
+        const uint64_t x = key[a], y = key[b];
+        if ((x > y) == ((a & size) == 0)) {
+          key[a] = y;
+          key[b] = x;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  int32_t n = 0;
+  float ent = 0.0f;
+  for (int32_t j0 = 0; j0 < pow2; j0 += kSortThreads) {
+    const int32_t j = j0 + tid;
+    const uint64_t k = j < pow2 ? key[j] : ~0ull;
+    bool head = k != ~0ull && (j == 0 || (key[j - 1] >> 32) != (k >> 32));
+    float q = 0.0f;
+    if (head) {
+      for (int32_t i = j; i < pow2 && (key[i] >> 32) == (k >> 32); ++i) q += p[uint32_t(key[i])];
+      q /= sum;
+      head = q != 0.0f;                     // an entry whose probability underflowed adds nothing
+      if (head) ent += q * logf(q);
+    }
+    const uint32_t w = __ballot_sync(FULL, head);
+    if (lane == 0) wcount[wid] = __popc(w);
+    __syncthreads();
+    int32_t at = n;
+    for (int i = 0; i < kSortThreads / 32; ++i) {
+      if (i < wid) at += wcount[i];
+      n += wcount[i];
+    }
+    __syncthreads();
+    if (head) {
+      at += __popc(w & lanemask_lt());
+      s.ids[t * K + at] = int32_t(k >> 32);
+      s.p[t * K + at] = q;
+    }
+  }
+  ent = reduce(ent, false);
+  if (tid == 0) {
+    s.cnt[t] = n;
+    s.ent[t] = ent;
+    s.flag[t] = n > 0;
+  }
+}
+
+// Walks a row's ascending entries as the tiles pass.
+struct Cursor {
+  const int32_t* ids;
+  const float* p;
+  int32_t left;      // entries not passed
+  int32_t next;      // id of the next one (INT_MAX: none)
+  __device__ void start(const Lists& l, int64_t orig, bool live, int32_t v0) {
+    left = 0;
+    next = 0x7FFFFFFF;
+    if (!live) return;
+    ids = l.ids + orig * l.K;
+    p = l.p + orig * l.K;
+    left = l.cnt[orig];
+    int32_t lo = 0, hi = left;       // first entry with id >= v0
+    while (lo < hi) {
+      const int32_t mid = (lo + hi) >> 1;
+      if (ids[mid] < v0) lo = mid + 1;
+      else hi = mid;
+    }
+    ids += lo;
+    p += lo;
+    left -= lo;
+    if (left > 0) next = *ids;
+  }
+  __device__ void step() {
+    ++ids;
+    ++p;
+    --left;
+    next = left > 0 ? *ids : 0x7FFFFFFF;
+  }
+};
+
+// z of 32 consecutive vocabulary rows
+__device__ __forceinline__ void to_z(float (&v)[32], float c, const float* bias2) {
+  const float4* b = reinterpret_cast<const float4*>(bias2);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float4 x = __ldg(b + q);
+    v[4 * q] = fmaf(v[4 * q], c, x.x);
+    v[4 * q + 1] = fmaf(v[4 * q + 1], c, x.y);
+    v[4 * q + 2] = fmaf(v[4 * q + 2], c, x.z);
+    v[4 * q + 3] = fmaf(v[4 * q + 3], c, x.w);
+  }
+}
+
+// ---- forward -----------------------------------------------------------------------------
+struct Part {
+  float m, l, dot;     // maximum, sum of 2^(z - m), sum q z (each per row and share)
+};
+
+template <bool kList>
+struct LossJob {
+  CUtensorMap maps[2];      // H, W (K-major)
+  int32_t wait_limit, bf16;
+  const int32_t* head;
+  const int32_t* map;
+  int32_t nt, nk;           // tiles along the vocabulary, steps along D
+  float c;
+  const float* bias2;
+  Lists lists;
+  float* part;              // [ctas + row blocks][3][128]
+
+  struct Walk {
+    int64_t lo, hi;
+    int32_t nt, nk;
+    __device__ bool get(int32_t i, mm::Tile& t) const {
+      const int64_t x = lo + i;
+      if (x >= hi) return false;
+      t.x = int32_t(x / nt);
+      t.y = int32_t(x - int64_t(t.x) * nt);
+      t.a = 0, t.b = 1;
+      t.a0 = t.x * mm::kBM;
+      t.b0 = t.y * mm::kBN;
+      t.ak = t.bk = 0;
+      t.nk = nk;
+      t.a_mn = t.b_mn = false;
+      t.bn = mm::kBN;
+      t.flags = (i == 0 || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == nt - 1 ? kLast : 0);
+      return true;
+    }
+  };
+  __device__ Walk walk() const {
+    const int64_t tot = int64_t((head[0] + mm::kBM - 1) / mm::kBM) * nt;
+    return Walk{share_lo(tot, gridDim.x, blockIdx.x), share_lo(tot, gridDim.x, blockIdx.x + 1), nt, nk};
+  }
+
+  struct Epi {
+    float m, l, dot;
+    int32_t tgt;
+    Cursor cur;
+    __device__ void tile(const LossJob& j, const mm::Tile& t, const mm::Acc& a) {
+      const int32_t n0 = t.y * mm::kBN;
+      if (t.flags & kFirst) {
+        m = neg_inf();
+        l = dot = 0.0f;
+        const int32_t r = t.a0 + a.warp * 32 + a.lane;
+        const bool live = r < j.head[0];
+        if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, n0);
+        else tgt = live ? j.lists.tgt[r] : -1;
+      }
+      for (int32_t c0 = 0; c0 < mm::kBN; c0 += 32) {
+        float z[32];
+        a.ld32(c0, z);
+        const int32_t v0 = n0 + c0;
+        to_z(z, j.c, j.bias2 + v0);
+        if constexpr (kList) {
+          if (__any_sync(FULL, cur.next < v0 + 32)) {
+            float* mine = a.stage + a.lane * 33;      // own row: no other lane reads it
+#pragma unroll
+            for (int k = 0; k < 32; ++k) mine[k] = z[k];
+            while (cur.next < v0 + 32) {
+              dot = fmaf(*cur.p, mine[cur.next - v0], dot);
+              cur.step();
+            }
+          }
+        } else {
+          const int32_t d = tgt - v0;
+          if (d >= 0 && d < 32) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              if (k == d) dot = z[k];
+            }
+          }
+        }
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = fmaxf(fmaxf(z[k], z[k + 8]), fmaxf(z[k + 16], z[k + 24]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = fmaxf(x[k], x[k + 4]);
+        const float cm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        if (cm > m) {
+          l *= ex2(m - cm);
+          m = cm;
+        }
+        const float base = m == neg_inf() ? 0.0f : m;
+        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 32; ++k) e[k & 3] += ex2(z[k] - base);
+        l += (e[0] + e[1]) + (e[2] + e[3]);
+      }
+      if (t.flags & kLast) {
+        float* o = j.part + (int64_t(blockIdx.x) + t.x) * (3 * mm::kBM) + a.warp * 32 + a.lane;
+        o[0] = m;
+        o[mm::kBM] = l;
+        o[2 * mm::kBM] = dot;
+      }
+    }
+  };
+  __device__ Epi epi() const { return Epi{}; }
+};
+
+// Joins a row's partial results in share order and sums the losses: the blocks' sums are
+// added by whichever block finishes last, in block order.
+__global__ void __launch_bounds__(mm::kBM)
+join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, int32_t ctas, const float* ent, float tau2,
+            int32_t reduction, float* lse2, double* sums, float* loss) {
+  __shared__ double red[mm::kBM / 32];
+  __shared__ bool last;
+  const int32_t n = head[0], mb = blockIdx.x;
+  const int32_t r = mb * mm::kBM + threadIdx.x;
+  const int32_t blocks = (n + mm::kBM - 1) / mm::kBM;
+  const int64_t tot = int64_t(blocks) * nt;
+  double mine = 0.0;
+  if (r < n) {
+    const int64_t c0 = share_of(tot, ctas, int64_t(mb) * nt), c1 = share_of(tot, ctas, int64_t(mb + 1) * nt - 1);
+    float m = neg_inf(), l = 0.0f, dot = 0.0f;
+    for (int64_t c = c0; c <= c1; ++c) {
+      if (share_lo(tot, ctas, c) == share_lo(tot, ctas, c + 1)) continue;    // an empty share
+      const float* o = part + (c + mb) * (3 * mm::kBM) + threadIdx.x;
+      const float pm = o[0], pl = o[mm::kBM];
+      dot += o[2 * mm::kBM];
+      const float nm = fmaxf(m, pm), base = nm == neg_inf() ? 0.0f : nm;
+      l = l * ex2(m - base) + pl * ex2(pm - base);
+      m = nm;
+    }
+    const float z = m + log2f(l);
+    lse2[r] = z;
+    const int32_t orig = map[r];
+    const float v = tau2 * fmaf(z - dot, kLn2, ent ? ent[orig] : 0.0f);
+    if (reduction == GSP_REDUCE_NONE) loss[orig] = v;
+    mine = double(v);
+  }
+  if (reduction == GSP_REDUCE_NONE) return;
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(FULL, mine, o);
+  if (lane_id() == 0) red[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < mm::kBM / 32; ++i) s += red[i];
+    sums[mb] = s;
+    __threadfence();
+    last = atomicAdd(head + 1, 1) == int32_t(gridDim.x) - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double s = 0.0;
+  for (int32_t i = threadIdx.x; i < blocks; i += mm::kBM) s += *reinterpret_cast<volatile double*>(sums + i);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
+  __syncthreads();
+  if (lane_id() == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double v = 0.0;
+    for (int i = 0; i < mm::kBM / 32; ++i) v += red[i];
+    *loss = float(reduction == GSP_REDUCE_MEAN ? v / (n > 0 ? n : 1) : v);
+  }
+}
+
+// ---- backward ----------------------------------------------------------------------------
+// Row coefficients of P: ga[r] = tau * grad_loss (divided by the rows of a mean) over their
+// largest finite size; lse2 of the padding rows +inf, so that their P is 0.  One CTA.
+__global__ void __launch_bounds__(1024)
+grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, int32_t bf16, float* ga, float* scale) {
+  __shared__ float red[32];
+  const int32_t n = s.head[0];
+  const int32_t np = (n + kRowPad - 1) / kRowPad * kRowPad;
+  const float mul = tau / float(reduction == GSP_REDUCE_MEAN ? (n > 0 ? n : 1) : 1);
+  float gmax = 0.0f;
+  if (reduction == GSP_REDUCE_NONE) {
+    for (int32_t r = threadIdx.x; r < n; r += 1024) {
+      const float g = fabsf(grad_loss[s.map[r]] * mul);
+      if (g < __uint_as_float(0x7F800000u)) gmax = fmaxf(gmax, g);
+    }
+    for (int o = 16; o > 0; o >>= 1) gmax = fmaxf(gmax, __shfl_xor_sync(FULL, gmax, o));
+    if (lane_id() == 0) red[threadIdx.x >> 5] = gmax;
+    __syncthreads();
+    gmax = red[lane_id()];
+    for (int o = 16; o > 0; o >>= 1) gmax = fmaxf(gmax, __shfl_xor_sync(FULL, gmax, o));
+  } else {
+    const float g = fabsf(*grad_loss * mul);
+    if (g < __uint_as_float(0x7F800000u)) gmax = g;
+  }
+  if (gmax == 0.0f) gmax = 1.0f;
+  const float top = bf16 ? 1.0f : 16384.0f;
+  if (threadIdx.x == 0) *scale = gmax / top;
+  for (int32_t r = threadIdx.x; r < np; r += 1024) {
+    if (r < n) {
+      ga[r] = (reduction == GSP_REDUCE_NONE ? grad_loss[s.map[r]] : *grad_loss) * mul / gmax * top;
+    } else {
+      ga[r] = 0.0f;
+      s.lse2[r] = __uint_as_float(0x7F800000u);
+    }
+  }
+  zero_tail_rows(s.h, s.Dp, n);
+}
+
+template <bool kList>
+struct LogitGradJob {
+  CUtensorMap maps[2];      // H, W (K-major)
+  int32_t wait_limit, bf16;
+  const int32_t* head;
+  const int32_t* map;
+  int32_t nk, v0, nt;       // the piece's first vocabulary row and 256-wide tiles
+  float c;
+  const float *bias2, *lse2, *ga;
+  Lists lists;
+  uint16_t* P;
+  int64_t pitch;
+  float* colpart;           // [row blocks][pitch], or null
+
+  struct Walk {
+    int64_t tot;
+    int32_t nt, nk, v0;
+    __device__ bool get(int32_t i, mm::Tile& t) const {
+      const int64_t x = int64_t(i) * gridDim.x + blockIdx.x;
+      if (x >= tot) return false;
+      t.x = int32_t(x / nt);
+      t.y = int32_t(x - int64_t(t.x) * nt);
+      t.a = 0, t.b = 1;
+      t.a0 = t.x * mm::kBM;
+      t.b0 = v0 + t.y * mm::kBN;
+      t.ak = t.bk = 0;
+      t.nk = nk;
+      t.a_mn = t.b_mn = false;
+      t.bn = mm::kBN;
+      t.flags = 0;
+      return true;
+    }
+  };
+  __device__ Walk walk() const { return Walk{int64_t((head[0] + mm::kBM - 1) / mm::kBM) * nt, nt, nk, v0}; }
+
+  struct Epi {
+    __device__ void tile(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
+      const int32_t r = t.a0 + a.warp * 32 + a.lane;
+      const bool live = r < j.head[0];
+      const float lse = j.lse2[r], ga = j.ga[r];
+      Cursor cur;
+      int32_t tgt = -1;
+      if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, t.b0);
+      else tgt = live ? j.lists.tgt[r] : -1;
+      uint16_t* row = j.P + int64_t(r) * j.pitch + t.y * mm::kBN;
+      for (int32_t c0 = 0; c0 < mm::kBN; c0 += 32) {
+        float z[32];
+        a.ld32(c0, z);
+        const int32_t v0 = t.b0 + c0;
+        to_z(z, j.c, j.bias2 + v0);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) z[k] = ga * ex2(z[k] - lse);
+        if (!live) {        // padding rows: 0 whatever their hidden states hold
+#pragma unroll
+          for (int k = 0; k < 32; ++k) z[k] = 0.0f;
+        }
+        if constexpr (kList) {
+          if (__any_sync(FULL, cur.next < v0 + 32)) {
+            float* mine = a.stage + a.lane * 33;
+#pragma unroll
+            for (int k = 0; k < 32; ++k) mine[k] = z[k];
+            while (cur.next < v0 + 32) {
+              mine[cur.next - v0] = fmaf(-ga, *cur.p, mine[cur.next - v0]);
+              cur.step();
+            }
+#pragma unroll
+            for (int k = 0; k < 32; ++k) z[k] = mine[k];
+          }
+        } else {
+          const int32_t d = tgt - v0;
+          if (d >= 0 && d < 32) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+              if (k == d) z[k] -= ga;
+            }
+          }
+        }
+        uint32_t w[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) w[k] = pack2(z[2 * k], z[2 * k + 1], j.bf16 != 0);
+        st256(row + c0, w);
+        st256(row + c0 + 16, w + 8);
+        if (j.colpart) a.cols[a.warp * mm::kBN + c0 + a.lane] = warp_col_sums(z, a.lane);
+      }
+      if (j.colpart) {
+        a.sync();
+        const int i = a.warp * 32 + a.lane;
+        float* o = j.colpart + int64_t(t.x) * j.pitch + t.y * mm::kBN;
+#pragma unroll
+        for (int h = 0; h < mm::kBN; h += 128) {
+          const float* q = a.cols + h + i;
+          o[h + i] = (q[0] + q[mm::kBN]) + (q[2 * mm::kBN] + q[3 * mm::kBN]);
+        }
+      }
+    }
+  };
+  __device__ Epi epi() const { return Epi{}; }
+};
+
+// d_bias of a piece: the row blocks' column sums, in order
+__global__ void __launch_bounds__(256)
+bias_grad_kernel(const int32_t* head, const float* colpart, int64_t pitch, int64_t cols, const float* scale, float* d_bias) {
+  const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (c >= cols) return;
+  const int32_t blocks = (head[0] + mm::kBM - 1) / mm::kBM;
+  float s = 0.0f;
+  for (int32_t b = 0; b < blocks; ++b) s += colpart[int64_t(b) * pitch + c];
+  d_bias[c] = s * *scale;
+}
+
+// ---- host --------------------------------------------------------------------------------
+struct Fwd {
+  int32_t* counts;
+  float* part;
+  double* sums;
+  void* wcopy;
+  int64_t bytes;
+};
+Fwd carve_fwd(void* base, const gsp_vocab_view* vw) {
+  Fwd f{};
+  Carver c{static_cast<char*>(base)};
+  const int64_t blocks = pad_rows(vw->T) / mm::kBM;
+  f.counts = c.take<int32_t>(pack_counts(vw->T));
+  f.part = c.take<float>((num_sms() + blocks) * 3 * mm::kBM);
+  f.sums = c.take<double>(blocks);
+  f.wcopy = c.take<char>(weight_copy_bytes(vw));
+  f.bytes = c.off;
+  return f;
+}
+struct Bwd {
+  float *ga, *scale, *colpart, *dh_acc;
+  uint16_t* P;
+  void* wcopy;
+  int64_t pitch, bytes;
+};
+Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
+  Bwd b{};
+  Carver c{static_cast<char*>(base)};
+  const int64_t Tp = pad_rows(vw->T);
+  b.pitch = piece_cols(Tp, vw->V);
+  b.ga = c.take<float>(Tp);
+  b.scale = c.take<float>(1);
+  b.colpart = c.take<float>(Tp / mm::kBM * b.pitch);
+  b.dh_acc = c.take<float>(b.pitch < vw->V ? Tp * up(vw->D, 32) : 0);
+  b.P = c.take<uint16_t>(Tp * b.pitch);
+  b.wcopy = c.take<char>(weight_copy_bytes(vw));
+  b.bytes = c.off;
+  return b;
+}
+
+int check_reduction(int32_t reduction, const char* what) {
+  GSP_REQUIRE(reduction >= GSP_REDUCE_NONE && reduction <= GSP_REDUCE_MEAN, GSP_ERR_ARG, "%s: unknown reduction %d", what,
+              reduction);
+  return GSP_OK;
+}
+
+template <bool kList>
+int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Lists& lists, float tau, int32_t reduction,
+                const float* ent, float* loss, cudaStream_t st) {
+  const uint16_t* w;
+  int64_t ldw;
+  int rc;
+  if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
+  LossJob<kList> j{};
+  const bool bf = is_bf16(vw);
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kBM))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN))) return rc;
+  j.wait_limit = gsp_get_wait_limit();
+  j.bf16 = bf;
+  j.head = s.head;
+  j.map = s.map;
+  j.nt = int32_t(s.Vp / mm::kBN);
+  j.nk = int32_t((vw->D + mm::kBK - 1) / mm::kBK);
+  j.c = kLog2e / tau;
+  j.bias2 = s.bias2;
+  j.lists = lists;
+  j.part = f.part;
+  if ((rc = ensure_smem(reinterpret_cast<const void*>(&mm::mma_kernel<LossJob<kList>>), mm::kSmem))) return rc;
+  const int ctas = num_sms();
+  mm::mma_kernel<LossJob<kList>><<<ctas, mm::kThreads, mm::kSmem, st>>>(j);
+  GSP_CHECK_LAUNCH();
+  if (reduction == GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, size_t(vw->T) * sizeof(float), st));
+  join_kernel<<<unsigned((vw->T + mm::kBM - 1) / mm::kBM), mm::kBM, 0, st>>>(s.head, s.map, f.part, j.nt, ctas, ent, tau * tau,
+                                                                           reduction, s.lse2, f.sums, loss);
+  GSP_CHECK_LAUNCH();
+  return GSP_OK;
+}
+
+template <bool kList>
+int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const Lists& lists, float tau, void* d_hidden,
+                 void* d_weight, float* d_bias, cudaStream_t st) {
+  const uint16_t* w;
+  int64_t ldw;
+  int rc;
+  if ((rc = weight_rows(vw, b.wcopy, &w, &ldw, st))) return rc;
+  LogitGradJob<kList> j{};
+  const bool bf = is_bf16(vw);
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kBM))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN))) return rc;
+  j.wait_limit = gsp_get_wait_limit();
+  j.bf16 = bf;
+  j.head = s.head;
+  j.map = s.map;
+  j.nk = int32_t((vw->D + mm::kBK - 1) / mm::kBK);
+  j.c = kLog2e / tau;
+  j.bias2 = s.bias2;
+  j.lse2 = s.lse2;
+  j.ga = b.ga;
+  j.lists = lists;
+  j.P = b.P;
+  j.pitch = b.pitch;
+  j.colpart = d_bias ? b.colpart : nullptr;
+  if ((rc = ensure_smem(reinterpret_cast<const void*>(&mm::mma_kernel<LogitGradJob<kList>>), mm::kSmem))) return rc;
+  for (int64_t v0 = 0; v0 < vw->V; v0 += b.pitch) {
+    const int64_t cols = min64(b.pitch, vw->V - v0);
+    j.v0 = int32_t(v0);
+    j.nt = int32_t((cols + mm::kBN - 1) / mm::kBN);
+    mm::mma_kernel<LogitGradJob<kList>><<<num_sms(), mm::kThreads, mm::kSmem, st>>>(j);
+    GSP_CHECK_LAUNCH();
+    if (d_bias) {
+      bias_grad_kernel<<<unsigned((cols + 255) / 256), 256, 0, st>>>(s.head, b.colpart, b.pitch, cols, b.scale, d_bias + v0);
+      GSP_CHECK_LAUNCH();
+    }
+    const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V};
+    if ((rc = grad_products(vw, s, w, ldw, pc, b.dh_acc, b.scale, d_hidden, d_weight, st))) return rc;
+  }
+  return GSP_OK;
+}
+
+}  // namespace
+
+int64_t loss_ws_bytes(const gsp_vocab_view* vw, bool backward) {
+  return backward ? carve_bwd(nullptr, vw).bytes : carve_fwd(nullptr, vw).bytes;
+}
+
+}  // namespace vocab
+}  // namespace gsp
+
+using namespace gsp;
+using namespace gsp::vocab;
+
+extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore_index, int32_t reduction,
+                            float* loss, void* state, int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream) {
+  int rc = check_view(vw, "vocab_cross_entropy");
+  if (rc) return rc;
+  if ((rc = check_reduction(reduction, "vocab_cross_entropy"))) return rc;
+  cudaStream_t st = as_stream(stream);
+  GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "vocab_cross_entropy: null loss");
+  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, true);
+  const Fwd f = carve_fwd(ws, vw);
+  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
+              "vocab_cross_entropy: state or workspace too small");
+  if (vw->T == 0) {
+    if (reduction != GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
+    return GSP_OK;
+  }
+  GSP_REQUIRE(targets && vw->hidden && vw->weight, GSP_ERR_ARG, "vocab_cross_entropy: null input");
+  if ((rc = pack_rows(vw, targets, ignore_index, nullptr, kLog2e, s, f.counts, st))) return rc;
+  Lists l{};
+  l.tgt = s.tgt;
+  return run_forward<false>(vw, s, f, l, 1.0f, reduction, nullptr, loss, st);
+}
+
+extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, const int64_t* ids, int64_t K, float tau,
+                                 int32_t reduction, float* loss, void* state, int64_t state_bytes, void* ws,
+                                 int64_t ws_bytes, void* stream) {
+  int rc = check_view(vw, "topk_distillation");
+  if (rc) return rc;
+  if ((rc = check_reduction(reduction, "topk_distillation"))) return rc;
+  cudaStream_t st = as_stream(stream);
+  GSP_REQUIRE(K >= 1 && K <= GSP_DISTILL_MAX_K, GSP_ERR_ARG, "topk_distillation: %lld teacher entries, 1 to %d are supported",
+              (long long)K, GSP_DISTILL_MAX_K);
+  GSP_REQUIRE(tau > 0.0f && tau < __builtin_inff(), GSP_ERR_ARG, "topk_distillation: temperature must be positive");
+  GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "topk_distillation: null loss");
+  const State s = carve_state(state, vw->T, vw->V, vw->D, K, true);
+  const Fwd f = carve_fwd(ws, vw);
+  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
+              "topk_distillation: state or workspace too small");
+  if (vw->T == 0) {
+    if (reduction != GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
+    return GSP_OK;
+  }
+  GSP_REQUIRE(scores && ids && vw->hidden && vw->weight, GSP_ERR_ARG, "topk_distillation: null input");
+  int32_t pow2 = 2;
+  while (pow2 < K) pow2 <<= 1;
+  teacher_kernel<<<unsigned(vw->T), kSortThreads, size_t(pow2) * 12, st>>>(scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, s);
+  GSP_CHECK_LAUNCH();
+  if ((rc = pack_rows(vw, nullptr, 0, s.flag, kLog2e / tau, s, f.counts, st))) return rc;
+  Lists l{};
+  l.cnt = s.cnt;
+  l.ids = s.ids;
+  l.p = s.p;
+  l.K = K;
+  return run_forward<true>(vw, s, f, l, tau, reduction, s.ent, loss, st);
+}
+
+extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, int64_t K, float tau, int32_t reduction,
+                                       const float* grad_loss, void* d_hidden, void* d_weight,
+                                       float* d_bias, void* state, int64_t state_bytes, void* ws, int64_t ws_bytes,
+                                       void* stream) {
+  int rc = check_view(vw, "vocab loss backward");
+  if (rc) return rc;
+  if ((rc = check_reduction(reduction, "vocab loss backward"))) return rc;
+  GSP_REQUIRE(kind == GSP_VOCAB_CE || kind == GSP_VOCAB_DISTILL, GSP_ERR_ARG, "vocab loss backward: unknown kind %d", kind);
+  const bool list = kind == GSP_VOCAB_DISTILL;
+  GSP_REQUIRE(!list || (K >= 1 && K <= GSP_DISTILL_MAX_K && tau > 0.0f && tau < __builtin_inff()), GSP_ERR_ARG,
+              "vocab loss backward: bad teacher entries or temperature");
+  cudaStream_t st = as_stream(stream);
+  const State s = carve_state(state, vw->T, vw->V, vw->D, list ? K : 0, true);
+  const Bwd b = carve_bwd(ws, vw);
+  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,
+              "vocab loss backward: state or workspace too small");
+  const size_t VD = size_t(vw->V) * size_t(vw->D);
+  if (vw->T == 0) {
+    if (d_weight) GSP_CUDA(cudaMemsetAsync(d_weight, 0, VD * 2, st));
+    if (d_bias) GSP_CUDA(cudaMemsetAsync(d_bias, 0, size_t(vw->V) * sizeof(float), st));
+    return GSP_OK;
+  }
+  GSP_REQUIRE(grad_loss && vw->weight, GSP_ERR_ARG, "vocab loss backward: null input");
+  if (d_hidden) GSP_CUDA(cudaMemsetAsync(d_hidden, 0, size_t(vw->T) * size_t(vw->D) * 2, st));
+  if (!list) tau = 1.0f;
+  grad_rows_kernel<<<1, 1024, 0, st>>>(s, grad_loss, reduction, tau, is_bf16(vw), b.ga, b.scale);
+  GSP_CHECK_LAUNCH();
+  Lists l{};
+  if (list) {
+    l.cnt = s.cnt;
+    l.ids = s.ids;
+    l.p = s.p;
+    l.K = K;
+    return run_backward<true>(vw, s, b, l, tau, d_hidden, d_weight, d_bias, st);
+  }
+  l.tgt = s.tgt;
+  return run_backward<false>(vw, s, b, l, tau, d_hidden, d_weight, d_bias, st);
+}

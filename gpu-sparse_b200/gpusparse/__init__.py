@@ -8,9 +8,13 @@ fallback: every entry point raises if the library or a CUDA device is missing.
 
 Beyond the reference: streamed index builds (build_streamed, build_from_host_csr),
 index persistence (save_index, load_index), a captured fixed-shape scorer
-(CapturedScorer), and, in gpusparse.distributed, doc-range sharding over the GPUs of a
-node.
+(CapturedScorer), the vocabulary head that term weights come from and the losses it is
+trained with (sparse_head, vocab_cross_entropy, topk_distillation, and encode_documents,
+encode_queries and build_index_from_hidden on top of it), and, in gpusparse.distributed,
+doc-range sharding over the GPUs of a node.
 """
+from .head import (build_index_from_hidden, encode_documents, encode_queries,  # noqa: F401
+                   sparse_head, topk_distillation, vocab_cross_entropy)
 from .index import (BLOCK_DOCS, BLOCK_SIZE, VOCAB_SIZE, GPUInvertedIndex,  # noqa: F401
                     build_from_csr_tensors, build_from_host_csr, build_gpu_index_from_csr,
                     build_gpu_inverted_index, build_streamed,

@@ -16,7 +16,8 @@ ROOT = os.path.dirname(PKG)                       # gpu-sparse_b200/
 CSRC = os.path.join(ROOT, "csrc")
 OBJ = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libgpusparse.so")
-SOURCES = ["runtime.cu", "synth.cu", "build.cu", "score.cu", "select.cu"]
+SOURCES = ["runtime.cu", "synth.cu", "build.cu", "score.cu", "select.cu", "vocab.cu",
+           "vocab_loss.cu", "sparse_head.cu"]
 NVCC = os.environ.get("NVCC", "nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
          "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall"]

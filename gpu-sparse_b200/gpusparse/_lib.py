@@ -24,7 +24,10 @@ GSP_ERR_TIMEOUT = 5
 GSP_ERR_UNSUPPORTED = 6
 GSP_ERR_BLOCK_PL = 7
 
-W_F32, W_BF16, W_U8 = 0, 1, 2
+W_F32, W_BF16, W_U8, W_F16 = 0, 1, 2, 3
+VOCAB_CE, VOCAB_DISTILL, VOCAB_HEAD = 0, 1, 2              # GSP_VOCAB_*
+REDUCE = {"none": 0, "sum": 1, "mean": 2}                  # GSP_REDUCE_*
+DISTILL_MAX_K = 1024                                       # GSP_DISTILL_MAX_K
 HEAD_AUTO, HEAD_CUDA_CORES, HEAD_TENSOR_CORES = 0, 1, 2   # gsp_set_head_mode
 CHECK_WS_BYTES = 16     # GSP_CHECK_WS_BYTES
 
@@ -38,7 +41,9 @@ EXPORTS = (
     "gsp_get_head_mode", "gsp_check_sorted", "gsp_chunk_bounds", "gsp_score_ws_bytes",
     "gsp_score_topk", "gsp_score_topk_noalloc", "gsp_score_topk_shared", "gsp_board_alloc",
     "gsp_board_free", "gsp_board_open", "gsp_board_close", "gsp_board_clear", "gsp_profile_enable", "gsp_profile_collect", "gsp_set_wait_limit", "gsp_get_wait_limit", "gsp_set_schedule_jitter", "gsp_get_schedule_jitter", "gsp_set_tree_limit", "gsp_get_tree_limit", "gsp_merge_ws_bytes", "gsp_merge_topk",
-    "gsp_compacted_ws_bytes", "gsp_compacted_topk",
+    "gsp_compacted_ws_bytes", "gsp_compacted_topk", "gsp_vocab_state_bytes", "gsp_vocab_ws_bytes",
+    "gsp_vocab_ce", "gsp_vocab_distill", "gsp_vocab_loss_backward", "gsp_sparse_head",
+    "gsp_sparse_head_backward", "gsp_dense_rows_count", "gsp_dense_rows_fill",
 )
 
 
@@ -52,6 +57,16 @@ class IndexView(ctypes.Structure):
         ("lengths", ctypes.c_void_p), ("block_starts", ctypes.c_void_p),
         ("n_head", ctypes.c_int32), ("head_wdtype", ctypes.c_int32), ("head_slot", ctypes.c_void_p),
         ("head_rows", ctypes.c_void_p), ("head_ld", ctypes.c_int64), ("head_lo", ctypes.c_void_p),
+    ]
+
+
+class VocabView(ctypes.Structure):
+    """struct gsp_vocab_view"""
+    _fields_ = [
+        ("T", ctypes.c_int64), ("V", ctypes.c_int64), ("D", ctypes.c_int64),
+        ("ld_hidden", ctypes.c_int64), ("ld_weight", ctypes.c_int64),
+        ("hidden", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("dtype", ctypes.c_int32), ("pad_", ctypes.c_int32),
     ]
 
 
@@ -132,6 +147,21 @@ def lib() -> ctypes.CDLL:
             "gsp_compacted_ws_bytes": (i64, [i64, i64, i64, i64]),
             "gsp_compacted_topk": (ctypes.c_int, [p, i64, i64, i64, p, i64, i64, p, p, p, i64,
                                                   p]),
+            "gsp_vocab_state_bytes": (i64, [i64, i64, i64, i64, i32]),
+            "gsp_vocab_ws_bytes": (i64, [ctypes.POINTER(VocabView), i32, i32]),
+            "gsp_vocab_ce": (ctypes.c_int, [ctypes.POINTER(VocabView), p, i64, i32, p, p, i64, p,
+                                            i64, p]),
+            "gsp_vocab_distill": (ctypes.c_int, [ctypes.POINTER(VocabView), p, p, i64,
+                                                 ctypes.c_float, i32, p, p, i64, p, i64, p]),
+            "gsp_vocab_loss_backward": (ctypes.c_int, [ctypes.POINTER(VocabView), i32, i64,
+                                                       ctypes.c_float, i32, p, p, p, p, p, i64, p,
+                                                       i64, p]),
+            "gsp_sparse_head": (ctypes.c_int, [ctypes.POINTER(VocabView), i64, p, p, p, p, i64, p,
+                                               i64, p]),
+            "gsp_sparse_head_backward": (ctypes.c_int, [ctypes.POINTER(VocabView), i64, p, p, p, p,
+                                                        p, p, p, i64, p, i64, p]),
+            "gsp_dense_rows_count": (ctypes.c_int, [p, i64, i64, ctypes.c_float, p, p]),
+            "gsp_dense_rows_fill": (ctypes.c_int, [p, i64, i64, ctypes.c_float, p, p, p, p]),
         }
         for name, (res, args) in sig.items():
             f = getattr(L, name)

@@ -1,0 +1,376 @@
+"""The vocabulary head: the projection that term weights come from, and its training losses.
+
+A learned-sparse encoder ends in a projection of its hidden states onto the vocabulary,
+s[t, v] = hidden[t] . weight[v] + bias[v].  The operators here run that projection on the
+tensor cores and reduce the logits where they are made, so none of them ever holds logits:
+
+* ``sparse_head``: term weights log1p(relu(max over a text's tokens of s)), [B, V];
+  ``encode_documents`` / ``encode_queries`` turn them into what the index builders and the
+  scorer take, ``build_index_from_hidden`` into an index;
+* ``vocab_cross_entropy``: softmax cross entropy over the vocabulary (masked tokens, or
+  with documents as the rows of ``weight`` a contrastive loss);
+* ``topk_distillation``: KL divergence from a teacher's top scores, in the (scores, ids)
+  form ``score_topk`` and ``compacted_topk`` return.
+
+Types: hidden and weight both bf16 or both fp16, bias in any floating type (used as fp32);
+logits and sums are fp32, and so are the results.  All three differentiate in hidden,
+weight and bias; gradients come in the inputs' types, and equal inputs give equal bits.
+Tokens that take no part (ignored targets, masked tokens, rows without teacher entries)
+are packed away on the GPU first: they cost nothing, and what they hold is never used.
+No call synchronises except ``encode_documents`` and ``build_index_from_hidden``, whose
+results' sizes depend on the data.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Iterable, Optional, Tuple
+
+import torch
+
+from . import _lib as L
+from .index import GPUInvertedIndex, build_from_csr_tensors
+from .scoring import compacted_topk
+
+_DTYPES = {torch.bfloat16: L.W_BF16, torch.float16: L.W_F16}
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x as rows of unit element stride that do not overlap, copied only if it has others."""
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _check(what: str, hidden, weight, bias):
+    L.require_cuda(hidden, "hidden")
+    L.require_cuda(weight, "weight")
+    if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
+        raise ValueError(f"{what}: hidden and weight must both be bfloat16 or both float16, got "
+                         f"{hidden.dtype} and {weight.dtype}")
+    if weight.dim() != 2 or hidden.dim() < 2 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: hidden must be [..., D] and weight [V, D], got "
+                         f"{tuple(hidden.shape)} and {tuple(weight.shape)}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"{what}: weight must not be empty")
+    if weight.device != hidden.device:
+        raise ValueError(f"{what}: weight must live on {hidden.device}")
+    if bias is not None:
+        if bias.shape != (weight.shape[0],) or not bias.dtype.is_floating_point:
+            raise ValueError(f"{what}: bias must be a floating tensor of {weight.shape[0]} entries")
+        if bias.device != hidden.device:
+            raise ValueError(f"{what}: bias must live on {hidden.device}")
+
+
+def _view(hidden, weight, bias) -> L.VocabView:
+    """View of row tensors (see _rows); hidden may be (T, D) of a backward call without data."""
+    v = L.VocabView()
+    if isinstance(hidden, torch.Tensor):
+        v.T, v.D = hidden.shape
+        v.ld_hidden = hidden.stride(0) if v.T > 1 else v.D
+        v.hidden = hidden.data_ptr()
+    else:
+        v.T, v.D = hidden
+        v.ld_hidden = v.D
+    v.V = weight.shape[0]
+    v.ld_weight = weight.stride(0) if v.V > 1 else v.D
+    v.weight = weight.data_ptr()
+    v.bias = bias.data_ptr() if bias is not None else None
+    v.dtype = _DTYPES[weight.dtype]
+    return v
+
+
+def _buffers(v: L.VocabView, K: int, kind: int, dev):
+    lib = L.lib()
+    sb = lib.gsp_vocab_state_bytes(v.T, v.V, v.D, K, kind)
+    wb = lib.gsp_vocab_ws_bytes(ctypes.byref(v), kind, 0)
+    if sb < 0 or wb < 0:
+        L.check(int(-min(sb, wb)), "vocabulary head")
+    return L.workspace(sb, dev), L.workspace(wb, dev)
+
+
+def _backward_ws(v: L.VocabView, kind: int, dev) -> torch.Tensor:
+    wb = L.lib().gsp_vocab_ws_bytes(ctypes.byref(v), kind, 1)
+    if wb < 0:
+        L.check(int(-wb), "vocabulary head")
+    return L.workspace(wb, dev)
+
+
+# ---------------------------------------------------------------------------- losses
+def _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction):
+    dev = hidden.device
+    with torch.cuda.device(dev):
+        v = _view(hidden, weight, bias)
+        K = ids.shape[1] if kind == L.VOCAB_DISTILL else 0
+        state, ws = _buffers(v, K, kind, dev)
+        loss = torch.empty(v.T if reduction == 0 else (), dtype=torch.float32, device=dev)
+        if kind == L.VOCAB_CE:
+            L.check(L.lib().gsp_vocab_ce(ctypes.byref(v), targets.data_ptr(), ignore_index, reduction,
+                                         loss.data_ptr(), state.data_ptr(), state.numel(),
+                                         ws.data_ptr(), ws.numel(), L.stream_of(dev)),
+                    "vocab_cross_entropy")
+        else:
+            L.check(L.lib().gsp_vocab_distill(ctypes.byref(v), scores.data_ptr(), ids.data_ptr(), K,
+                                              tau, reduction, loss.data_ptr(), state.data_ptr(),
+                                              state.numel(), ws.data_ptr(), ws.numel(),
+                                              L.stream_of(dev)), "topk_distillation")
+    return loss, state, K
+
+
+class _VocabLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, kind, targets, ignore_index, scores, ids, tau, reduction):
+        loss, state, K = _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids,
+                                       tau, reduction)
+        ctx.save_for_backward(weight)
+        ctx.state, ctx.T, ctx.args = state, hidden.shape[0], (kind, K, tau, reduction)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (weight,) = ctx.saved_tensors
+        kind, K, tau, reduction = ctx.args
+        need_h, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = weight.device
+        with torch.cuda.device(dev):
+            v = _view((ctx.T, weight.shape[1]), weight, None)
+            grad = grad.to(torch.float32).contiguous()
+            ws = _backward_ws(v, kind, dev)
+            dh = torch.empty((v.T, v.D), dtype=weight.dtype, device=dev) if need_h else None
+            dw = torch.empty((v.V, v.D), dtype=weight.dtype, device=dev) if need_w else None
+            db = torch.empty(v.V, dtype=torch.float32, device=dev) if need_b else None
+            L.check(L.lib().gsp_vocab_loss_backward(
+                ctypes.byref(v), kind, K, tau, reduction, grad.data_ptr(), L.ptr(dh), L.ptr(dw),
+                L.ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), ws.numel(),
+                L.stream_of(dev)), "vocab loss backward")
+        return (dh, dw, db) + (None,) * 7
+
+
+def _loss(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction):
+    lead = hidden.shape[:-1]
+    hidden = _rows(hidden.reshape(-1, hidden.shape[-1]))
+    weight = _rows(weight)
+    if bias is not None:
+        bias = bias.to(torch.float32).contiguous()
+    red = L.REDUCE[reduction]
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        loss = _VocabLoss.apply(hidden, weight, bias, kind, targets, ignore_index, scores, ids, tau, red)
+    else:
+        loss = _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, red)[0]
+    return loss.reshape(lead) if red == 0 else loss
+
+
+def _check_reduction(what: str, reduction: str) -> None:
+    if reduction not in L.REDUCE:
+        raise ValueError(f"{what}: reduction must be 'mean', 'sum' or 'none', got {reduction!r}")
+
+
+def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor,
+                        bias: Optional[torch.Tensor] = None, ignore_index: int = -100,
+                        reduction: str = "mean") -> torch.Tensor:
+    """Softmax cross entropy of hidden @ weight.T + bias against ``targets``, in fp32.
+
+    hidden [..., D], weight [V, D], targets integer [...].  Tokens whose target is
+    ``ignore_index`` or lies outside [0, V) take no part: they add no loss, get zero
+    gradients, and their hidden states are never used.  ``reduction`` "mean" divides by the
+    tokens that take part (0 when there are none), "none" gives the losses in targets' shape.
+    """
+    _check("vocab_cross_entropy", hidden, weight, bias)
+    _check_reduction("vocab_cross_entropy", reduction)
+    if targets.shape != hidden.shape[:-1] or targets.dtype.is_floating_point or \
+            targets.dtype in (torch.bool, torch.complex64, torch.complex128):
+        raise ValueError(f"vocab_cross_entropy: targets must be an integer tensor of shape "
+                         f"{tuple(hidden.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
+    if targets.device != hidden.device:
+        raise ValueError(f"vocab_cross_entropy: targets must live on {hidden.device}")
+    targets = targets.reshape(-1).to(torch.int64).contiguous()
+    return _loss(L.VOCAB_CE, hidden, weight, bias, targets, int(ignore_index), None, None, 1.0,
+                 reduction)
+
+
+def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_scores: torch.Tensor,
+                      teacher_ids: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                      temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
+    """Distillation from a teacher's top scores: with p = softmax(teacher_scores /
+    temperature) over a token's K entries, temperature^2 KL(p || softmax(s / temperature)),
+    s = hidden @ weight.T + bias, in fp32.
+
+    hidden [..., D], weight [V, D], teacher_scores and teacher_ids [..., K] with K <= 1024,
+    in any order (``score_topk`` and ``compacted_topk`` return this pair).  Entries with an
+    id outside [0, V) or a score of -inf are left out, an id listed twice adds its
+    probabilities, and a token without entries takes no part (as an ignored target in
+    ``vocab_cross_entropy``).  No gradient flows to the teacher's scores.
+    """
+    _check("topk_distillation", hidden, weight, bias)
+    _check_reduction("topk_distillation", reduction)
+    if teacher_scores.shape != teacher_ids.shape or \
+            teacher_scores.shape[:-1] != hidden.shape[:-1] or teacher_scores.dim() != hidden.dim():
+        raise ValueError(f"topk_distillation: teacher scores and ids must be "
+                         f"{tuple(hidden.shape[:-1])} + [K], got {tuple(teacher_scores.shape)} and "
+                         f"{tuple(teacher_ids.shape)}")
+    if teacher_ids.dtype.is_floating_point or teacher_ids.dtype == torch.bool:
+        raise ValueError("topk_distillation: teacher ids must be an integer tensor")
+    if teacher_scores.device != hidden.device or teacher_ids.device != hidden.device:
+        raise ValueError(f"topk_distillation: teacher scores and ids must live on {hidden.device}")
+    K = teacher_ids.shape[-1]
+    if not 1 <= K <= L.DISTILL_MAX_K:
+        raise ValueError(f"topk_distillation: {K} teacher entries, 1 to {L.DISTILL_MAX_K} are supported")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError("topk_distillation: temperature must be positive")
+    scores = teacher_scores.detach().reshape(-1, K).to(torch.float32).contiguous()
+    ids = teacher_ids.reshape(-1, K).to(torch.int64).contiguous()
+    return _loss(L.VOCAB_DISTILL, hidden, weight, bias, None, 0, scores, ids, float(temperature),
+                 reduction)
+
+
+# ---------------------------------------------------------------------------- sparse head
+def _head_forward(hidden, weight, bias, mask, Lt: int, train: bool):
+    dev = hidden.device
+    with torch.cuda.device(dev):
+        v = _view(hidden, weight, bias)
+        B = v.T // Lt
+        state, ws = _buffers(v, 0, L.VOCAB_HEAD, dev)
+        y = torch.empty((B, v.V), dtype=torch.float32, device=dev)
+        win = torch.empty((B, v.V), dtype=torch.int32, device=dev) if train else None
+        L.check(L.lib().gsp_sparse_head(ctypes.byref(v), Lt, L.ptr(mask), y.data_ptr(), L.ptr(win),
+                                        state.data_ptr(), state.numel(), ws.data_ptr(), ws.numel(),
+                                        L.stream_of(dev)), "sparse_head")
+    return y, win, state
+
+
+class _SparseHead(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, mask, Lt):
+        y, win, state = _head_forward(hidden, weight, bias, mask, Lt, True)
+        ctx.save_for_backward(weight, y)
+        ctx.win, ctx.state, ctx.T, ctx.Lt = win, state, hidden.shape[0], Lt
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        weight, y = ctx.saved_tensors
+        need_h, need_w, need_b = ctx.needs_input_grad[:3]
+        dev = weight.device
+        with torch.cuda.device(dev):
+            v = _view((ctx.T, weight.shape[1]), weight, None)
+            dy = dy.to(torch.float32).contiguous()
+            ws = _backward_ws(v, L.VOCAB_HEAD, dev)
+            dh = torch.empty((v.T, v.D), dtype=weight.dtype, device=dev) if need_h else None
+            dw = torch.empty((v.V, v.D), dtype=weight.dtype, device=dev) if need_w else None
+            db = torch.empty(v.V, dtype=torch.float32, device=dev) if need_b else None
+            L.check(L.lib().gsp_sparse_head_backward(
+                ctypes.byref(v), ctx.Lt, y.data_ptr(), ctx.win.data_ptr(), dy.data_ptr(), L.ptr(dh),
+                L.ptr(dw), L.ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(),
+                ws.numel(), L.stream_of(dev)), "sparse_head backward")
+        return dh, dw, db, None, None
+
+
+def sparse_head(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Term weights fp32 [B, V] of B texts: log1p(relu(max over the text's tokens of
+    hidden @ weight.T + bias)).
+
+    hidden [B, L, D], weight [V, D], mask [B, L] (nonzero or True = the token takes part, in
+    any pattern; None = all do).  A text without tokens has zero weights.  The gradient goes
+    to the token that won the maximum, the first one on ties.
+    """
+    _check("sparse_head", hidden, weight, bias)
+    if hidden.dim() != 3:
+        raise ValueError(f"sparse_head: hidden must be [B, L, D], got {tuple(hidden.shape)}")
+    B, Lt, D = hidden.shape
+    V = weight.shape[0]
+    if mask is not None:
+        if mask.shape != (B, Lt):
+            raise ValueError(f"sparse_head: mask must be {(B, Lt)}, got {tuple(mask.shape)}")
+        if mask.device != hidden.device:
+            raise ValueError(f"sparse_head: mask must live on {hidden.device}")
+        mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+    if Lt == 0:
+        return torch.zeros((B, V), dtype=torch.float32, device=hidden.device)
+    if B > 65534:
+        raise ValueError(f"sparse_head: {B} texts in one call, at most 65534 are supported")
+    rows = _rows(hidden.reshape(B * Lt, D))
+    weight = _rows(weight)
+    if bias is not None:
+        bias = bias.to(torch.float32).contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        return _SparseHead.apply(rows, weight, bias, mask, Lt)
+    return _head_forward(rows, weight, bias, mask, Lt, False)[0]
+
+
+# ---------------------------------------------------------------------------- index and queries
+def encode_documents(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                     mask: Optional[torch.Tensor] = None, min_weight: float = 0.0):
+    """Documents as CSR rows for the index builders: ``(indptr int64 [B + 1], indices int32,
+    data fp32)`` on the GPU, the terms of ``sparse_head`` with a weight above ``min_weight``
+    (>= 0) in ascending order.  Synchronises once for the number of terms."""
+    if not min_weight >= 0.0:
+        raise ValueError("encode_documents: min_weight must be >= 0")
+    with torch.no_grad():
+        y = sparse_head(hidden, weight, bias, mask)
+    B, V = y.shape
+    dev = y.device
+    lib = L.lib()
+    with torch.cuda.device(dev):
+        st = L.stream_of(dev)
+        nnz = torch.empty(B, dtype=torch.int32, device=dev)
+        indptr = torch.empty(B + 1, dtype=torch.int64, device=dev)
+        ws = L.workspace(lib.gsp_scan_ws_bytes(B), dev)
+        L.check(lib.gsp_dense_rows_count(L.ptr(y), B, V, min_weight, L.ptr(nnz), st), "encode_documents")
+        L.check(lib.gsp_scan_i32(L.ptr(nnz), B, L.ptr(indptr), L.ptr(ws), ws.numel(), st),
+                "encode_documents")
+        total = int(indptr[B].item())
+        indices = torch.empty(total, dtype=torch.int32, device=dev)
+        data = torch.empty(total, dtype=torch.float32, device=dev)
+        L.check(lib.gsp_dense_rows_fill(L.ptr(y), B, V, min_weight, L.ptr(indptr), L.ptr(indices),
+                                        L.ptr(data), st), "encode_documents")
+    return indptr, indices, data
+
+
+def encode_queries(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   mask: Optional[torch.Tensor] = None, max_terms: int = 128
+                   ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Queries as the scorer takes them: term ids int32 and weights fp32, both [B, max_terms]
+    (-1 / 0 padded), the ``max_terms`` strongest terms of ``sparse_head``, ties by ascending
+    term id."""
+    if max_terms < 1:
+        raise ValueError("encode_queries: max_terms must be positive")
+    with torch.no_grad():
+        y = sparse_head(hidden, weight, bias, mask)
+        B, V = y.shape
+        tau = torch.full((B,), torch.finfo(torch.float32).tiny, device=y.device)
+        w, t = compacted_topk(y, tau, max_terms)
+        pad = w == float("-inf")
+        qi = torch.where(pad, torch.full_like(t, -1), t).to(torch.int32)
+        qs = torch.where(pad, torch.zeros_like(w), w)
+        if qi.shape[1] < max_terms:
+            qi = torch.nn.functional.pad(qi, (0, max_terms - qi.shape[1]), value=-1)
+            qs = torch.nn.functional.pad(qs, (0, max_terms - qs.shape[1]))
+    return qi, qs
+
+
+def build_index_from_hidden(batches: Iterable, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                            min_weight: float = 0.0, weight_dtype: str = "fp32",
+                            doc_base: int = 0) -> GPUInvertedIndex:
+    """Index of the documents whose hidden states ``batches`` yields, in order: each batch
+    hidden [B, L, D], or a pair (hidden, mask).  The vocabulary is weight's rows; the other
+    arguments are ``encode_documents``' and ``build_from_csr_tensors``'."""
+    ptrs, indices, data = [], [], []
+    base = 0
+    for batch in batches:
+        hidden, mask = batch if isinstance(batch, (tuple, list)) else (batch, None)
+        ip, ix, dt = encode_documents(hidden, weight, bias, mask, min_weight)
+        ptrs.append(ip[:-1] + base)
+        indices.append(ix)
+        data.append(dt)
+        base += ix.numel()
+    dev = weight.device
+    ptrs.append(torch.full((1,), base, dtype=torch.int64, device=dev))
+    empty_i = torch.empty(0, dtype=torch.int32, device=dev)
+    empty_f = torch.empty(0, dtype=torch.float32, device=dev)
+    return build_from_csr_tensors(torch.cat(ptrs), torch.cat(indices or [empty_i]),
+                                  torch.cat(data or [empty_f]), weight.shape[0], dev,
+                                  weight_dtype=weight_dtype, doc_base=doc_base)

@@ -52,6 +52,7 @@ extern "C" {
 #define GSP_W_F32 0
 #define GSP_W_BF16 1
 #define GSP_W_U8 2
+#define GSP_W_F16 3            /* vocabulary head only */
 
 const char* gsp_last_error(void);
 int gsp_version(void);
@@ -341,6 +342,88 @@ int64_t gsp_compacted_ws_bytes(int64_t B, int64_t L, int64_t k, int64_t max_cand
 int gsp_compacted_topk(const float* scores, int64_t B, int64_t L, int64_t stride,
                        const float* tau, int64_t k, int64_t max_cand, float* out_v,
                        int64_t* out_i, void* ws, int64_t ws_bytes, void* stream);
+
+/* ---------------------------------------------------------------- vocabulary head */
+/* The projection that term weights come from and the losses it is trained with (no
+ * counterpart in the reference's scoring path; its encoders run this step in torch before
+ * they build an index, src/real_splade_benchmark.py).  For hidden states H [T, D] and
+ * projection rows W [V, D] (both bf16 or both fp16), s[t, v] = H[t] . W[v] + bias[v] are the
+ * logits.  No call stores them: products run on the tensor cores with fp32 accumulators and
+ * are reduced where they are made.  Results do not depend on scheduling (no floating-point
+ * atomics).  A bounded wait that runs out (gsp_set_wait_limit) gives NaN results. */
+typedef struct gsp_vocab_view {
+    int64_t T;                 /* tokens (for the sparse head: texts x length) */
+    int64_t V;
+    int64_t D;
+    int64_t ld_hidden;         /* elements between rows of hidden (>= D) */
+    int64_t ld_weight;         /* elements between rows of weight (>= D) */
+    const void* hidden;
+    const void* weight;
+    const float* bias;         /* [V], or NULL */
+    int32_t dtype;             /* GSP_W_BF16 or GSP_W_F16, of hidden, weight and their gradients */
+    int32_t pad_;
+} gsp_vocab_view;
+
+#define GSP_VOCAB_CE 0
+#define GSP_VOCAB_DISTILL 1
+#define GSP_VOCAB_HEAD 2
+#define GSP_REDUCE_NONE 0
+#define GSP_REDUCE_SUM 1
+#define GSP_REDUCE_MEAN 2
+#define GSP_DISTILL_MAX_K 1024
+
+/* A forward call leaves in `state` (gsp_vocab_state_bytes; K = teacher entries per row, else
+ * 0) what its backward call needs: the rows that took part, packed, their softmax
+ * denominators and the teacher's probabilities.  The caller's hidden and targets are not
+ * read again.  ws is scratch of the one call (gsp_vocab_ws_bytes, backward 0 or 1); no call
+ * allocates, synchronises or keeps anything else, so calls can be captured, and calls with
+ * their own buffers can overlap.  Both functions return a negative status on error. */
+int64_t gsp_vocab_state_bytes(int64_t T, int64_t V, int64_t D, int64_t K, int32_t kind);
+int64_t gsp_vocab_ws_bytes(const gsp_vocab_view* vw, int32_t kind, int32_t backward);
+
+/* Softmax cross entropy of every row whose target lies in [0, V) and is not ignore_index;
+ * the other rows take no part (their hidden states are never used, whatever they hold).
+ * loss: fp32, one value (sum, or mean over the rows that take part, 0 when there are none)
+ * or [T] (GSP_REDUCE_NONE, 0 for rows that take no part). */
+int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore_index, int32_t reduction, float* loss,
+                 void* state, int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream);
+/* Distillation from a teacher's top scores (scores fp32, ids int64, both [T, K], K <=
+ * GSP_DISTILL_MAX_K): with p = softmax(scores / tau) over a row's entries, the loss of the
+ * row is tau^2 KL(p || softmax(s / tau)).  Entries with an id outside [0, V) or a score of
+ * -inf (the padding of gsp_score_topk and gsp_compacted_topk) are left out, an id listed
+ * twice adds its probabilities, and a row without entries takes no part. */
+int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, const int64_t* ids, int64_t K, float tau,
+                      int32_t reduction, float* loss, void* state, int64_t state_bytes, void* ws, int64_t ws_bytes,
+                      void* stream);
+/* Gradients of either loss from the state its forward call left (vw with the same sizes and
+ * weight; hidden unused): d_hidden [T, D] and d_weight [V, D] in dtype, d_bias fp32 [V], each
+ * contiguous and each optional (NULL).  grad_loss: fp32, one value, or [T] with
+ * GSP_REDUCE_NONE.  K and tau are the forward call's, for GSP_VOCAB_DISTILL.  The softmax is computed again, for a piece of the vocabulary at a time
+ * (at most 512 MiB of ws); its gradient is rounded to dtype as an operand of the two
+ * products that follow. */
+int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, int64_t K, float tau, int32_t reduction,
+                            const float* grad_loss, void* d_hidden, void* d_weight, float* d_bias,
+                            void* state, int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream);
+
+/* Sparse head: term weights of B = T / L texts of L tokens (mask uint8 [T], 0 = the token takes
+ * no part, NULL = all do; any pattern),
+ *   y[b, v] = log1p(max(0, max over the text's tokens of s[t, v]))     fp32 [B, V],
+ * 0 for a text without tokens.  win (int32 [B, V], or NULL when no backward call follows) gets
+ * the packed row of the token that won, the first on ties, or -1 where y is 0. */
+int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_t* mask, float* y, int32_t* win, void* state,
+                    int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream);
+/* Its gradients from dy fp32 [B, V] and what the forward call left (vw with the same sizes and
+ * weight; hidden unused): ds = dy exp(-y) goes to the winning token.  Outputs as in
+ * gsp_vocab_loss_backward. */
+int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, const float* y, const int32_t* win, const float* dy,
+                             void* d_hidden, void* d_weight, float* d_bias, void* state, int64_t state_bytes, void* ws,
+                             int64_t ws_bytes, void* stream);
+/* Rows of a dense [B, V] fp32 matrix (the sparse head's y) as CSR rows for the index builders:
+ * nnz[b] = entries > min_weight, then (after a scan of nnz into indptr, gsp_scan_i32) their
+ * columns and values in ascending column order. */
+int gsp_dense_rows_count(const float* y, int64_t B, int64_t V, float min_weight, int32_t* nnz, void* stream);
+int gsp_dense_rows_fill(const float* y, int64_t B, int64_t V, float min_weight, const int64_t* indptr, int32_t* indices,
+                        float* data, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,536 @@
+"""The vocabulary head's operators on the GPU against their definitions in 64 bits."""
+import pytest
+import torch
+
+import head_reference as R
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+BF, HF = torch.bfloat16, torch.float16
+
+
+def make(T, V, D, dt, seed=0, bias=True):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(T, D, generator=g).to(dt)
+    w = (torch.randn(V, D, generator=g) * (2.0 / D ** 0.5)).to(dt)
+    b = torch.randn(V, generator=g) * 0.5 if bias else None
+    return h.to(DEV), w.to(DEV), b.to(DEV) if bias else None
+
+
+def leaf(x):
+    return x.detach().clone().requires_grad_(True) if x is not None else None
+
+
+def one_hot(targets, V, live):
+    q = torch.zeros(len(targets), V, dtype=torch.float64, device=DEV)
+    q[live, targets[live]] = 1.0
+    return q
+
+
+def check_ce(h, w, b, targets, ignore=-100, reduction="mean", grad=None):
+    import gpusparse
+    T, V = h.shape[0], w.shape[0]
+    live = (targets >= 0) & (targets < V) & (targets != ignore)
+    n = max(int(live.sum()), 1)
+    if reduction == "none":
+        rows = grad
+    else:
+        scale = 1.0 if grad is None else float(grad)
+        rows = torch.full((T,), scale / (n if reduction == "mean" else 1), device=DEV)
+    ref, (rh, rw, rb) = R.softmax_loss(h, w, b, one_hot(targets, V, live), live, 1.0, rows, h.dtype)
+    hl, wl, bl = h.requires_grad_(True), w.requires_grad_(True), leaf(b)
+    loss = gpusparse.vocab_cross_entropy(hl, wl, targets, bias=bl, ignore_index=ignore, reduction=reduction)
+    assert loss.dtype == torch.float32
+    if reduction == "none":
+        R.assert_within(loss.detach(), ref, "loss")
+    else:
+        div = n if reduction == "mean" else 1
+        R.assert_within(loss.detach(), (ref[0].sum() / div, ref[1].sum() / div + 2.0 ** -23 * ref[0].sum().abs() / div), "loss")
+    leaves = [x for x in (hl, wl, bl) if x is not None]
+    go = rows if reduction == "none" else torch.tensor(1.0 if grad is None else float(grad), device=DEV)
+    got = torch.autograd.grad(loss, leaves, go.to(torch.float32))
+    R.assert_within(got[0], rh, "dh")
+    R.assert_within(got[1], rw, "dw")
+    if b is not None:
+        R.assert_within(got[2], rb, "db")
+    assert got[0].dtype == h.dtype and got[1].dtype == w.dtype
+    assert (got[0][~live] == 0).all()
+    return loss.detach(), got
+
+
+@pytest.mark.parametrize("T,V,D,dt,frac,bias", [
+    (1, 256, 64, BF, 1.0, True),
+    (1, 1, 1, BF, 1.0, True),
+    (3, 7, 8, HF, 1.0, False),
+    (130, 1000, 331, HF, 0.6, True),
+    (300, 513, 72, BF, 0.5, False),
+    (257, 255, 65, BF, 1.0, True),
+    (64, 30522, 768, BF, 1.0, True),
+    (5, 30522, 1024, HF, 1.0, False),
+    (3000, 300, 128, BF, 0.15, True),
+])
+def test_cross_entropy(T, V, D, dt, frac, bias):
+    h, w, b = make(T, V, D, dt, seed=T + V, bias=bias)
+    g = torch.Generator().manual_seed(T)
+    targets = torch.randint(0, V, (T,), generator=g)
+    targets[torch.rand(T, generator=g) >= frac] = -100
+    check_ce(h, w, b, targets.to(DEV), grad=1.0 if dt == BF else 1024.0)
+
+
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_cross_entropy_reductions(reduction, dt):
+    h, w, b = make(200, 777, 96, dt, seed=5)
+    g = torch.Generator().manual_seed(1)
+    targets = torch.randint(0, 777, (200,), generator=g)
+    targets[::7] = -100
+    grad = torch.randn(200, generator=g).to(DEV) if reduction == "none" else 0.37
+    check_ce(h, w, b, targets.to(DEV), reduction=reduction, grad=grad)
+
+
+def test_cross_entropy_ignored_rows_hold_anything():
+    """Ignored tokens and targets outside the vocabulary: NaN and infinities in their hidden
+    states reach nothing; the others' results are those without these rows, bit for bit."""
+    import gpusparse
+    h, w, b = make(140, 500, 80, BF, seed=6)
+    targets = torch.arange(140, device=DEV) * 3
+    targets[5], targets[9], targets[11], targets[139] = -100, 500, -7, 33
+    bad = [5, 9, 11, 139]
+    h[5], h[9], h[11], h[139] = float("nan"), float("inf"), float("-inf"), float("nan")
+    loss, got = check_ce(h, w, b, targets, ignore=33)
+    keep = torch.tensor([r for r in range(140) if r not in bad and int(targets[r]) != 33], device=DEV)
+    hl, wl, bl = leaf(h[keep]), leaf(w), leaf(b)
+    l2 = gpusparse.vocab_cross_entropy(hl, wl, targets[keep], bias=bl, ignore_index=33)
+    g2 = torch.autograd.grad(l2, (hl, wl, bl))
+    assert torch.equal(loss, l2) and torch.equal(got[0][keep], g2[0])
+    assert torch.equal(got[1], g2[1]) and torch.equal(got[2], g2[2])
+
+
+def test_cross_entropy_without_any_target():
+    import gpusparse
+    h, w, b = make(70, 300, 64, BF, seed=7)
+    hl, wl, bl = leaf(h), leaf(w), leaf(b)
+    loss = gpusparse.vocab_cross_entropy(hl, wl, torch.full((70,), -100, device=DEV), bias=bl)
+    grads = torch.autograd.grad(loss, (hl, wl, bl))
+    assert float(loss.detach()) == 0.0 and all((x == 0).all() for x in grads)
+    hl = leaf(h[:0])
+    loss = gpusparse.vocab_cross_entropy(hl, wl, torch.zeros(0, dtype=torch.int64, device=DEV))
+    grads = torch.autograd.grad(loss, (hl, wl))
+    assert float(loss.detach()) == 0.0 and (grads[1] == 0).all() and grads[0].shape == (0, 64)
+
+
+def test_cross_entropy_masked_vocabulary():
+    """A bias of -inf (or the type's lowest value) takes words out of the vocabulary."""
+    h, w, b = make(40, 600, 64, BF, seed=8)
+    b[100:400] = float("-inf")
+    b[400:450] = torch.finfo(torch.float32).min
+    targets = torch.arange(40, device=DEV)
+    loss, got = check_ce(h, w, b, targets)
+    assert (got[1][100:450] == 0).all() and (got[2][100:450] == 0).all()
+
+
+def test_cross_entropy_layouts():
+    """Row strides, unaligned starts, leading dimensions, int32 targets, a 16-bit bias."""
+    import gpusparse
+    g = torch.Generator().manual_seed(3)
+    wide = torch.randn(6, 10, 131, generator=g).to(BF).to(DEV)
+    ww = (torch.randn(450, 140, generator=g) * 0.2).to(BF).to(DEV)
+    b = torch.randn(450, generator=g).to(BF).to(DEV)
+    targets = torch.randint(0, 450, (6, 10), generator=g).to(DEV)
+    a = dict(h=wide[..., 3:123], w=ww[:, 5:125])
+    dense = gpusparse.vocab_cross_entropy(a["h"].contiguous(), a["w"].contiguous(), targets, bias=b.float())
+    assert torch.equal(gpusparse.vocab_cross_entropy(a["h"], a["w"], targets.to(torch.int32), bias=b), dense)
+    by_row = gpusparse.vocab_cross_entropy(a["h"], a["w"], targets, bias=b, reduction="none")
+    assert by_row.shape == (6, 10)
+    t = a["w"].t().contiguous().t()                      # columns contiguous
+    assert torch.equal(gpusparse.vocab_cross_entropy(a["h"], t, targets, bias=b), dense)
+    # broadcast rows: the gradient of the shared row is the sum over its uses
+    one = leaf(wide[0, :1, 3:123])
+    loss = gpusparse.vocab_cross_entropy(one.expand(9, 120), a["w"], targets[0, :9])
+    (d1,) = torch.autograd.grad(loss, one)
+    rep = leaf(one.expand(9, 120))
+    (d9,) = torch.autograd.grad(gpusparse.vocab_cross_entropy(rep, a["w"], targets[0, :9]), rep)
+    assert d1.shape == one.shape and torch.allclose(d1.float(), d9.float().sum(0, keepdim=True), rtol=2 ** -7, atol=1e-3)
+
+
+def test_cross_entropy_gradient_matches_differences():
+    """The gradient along a direction against a central difference of the 64-bit loss."""
+    import gpusparse
+    h, w, b = make(60, 400, 64, BF, seed=12)
+    targets = torch.arange(60, device=DEV) * 5
+    hl, wl, bl = leaf(h), leaf(w), leaf(b)
+    grads = torch.autograd.grad(gpusparse.vocab_cross_entropy(hl, wl, targets, bias=bl), (hl, wl, bl))
+    g = torch.Generator().manual_seed(4)
+    for i, (x, d) in enumerate(zip((h, w, b), grads)):
+        v = torch.randn(x.shape, generator=g).to(DEV).double()
+
+        def f(step):
+            p = [h.double(), w.double(), b.double()]
+            p[i] = p[i] + step * v
+            return torch.nn.functional.cross_entropy(p[0] @ p[1].t() + p[2], targets)
+        diff = (f(1e-5) - f(-1e-5)) / 2e-5
+        # sum of independent roundings of at most 2^-8 of each term (its own and P's), by the
+        # triangle inequality over the terms
+        bound = 2.0 ** -7 * (d.double().abs() * v.abs()).sum() + 1e-6
+        assert abs(float((d.double() * v).sum() - diff)) <= float(bound)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_cross_entropy_in_pieces(dt):
+    """More rows x vocabulary than one piece of the backward pass holds: d_hidden is carried
+    over the pieces in fp32; the reference is the same formula in fp64 on the GPU, row blocks
+    at a time."""
+    import gpusparse
+    T, V, D = 20000, 15000, 40
+    h, w, b = make(T, V, D, dt, seed=9)
+    g = torch.Generator().manual_seed(2)
+    targets = torch.randint(0, V, (T,), generator=g).to(DEV)
+    hl, wl, bl = leaf(h), leaf(w), leaf(b)
+    loss = gpusparse.vocab_cross_entropy(hl, wl, targets, bias=bl, reduction="sum")
+    got = torch.autograd.grad(loss, (hl, wl, bl), torch.tensor(1.0, device=DEV))
+    hd, wd, total = h.double(), w.double(), 0.0
+    dw = torch.zeros(V, D, dtype=torch.float64, device=DEV)
+    db = torch.zeros(V, dtype=torch.float64, device=DEV)
+    bw = torch.zeros_like(dw)
+    u = R.U[dt]
+    for lo in range(0, T, 2500):
+        r = slice(lo, lo + 2500)
+        s = hd[r] @ wd.t() + b.double()
+        P = torch.softmax(s, 1)
+        total += float((torch.logsumexp(s, 1) - s.gather(1, targets[r, None]).squeeze(1)).sum())
+        P[torch.arange(2500, device=DEV), targets[r]] -= 1.0
+        dh = P @ wd
+        # P: u + 2^-13 relative (logit errors of 48 * 2^-23 * sum |h||w| < 2^-15, twice), 2^-39
+        # absolute in fp16; the sums' own roundings (V + T) 2^-23 are below 2^-8 of u each
+        aP = P.abs() * (u + 2.0 ** -13 + V * 2.0 ** -23) + 2.0 ** -39
+        bound = (aP @ wd.abs()) * (1 + u) + u * dh.abs() + R.SUB[dt]
+        assert ((got[0][r].double() - dh).abs() <= bound).all()
+        dw += P.t() @ hd[r]
+        bw += aP.t() @ hd[r].abs()
+        db += P.sum(0)
+    bound = (bw + T * 2.0 ** -23 * bw / u) * (1 + u) + u * dw.abs() + R.SUB[dt]
+    assert ((got[1].double() - dw).abs() <= bound).all()
+    assert abs(float(loss) - total) <= 2.0 ** -13 * T
+    # column sums of 20000 unrounded terms: 2^-13 of the terms' absolute sum (<= 2 per column on
+    # average, counted as the target count + the softmax mass)
+    mass = torch.bincount(targets, minlength=V).double() * 2 + db.abs()
+    assert ((got[2].double() - db).abs() <= (2.0 ** -13 + T * 2.0 ** -24) * (mass + 1)).all()
+
+
+# ---------------------------------------------------------------------------- distillation
+def teacher(T, V, K, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(T)])
+    scores = torch.sort(torch.randn(T, K, generator=g) * 2 + 6, dim=1, descending=True).values
+    return scores.to(DEV), ids.to(DEV)
+
+
+def check_distill(h, w, b, scores, ids, tau, reduction="mean", grad=1.0):
+    import gpusparse
+    T, V = h.shape[0], w.shape[0]
+    ok = (ids >= 0) & (ids < V) & (scores > float("-inf"))
+    live = ok.any(1)
+    x = torch.where(ok, scores.double(), float("-inf")) / tau
+    p = torch.where(ok, torch.exp(x - torch.where(live, x.max(1).values, 0.0)[:, None]), 0.0)
+    p = p / torch.where(live, p.sum(1), 1.0)[:, None]
+    q = torch.zeros(T, V, dtype=torch.float64, device=DEV)
+    q.scatter_add_(1, torch.where(ok, ids, 0), p)
+    n = max(int(live.sum()), 1)
+    rows = torch.full((T,), grad / (n if reduction == "mean" else 1), device=DEV)
+    ref, (rh, rw, rb) = R.softmax_loss(h, w, b, q, live, tau, rows, h.dtype)
+    hl, wl, bl = leaf(h), leaf(w), leaf(b)
+    loss = gpusparse.topk_distillation(hl, wl, scores, ids, bias=bl, temperature=tau, reduction=reduction)
+    div = n if reduction == "mean" else 1
+    R.assert_within(loss.detach(), (ref[0].sum() / div, ref[1].sum() / div + 2.0 ** -23 * ref[0].sum().abs() / div), "loss")
+    leaves = [t for t in (hl, wl, bl) if t is not None]
+    got = torch.autograd.grad(loss, leaves, torch.tensor(grad, device=DEV))
+    R.assert_within(got[0], rh, "dh")
+    R.assert_within(got[1], rw, "dw")
+    if b is not None:
+        R.assert_within(got[2], rb, "db")
+    return loss.detach(), got
+
+
+@pytest.mark.parametrize("T,V,D,K,tau,dt,bias", [
+    (1, 300, 64, 1, 1.0, BF, True),
+    (33, 700, 72, 10, 2.0, BF, True),
+    (140, 2000, 100, 100, 0.7, HF, False),
+    (70, 5000, 256, 1000, 1.0, BF, True),
+    (9, 1024, 64, 1024, 1.5, HF, True),
+    (260, 257, 33, 37, 1.0, BF, False),
+])
+def test_distillation(T, V, D, K, tau, dt, bias):
+    h, w, b = make(T, V, D, dt, seed=T, bias=bias)
+    scores, ids = teacher(T, V, K, seed=K)
+    check_distill(h, w, b, scores, ids, tau, grad=1.0 if dt == BF else 512.0)
+
+
+def test_distillation_padding_duplicates_and_empty_rows():
+    h, w, b = make(50, 400, 64, BF, seed=21)
+    scores, ids = teacher(50, 400, 16, seed=3)
+    scores[3, 10:], ids[3, 10:] = float("-inf"), 0          # compacted_topk's padding
+    scores[4, 5:], ids[4, 5:] = float("-inf"), -1           # score_topk's padding
+    ids[5] = 77                                             # one word for all
+    ids[6, 4], ids[6, 9] = ids[6, 0].clone(), ids[6, 0].clone()
+    ids[7, 2], ids[7, 3] = 400, -5                          # outside the vocabulary
+    scores[8] = float("-inf")                               # nothing left
+    scores[9, 3] = torch.finfo(torch.float32).min           # probability 0
+    ids[10] = -1
+    h[8], h[10] = float("nan"), float("inf")
+    loss, got = check_distill(h, w, b, scores, ids, 1.3)
+    assert (got[0][8] == 0).all() and (got[0][10] == 0).all()
+    check_distill(h, w, b, scores, ids, 1.3, reduction="sum", grad=0.25)
+
+
+def test_distillation_from_one_entry_is_cross_entropy():
+    import gpusparse
+    h, w, b = make(90, 600, 64, BF, seed=22)
+    ids = torch.arange(90, device=DEV) * 6
+    a, ga = check_ce(h, w, b, ids)
+    c, gc = check_distill(h, w, b, torch.zeros(90, 1, device=DEV), ids[:, None], 1.0)
+    assert torch.equal(a, c) and all(torch.equal(x, y) for x, y in zip(ga, gc))
+
+
+# ---------------------------------------------------------------------------- sparse head
+def head_inputs(B, Lt, V, D, dt, seed, bias_mean=-1.0):
+    """Fixed-point values whose products sum without rounding: maxima and their ties are the
+    same in every order of summation."""
+    g = torch.Generator().manual_seed(seed)
+
+    def grid(x, step):
+        return torch.round(x / step) * step
+    h = grid(torch.randn(B, Lt, D, generator=g).clamp(-3.9, 3.9), 2.0 ** -5).to(dt)
+    w = grid((torch.randn(V, D, generator=g) / D ** 0.5).clamp(-0.24, 0.24), 2.0 ** -10).to(dt)
+    b = grid(torch.randn(V, generator=g) * 0.5 + bias_mean, 2.0 ** -10)
+    dy = torch.randn(B, V, generator=g)
+    return h.to(DEV), w.to(DEV), b.to(DEV), dy.to(DEV)
+
+
+def check_head(h, w, b, mask, dy):
+    import gpusparse
+    ref, (rh, rw, rb) = R.sparse_head(h, w, b, mask != 0 if mask is not None else
+                                      torch.ones(h.shape[:2], dtype=torch.bool, device=DEV), dy, h.dtype)
+    with torch.no_grad():
+        y0 = gpusparse.sparse_head(h, w, bias=b, mask=mask)
+    hl, wl, bl = leaf(h), leaf(w), leaf(b)
+    y = gpusparse.sparse_head(hl, wl, bias=bl, mask=mask)
+    assert torch.equal(y, y0)
+    R.assert_within(y.detach(), ref, "y")
+    leaves = [x for x in (hl, wl, bl) if x is not None]
+    got = torch.autograd.grad(y, leaves, dy)
+    R.assert_within(got[0].reshape(-1, h.shape[2]), rh, "dh")
+    R.assert_within(got[1], rw, "dw")
+    if b is not None:
+        R.assert_within(got[2], rb, "db")
+    return y.detach(), got
+
+
+@pytest.mark.parametrize("B,Lt,V,D,dt", [
+    (1, 1, 5, 8, BF),
+    (1, 16, 30522, 256, BF),
+    (1, 700, 300, 64, BF),          # one text over many shares
+    (3, 700, 300, 72, HF),
+    (40, 9, 1000, 331, BF),
+    (130, 33, 257, 64, HF),
+    (5, 256, 4000, 128, BF),
+    (2, 300, 128, 1000, BF),
+])
+def test_sparse_head(B, Lt, V, D, dt):
+    h, w, b, dy = head_inputs(B, Lt, V, D, dt, seed=B + Lt)
+    check_head(h, w, b, None, dy)
+    g = torch.Generator().manual_seed(B)
+    mask = (torch.rand(B, Lt, generator=g) < 0.6).to(DEV)        # any pattern
+    if B > 2:
+        mask[1] = False
+    check_head(h, w, b, mask, dy)
+    check_head(h, w, None, mask, dy)
+
+
+def test_sparse_head_masked_tokens_hold_anything():
+    h, w, b, dy = head_inputs(6, 50, 500, 64, BF, seed=31)
+    mask = torch.zeros(6, 50, dtype=torch.bool, device=DEV)
+    for i, n in enumerate([50, 20, 0, 1, 33, 7]):
+        mask[i, :n] = True
+    y, got = check_head(h, w, b, mask, dy)
+    h2 = h.clone()
+    h2[~mask] = float("nan")
+    y2, got2 = check_head(h2, w, b, mask.to(torch.int64), dy)
+    assert torch.equal(y, y2) and all(torch.equal(a, c) for a, c in zip(got, got2))
+    assert (y[2] == 0).all() and (got[0][2] == 0).all()
+
+
+def test_sparse_head_ties_go_to_the_first_token():
+    import gpusparse
+    h, w, b, dy = head_inputs(3, 40, 300, 64, BF, seed=32)
+    h[:, 20:] = h[:, :20]                     # every token twice
+    _, got = check_head(h, w, b, None, dy)
+    assert (got[0][:, 20:] == 0).all()
+
+
+def test_sparse_head_propagates_nan_of_tokens_that_take_part():
+    import gpusparse
+    h, w, b, dy = head_inputs(3, 40, 300, 64, BF, seed=33)
+    h[1, 17] = float("nan")
+    y = gpusparse.sparse_head(h, w, bias=b)
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2]).all()
+
+
+def test_sparse_head_without_texts_or_tokens():
+    import gpusparse
+    h, w, b, _ = head_inputs(3, 4, 50, 16, BF, seed=34)
+    assert gpusparse.sparse_head(h[:0], w, bias=b).shape == (0, 50)
+    assert (gpusparse.sparse_head(h[:, :0], w, bias=b) == 0).all()
+    none = torch.zeros(3, 4, dtype=torch.bool, device=DEV)
+    wl = leaf(w)
+    y = gpusparse.sparse_head(h, wl, bias=b, mask=none)
+    (dw,) = torch.autograd.grad(y.sum(), wl)
+    assert (y == 0).all() and (dw == 0).all()
+
+
+# ---------------------------------------------------------------------------- how calls run
+def step(h, w, b, targets, scores, ids):
+    import gpusparse
+    loss = gpusparse.vocab_cross_entropy(h, w, targets, bias=b) + \
+        gpusparse.topk_distillation(h, w, scores, ids, bias=b) + \
+        gpusparse.sparse_head(h[None], w, bias=b).mean()
+    return (loss.detach(),) + torch.autograd.grad(loss, (h, w, b))
+
+
+def step_inputs(seed):
+    h, w, b = make(300, 900, 96, BF, seed=seed)
+    targets = torch.arange(300, device=DEV) * 3
+    scores, ids = teacher(300, 900, 12, seed=seed)
+    return leaf(h), leaf(w), leaf(b), targets, scores, ids
+
+
+def test_equal_inputs_give_equal_bits_on_any_stream():
+    a = step(*step_inputs(41))
+    s = torch.cuda.Stream()
+    inputs = step_inputs(41)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        c = step(*inputs)
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))
+
+
+def test_captured_training_step_replays_on_new_inputs():
+    """Forward and backward in one CUDA graph, then other values in the same tensors; two
+    graphs captured over the same leaves keep their own buffers."""
+    inputs = step_inputs(42)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(*inputs)
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(*inputs)
+        graphs.append((g, out))
+    other = step_inputs(43)
+    want = step(*other)
+    with torch.no_grad():
+        for x, y in zip(inputs, other):
+            x.copy_(y)
+    for g, _ in graphs:
+        g.replay()
+    for _, out in graphs:
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+
+
+def test_wait_that_runs_out_shows_in_the_result():
+    """With no polls allowed some wait gives up: the results are NaN, nothing hangs, and the
+    next call is right again."""
+    import gpusparse
+    import gpusparse._lib as L
+    h, w, b = make(300, 900, 512, BF, seed=44)
+    targets = torch.arange(300, device=DEV) * 3
+    want = gpusparse.vocab_cross_entropy(h, w, targets, bias=b)
+    lib = L.lib()
+    default = lib.gsp_get_wait_limit()
+    L.check(lib.gsp_set_wait_limit(0), "wait limit")
+    try:
+        got = [gpusparse.vocab_cross_entropy(h, w, targets, bias=b) for _ in range(3)]
+        y = gpusparse.sparse_head(h[None], w, bias=b)
+        torch.cuda.synchronize()
+    finally:
+        L.check(lib.gsp_set_wait_limit(default), "wait limit")
+    assert any(torch.isnan(x).item() for x in got)
+    assert torch.isnan(y).any()
+    assert torch.equal(gpusparse.vocab_cross_entropy(h, w, targets, bias=b), want)
+
+
+def test_backward_twice_and_changed_inputs():
+    import gpusparse
+    h, w, b = make(100, 400, 64, BF, seed=45)
+    targets = torch.arange(100, device=DEV)
+    hl, wl, bl = leaf(h), leaf(w), leaf(b)
+    loss = gpusparse.vocab_cross_entropy(hl, wl, targets, bias=bl)
+    first = torch.autograd.grad(loss, (hl, wl, bl), retain_graph=True)
+    targets.fill_(7)                              # the forward call kept its own
+    second = torch.autograd.grad(loss, (hl, wl, bl), retain_graph=True)
+    assert all(torch.equal(x, y) for x, y in zip(first, second))
+    only = torch.autograd.grad(loss, (wl,), retain_graph=True)
+    assert torch.equal(only[0], first[1])
+    with torch.no_grad():
+        wl.add_(1.0)                              # the weight is needed unchanged
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, (hl,))
+
+
+# ---------------------------------------------------------------------------- refusals
+def test_refusals():
+    import gpusparse
+    h, w, b = make(10, 50, 16, BF, seed=51)
+    t = torch.zeros(10, dtype=torch.int64, device=DEV)
+    ce, di, sh = gpusparse.vocab_cross_entropy, gpusparse.topk_distillation, gpusparse.sparse_head
+    s, i = torch.zeros(10, 4, device=DEV), torch.zeros(10, 4, dtype=torch.int64, device=DEV)
+    for bad in (lambda: ce(h.float(), w.float(), t), lambda: ce(h, w.half(), t), lambda: ce(h, w[:, :8], t),
+                lambda: ce(h, w, t[:5]), lambda: ce(h, w, t.float()), lambda: ce(h, w, t, bias=b[:9]),
+                lambda: ce(h, w, t, reduction="median"), lambda: ce(h, w[:0], t),
+                lambda: ce(h, w, t.cpu()), lambda: ce(h, w.cpu(), t.cpu()) if False else ce(h, w, t, bias=b.cpu()),
+                lambda: di(h, w, s, i[:, :3]), lambda: di(h, w, s, i, temperature=0.0),
+                lambda: di(h, w, s, i, temperature=float("inf")), lambda: di(h, w, s, s),
+                lambda: di(h, w, torch.zeros(10, 1025, device=DEV), torch.zeros(10, 1025, dtype=torch.int64, device=DEV)),
+                lambda: di(h, w, s[:, :0], i[:, :0]), lambda: sh(h, w), lambda: sh(h[None], w, mask=t[None, :3]),
+                lambda: gpusparse.encode_queries(h[None], w, max_terms=0),
+                lambda: gpusparse.encode_documents(h[None], w, min_weight=-1.0)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        ce(h.cpu(), w, t)
+
+
+# ---------------------------------------------------------------------------- used together
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_encode_index_search_and_distil(dt):
+    """Documents and queries through the head, an index of the documents, the scorer's top-k
+    against the dense product of the weights, and a distillation step on what it returned."""
+    import gpusparse
+    V, D, N, Q = 2000, 64, 300, 20
+    h, w, b, _ = head_inputs(N, 24, V, D, dt, seed=61, bias_mean=-3.0)
+    hq = head_inputs(Q, 8, V, D, dt, seed=62)[0]
+    mask = (torch.arange(24, device=DEV)[None, :] < torch.randint(1, 25, (N, 1), generator=torch.Generator().manual_seed(5)).to(DEV))
+    yd = gpusparse.sparse_head(h, w, bias=b, mask=mask)
+    ip, ix, dtv = gpusparse.encode_documents(h, w, bias=b, mask=mask)
+    dense = torch.zeros_like(yd)
+    rows = torch.repeat_interleave(torch.arange(N, device=DEV), ip[1:] - ip[:-1])
+    dense[rows, ix.long()] = dtv
+    assert torch.equal(dense, yd)
+    index = gpusparse.build_index_from_hidden([(h[:128], mask[:128]), (h[128:], mask[128:])], w, bias=b)
+    assert index.num_docs == N and index.vocab_size == V
+    qi, qs = gpusparse.encode_queries(hq, w, bias=b, max_terms=512)
+    yq = gpusparse.sparse_head(hq, w, bias=b)
+    assert int((yq > 0).sum(1).max()) <= 512
+    back = torch.zeros(Q, V + 1, device=DEV).scatter_(1, qi.long() % (V + 1), qs)[:, :V]
+    assert torch.equal(back, yq)
+    scores, ids = gpusparse.triton_fused_score(index, qi, qs, top_k=50)
+    full = yq.double() @ yd.double().t()
+    want = full.topk(50, dim=1).values
+    assert torch.allclose(scores.double(), want, rtol=1e-5, atol=1e-6)
+    assert torch.allclose(full.gather(1, ids), want, rtol=1e-5, atol=1e-6)
+    # a student that scores the documents by dense vectors learns the ranking
+    sq, sd = make(Q, N, D, dt, seed=63, bias=False)[:2]
+    check_distill(sq, sd, None, scores, ids, 2.0, grad=1.0 if dt == BF else 256.0)
