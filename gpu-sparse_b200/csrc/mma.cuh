@@ -2,28 +2,35 @@
 //
 //   acc[m, n] = sum over k of A[m, k] * B[n, k]      (16-bit operands, fp32 accumulators)
 //
-// One persistent CTA per SM walks a list of output tiles; what happens to a finished tile
-// is the job's epilogue, which reads the accumulators from tensor memory and reduces or
+// A pair of CTAs (one cluster, two SMs) works on one output tile of 256 x 256 at a time: each
+// CTA holds half of A's rows and half of B's and computes its 128 rows of the tile against all
+// of B (tcgen05 cta_group::2), so every operand byte that reaches an SM feeds twice the products
+// it would feed alone.  Pairs are persistent and walk a list of tiles; what happens to a finished
+// tile is the job's epilogue, which reads the accumulators from tensor memory and reduces or
 // stores them, so no product has to be written out to be used.  Warp roles:
-//   warp 0     TMA producer: one lane streams the operands of every 64-deep step through a
-//              ring of shared-memory stages
-//   warp 1     MMA issuer: one lane issues four 16-deep tcgen05.mma per stage
-//   warp 2     owns the tensor memory (two accumulators of 128 x 256, so that the products
-//              of a tile run while the epilogue drains the one before)
-//   warps 4-7  epilogue: thread i owns accumulator row i (tensor-memory lane i)
+//   warp 0      TMA producer: one lane streams this CTA's operand halves of every 64-deep step
+//               through a ring of shared-memory stages; the copies of both CTAs signal the
+//               first CTA's barrier
+//   warp 1      MMA issuer (first CTA of the pair only): one lane issues four 16-deep
+//               tcgen05.mma per stage for both CTAs
+//   warp 2      owns the tensor memory (two accumulators of 128 x 256 per CTA, so that the
+//               products of a tile run while the epilogue drains the one before)
+//   warps 4-11  epilogue: thread i of each group of four warps owns accumulator row i (tensor-
+//               memory lane i), the first group the lower half of the columns, the second the
+//               upper; two warps per scheduler hide each other's latencies
 // An operand is either K-major (rows of A or B contiguous along k) or MN-major (contiguous
 // along m or n); both are read in place with 128-byte swizzled boxes, so no transposed copy
 // is ever made.
 //
-// Every wait is bounded.  A role whose wait runs out raises the CTA's fault flag and winds
+// Every wait is bounded.  A role whose wait runs out raises its CTA's fault flag and winds
 // down after its copies and products in flight have landed; the epilogue then sees NaN
 // accumulators for that and all later tiles of the CTA, so the results show it.
 //
 // A job type provides
-//   Walk walk() const            per-thread view of this CTA's tile list
-//   Walk::get(i, Tile&)          the i-th tile of this CTA, false past the end
-//   Epi  epi(...)                per-thread epilogue state, called once per tile with the
-//                                accumulators (Acc)
+//   kStages, kScratch            depth of the operand ring, bytes of epilogue scratch
+//   Walk walk(pair, pairs)       per-thread view of a pair's tile list
+//   Walk::next(Tile&)            the next tile, false past the end
+//   Epi epi()                    per-thread epilogue state; tile() is called once per tile
 #pragma once
 #include "common.cuh"
 
@@ -32,22 +39,22 @@
 namespace gsp {
 namespace mm {
 
-constexpr int kBM = 128;                 // rows of A per tile
+constexpr int kRows = 128;               // rows of A per CTA
+constexpr int kBM = 2 * kRows;           // rows of A per tile
 constexpr int kBN = 256;                 // most rows of B per tile
 constexpr int kBK = 64;                  // depth of one stage: 128 bytes of a 16-bit operand
-constexpr int kStages = 4;
-constexpr int kThreads = 256;
 constexpr int kEpiWarp0 = 4;             // first epilogue warp (a multiple of 4: warp % 4 is
                                          // the tensor-memory quarter it may read)
-constexpr int kABytes = kBM * kBK * 2;
-constexpr int kBBytes = kBN * kBK * 2;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
+constexpr int kABytes = kRows * kBK * 2;
+constexpr int kBBytes = kBN / 2 * kBK * 2;
 constexpr int kStageBytes = kABytes + kBBytes;
-constexpr int kScratch = 4 * 32 * 33 * 4 + 2 * 4 * kBN * 4;   // epilogue scratch
-constexpr int kOffScratch = kStages * kStageBytes;
-constexpr int kOffBar = kOffScratch + kScratch;
-constexpr int kSmem = kOffBar + 256 + 1024;   // + alignment slack
-static_assert(kSmem <= 232448, "stages exceed shared memory");
 constexpr int kTmemCols = 2 * kBN;
+template <class Job>
+constexpr int smem_bytes() {
+  return Job::kStages * kStageBytes + Job::kScratch + 256 + 1024;   // + barriers, alignment slack
+}
 
 // One output tile.  a/b select the operand maps; a0/b0 are the tile's first row (m or n) of
 // each operand, ak/bk the first k of it.
@@ -57,7 +64,7 @@ struct Tile {
   int32_t ak, bk;
   int32_t nk;            // 64-deep steps; 0: the product is zero
   bool a_mn, b_mn;       // operand is MN-major
-  int32_t bn;            // rows of B of this tile (the map's box for a K-major B)
+  int32_t bn;            // rows of B of this tile (a K-major B's map has boxes of half of it)
   int32_t x, y, flags;   // the job's own coordinates
 };
 
@@ -96,21 +103,46 @@ __device__ __forceinline__ void bar_land(uint64_t* b, uint32_t parity) {
     __nanosleep(32);
   }
 }
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint64_t* bar) {
+// the address of the first CTA's copy of a shared-memory object of this CTA
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(su32(p)));
+  return r;
+}
+__device__ __forceinline__ uint32_t cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// this CTA's copy of a box, counted at the barrier `bar` (a cluster address, in either CTA)
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          su32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(su32(bar))
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+      "[%4];" ::"r"(su32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
+// arrives once the products issued so far are done, at this CTA's barrier or at both CTAs'
+__device__ __forceinline__ void commit_own(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(su32(bar)) : "memory");
+}
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                   su32(bar)),
+               "h"(uint16_t(3))
+               : "memory");
 }
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a),
+      "{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a),
       "l"(b), "r"(idesc), "r"(acc));
 }
 // thread i of the warp gets columns c .. c+31 of tensor-memory lane (quarter base + i)
@@ -146,13 +178,17 @@ __device__ __forceinline__ uint32_t inst_desc(bool bf16, bool a_mn, bool b_mn, i
          (uint32_t(bn >> 3) << 17) | (uint32_t(kBM >> 4) << 24);
 }
 
-// Accumulators of a finished tile as an epilogue warp sees them.
+// A finished tile's accumulators as an epilogue warp sees them: row `row` of the tile's A, and
+// of the columns [c_lo, c_hi).
 struct Acc {
   uint32_t taddr;        // this warp's quarter of the tile's tensor-memory columns
+  uint32_t free_bar;     // counts the warps that are done with the accumulators
   bool zero, bad;        // nk == 0; a wait ran out
-  float* stage;          // 32 x 33 floats of this warp
-  float* cols;           // [4 warps][kBN] floats of this tile (alternating buffers)
-  int warp, lane;        // epilogue warp 0..3
+  unsigned char* scratch;
+  int warp, lane;        // epilogue warp 0..7
+  int half, lane_row;    // column half; row of this CTA's 128
+  int buf;               // alternates from tile to tile
+  int32_t rank, row, c_lo, c_hi;
   __device__ __forceinline__ void ld32(int32_t c, float (&v)[32]) const {
     if (bad || zero) {
       const float f = bad ? __uint_as_float(0x7FC00000u) : 0.0f;
@@ -163,24 +199,37 @@ struct Acc {
       tmem_ld32(taddr + uint32_t(c), v);
     }
   }
-  // the four epilogue warps
-  __device__ __forceinline__ void sync() const { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+  // every epilogue warp, once per tile, after its last ld32: the accumulators may be overwritten
+  __device__ __forceinline__ void release() const {
+    fence_before();
+    __syncwarp();
+    if (lane == 0) arrive_remote(free_bar);
+  }
+  // this CTA's epilogue warps
+  __device__ __forceinline__ void sync() const {
+    __syncwarp();
+    asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");
+  }
 };
 
 template <class Job>
-__global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Job job) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Job job) {
+  constexpr int kStages = Job::kStages;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* smem =
       reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOffBar);   // [kStages]
-  uint64_t* empty = full + kStages;                               // [kStages]
-  uint64_t* acc_full = empty + kStages;                           // [2]
-  uint64_t* acc_empty = acc_full + 2;                             // [2]
+  unsigned char* scratch = smem + kStages * kStageBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(scratch + Job::kScratch);   // [kStages], used in the first CTA
+  uint64_t* empty = full + kStages;                                        // [kStages]
+  uint64_t* acc_full = empty + kStages;                                    // [2]
+  uint64_t* acc_empty = acc_full + 2;                                      // [2], used in the first CTA
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int32_t* fault = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
   const int wid = threadIdx.x >> 5, lane = lane_id();
   const int32_t limit = job.wait_limit;
+  const int32_t rank = int32_t(cta_rank());
+  const int32_t pair = int32_t(blockIdx.x) >> 1, pairs = int32_t(gridDim.x) >> 1;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
@@ -189,64 +238,74 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
     }
     for (int i = 0; i < 2; ++i) {
       bar_init(acc_full + i, 1);
-      bar_init(acc_empty + i, 4);
+      bar_init(acc_empty + i, 2 * kEpiWarps);
     }
     bar_init(drain, 1);
     *fault = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (wid == 2) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)),
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(su32(tmem_slot)),
                  "r"(kTmemCols));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
   }
   fence_before();
   __syncthreads();
+  cluster_sync();
   fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   if (wid == 0) {
     if (lane == 0) {
-      auto walk = job.walk();
+      auto walk = job.walk(pair, pairs);
       Tile t;
       uint32_t it = 0;
       bool ok = true;
-      for (int32_t i = 0; ok && walk.get(i, t); ++i) {
+      while (ok && walk.next(t)) {
         const CUtensorMap* ma = &job.maps[t.a];
         const CUtensorMap* mb = &job.maps[t.b];
-        const uint32_t bytes = uint32_t(kABytes + t.bn * kBK * 2);
+        const int32_t nb = t.bn / 2, a0 = t.a0 + rank * kRows, b0 = t.b0 + rank * nb;
+        const uint32_t bytes = 2 * uint32_t(kABytes + nb * kBK * 2);
         for (int32_t k = 0; k < t.nk; ++k, ++it) {
           const uint32_t s = it % kStages, n = it / kStages;
           if (n > 0) ok = bar_wait(empty + s, (n - 1) & 1, limit, fault);
           if (!ok) break;
           unsigned char* as = smem + s * kStageBytes;
           unsigned char* bs = as + kABytes;
-          bar_expect(full + s, bytes);
+          const uint32_t bar = in_first_cta(full + s);
+          if (rank == 0) bar_expect(full + s, bytes);
           if (!t.a_mn) {
-            tma_2d(as, ma, t.ak + k * kBK, t.a0, full + s);
+            tma_2d(as, ma, t.ak + k * kBK, a0, bar);
           } else {
-            for (int32_t j = 0; j < kBM / 64; ++j) tma_2d(as + j * 8192, ma, t.a0 + j * 64, t.ak + k * kBK, full + s);
+            for (int32_t j = 0; j < kRows / 64; ++j) tma_2d(as + j * 8192, ma, a0 + j * 64, t.ak + k * kBK, bar);
           }
           if (!t.b_mn) {
-            tma_2d(bs, mb, t.bk + k * kBK, t.b0, full + s);
+            tma_2d(bs, mb, t.bk + k * kBK, b0, bar);
           } else {
-            for (int32_t j = 0; j < t.bn / 64; ++j) tma_2d(bs + j * 8192, mb, t.b0 + j * 64, t.bk + k * kBK, full + s);
+            for (int32_t j = 0; j < nb / 64; ++j) tma_2d(bs + j * 8192, mb, b0 + j * 64, t.bk + k * kBK, bar);
           }
         }
       }
       if (!ok) *fault = 1;
-      for (uint32_t i = 0; i < kStages && i < it; ++i) {
-        const uint32_t j = it - 1 - i;
-        bar_land(full + j % kStages, (j / kStages) & 1);
+      if (rank == 0) {
+        for (uint32_t i = 0; i < uint32_t(kStages) && i < it; ++i) {
+          const uint32_t j = it - 1 - i;
+          bar_land(full + j % kStages, (j / kStages) & 1);
+        }
+      } else if (!ok) {
+        // the second CTA's copies count at a barrier it cannot wait on: without a fault the
+        // products that read them have finished; with one, a millisecond is far more than any
+        // copy takes
+        for (int i = 0; i < 1024; ++i) __nanosleep(1000);
       }
     }
   } else if (wid == 1) {
-    if (lane == 0) {
-      auto walk = job.walk();
+    if (lane == 0 && rank == 0) {
+      auto walk = job.walk(pair, pairs);
       Tile t;
       uint32_t it = 0;
       bool ok = true;
-      for (int32_t i = 0; ok && walk.get(i, t); ++i) {
+      for (int32_t i = 0; ok && walk.next(t); ++i) {
         const int32_t buf = i & 1, use = i >> 1;
         if (use > 0) ok = bar_wait(acc_empty + buf, (use - 1) & 1, limit, fault);
         if (!ok) break;
@@ -263,26 +322,28 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
           const uint64_t da = desc(as, t.a_mn), db = desc(as + kABytes, t.b_mn);
 #pragma unroll
           for (int q = 0; q < kBK / 16; ++q) mma_f16(d, da + q * step_a, db + q * step_b, id, (k > 0 || q > 0) ? 1u : 0u);
-          commit(empty + s);
+          commit_both(empty + s);
         }
         if (!ok) break;
-        commit(acc_full + buf);
+        commit_both(acc_full + buf);
       }
       if (!ok) *fault = 1;
-      commit(drain);          // every product issued has finished before the memory is given back
+      commit_own(drain);          // every product issued has finished before the memory is given back
       bar_land(drain, 0);
     }
   } else if (wid >= kEpiWarp0) {
-    auto walk = job.walk();
+    auto walk = job.walk(pair, pairs);
     auto epi = job.epi();
     Tile t;
     Acc acc;
     acc.warp = wid - kEpiWarp0;
     acc.lane = lane;
-    acc.stage = reinterpret_cast<float*>(smem + kOffScratch) + acc.warp * 32 * 33;
-    float* cols = reinterpret_cast<float*>(smem + kOffScratch + 4 * 32 * 33 * 4);
+    acc.half = acc.warp >> 2;
+    acc.lane_row = (acc.warp & 3) * 32 + lane;
+    acc.rank = rank;
+    acc.scratch = scratch;
     bool ok = true;
-    for (int32_t i = 0; walk.get(i, t); ++i) {
+    for (int32_t i = 0; walk.next(t); ++i) {
       const int32_t buf = i & 1, use = i >> 1;
       if (ok) {
         ok = bar_wait(acc_full + buf, use & 1, limit, fault);
@@ -290,22 +351,36 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant_
         ok = __all_sync(FULL, ok);
       }
       fence_after();
-      acc.taddr = tmem + (uint32_t(32 * acc.warp) << 16) + uint32_t(buf * kBN);
+      acc.taddr = tmem + (uint32_t(32 * (acc.warp & 3)) << 16) + uint32_t(buf * kBN);
+      acc.free_bar = in_first_cta(acc_empty + buf);
       acc.zero = t.nk == 0;
       acc.bad = !ok;
-      acc.cols = cols + buf * 4 * kBN;
+      acc.buf = buf;
+      acc.row = t.a0 + rank * kRows + acc.lane_row;
+      acc.c_lo = acc.half * (t.bn / 2);
+      acc.c_hi = acc.c_lo + t.bn / 2;
       epi.tile(job, t, acc);
-      fence_before();
-      __syncwarp();
-      if (lane == 0) bar_arrive(acc_empty + buf);
     }
   }
+  __syncwarp();
   fence_before();
   __syncthreads();
+  cluster_sync();         // neither CTA's memory goes away while the other may still use it
   if (wid == 2) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
   }
+}
+
+// Launches a job on every pair of SMs.
+inline int pair_ctas() { return num_sms() & ~1; }
+template <class Job>
+int launch(const Job& job, cudaStream_t st) {
+  const int rc = ensure_smem(reinterpret_cast<const void*>(&mma_kernel<Job>), smem_bytes<Job>());
+  if (rc) return rc;
+  mma_kernel<Job><<<pair_ctas(), kThreads, smem_bytes<Job>(), st>>>(job);
+  GSP_CHECK_LAUNCH();
+  return GSP_OK;
 }
 
 }  // namespace mm

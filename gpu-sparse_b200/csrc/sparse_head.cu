@@ -5,9 +5,10 @@
 // packed tokens in its columns, so that the maximum over a text's tokens runs along one
 // thread's registers: one compare per logit, no exchange between threads, and log1p only on
 // the maximum (it is monotone).  Tiles are ordered tokens-fastest and cut into equal shares,
-// one per CTA; the running maximum is carried from tile to tile, and a text that a share's
-// border cuts leaves its partial maxima for a joining kernel.  Texts may so have any length,
-// and no work is lost to their padding.
+// one per pair of CTAs.  The texts open at the end of a column half are carried to the thread
+// that has the same vocabulary row in the next half (shared memory, a named barrier in each
+// direction), and a text that a share's border cuts leaves its partial maxima for a joining
+// kernel.  Texts may so have any length, and no work is lost to their padding.
 //
 // Backward.  Each (text, term) with y > 0 sends ds = dy exp(-y) to its winning token; as a
 // matrix P [tokens, V] with one entry per (text, term) this is the shape of the losses'
@@ -18,10 +19,16 @@ namespace gsp {
 namespace vocab {
 namespace {
 
-constexpr int kFirst = 1, kLast = 2;
+constexpr int kFirst = 1, kLast = 2;      // of a share along one row of tiles
+constexpr int kBegin = 4, kEnd = 8;       // of a share
 
 template <bool kWin>
 struct HeadJob {
+  // scratch: per warp 16 finished maxima and tokens per lane; per column half the carry
+  static constexpr int kSlots = 16;
+  static constexpr int kSlotBytes = kSlots * 32 * 4 * 2;
+  static constexpr int kCarryOff = mm::kEpiWarps * kSlotBytes;
+  static constexpr int kStages = 5, kScratch = kCarryOff + 2 * (mm::kRows * 8 + 16);
   CUtensorMap maps[2];      // W, H (K-major)
   int32_t wait_limit, bf16;
   const int32_t* head;
@@ -30,17 +37,15 @@ struct HeadJob {
   const float* bias;
   float* y;
   int32_t* win;
-  float* part_m;            // [ctas][2][128]
+  float* part_m;            // [pairs][2: begun elsewhere, open at the end][kBM]
   int32_t* part_i;
 
   struct Walk {
-    int64_t lo, hi;
-    int32_t ntt, nk, bn;
-    __device__ bool get(int32_t i, mm::Tile& t) const {
-      const int64_t x = lo + i;
+    int32_t lo, x, hi, ntt, nk, bn;
+    __device__ bool next(mm::Tile& t) {
       if (x >= hi) return false;
-      t.x = int32_t(x / ntt);
-      t.y = int32_t(x - int64_t(t.x) * ntt);
+      t.x = x / ntt;
+      t.y = x - t.x * ntt;
       t.a = 0, t.b = 1;
       t.a0 = t.x * mm::kBM;
       t.b0 = t.y * bn;
@@ -48,84 +53,141 @@ struct HeadJob {
       t.nk = nk;
       t.a_mn = t.b_mn = false;
       t.bn = bn;
-      t.flags = (i == 0 || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == ntt - 1 ? kLast : 0);
+      t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == ntt - 1 ? kLast : 0) | (x == lo ? kBegin : 0) |
+                (x == hi - 1 ? kEnd : 0);
+      ++x;
       return true;
     }
   };
-  __device__ Walk walk() const {
-    const int32_t ntt = (head[0] + bn - 1) / bn;
-    const int64_t tot = int64_t(ntt) * nvt;
-    return Walk{share_lo(tot, gridDim.x, blockIdx.x), share_lo(tot, gridDim.x, blockIdx.x + 1), ntt, nk, bn};
+  __device__ Walk walk(int32_t pair, int32_t pairs) const {
+    const int32_t ntt = (head[0] + bn - 1) / bn, tot = ntt * nvt, lo = share_lo(tot, pairs, pair);
+    return Walk{lo, lo, share_lo(tot, pairs, pair + 1), ntt, nk, bn};
   }
 
   struct Epi {
-    float m;
-    int32_t idx;
-    bool cut;            // the open text began before this share
-    __device__ void flush(const HeadJob& j, int32_t text, int32_t v, float bias, int slot_row) {
-      if (cut) {
-        const int64_t o = int64_t(blockIdx.x) * 2 * mm::kBM + slot_row;
-        j.part_m[o] = m;
-        if (kWin) j.part_i[o] = idx;
-      } else if (v < j.V) {
-        const float x = m + bias;
-        const int64_t o = int64_t(text) * j.V + v;
-        j.y[o] = x > 0.0f ? log1pf(x) : (x != x ? x : 0.0f);
-        if (kWin) j.win[o] = x > 0.0f ? idx : -1;
-      }
-      cut = false;
-      m = neg_inf();
-      idx = -1;
+    __device__ static void put(const HeadJob& j, int32_t row, int32_t v, float bias, float m, int32_t idx) {
+      if (v >= j.V) return;
+      const float x = m + bias;
+      const int64_t o = int64_t(j.map[row] / j.L) * j.V + v;
+      j.y[o] = x > 0.0f ? log1pf(x) : (x != x ? x : 0.0f);
+      if (kWin) j.win[o] = x > 0.0f ? idx : -1;
+    }
+    __device__ static void part(const HeadJob& j, const mm::Acc& a, int which, float m, int32_t idx) {
+      const int64_t o = (int64_t(blockIdx.x >> 1) * 2 + which) * mm::kBM + a.rank * mm::kRows + a.lane_row;
+      j.part_m[o] = m;
+      if (kWin) j.part_i[o] = idx;
     }
     __device__ void tile(const HeadJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const int32_t n = j.head[0];
-      if (t.flags & kFirst) {
-        m = neg_inf();
-        idx = -1;
-        cut = t.b0 > 0 && j.map[t.b0 - 1] / j.L == j.map[t.b0] / j.L;
-      }
-      const int slot_row = a.warp * 32 + a.lane;
-      const int32_t v = t.a0 + slot_row;
+      const int32_t n = j.head[0], v = a.row;
       const float bias = j.bias && v < j.V ? __ldg(j.bias + v) : 0.0f;
-      bool open = false;
-      for (int32_t c0 = 0; c0 < t.bn; c0 += 32) {
-        const int32_t r0 = t.b0 + c0;
-        if (r0 >= n) break;
+      const int32_t r_lo = t.b0 + a.c_lo, r_hi = min(t.b0 + a.c_hi, n);
+      float* slot_m = reinterpret_cast<float*>(a.scratch + a.warp * kSlotBytes) + a.lane;
+      int32_t* slot_i = reinterpret_cast<int32_t*>(slot_m + kSlots * 32);
+      // which of this half's columns end a text (all loads at once: one latency per tile)
+      uint32_t ends[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const int32_t r = r_lo + 32 * w + a.lane;
+        bool e = false;
+        if (r < r_hi) e = r + 1 == n || j.map[r] / j.L != j.map[r + 1] / j.L;
+        ends[w] = __ballot_sync(FULL, e);
+      }
+      float m = neg_inf(), head_m = neg_inf();
+      int32_t idx = -1, head_i = -1, head_row = -1;     // head: the first text that ends here
+#pragma unroll 1
+      for (int w = 0; w < 4; ++w) {
+        const int32_t r0 = r_lo + 32 * w;
+        if (r0 >= r_hi) break;
         float z[32];
-        a.ld32(c0, z);
-        // text of every column, and which columns end one
-        const int32_t r = r0 + a.lane;
-        const int32_t text = r < n ? j.map[r] / j.L : -1;
-        const int32_t after = r + 1 < n ? j.map[r + 1] / j.L : -1;
-        const uint32_t ends = __ballot_sync(FULL, r < n && text != after);
-        int32_t won = -1;
-        if (ends == 0) {
-          // whole block inside a text
+        a.ld32(a.c_lo + 32 * w, z);
+        if (r0 + 32 >= r_hi) a.release();
+        const uint32_t word = w < 2 ? (w == 0 ? ends[0] : ends[1]) : (w == 2 ? ends[2] : ends[3]);
+        // 16 columns at a time; columns past the last row are past the last text's end
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            if (kWin) won = z[k] > m ? k : won;
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(z[k]));
-          }
-          if (kWin && won >= 0) idx = r0 + won;
-          open = true;
-        } else {
-          const int32_t live = min(32, n - r0);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t bits = (word >> (16 * h)) & 0xFFFFu;
+          const int32_t rb = r0 + 16 * h;
+          int32_t won = -1;
+          if (bits == 0) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            if (k < live) {
-              if (kWin) idx = z[k] > m ? r0 + k : idx;
-              asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(z[k]));
-              if ((ends >> k) & 1) flush(j, __shfl_sync(FULL, text, k), v, bias, slot_row);
+            for (int k = 0; k < 16; ++k) {
+              if (kWin) won = z[16 * h + k] > m ? k : won;
+              asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(z[16 * h + k]));
+            }
+            if (kWin && won >= 0) idx = rb + won;
+          } else {
+            int32_t e = 0;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              if (kWin) idx = z[16 * h + k] > m ? rb + k : idx;
+              asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(z[16 * h + k]));
+              if ((bits >> k) & 1) {
+                slot_m[e * 32] = m;
+                if (kWin) slot_i[e * 32] = idx;
+                ++e;
+                m = neg_inf();
+                idx = -1;
+              }
+            }
+            for (int32_t q = 0; q < e; ++q) {
+              const int32_t row = rb + __ffs(bits) - 1;
+              bits &= bits - 1;
+              const float x = slot_m[q * 32];
+              const int32_t xi = kWin ? slot_i[q * 32] : 0;
+              if (head_row < 0) {
+                head_row = row;
+                head_m = x;
+                head_i = xi;
+              } else {
+                put(j, row, v, bias, x, xi);
+              }
             }
           }
-          open = !((ends >> (live - 1)) & 1);
         }
       }
-      if ((t.flags & kLast) && open) {
-        const int64_t o = (int64_t(blockIdx.x) * 2 + 1) * mm::kBM + slot_row;
-        j.part_m[o] = m;
-        if (kWin) j.part_i[o] = idx;
+      if (r_lo >= r_hi) a.release();
+      // the text open at this half's start: what the halves before it in the share found
+      unsigned char* carry = a.scratch + kCarryOff;
+      constexpr int kCarryBytes = mm::kRows * 8 + 16;
+      float* in_m = reinterpret_cast<float*>(carry + (1 - a.half) * kCarryBytes) + a.lane_row;
+      float* out_m = reinterpret_cast<float*>(carry + a.half * kCarryBytes) + a.lane_row;
+      int32_t* in_cut = reinterpret_cast<int32_t*>(carry + (1 - a.half) * kCarryBytes + mm::kRows * 8);
+      int32_t* out_cut = reinterpret_cast<int32_t*>(carry + a.half * kCarryBytes + mm::kRows * 8);
+      float cm = neg_inf();
+      int32_t ci = -1;
+      bool cut;
+      // the two halves' threads take turns over all of the share, so neither overtakes the other
+      __syncwarp();
+      if (a.half == 1 || !(t.flags & kBegin)) asm volatile("bar.sync %0, 256;" ::"r"(3 - a.half) : "memory");
+      if ((t.flags & kFirst) && a.half == 0) {
+        cut = t.b0 > 0 && j.map[t.b0 - 1] / j.L == j.map[t.b0] / j.L;    // began in an earlier share
+      } else {
+        cm = in_m[0];
+        if (kWin) ci = reinterpret_cast<int32_t*>(in_m)[mm::kRows];
+        cut = *in_cut != 0;
       }
+      float open_m = m;
+      int32_t open_i = idx;
+      if (head_row >= 0) {
+        const int32_t hi = kWin && head_m > cm ? head_i : ci;
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(head_m) : "f"(cm));
+        if (cut) part(j, a, 0, head_m, hi);
+        else put(j, head_row, v, bias, head_m, hi);
+        cut = false;
+      } else {
+        if (kWin) open_i = m > cm ? idx : ci;
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(open_m) : "f"(cm));
+      }
+      if ((t.flags & kLast) && a.half == 1) {
+        const int32_t end = min(t.b0 + t.bn, n);
+        if (end < n && j.map[end] / j.L == j.map[end - 1] / j.L) part(j, a, 1, open_m, open_i);
+      } else {
+        out_m[0] = open_m;
+        if (kWin) reinterpret_cast<int32_t*>(out_m)[mm::kRows] = open_i;
+        if (a.lane_row == 0) *out_cut = cut;
+      }
+      __syncwarp();
+      if (a.half == 0 || !(t.flags & kEnd)) asm volatile("bar.arrive %0, 256;" ::"r"(2 + a.half) : "memory");
     }
   };
   __device__ Epi epi() const { return Epi{}; }
@@ -134,8 +196,8 @@ struct HeadJob {
 struct JoinParams {
   const int32_t *head, *map;
   const uint8_t* mask;
-  int32_t L, bn, ctas;
-  int64_t B, V, nvt;
+  int32_t L, bn, pairs, nvt;
+  int64_t B, V;
   const float* bias;
   const float* part_m;
   const int32_t* part_i;
@@ -143,16 +205,14 @@ struct JoinParams {
   int32_t* win;
 };
 
-// Blocks [0, ctas): a text that began in an earlier share and ends in this one is joined from
+// Blocks [0, pairs): a text that began in an earlier share and ends in this one is joined from
 // the shares it crosses, in order.  Blocks past them: texts without tokens get zero rows.
 __global__ void __launch_bounds__(mm::kBM) head_join_kernel(const JoinParams p) {
   const int32_t n = p.head[0];
-  if (int32_t(blockIdx.x) >= p.ctas) {
-    const int64_t b = int64_t(blockIdx.x) - p.ctas;
-    bool any = p.mask == nullptr && p.L > 0;
-    if (p.mask) {
-      for (int64_t t = threadIdx.x; t < p.L; t += mm::kBM) any |= p.mask[b * p.L + t] != 0;
-    }
+  if (int32_t(blockIdx.x) >= p.pairs) {
+    const int64_t b = int64_t(blockIdx.x) - p.pairs;
+    bool any = false;
+    for (int64_t t = threadIdx.x; t < p.L; t += mm::kBM) any |= p.mask[b * p.L + t] != 0;
     if (__syncthreads_or(any)) return;
     for (int64_t v = threadIdx.x; v < p.V; v += mm::kBM) {
       p.y[b * p.V + v] = 0.0f;
@@ -160,35 +220,30 @@ __global__ void __launch_bounds__(mm::kBM) head_join_kernel(const JoinParams p) 
     }
     return;
   }
-  const int32_t ntt = (n + p.bn - 1) / p.bn;
-  const int64_t tot = int64_t(ntt) * p.nvt, c = blockIdx.x;
-  const int64_t lo = share_lo(tot, p.ctas, c), hi = share_lo(tot, p.ctas, c + 1);
+  const int32_t ntt = (n + p.bn - 1) / p.bn, tot = ntt * p.nvt, c = blockIdx.x;
+  const int32_t lo = share_lo(tot, p.pairs, c), hi = share_lo(tot, p.pairs, c + 1);
   if (lo >= hi) return;
-  const int64_t vt = lo / ntt, t0 = lo - vt * ntt;
-  if (t0 == 0) return;
-  const int64_t r0 = t0 * p.bn;
+  const int32_t vt = lo / ntt, r0 = (lo - vt * ntt) * p.bn;
+  if (r0 == 0) return;
   const int32_t text = p.map[r0] / p.L;
   if (p.map[r0 - 1] / p.L != text) return;
   // does it end inside this share?
-  const int64_t row_end = min64(n, (min64(hi, (vt + 1) * ntt) - vt * ntt) * p.bn);
+  const int64_t row_end = min64(n, int64_t(min(hi, (vt + 1) * ntt) - vt * ntt) * p.bn);
   if (row_end < n && p.map[row_end] / p.L == text) return;
-  int64_t first = c - 1;
+  int32_t first = c - 1;
   for (;; --first) {
-    const int64_t l0 = share_lo(tot, p.ctas, first);
-    if (l0 == share_lo(tot, p.ctas, first + 1)) continue;      // an empty share
-    const int64_t at = (l0 - vt * ntt) * p.bn;                 // its first row for this tile row
+    const int64_t at = int64_t(share_lo(tot, p.pairs, first) - vt * ntt) * p.bn;   // its first row along this tile row
     if (at <= 0 || p.map[at - 1] / p.L != text) break;
   }
   float m = neg_inf();
   int32_t idx = -1;
-  for (int64_t s = first; s <= c; ++s) {
-    if (share_lo(tot, p.ctas, s) == share_lo(tot, p.ctas, s + 1)) continue;
-    const int64_t o = (s * 2 + (s == c ? 0 : 1)) * mm::kBM + threadIdx.x;
+  for (int32_t s = first; s <= c; ++s) {
+    const int64_t o = (int64_t(s) * 2 + (s == c ? 0 : 1)) * mm::kBM + threadIdx.x;
     const float x = p.part_m[o];
     if (p.win && x > m) idx = p.part_i[o];
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x));
   }
-  const int64_t v = vt * mm::kBM + threadIdx.x;
+  const int64_t v = int64_t(vt) * mm::kBM + threadIdx.x;
   if (v >= p.V) return;
   const float x = m + (p.bias ? p.bias[v] : 0.0f);
   p.y[text * p.V + v] = x > 0.0f ? log1pf(x) : (x != x ? x : 0.0f);
@@ -334,15 +389,16 @@ Fwd carve_fwd(void* base, const gsp_vocab_view* vw) {
   Fwd f{};
   Carver c{static_cast<char*>(base)};
   f.counts = c.take<int32_t>(pack_counts(vw->T));
-  f.part_m = c.take<float>(int64_t(num_sms()) * 2 * mm::kBM);
-  f.part_i = c.take<int32_t>(int64_t(num_sms()) * 2 * mm::kBM);
+  f.part_m = c.take<float>(int64_t(mm::pair_ctas()) * mm::kBM);
+  f.part_i = c.take<int32_t>(int64_t(mm::pair_ctas()) * mm::kBM);
   f.wcopy = c.take<char>(weight_copy_bytes(vw));
   f.bytes = c.off;
   return f;
 }
 struct Bwd {
   uint32_t* absmax;
-  float *scale, *dh_acc;
+  float* scale;
+  GradScratch grad;
   uint16_t* P;
   void* wcopy;
   int64_t pitch, bytes;
@@ -354,23 +410,11 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
   b.pitch = piece_cols(Tp, vw->V);
   b.absmax = c.take<uint32_t>(1);
   b.scale = c.take<float>(1);
-  b.dh_acc = c.take<float>(b.pitch < vw->V ? Tp * up(vw->D, 32) : 0);
+  b.grad = carve_grad(c, vw, Tp, b.pitch);
   b.P = c.take<uint16_t>(Tp * b.pitch);
   b.wcopy = c.take<char>(weight_copy_bytes(vw));
   b.bytes = c.off;
   return b;
-}
-
-template <bool kWin>
-int launch_head(const gsp_vocab_view* vw, HeadJob<kWin>& j, const State& s, const uint16_t* w, int64_t ldw, cudaStream_t st) {
-  const bool bf = is_bf16(vw);
-  int rc;
-  if ((rc = make_map(&j.maps[0], bf, w, vw->D, vw->V, ldw, mm::kBM))) return rc;
-  if ((rc = make_map(&j.maps[1], bf, s.h, s.Dp, s.Tp, s.Dp, j.bn))) return rc;
-  if ((rc = ensure_smem(reinterpret_cast<const void*>(&mm::mma_kernel<HeadJob<kWin>>), mm::kSmem))) return rc;
-  mm::mma_kernel<HeadJob<kWin>><<<num_sms(), mm::kThreads, mm::kSmem, st>>>(j);
-  GSP_CHECK_LAUNCH();
-  return GSP_OK;
 }
 
 template <bool kWin>
@@ -391,7 +435,11 @@ int run_head(const gsp_vocab_view* vw, const State& s, const Fwd& f, int32_t L, 
   j.win = win;
   j.part_m = f.part_m;
   j.part_i = f.part_i;
-  return launch_head<kWin>(vw, j, s, w, ldw, st);
+  const bool bf = is_bf16(vw);
+  int rc;
+  if ((rc = make_map(&j.maps[0], bf, w, vw->D, vw->V, ldw, mm::kRows))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, s.h, s.Dp, s.Tp, s.Dp, bn / 2))) return rc;
+  return mm::launch(j, st);
 }
 
 int check_texts(const gsp_vocab_view* vw, int64_t L, const char* what) {
@@ -443,7 +491,7 @@ extern "C" int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_
   if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
   // columns of a tile: no more than the tokens need (a single query's product is then as short
   // as reading W allows)
-  const int32_t bn = int32_t(vw->T >= mm::kBN ? mm::kBN : up(vw->T, 32));
+  const int32_t bn = int32_t(vw->T >= mm::kBN ? mm::kBN : up(vw->T, 64));
   rc = win ? run_head<true>(vw, s, f, int32_t(L), bn, y, win, w, ldw, st)
            : run_head<false>(vw, s, f, int32_t(L), bn, y, win, w, ldw, st);
   if (rc) return rc;
@@ -453,16 +501,16 @@ extern "C" int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_
   p.mask = mask;
   p.L = int32_t(L);
   p.bn = bn;
-  p.ctas = num_sms();
+  p.pairs = mm::pair_ctas() / 2;
   p.B = vw->T / L;
   p.V = vw->V;
-  p.nvt = (vw->V + mm::kBM - 1) / mm::kBM;
+  p.nvt = int32_t((vw->V + mm::kBM - 1) / mm::kBM);
   p.bias = vw->bias;
   p.part_m = f.part_m;
   p.part_i = f.part_i;
   p.y = y;
   p.win = win;
-  head_join_kernel<<<unsigned(p.ctas + (mask ? p.B : 0)), mm::kBM, 0, st>>>(p);
+  head_join_kernel<<<unsigned(p.pairs + (mask ? p.B : 0)), mm::kBM, 0, st>>>(p);
   GSP_CHECK_LAUNCH();
   return GSP_OK;
 }
@@ -523,7 +571,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
     spread_kernel<<<dim3(unsigned((b.pitch / 8 + 255) / 256), unsigned(B + 1), unsigned(zs)), 256, 0, st>>>(p);
     GSP_CHECK_LAUNCH();
     const GradPiece pc{b.P, b.pitch, v0, p.cols, v0 == 0, v0 + p.cols >= vw->V};
-    if ((rc = grad_products(vw, s, w, ldw, pc, b.dh_acc, b.scale, d_hidden, d_weight, st))) return rc;
+    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
 }

@@ -116,7 +116,35 @@ __global__ void __launch_bounds__(256) copy_weight_kernel(const uint16_t* w, int
 }
 
 // ---- backward products -------------------------------------------------------------------
+// Both products' tiles form one list, first dH's (256 rows x 256 of D, k along the piece's
+// vocabulary), then dW's (256 vocabulary rows x 256 of D, k along the rows).  Tile counts and
+// depths differ by orders of magnitude with the sizes (32 rows: 3 dH tiles of 477 steps, 360 dW
+// tiles of one), so the list is cut by steps and not by tiles: every pair of CTAs gets the same
+// number of steps, and a tile cut by a border is finished from its fp32 fragments by
+// frag_kernel, in list order.  Pairs are dealt to the 256-wide tiles of D in turn, so that the
+// pairs that read the same rows of P run side by side.
+constexpr int kTileCost = 3;      // steps an epilogue counts for in the cut
+
+struct GradList {
+  int32_t nh, nw, nkh, nkw;       // tiles of each kind along this D tile, steps of each
+  __device__ int64_t total() const { return int64_t(nh) * (nkh + kTileCost) + int64_t(nw) * (nkw + kTileCost); }
+  // tile of position x, its first position, its steps
+  __device__ void at(int64_t x, bool* is_h, int32_t* blk, int64_t* start, int32_t* nk) const {
+    const int64_t lh = nkh + kTileCost, lw = nkw + kTileCost, h_end = nh * lh;
+    if (x < h_end) {
+      *is_h = true, *nk = nkh;
+      *blk = int32_t(x / lh);
+      *start = *blk * lh;
+    } else {
+      *is_h = false, *nk = nkw;
+      *blk = int32_t((x - h_end) / lw);
+      *start = h_end + *blk * lw;
+    }
+  }
+};
+
 struct GradJob {
+  static constexpr int kStages = 6, kScratch = 0;
   CUtensorMap maps[4];       // P K-major, P MN-major, W MN-major, H MN-major
   int32_t wait_limit, bf16;
   const int32_t* n_rows;
@@ -127,91 +155,183 @@ struct GradJob {
   bool want_h, want_w, vec_h, vec_w;
   float* dh_acc;
   int32_t ld_acc;
+  float* frag;               // [pairs][2: begun elsewhere, ends elsewhere][2 CTAs][128][256]
   const float* scale;        // null: 1
   uint16_t *dh, *dw;
 
+  __device__ GradList list() const {
+    const int32_t n = *n_rows;
+    return GradList{want_h ? (n + mm::kBM - 1) / mm::kBM : 0, want_w ? (cols + mm::kBM - 1) / mm::kBM : 0, (cols + 63) / 64,
+                    (n + 63) / 64};
+  }
+  __device__ float* fragment(int32_t pair, bool ends_elsewhere, int32_t rank) const {
+    return frag + ((int64_t(pair) * 2 + ends_elsewhere) * 2 + rank) * mm::kRows * mm::kBN;
+  }
+
+  static constexpr int kIsH = 1, kFrag = 2, kEndsElsewhere = 4;
   struct Walk {
-    int32_t nh, nw, rows, cols, v0, nbs, D;
-    bool h_first;
-    __device__ bool get(int32_t i, mm::Tile& t) const {
-      int64_t x = int64_t(i) * gridDim.x + blockIdx.x;
-      if (x >= nh + nw) return false;
-      // tiles with the longer sums first, so that the last ones to start are short
-      bool is_h = h_first ? x < nh : x >= nw;
-      if (h_first ? !is_h : is_h) x -= h_first ? nh : nw;
-      const int32_t blk = int32_t(x / nbs), nb = int32_t(x - int64_t(blk) * nbs);
-      t.b0 = nb * mm::kBN;
-      t.bn = min(mm::kBN, (D - t.b0 + 63) / 64 * 64);
-      t.a0 = blk * mm::kBM;
-      t.ak = 0;
-      t.b_mn = true;
-      if (is_h) {
-        t.a = 0, t.b = 2, t.a_mn = false, t.bk = v0, t.nk = (cols + 63) / 64;
-      } else {
-        t.a = 1, t.b = 3, t.a_mn = true, t.bk = 0, t.nk = (rows + 63) / 64;
+    GradList l;
+    int64_t x, x1;
+    int32_t nb, nb_step, nbs, D, v0;
+    __device__ bool next(mm::Tile& t) {
+      for (;;) {
+        if (x >= x1) {             // with more D tiles than pairs a pair takes several, whole
+          nb += nb_step;
+          if (nb >= nbs) return false;
+          x = 0;
+          continue;
+        }
+        bool is_h;
+        int32_t blk, nk;
+        int64_t start;
+        l.at(x, &is_h, &blk, &start, &nk);
+        const int64_t end = start + nk + kTileCost, y = x1 < end ? x1 : end;
+        const int32_t k0 = int32_t(min64(x - start, nk)), k1 = int32_t(min64(y - start, nk));
+        const bool whole_zero = nk == 0 && x == start;
+        x = y;
+        if (k0 >= k1 && !whole_zero) continue;      // only the tail of a tile's cost
+        t.b0 = nb * mm::kBN;
+        t.bn = D - t.b0 > 128 ? 256 : 128;
+        t.a0 = blk * mm::kBM;
+        t.ak = k0 * mm::kBK;
+        t.b_mn = true;
+        t.a = is_h ? 0 : 1;
+        t.b = is_h ? 2 : 3;
+        t.a_mn = !is_h;
+        t.bk = (is_h ? v0 : 0) + k0 * mm::kBK;
+        t.nk = k1 - k0;
+        t.x = blk;
+        t.y = nb;
+        t.flags = (is_h ? kIsH : 0) | (k0 > 0 || k1 < nk ? kFrag : 0) | (k1 < nk && k0 == 0 ? kEndsElsewhere : 0);
+        return true;
       }
-      t.x = blk;
-      t.y = nb;
-      t.flags = is_h;
-      return true;
     }
   };
-  __device__ Walk walk() const {
-    const int32_t n = *n_rows;
-    const int32_t nh = want_h ? (n + mm::kBM - 1) / mm::kBM * nbs : 0;
-    const int32_t nw = want_w ? (cols + mm::kBM - 1) / mm::kBM * nbs : 0;
-    return Walk{nh, nw, n, cols, v0, nbs, D, cols >= n};
+  __device__ Walk walk(int32_t pair, int32_t pairs) const {
+    const GradList l = list();
+    const int64_t tot = l.total();
+    if (nbs > pairs) return Walk{l, tot > 0 ? 0 : 1, tot, pair, tot > 0 ? pairs : nbs, nbs, D, v0};
+    const int32_t groups = pairs / nbs, g = pair / nbs;      // pairs past groups * nbs stay idle
+    if (g >= groups) return Walk{l, 0, 0, 0, nbs, nbs, D, v0};
+    return Walk{l, g * tot / groups, (g + 1) * tot / groups, pair % nbs, nbs, nbs, D, v0};
+  }
+
+  // 8 columns from c of a finished row: r a packed row (dH) or a vocabulary row of the piece (dW)
+  __device__ void finish8(bool is_h, int32_t r, int32_t c, float (&v)[8]) const {
+    if (c >= D) return;
+    uint16_t* out;
+    bool vec;
+    const float sc = scale ? *scale : 1.0f;
+    if (is_h) {
+      if (r >= *n_rows) return;
+      float* acc = dh_acc + int64_t(r) * ld_acc + c;
+      if (!first) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += acc[k];
+      }
+      if (!last) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = v[k];
+        return;
+      }
+      out = dh + int64_t(map[r]) * D + c;
+      vec = vec_h;
+    } else {
+      if (r >= cols) return;
+      out = dw + int64_t(v0 + r) * D + c;
+      vec = vec_w;
+    }
+    const bool bf = bf16 != 0;
+    uint4 o;
+    uint32_t* u = &o.x;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) u[k] = pack2(v[2 * k] * sc, v[2 * k + 1] * sc, bf);
+    if (vec) {
+      *reinterpret_cast<uint4*>(out) = o;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (c + k < D) out[k] = uint16_t(u[k >> 1] >> (16 * (k & 1)));
+      }
+    }
   }
 
   struct Epi {
     __device__ void tile(const GradJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const int32_t r = t.a0 + a.warp * 32 + a.lane;
+      const int32_t r = a.row;
       const float sc = j.scale ? *j.scale : 1.0f;
-      const bool bf = j.bf16 != 0;
-      if (t.flags) {
-        const bool live = r < *j.n_rows;
-        uint16_t* row = live && j.last ? j.dh + int64_t(j.map[r]) * j.D : nullptr;
-        float* acc = j.dh_acc + int64_t(r) * j.ld_acc;
-        for (int32_t c = 0; c < t.bn; c += 32) {
-          float v[32];
-          a.ld32(c, v);
-          if (!live || t.b0 + c >= j.ld_acc) continue;
-          uint32_t* u = reinterpret_cast<uint32_t*>(v);
-          if (!j.first) {
+      const bool bf = j.bf16 != 0, is_h = t.flags & kIsH;
+      const bool live = is_h ? r < *j.n_rows : r < j.cols;
+      float* acc = j.dh_acc + int64_t(r) * j.ld_acc;
+      uint16_t* row = nullptr;
+      if (live) row = is_h ? j.dh + int64_t(j.map[r]) * j.D : j.dw + int64_t(j.v0 + r) * j.D;
+      float* frag = j.fragment(int32_t(blockIdx.x) >> 1, (t.flags & kEndsElsewhere) != 0, a.rank) + a.lane_row * mm::kBN;
+      for (int32_t c = a.c_lo; c < a.c_hi; c += 32) {
+        float v[32];
+        a.ld32(c, v);
+        uint32_t* u = reinterpret_cast<uint32_t*>(v);
+        const int32_t d0 = t.b0 + c;
+        if (!live || d0 >= j.D) continue;
+        if (t.flags & kFrag) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t o[8];
-              ld256(acc + t.b0 + c + 8 * q, o);
+          for (int q = 0; q < 4; ++q) st256(frag + c + 8 * q, u + 8 * q);
+          continue;
+        }
+        if (is_h && !j.first) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k) v[8 * q + k] += __uint_as_float(o[k]);
-            }
-          }
-          if (j.last) {
+          for (int q = 0; q < 4; ++q) {
+            uint32_t o[8];
+            ld256(acc + d0 + 8 * q, o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) v[k] *= sc;
-            store_row16(row, t.b0 + c, j.D, v, bf, j.vec_h);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) st256(acc + t.b0 + c + 8 * q, u + 8 * q);
+            for (int k = 0; k < 8; ++k) v[8 * q + k] += __uint_as_float(o[k]);
           }
         }
-      } else {
-        const int32_t v_row = j.v0 + r;
-        const bool live = r < j.cols && v_row < j.V;
-        uint16_t* row = j.dw + int64_t(v_row) * j.D;
-        for (int32_t c = 0; c < t.bn; c += 32) {
-          float v[32];
-          a.ld32(c, v);
-          if (!live) continue;
+        if (is_h && !j.last) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) v[k] *= sc;
-          store_row16(row, t.b0 + c, j.D, v, bf, j.vec_w);
+          for (int q = 0; q < 4; ++q) st256(acc + d0 + 8 * q, u + 8 * q);
+          continue;
         }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] *= sc;
+        store_row16(row, d0, j.D, v, bf, is_h ? j.vec_h : j.vec_w);
       }
+      a.release();
     }
   };
   __device__ Epi epi() const { return Epi{}; }
 };
+
+// Finishes the tiles that a border between two shares cuts: the pair whose share holds a tile's
+// last step adds the fragments in list order.  Block (pair, CTA of the pair, 8 rows): a warp per
+// row, 8 columns per lane.
+__global__ void __launch_bounds__(256) frag_kernel(const __grid_constant__ GradJob j, int32_t pairs) {
+  const GradList l = j.list();
+  const int64_t tot = l.total();
+  const int32_t groups = pairs / j.nbs, pair = blockIdx.x;
+  const int32_t g = pair / j.nbs, nb = pair % j.nbs;
+  if (g >= groups) return;
+  const int64_t x0 = g * tot / groups, x1 = (g + 1) * tot / groups;
+  if (x0 >= x1) return;
+  bool is_h;
+  int32_t blk, nk;
+  int64_t start;
+  l.at(x0, &is_h, &blk, &start, &nk);
+  if (x0 == start || x0 - start >= nk || x1 - start < nk) return;    // begins here, or ends elsewhere
+  int32_t first = g - 1;
+  while (first * tot / groups > start) --first;
+  const int32_t rank = blockIdx.y, row = blockIdx.z * 8 + (threadIdx.x >> 5), c = lane_id() * 8;
+  const int32_t r = blk * mm::kBM + rank * mm::kRows + row;
+  if (r >= (is_h ? *j.n_rows : j.cols) || nb * mm::kBN + c >= j.D) return;
+  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+  for (int32_t s = first; s <= g; ++s) {
+    if (s * tot / groups == (s + 1) * tot / groups) continue;        // an empty share
+    uint32_t o[8];
+    ld256(j.fragment(s * j.nbs + nb, s == first, rank) + row * mm::kBN + c, o);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += __uint_as_float(o[k]);
+  }
+  j.finish8(is_h, r, nb * mm::kBN + c, v);
+}
 
 }  // namespace
 
@@ -247,6 +367,8 @@ int check_view(const gsp_vocab_view* vw, const char* what) {
   GSP_REQUIRE(vw->V >= 1 && vw->V <= (int64_t(1) << 30), GSP_ERR_ARG, "%s: %lld vocabulary rows out of range", what,
               (long long)vw->V);
   GSP_REQUIRE(vw->D >= 1 && vw->D <= (int64_t(1) << 20), GSP_ERR_ARG, "%s: width %lld out of range", what, (long long)vw->D);
+  GSP_REQUIRE(up256(vw->T) / 256 * (up256(vw->V) / 256) < (int64_t(1) << 31), GSP_ERR_ARG,
+              "%s: %lld tokens x %lld vocabulary rows are too many for one call", what, (long long)vw->T, (long long)vw->V);
   GSP_REQUIRE(vw->ld_hidden >= vw->D && vw->ld_weight >= vw->D, GSP_ERR_ARG, "%s: row stride smaller than the width", what);
   return GSP_OK;
 }
@@ -329,13 +451,20 @@ int64_t piece_cols(int64_t Tp, int64_t V) {
   return up((all + pieces - 1) / pieces, kRowPad);
 }
 
+GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t pitch) {
+  GradScratch g{};
+  g.dh_acc = c.take<float>(pitch < vw->V ? Tp * up(vw->D, 32) : 0);
+  g.frag = c.take<float>(int64_t(mm::pair_ctas()) * 2 * mm::kRows * mm::kBN);
+  return g;
+}
+
 int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, int64_t ldw, const GradPiece& pc,
-                  float* dh_acc, const float* scale, void* d_hidden, void* d_weight, cudaStream_t st) {
+                  const GradScratch& g, const float* scale, void* d_hidden, void* d_weight, cudaStream_t st) {
   if (!d_hidden && !d_weight) return GSP_OK;
   GradJob j{};
   const bool bf = is_bf16(vw);
   int rc;
-  if ((rc = make_map(&j.maps[0], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kBM))) return rc;
+  if ((rc = make_map(&j.maps[0], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kRows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kBK))) return rc;
   if ((rc = make_map(&j.maps[2], bf, w, vw->D, vw->V, ldw, mm::kBK))) return rc;
   if ((rc = make_map(&j.maps[3], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kBK))) return rc;
@@ -354,13 +483,16 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.want_w = d_weight != nullptr;
   j.vec_h = vw->D % 16 == 0 && (reinterpret_cast<uintptr_t>(d_hidden) & 31) == 0;
   j.vec_w = vw->D % 16 == 0 && (reinterpret_cast<uintptr_t>(d_weight) & 31) == 0;
-  j.dh_acc = dh_acc;
+  j.dh_acc = g.dh_acc;
   j.ld_acc = int32_t(up(vw->D, 32));
+  j.frag = g.frag;
   j.scale = scale;
   j.dh = static_cast<uint16_t*>(d_hidden);
   j.dw = static_cast<uint16_t*>(d_weight);
-  if ((rc = ensure_smem(reinterpret_cast<const void*>(&mm::mma_kernel<GradJob>), mm::kSmem))) return rc;
-  mm::mma_kernel<GradJob><<<num_sms(), mm::kThreads, mm::kSmem, st>>>(j);
+  if ((rc = mm::launch(j, st))) return rc;
+  const int32_t pairs = mm::pair_ctas() / 2;
+  if (j.nbs > pairs) return GSP_OK;      // no tile is cut
+  frag_kernel<<<dim3(unsigned(pairs), 2, mm::kRows / 8), 256, 0, st>>>(j, pairs);
   GSP_CHECK_LAUNCH();
   return GSP_OK;
 }

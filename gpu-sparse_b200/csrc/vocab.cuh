@@ -63,14 +63,19 @@ inline int64_t pack_counts(int64_t T) { return (T + 255) / 256 + 1; }
 // Backward products over a piece of the vocabulary [v0, v0 + cols): P [Tp, pitch] is the
 // gradient of the piece's logits,
 //   dH (+)= P W[v0 : v0 + cols],   dW[v0 : v0 + cols] = P^T H,
-// in one launch.  dh_acc [Tp, up(D, 32)] carries dH in fp32 between pieces.
+// in one launch.  Between pieces dH is carried in fp32.
 struct GradPiece {
   const uint16_t* P;
   int64_t pitch, v0, cols;
   bool first, last;
 };
+struct GradScratch {
+  float* dh_acc;      // [Tp, up(D, 32)], or null when there is one piece
+  float* frag;        // partial tiles
+};
+GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t pitch);
 int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, int64_t ldw, const GradPiece& pc,
-                  float* dh_acc, const float* scale, void* d_hidden, void* d_weight, cudaStream_t st);
+                  const GradScratch& g, const float* scale, void* d_hidden, void* d_weight, cudaStream_t st);
 // columns of one piece: P takes at most kPieceBytes
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
 int64_t piece_cols(int64_t Tp, int64_t V);
@@ -111,8 +116,8 @@ __device__ __forceinline__ void ld256(const void* p, uint32_t* r) {
                : "l"(p)
                : "memory");
 }
-// 32 accumulators of one row -> 16-bit, columns c0 .. min(c0 + 32, D); vec: row starts on a
-// 32-byte boundary and D is a multiple of 16
+// 32 accumulators of one row -> 16-bit, columns c0 .. min(c0 + 32, D); vec: rows start on
+// 32-byte boundaries and D is a multiple of 16
 __device__ __forceinline__ void store_row16(uint16_t* row, int32_t c0, int32_t D, const float (&v)[32], bool bf16, bool vec) {
   uint32_t w[16];
 #pragma unroll
@@ -142,9 +147,14 @@ __device__ __forceinline__ float warp_col_sums(float (&v)[32], int lane) {
   return v[0];
 }
 
-// CTA c's share [lo, hi) of `tot` tiles in a row, and the CTA that owns tile x
-__host__ __device__ __forceinline__ int64_t share_lo(int64_t tot, int64_t ctas, int64_t c) { return c * tot / ctas; }
-__host__ __device__ __forceinline__ int64_t share_of(int64_t tot, int64_t ctas, int64_t x) { return ((x + 1) * ctas - 1) / tot; }
+// A list of `tot` tiles in equal consecutive shares: share c is [share_lo(c), share_lo(c + 1)),
+// tile x lies in share share_of(x).  No share is empty unless all later ones are.
+__host__ __device__ __forceinline__ int32_t share_lo(int32_t tot, int32_t shares, int32_t c) {
+  return tot <= shares ? (c < tot ? c : tot) : int32_t(uint64_t(c) * uint32_t(tot) / uint32_t(shares));
+}
+__host__ __device__ __forceinline__ int32_t share_of(int32_t tot, int32_t shares, int32_t x) {
+  return tot <= shares ? x : int32_t(((uint64_t(x) + 1) * uint32_t(shares) - 1) / uint32_t(tot));
+}
 
 }  // namespace vocab
 }  // namespace gsp

@@ -6,11 +6,11 @@
 //   lse2 = log2 sum_v 2^z[v],   loss = tau^2 (sum_j q_j log q_j + ln 2 (lse2 - sum_j q_j z_j))
 //   dloss/ds[v] = tau (2^(z[v] - lse2) - q[v])
 //
-// Forward.  The tiles (128 rows x 256 vocabulary rows) of all rows are one long list, row
-// block by row block, cut into equal shares, one per CTA, so every SM has the same work
-// whatever the sizes.  The epilogue thread that owns a row carries its running maximum, sum
-// and target dot product in registers along the share and writes them once per row block; a
-// second kernel joins the partial results (in share order) and sums the losses.
+// Forward.  The tiles (256 rows x 256 vocabulary rows) of all rows are one long list, row
+// block by row block, cut into equal shares, one per pair of CTAs, so every SM has the same work
+// whatever the sizes.  The two epilogue threads that own a row (a column half each) carry its
+// running maximum, sum and target dot product in registers along the share and write them once
+// per row block; a second kernel joins the partial results (in share order) and sums the losses.
 //
 // Backward.  Per piece of the vocabulary: the logits' tiles again, whose epilogue turns them
 // into P = gradient of the logits, rounded once to 16 bits, then the two products of
@@ -158,6 +158,9 @@ struct Cursor {
     left -= lo;
     if (left > 0) next = *ids;
   }
+  __device__ void skip_to(int32_t v0) {      // entries of the other column half
+    while (next < v0) step();
+  }
   __device__ void step() {
     ++ids;
     ++p;
@@ -180,12 +183,15 @@ __device__ __forceinline__ void to_z(float (&v)[32], float c, const float* bias2
 }
 
 // ---- forward -----------------------------------------------------------------------------
-struct Part {
-  float m, l, dot;     // maximum, sum of 2^(z - m), sum q z (each per row and share)
-};
+// Partial results of a (share, row block): [2 column halves][maximum, sum of 2^(z - m),
+// sum q z][kBM rows], at index share + row block (which no two of them have in common, since
+// along the list one of the two always grows).
+constexpr int kPart = 2 * 3 * mm::kBM;
+constexpr int kListScratch = mm::kEpiWarps * 32 * 33 * 4;      // a padded 32 x 32 block per warp
 
 template <bool kList>
 struct LossJob {
+  static constexpr int kStages = kList ? 5 : 6, kScratch = kList ? kListScratch : 0;
   CUtensorMap maps[2];      // H, W (K-major)
   int32_t wait_limit, bf16;
   const int32_t* head;
@@ -194,16 +200,14 @@ struct LossJob {
   float c;
   const float* bias2;
   Lists lists;
-  float* part;              // [ctas + row blocks][3][128]
+  float* part;              // [pairs + row blocks][kPart]
 
   struct Walk {
-    int64_t lo, hi;
-    int32_t nt, nk;
-    __device__ bool get(int32_t i, mm::Tile& t) const {
-      const int64_t x = lo + i;
+    int32_t lo, x, hi, nt, nk;
+    __device__ bool next(mm::Tile& t) {
       if (x >= hi) return false;
-      t.x = int32_t(x / nt);
-      t.y = int32_t(x - int64_t(t.x) * nt);
+      t.x = x / nt;
+      t.y = x - t.x * nt;
       t.a = 0, t.b = 1;
       t.a0 = t.x * mm::kBM;
       t.b0 = t.y * mm::kBN;
@@ -211,13 +215,14 @@ struct LossJob {
       t.nk = nk;
       t.a_mn = t.b_mn = false;
       t.bn = mm::kBN;
-      t.flags = (i == 0 || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == nt - 1 ? kLast : 0);
+      t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == nt - 1 ? kLast : 0);
+      ++x;
       return true;
     }
   };
-  __device__ Walk walk() const {
-    const int64_t tot = int64_t((head[0] + mm::kBM - 1) / mm::kBM) * nt;
-    return Walk{share_lo(tot, gridDim.x, blockIdx.x), share_lo(tot, gridDim.x, blockIdx.x + 1), nt, nk};
+  __device__ Walk walk(int32_t pair, int32_t pairs) const {
+    const int32_t tot = (head[0] + mm::kBM - 1) / mm::kBM * nt, lo = share_lo(tot, pairs, pair);
+    return Walk{lo, lo, share_lo(tot, pairs, pair + 1), nt, nk};
   }
 
   struct Epi {
@@ -229,19 +234,21 @@ struct LossJob {
       if (t.flags & kFirst) {
         m = neg_inf();
         l = dot = 0.0f;
-        const int32_t r = t.a0 + a.warp * 32 + a.lane;
+        const int32_t r = a.row;
         const bool live = r < j.head[0];
-        if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, n0);
+        if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, n0 + a.c_lo);
         else tgt = live ? j.lists.tgt[r] : -1;
       }
-      for (int32_t c0 = 0; c0 < mm::kBN; c0 += 32) {
+      if constexpr (kList) cur.skip_to(n0 + a.c_lo);
+      for (int32_t c0 = a.c_lo; c0 < a.c_hi; c0 += 32) {
         float z[32];
         a.ld32(c0, z);
+        if (c0 + 32 == a.c_hi) a.release();
         const int32_t v0 = n0 + c0;
         to_z(z, j.c, j.bias2 + v0);
         if constexpr (kList) {
           if (__any_sync(FULL, cur.next < v0 + 32)) {
-            float* mine = a.stage + a.lane * 33;      // own row: no other lane reads it
+            float* mine = reinterpret_cast<float*>(a.scratch) + (a.warp * 32 + a.lane) * 33;   // no other lane's
 #pragma unroll
             for (int k = 0; k < 32; ++k) mine[k] = z[k];
             while (cur.next < v0 + 32) {
@@ -275,7 +282,7 @@ struct LossJob {
         l += (e[0] + e[1]) + (e[2] + e[3]);
       }
       if (t.flags & kLast) {
-        float* o = j.part + (int64_t(blockIdx.x) + t.x) * (3 * mm::kBM) + a.warp * 32 + a.lane;
+        float* o = j.part + (int64_t(blockIdx.x >> 1) + t.x) * kPart + a.half * 3 * mm::kBM + a.rank * mm::kRows + a.lane_row;
         o[0] = m;
         o[mm::kBM] = l;
         o[2 * mm::kBM] = dot;
@@ -285,60 +292,75 @@ struct LossJob {
   __device__ Epi epi() const { return Epi{}; }
 };
 
-// Joins a row's partial results in share order and sums the losses: the blocks' sums are
-// added by whichever block finishes last, in block order.
-__global__ void __launch_bounds__(mm::kBM)
-join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, int32_t ctas, const float* ent, float tau2,
+// Joins a row's partial results and sums the losses.  A block has 32 rows: each of its 8 warps
+// joins a run of consecutive shares (one row may have as many as there are pairs), the first
+// then joins the warps' results in order.  The blocks' sums are added by whichever block
+// finishes last, in block order.
+constexpr int kJoinRows = 32, kJoinWarps = 8;
+struct RowSum {
+  float m, l, dot;
+  __device__ void add(float pm, float pl, float pd) {
+    const float nm = fmaxf(m, pm), base = nm == neg_inf() ? 0.0f : nm;
+    l = l * ex2(m - base) + pl * ex2(pm - base);
+    m = nm;
+    dot += pd;
+  }
+};
+__global__ void __launch_bounds__(32 * kJoinWarps)
+join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, int32_t pairs, const float* ent, float tau2,
             int32_t reduction, float* lse2, double* sums, float* loss) {
-  __shared__ double red[mm::kBM / 32];
+  __shared__ float got[3][kJoinWarps][kJoinRows];
+  __shared__ double red[kJoinWarps];
   __shared__ bool last;
-  const int32_t n = head[0], mb = blockIdx.x;
-  const int32_t r = mb * mm::kBM + threadIdx.x;
-  const int32_t blocks = (n + mm::kBM - 1) / mm::kBM;
-  const int64_t tot = int64_t(blocks) * nt;
-  double mine = 0.0;
+  const int32_t n = head[0], wid = threadIdx.x >> 5, lane = lane_id();
+  const int32_t r = int32_t(blockIdx.x) * kJoinRows + lane, mb = r / mm::kBM;
+  const int32_t tot = (n + mm::kBM - 1) / mm::kBM * nt;
+  RowSum s{neg_inf(), 0.0f, 0.0f};
   if (r < n) {
-    const int64_t c0 = share_of(tot, ctas, int64_t(mb) * nt), c1 = share_of(tot, ctas, int64_t(mb + 1) * nt - 1);
-    float m = neg_inf(), l = 0.0f, dot = 0.0f;
-    for (int64_t c = c0; c <= c1; ++c) {
-      if (share_lo(tot, ctas, c) == share_lo(tot, ctas, c + 1)) continue;    // an empty share
-      const float* o = part + (c + mb) * (3 * mm::kBM) + threadIdx.x;
-      const float pm = o[0], pl = o[mm::kBM];
-      dot += o[2 * mm::kBM];
-      const float nm = fmaxf(m, pm), base = nm == neg_inf() ? 0.0f : nm;
-      l = l * ex2(m - base) + pl * ex2(pm - base);
-      m = nm;
+    const int32_t c0 = share_of(tot, pairs, mb * nt), c1 = share_of(tot, pairs, (mb + 1) * nt - 1) + 1;
+    const int32_t per = (c1 - c0 + kJoinWarps - 1) / kJoinWarps, lo = c0 + wid * per, hi = min(c1, lo + per);
+#pragma unroll 4
+    for (int32_t c = lo; c < hi; ++c) {
+      const float* o = part + int64_t(c + mb) * kPart + r % mm::kBM;
+      s.add(o[0], o[mm::kBM], o[2 * mm::kBM]);
+      o += 3 * mm::kBM;
+      s.add(o[0], o[mm::kBM], o[2 * mm::kBM]);
     }
-    const float z = m + log2f(l);
-    lse2[r] = z;
-    const int32_t orig = map[r];
-    const float v = tau2 * fmaf(z - dot, kLn2, ent ? ent[orig] : 0.0f);
-    if (reduction == GSP_REDUCE_NONE) loss[orig] = v;
-    mine = double(v);
+  }
+  got[0][wid][lane] = s.m;
+  got[1][wid][lane] = s.l;
+  got[2][wid][lane] = s.dot;
+  __syncthreads();
+  if (wid == 0) {
+    double mine = 0.0;
+    if (r < n) {
+      for (int w = 1; w < kJoinWarps; ++w) s.add(got[0][w][lane], got[1][w][lane], got[2][w][lane]);
+      const float z = s.m + log2f(s.l);
+      lse2[r] = z;
+      const int32_t orig = map[r];
+      const float v = tau2 * fmaf(z - s.dot, kLn2, ent ? ent[orig] : 0.0f);
+      if (reduction == GSP_REDUCE_NONE) loss[orig] = v;
+      mine = double(v);
+    }
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(FULL, mine, o);
+    if (lane == 0) {
+      sums[blockIdx.x] = mine;
+      __threadfence();
+      last = atomicAdd(head + 1, 1) == int32_t(gridDim.x) - 1;
+    }
   }
   if (reduction == GSP_REDUCE_NONE) return;
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(FULL, mine, o);
-  if (lane_id() == 0) red[threadIdx.x >> 5] = mine;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double s = 0.0;
-    for (int i = 0; i < mm::kBM / 32; ++i) s += red[i];
-    sums[mb] = s;
-    __threadfence();
-    last = atomicAdd(head + 1, 1) == int32_t(gridDim.x) - 1;
-  }
   __syncthreads();
   if (!last) return;
   __threadfence();
-  double s = 0.0;
-  for (int32_t i = threadIdx.x; i < blocks; i += mm::kBM) s += *reinterpret_cast<volatile double*>(sums + i);
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
-  __syncthreads();
-  if (lane_id() == 0) red[threadIdx.x >> 5] = s;
+  double v = 0.0;
+  for (int32_t i = threadIdx.x; i < int32_t(gridDim.x); i += 32 * kJoinWarps) v += *reinterpret_cast<volatile double*>(sums + i);
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  if (lane == 0) red[wid] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
-    double v = 0.0;
-    for (int i = 0; i < mm::kBM / 32; ++i) v += red[i];
+    v = 0.0;
+    for (int i = 0; i < kJoinWarps; ++i) v += red[i];
     *loss = float(reduction == GSP_REDUCE_MEAN ? v / (n > 0 ? n : 1) : v);
   }
 }
@@ -383,6 +405,8 @@ grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, 
 
 template <bool kList>
 struct LogitGradJob {
+  static constexpr int kColBytes = 2 * 4 * mm::kBN * 4;      // column sums of 4 x 32 rows, two buffers
+  static constexpr int kStages = kList ? 5 : 6, kScratch = kColBytes + (kList ? kListScratch : 0);
   CUtensorMap maps[2];      // H, W (K-major)
   int32_t wait_limit, bf16;
   const int32_t* head;
@@ -393,16 +417,15 @@ struct LogitGradJob {
   Lists lists;
   uint16_t* P;
   int64_t pitch;
-  float* colpart;           // [row blocks][pitch], or null
+  float* colpart;           // [128-row blocks][pitch], or null
 
   struct Walk {
-    int64_t tot;
-    int32_t nt, nk, v0;
-    __device__ bool get(int32_t i, mm::Tile& t) const {
-      const int64_t x = int64_t(i) * gridDim.x + blockIdx.x;
+    int32_t x, step, tot, nt, nk, v0;
+    __device__ bool next(mm::Tile& t) {
       if (x >= tot) return false;
-      t.x = int32_t(x / nt);
-      t.y = int32_t(x - int64_t(t.x) * nt);
+      t.x = x / nt;
+      t.y = x - t.x * nt;
+      x += step;
       t.a = 0, t.b = 1;
       t.a0 = t.x * mm::kBM;
       t.b0 = v0 + t.y * mm::kBN;
@@ -414,21 +437,25 @@ struct LogitGradJob {
       return true;
     }
   };
-  __device__ Walk walk() const { return Walk{int64_t((head[0] + mm::kBM - 1) / mm::kBM) * nt, nt, nk, v0}; }
+  __device__ Walk walk(int32_t pair, int32_t pairs) const {
+    return Walk{pair, pairs, (head[0] + mm::kBM - 1) / mm::kBM * nt, nt, nk, v0};
+  }
 
   struct Epi {
     __device__ void tile(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const int32_t r = t.a0 + a.warp * 32 + a.lane;
+      const int32_t r = a.row;
       const bool live = r < j.head[0];
       const float lse = j.lse2[r], ga = j.ga[r];
       Cursor cur;
       int32_t tgt = -1;
-      if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, t.b0);
+      if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, t.b0 + a.c_lo);
       else tgt = live ? j.lists.tgt[r] : -1;
       uint16_t* row = j.P + int64_t(r) * j.pitch + t.y * mm::kBN;
-      for (int32_t c0 = 0; c0 < mm::kBN; c0 += 32) {
+      float* cols = reinterpret_cast<float*>(a.scratch) + a.buf * 4 * mm::kBN;
+      for (int32_t c0 = a.c_lo; c0 < a.c_hi; c0 += 32) {
         float z[32];
         a.ld32(c0, z);
+        if (c0 + 32 == a.c_hi) a.release();
         const int32_t v0 = t.b0 + c0;
         to_z(z, j.c, j.bias2 + v0);
 #pragma unroll
@@ -439,7 +466,7 @@ struct LogitGradJob {
         }
         if constexpr (kList) {
           if (__any_sync(FULL, cur.next < v0 + 32)) {
-            float* mine = a.stage + a.lane * 33;
+            float* mine = reinterpret_cast<float*>(a.scratch + kColBytes) + (a.warp * 32 + a.lane) * 33;
 #pragma unroll
             for (int k = 0; k < 32; ++k) mine[k] = z[k];
             while (cur.next < v0 + 32) {
@@ -463,31 +490,38 @@ struct LogitGradJob {
         for (int k = 0; k < 16; ++k) w[k] = pack2(z[2 * k], z[2 * k + 1], j.bf16 != 0);
         st256(row + c0, w);
         st256(row + c0 + 16, w + 8);
-        if (j.colpart) a.cols[a.warp * mm::kBN + c0 + a.lane] = warp_col_sums(z, a.lane);
+        if (j.colpart) cols[(a.warp & 3) * mm::kBN + c0 + a.lane] = warp_col_sums(z, a.lane);
       }
       if (j.colpart) {
         a.sync();
-        const int i = a.warp * 32 + a.lane;
-        float* o = j.colpart + int64_t(t.x) * j.pitch + t.y * mm::kBN;
-#pragma unroll
-        for (int h = 0; h < mm::kBN; h += 128) {
-          const float* q = a.cols + h + i;
-          o[h + i] = (q[0] + q[mm::kBN]) + (q[2 * mm::kBN] + q[3 * mm::kBN]);
-        }
+        const int c = a.warp * 32 + a.lane;
+        const float* q = cols + c;
+        j.colpart[int64_t(t.x * 2 + a.rank) * j.pitch + t.y * mm::kBN + c] =
+            (q[0] + q[mm::kBN]) + (q[2 * mm::kBN] + q[3 * mm::kBN]);
       }
     }
   };
   __device__ Epi epi() const { return Epi{}; }
 };
 
-// d_bias of a piece: the row blocks' column sums, in order
+// d_bias of a piece: the row blocks' column sums.  8 warps share the blocks of 32 columns; their
+// sums are added in order.
 __global__ void __launch_bounds__(256)
 bias_grad_kernel(const int32_t* head, const float* colpart, int64_t pitch, int64_t cols, const float* scale, float* d_bias) {
-  const int64_t c = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (c >= cols) return;
-  const int32_t blocks = (head[0] + mm::kBM - 1) / mm::kBM;
+  __shared__ float got[8][32];
+  const int wid = threadIdx.x >> 5, lane = lane_id();
+  const int64_t c = int64_t(blockIdx.x) * 32 + lane;
+  const int32_t blocks = (head[0] + mm::kRows - 1) / mm::kRows;
   float s = 0.0f;
-  for (int32_t b = 0; b < blocks; ++b) s += colpart[int64_t(b) * pitch + c];
+  if (c < cols) {
+#pragma unroll 4
+    for (int32_t b = wid; b < blocks; b += 8) s += colpart[int64_t(b) * pitch + c];
+  }
+  got[wid][lane] = s;
+  __syncthreads();
+  if (wid > 0 || c >= cols) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) s += got[w][lane];
   d_bias[c] = s * *scale;
 }
 
@@ -502,16 +536,16 @@ struct Fwd {
 Fwd carve_fwd(void* base, const gsp_vocab_view* vw) {
   Fwd f{};
   Carver c{static_cast<char*>(base)};
-  const int64_t blocks = pad_rows(vw->T) / mm::kBM;
   f.counts = c.take<int32_t>(pack_counts(vw->T));
-  f.part = c.take<float>((num_sms() + blocks) * 3 * mm::kBM);
-  f.sums = c.take<double>(blocks);
+  f.part = c.take<float>((mm::pair_ctas() / 2 + pad_rows(vw->T) / mm::kBM) * kPart);
+  f.sums = c.take<double>(pad_rows(vw->T) / kJoinRows);
   f.wcopy = c.take<char>(weight_copy_bytes(vw));
   f.bytes = c.off;
   return f;
 }
 struct Bwd {
-  float *ga, *scale, *colpart, *dh_acc;
+  float *ga, *scale, *colpart;
+  GradScratch grad;
   uint16_t* P;
   void* wcopy;
   int64_t pitch, bytes;
@@ -523,8 +557,8 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
   b.pitch = piece_cols(Tp, vw->V);
   b.ga = c.take<float>(Tp);
   b.scale = c.take<float>(1);
-  b.colpart = c.take<float>(Tp / mm::kBM * b.pitch);
-  b.dh_acc = c.take<float>(b.pitch < vw->V ? Tp * up(vw->D, 32) : 0);
+  b.colpart = c.take<float>(Tp / mm::kRows * b.pitch);
+  b.grad = carve_grad(c, vw, Tp, b.pitch);
   b.P = c.take<uint16_t>(Tp * b.pitch);
   b.wcopy = c.take<char>(weight_copy_bytes(vw));
   b.bytes = c.off;
@@ -546,8 +580,8 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Li
   if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
   LossJob<kList> j{};
   const bool bf = is_bf16(vw);
-  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kBM))) return rc;
-  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN))) return rc;
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kRows))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.head = s.head;
@@ -558,13 +592,10 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Li
   j.bias2 = s.bias2;
   j.lists = lists;
   j.part = f.part;
-  if ((rc = ensure_smem(reinterpret_cast<const void*>(&mm::mma_kernel<LossJob<kList>>), mm::kSmem))) return rc;
-  const int ctas = num_sms();
-  mm::mma_kernel<LossJob<kList>><<<ctas, mm::kThreads, mm::kSmem, st>>>(j);
-  GSP_CHECK_LAUNCH();
+  if ((rc = mm::launch(j, st))) return rc;
   if (reduction == GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, size_t(vw->T) * sizeof(float), st));
-  join_kernel<<<unsigned((vw->T + mm::kBM - 1) / mm::kBM), mm::kBM, 0, st>>>(s.head, s.map, f.part, j.nt, ctas, ent, tau * tau,
-                                                                           reduction, s.lse2, f.sums, loss);
+  join_kernel<<<unsigned((vw->T + kJoinRows - 1) / kJoinRows), 32 * kJoinWarps, 0, st>>>(
+      s.head, s.map, f.part, j.nt, mm::pair_ctas() / 2, ent, tau * tau, reduction, s.lse2, f.sums, loss);
   GSP_CHECK_LAUNCH();
   return GSP_OK;
 }
@@ -578,8 +609,8 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
   if ((rc = weight_rows(vw, b.wcopy, &w, &ldw, st))) return rc;
   LogitGradJob<kList> j{};
   const bool bf = is_bf16(vw);
-  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kBM))) return rc;
-  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN))) return rc;
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kRows))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.head = s.head;
@@ -593,19 +624,17 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
   j.P = b.P;
   j.pitch = b.pitch;
   j.colpart = d_bias ? b.colpart : nullptr;
-  if ((rc = ensure_smem(reinterpret_cast<const void*>(&mm::mma_kernel<LogitGradJob<kList>>), mm::kSmem))) return rc;
   for (int64_t v0 = 0; v0 < vw->V; v0 += b.pitch) {
     const int64_t cols = min64(b.pitch, vw->V - v0);
     j.v0 = int32_t(v0);
     j.nt = int32_t((cols + mm::kBN - 1) / mm::kBN);
-    mm::mma_kernel<LogitGradJob<kList>><<<num_sms(), mm::kThreads, mm::kSmem, st>>>(j);
-    GSP_CHECK_LAUNCH();
+    if ((rc = mm::launch(j, st))) return rc;
     if (d_bias) {
-      bias_grad_kernel<<<unsigned((cols + 255) / 256), 256, 0, st>>>(s.head, b.colpart, b.pitch, cols, b.scale, d_bias + v0);
+      bias_grad_kernel<<<unsigned((cols + 31) / 32), 256, 0, st>>>(s.head, b.colpart, b.pitch, cols, b.scale, d_bias + v0);
       GSP_CHECK_LAUNCH();
     }
     const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V};
-    if ((rc = grad_products(vw, s, w, ldw, pc, b.dh_acc, b.scale, d_hidden, d_weight, st))) return rc;
+    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
 }
