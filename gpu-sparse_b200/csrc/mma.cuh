@@ -30,7 +30,8 @@
 //   kStages, kScratch            depth of the operand ring, bytes of epilogue scratch
 //   Walk walk(pair, pairs)       per-thread view of a pair's tile list
 //   Walk::next(Tile&)            the next tile, false past the end
-//   Epi epi()                    per-thread epilogue state; tile() is called once per tile
+//   Epi epi()                    per-thread epilogue state; per tile, begin() is called while its
+//                                products run (loads that they hide) and tile() when they are done
 #pragma once
 #include "common.cuh"
 
@@ -345,6 +346,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
     bool ok = true;
     for (int32_t i = 0; walk.next(t); ++i) {
       const int32_t buf = i & 1, use = i >> 1;
+      acc.buf = buf;
+      acc.row = t.a0 + rank * kRows + acc.lane_row;
+      acc.c_lo = acc.half * (t.bn / 2);
+      acc.c_hi = acc.c_lo + t.bn / 2;
+      epi.begin(job, t, acc);
       if (ok) {
         ok = bar_wait(acc_full + buf, use & 1, limit, fault);
         if (!ok) *fault = 1;
@@ -355,10 +361,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
       acc.free_bar = in_first_cta(acc_empty + buf);
       acc.zero = t.nk == 0;
       acc.bad = !ok;
-      acc.buf = buf;
-      acc.row = t.a0 + rank * kRows + acc.lane_row;
-      acc.c_lo = acc.half * (t.bn / 2);
-      acc.c_hi = acc.c_lo + t.bn / 2;
       epi.tile(job, t, acc);
     }
   }

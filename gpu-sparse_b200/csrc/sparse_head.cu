@@ -77,14 +77,10 @@ struct HeadJob {
       j.part_m[o] = m;
       if (kWin) j.part_i[o] = idx;
     }
-    __device__ void tile(const HeadJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const int32_t n = j.head[0], v = a.row;
-      const float bias = j.bias && v < j.V ? __ldg(j.bias + v) : 0.0f;
-      const int32_t r_lo = t.b0 + a.c_lo, r_hi = min(t.b0 + a.c_hi, n);
-      float* slot_m = reinterpret_cast<float*>(a.scratch + a.warp * kSlotBytes) + a.lane;
-      int32_t* slot_i = reinterpret_cast<int32_t*>(slot_m + kSlots * 32);
-      // which of this half's columns end a text (all loads at once: one latency per tile)
-      uint32_t ends[4];
+    uint32_t ends[4];      // which of this half's columns end a text
+    bool cut;              // the text open at the half's start began in an earlier share
+    __device__ void begin(const HeadJob& j, const mm::Tile& t, const mm::Acc& a) {
+      const int32_t n = j.head[0], r_lo = t.b0 + a.c_lo, r_hi = min(t.b0 + a.c_hi, n);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int32_t r = r_lo + 32 * w + a.lane;
@@ -92,6 +88,14 @@ struct HeadJob {
         if (r < r_hi) e = r + 1 == n || j.map[r] / j.L != j.map[r + 1] / j.L;
         ends[w] = __ballot_sync(FULL, e);
       }
+      if ((t.flags & kFirst) && a.half == 0) cut = t.b0 > 0 && j.map[t.b0 - 1] / j.L == j.map[t.b0] / j.L;
+    }
+    __device__ void tile(const HeadJob& j, const mm::Tile& t, const mm::Acc& a) {
+      const int32_t n = j.head[0], v = a.row;
+      const float bias = j.bias && v < j.V ? __ldg(j.bias + v) : 0.0f;
+      const int32_t r_lo = t.b0 + a.c_lo, r_hi = min(t.b0 + a.c_hi, n);
+      float* slot_m = reinterpret_cast<float*>(a.scratch + a.warp * kSlotBytes) + a.lane;
+      int32_t* slot_i = reinterpret_cast<int32_t*>(slot_m + kSlots * 32);
       float m = neg_inf(), head_m = neg_inf();
       int32_t idx = -1, head_i = -1, head_row = -1;     // head: the first text that ends here
 #pragma unroll 1
@@ -155,13 +159,10 @@ struct HeadJob {
       int32_t* out_cut = reinterpret_cast<int32_t*>(carry + a.half * kCarryBytes + mm::kRows * 8);
       float cm = neg_inf();
       int32_t ci = -1;
-      bool cut;
       // the two halves' threads take turns over all of the share, so neither overtakes the other
       __syncwarp();
       if (a.half == 1 || !(t.flags & kBegin)) asm volatile("bar.sync %0, 256;" ::"r"(3 - a.half) : "memory");
-      if ((t.flags & kFirst) && a.half == 0) {
-        cut = t.b0 > 0 && j.map[t.b0 - 1] / j.L == j.map[t.b0] / j.L;    // began in an earlier share
-      } else {
+      if (!(t.flags & kFirst) || a.half == 1) {
         cm = in_m[0];
         if (kWin) ci = reinterpret_cast<int32_t*>(in_m)[mm::kRows];
         cut = *in_cut != 0;

@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(256) copy_weight_kernel(const uint16_t* w, int
 // number of steps, and a tile cut by a border is finished from its fp32 fragments by
 // frag_kernel, in list order.  Pairs are dealt to the 256-wide tiles of D in turn, so that the
 // pairs that read the same rows of P run side by side.
+constexpr int kPadBytes = 32 * 33 * 4;      // a warp's 32 x 32 block
 constexpr int kTileCost = 3;      // steps an epilogue counts for in the cut
 
 struct GradList {
@@ -144,7 +145,7 @@ struct GradList {
 };
 
 struct GradJob {
-  static constexpr int kStages = 6, kScratch = 0;
+  static constexpr int kStages = 6, kScratch = mm::kEpiWarps * kPadBytes;
   CUtensorMap maps[4];       // P K-major, P MN-major, W MN-major, H MN-major
   int32_t wait_limit, bf16;
   const int32_t* n_rows;
@@ -164,6 +165,8 @@ struct GradJob {
     return GradList{want_h ? (n + mm::kBM - 1) / mm::kBM : 0, want_w ? (cols + mm::kBM - 1) / mm::kBM : 0, (cols + 63) / 64,
                     (n + 63) / 64};
   }
+  // shares per D tile: pairs past groups * nbs stay idle, and no share is empty
+  __device__ int32_t groups(int32_t pairs, int64_t tot) const { return int32_t(min64(pairs / nbs, tot)); }
   __device__ float* fragment(int32_t pair, bool ends_elsewhere, int32_t rank) const {
     return frag + ((int64_t(pair) * 2 + ends_elsewhere) * 2 + rank) * mm::kRows * mm::kBN;
   }
@@ -211,7 +214,7 @@ struct GradJob {
     const GradList l = list();
     const int64_t tot = l.total();
     if (nbs > pairs) return Walk{l, tot > 0 ? 0 : 1, tot, pair, tot > 0 ? pairs : nbs, nbs, D, v0};
-    const int32_t groups = pairs / nbs, g = pair / nbs;      // pairs past groups * nbs stay idle
+    const int32_t groups = this->groups(pairs, tot), g = pair / nbs;
     if (g >= groups) return Walk{l, 0, 0, 0, nbs, nbs, D, v0};
     return Walk{l, g * tot / groups, (g + 1) * tot / groups, pair % nbs, nbs, nbs, D, v0};
   }
@@ -257,27 +260,34 @@ struct GradJob {
   }
 
   struct Epi {
+    bool is_h, live;
+    uint16_t* row;
+    float sc;
+    __device__ void begin(const GradJob& j, const mm::Tile& t, const mm::Acc& a) {
+      is_h = t.flags & kIsH;
+      live = is_h ? a.row < *j.n_rows : a.row < j.cols;
+      row = nullptr;
+      if (live) row = is_h ? j.dh + int64_t(j.map[a.row]) * j.D : j.dw + int64_t(j.v0 + a.row) * j.D;
+      sc = j.scale ? *j.scale : 1.0f;
+    }
     __device__ void tile(const GradJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const int32_t r = a.row;
-      const float sc = j.scale ? *j.scale : 1.0f;
-      const bool bf = j.bf16 != 0, is_h = t.flags & kIsH;
-      const bool live = is_h ? r < *j.n_rows : r < j.cols;
-      float* acc = j.dh_acc + int64_t(r) * j.ld_acc;
-      uint16_t* row = nullptr;
-      if (live) row = is_h ? j.dh + int64_t(j.map[r]) * j.D : j.dw + int64_t(j.v0 + r) * j.D;
+      const bool bf = j.bf16 != 0, vec = is_h ? j.vec_h : j.vec_w;
+      float* acc = j.dh_acc + int64_t(a.row) * j.ld_acc;
       float* frag = j.fragment(int32_t(blockIdx.x) >> 1, (t.flags & kEndsElsewhere) != 0, a.rank) + a.lane_row * mm::kBN;
       for (int32_t c = a.c_lo; c < a.c_hi; c += 32) {
         float v[32];
         a.ld32(c, v);
+        if (c + 32 == a.c_hi) a.release();
         uint32_t* u = reinterpret_cast<uint32_t*>(v);
         const int32_t d0 = t.b0 + c;
-        if (!live || d0 >= j.D) continue;
+        if (d0 >= j.D) continue;
         if (t.flags & kFrag) {
+          if (!live) continue;
 #pragma unroll
           for (int q = 0; q < 4; ++q) st256(frag + c + 8 * q, u + 8 * q);
           continue;
         }
-        if (is_h && !j.first) {
+        if (is_h && !j.first && live) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             uint32_t o[8];
@@ -287,15 +297,32 @@ struct GradJob {
           }
         }
         if (is_h && !j.last) {
+          if (!live) continue;
 #pragma unroll
           for (int q = 0; q < 4; ++q) st256(acc + d0 + 8 * q, u + 8 * q);
           continue;
         }
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] *= sc;
-        store_row16(row, d0, j.D, v, bf, is_h ? j.vec_h : j.vec_w);
+        if (vec) {
+          if (live) store_row16(row, d0, j.D, v, bf);
+        } else {
+          // rows that start anywhere: the warp's block is turned in shared memory, so that a
+          // store has the 32 columns of one row and not one column of 32 rows
+          float* block = reinterpret_cast<float*>(a.scratch + a.warp * kPadBytes);
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 32; ++k) block[a.lane * 33 + k] = v[k];
+          __syncwarp();
+          const uint64_t mine = reinterpret_cast<uint64_t>(row);
+#pragma unroll 4
+          for (int q = 0; q < 32; ++q) {
+            uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(FULL, mine, q));
+            const float x = block[q * 33 + a.lane];
+            if (to && d0 + a.lane < j.D) to[d0 + a.lane] = uint16_t(pack2(x, 0.0f, bf));
+          }
+        }
       }
-      a.release();
     }
   };
   __device__ Epi epi() const { return Epi{}; }
@@ -307,24 +334,22 @@ struct GradJob {
 __global__ void __launch_bounds__(256) frag_kernel(const __grid_constant__ GradJob j, int32_t pairs) {
   const GradList l = j.list();
   const int64_t tot = l.total();
-  const int32_t groups = pairs / j.nbs, pair = blockIdx.x;
+  const int32_t groups = j.groups(pairs, tot), pair = blockIdx.x;
   const int32_t g = pair / j.nbs, nb = pair % j.nbs;
   if (g >= groups) return;
   const int64_t x0 = g * tot / groups, x1 = (g + 1) * tot / groups;
-  if (x0 >= x1) return;
   bool is_h;
   int32_t blk, nk;
   int64_t start;
   l.at(x0, &is_h, &blk, &start, &nk);
   if (x0 == start || x0 - start >= nk || x1 - start < nk) return;    // begins here, or ends elsewhere
-  int32_t first = g - 1;
-  while (first * tot / groups > start) --first;
+  const int32_t first = int32_t(((start + 1) * groups - 1) / tot);   // the share that holds the tile's first step
   const int32_t rank = blockIdx.y, row = blockIdx.z * 8 + (threadIdx.x >> 5), c = lane_id() * 8;
   const int32_t r = blk * mm::kBM + rank * mm::kRows + row;
   if (r >= (is_h ? *j.n_rows : j.cols) || nb * mm::kBN + c >= j.D) return;
   float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
   for (int32_t s = first; s <= g; ++s) {
-    if (s * tot / groups == (s + 1) * tot / groups) continue;        // an empty share
     uint32_t o[8];
     ld256(j.fragment(s * j.nbs + nb, s == first, rank) + row * mm::kBN + c, o);
 #pragma unroll
@@ -352,8 +377,9 @@ State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool l
   if (K > 0) {
     s.cnt = c.take<int32_t>(T);
     s.ent = c.take<float>(T);
-    s.ids = c.take<int32_t>(T * K);
-    s.p = c.take<float>(T * K);
+    s.Kp = up(K, 4);
+    s.ids = c.take<int32_t>(T * s.Kp + 4);      // a row is read four entries at a time, and one
+    s.p = c.take<float>(T * s.Kp + 4);          // four ahead
     s.flag = c.take<uint8_t>(T);
   }
   s.bytes = c.off;

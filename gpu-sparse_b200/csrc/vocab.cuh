@@ -36,11 +36,12 @@ struct State {
   int32_t* tgt;       // [Tp] target of every packed row (cross entropy)
   int32_t* cnt;       // [T] teacher entries of every row (distillation)
   float* ent;         // [T] sum p log p (distillation)
-  int32_t* ids;       // [T, K] ascending, distinct (distillation)
-  float* p;           // [T, K] (distillation)
+  int32_t* ids;       // [T, Kp] ascending, distinct, kNoId past a row's cnt (distillation)
+  float* p;           // [T, Kp] (distillation)
   uint8_t* flag;      // [T] row takes part (distillation)
-  int64_t Tp, Dp, Vp, bytes;
+  int64_t Tp, Dp, Vp, Kp, bytes;
 };
+constexpr int32_t kNoId = 0x7FFFFFFF;
 State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool loss);
 
 int check_view(const gsp_vocab_view* vw, const char* what);
@@ -116,35 +117,76 @@ __device__ __forceinline__ void ld256(const void* p, uint32_t* r) {
                : "l"(p)
                : "memory");
 }
-// 32 accumulators of one row -> 16-bit, columns c0 .. min(c0 + 32, D); vec: rows start on
-// 32-byte boundaries and D is a multiple of 16
-__device__ __forceinline__ void store_row16(uint16_t* row, int32_t c0, int32_t D, const float (&v)[32], bool bf16, bool vec) {
+// 32 accumulators of one row -> 16-bit, columns c0 .. min(c0 + 32, D); the row starts on a
+// 32-byte boundary and D is a multiple of 16
+__device__ __forceinline__ void store_row16(uint16_t* row, int32_t c0, int32_t D, const float (&v)[32], bool bf16) {
   uint32_t w[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
-  if (vec) {
-    if (c0 < D) st256(row + c0, w);
-    if (c0 + 16 < D) st256(row + c0 + 16, w + 8);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      if (c0 + j < D) row[c0 + j] = uint16_t(w[j >> 1] >> (16 * (j & 1)));
-    }
-  }
+  st256(row + c0, w);
+  if (c0 + 16 < D) st256(row + c0 + 16, w + 8);
 }
-// Lane l receives the sum over the warp's lanes of v[l] (a butterfly that halves the columns
-// it carries at every step; the order of the additions is fixed).
-__device__ __forceinline__ float warp_col_sums(float (&v)[32], int lane) {
+// two fp32 operations per instruction (sm_100a)
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(F2 x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// A warp's 32 x 32 block (lane = row) through shared memory (32 rows of kBlockLd floats, which
+// keeps 16-byte accesses free of bank conflicts).
+constexpr int kBlockLd = 36;
+constexpr int kBlockBytes = 32 * kBlockLd * 4;
+__device__ __forceinline__ void block_put(float* block, const float (&v)[32], int lane) {
+  float4* o = reinterpret_cast<float4*>(block + lane * kBlockLd);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const bool upper = (lane & o) != 0;
+  for (int q = 0; q < 8; ++q) o[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+}
+// Column sums of the block: lane l receives those of columns 4 (l % 8) .. + 3 over the rows
+// l / 8 + 4 i, then the four lanes with the same columns add theirs (in a fixed order).
+__device__ __forceinline__ float4 block_col_sums(const float* block, int lane) {
+  const float* p = block + (lane >> 3) * kBlockLd + (lane & 7) * 4;
+  F2 a = f2(0.0f, 0.0f), b = a;
 #pragma unroll
-    for (int j = 0; j < o; ++j) {
-      const float keep = upper ? v[j + o] : v[j], give = upper ? v[j] : v[j + o];
-      v[j] = keep + __shfl_xor_sync(FULL, give, o);
-    }
+  for (int i = 0; i < 8; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(p + 4 * i * kBlockLd);
+    a = add2(a, f2(x.x, x.y));
+    b = add2(b, f2(x.z, x.w));
   }
-  return v[0];
+  float4 s;
+  split(a, s.x, s.y);
+  split(b, s.z, s.w);
+#pragma unroll
+  for (int o = 8; o <= 16; o <<= 1) {
+    s.x += __shfl_xor_sync(FULL, s.x, o);
+    s.y += __shfl_xor_sync(FULL, s.y, o);
+    s.z += __shfl_xor_sync(FULL, s.z, o);
+    s.w += __shfl_xor_sync(FULL, s.w, o);
+  }
+  return s;
 }
 
 // A list of `tot` tiles in equal consecutive shares: share c is [share_lo(c), share_lo(c + 1)),

@@ -35,7 +35,7 @@ struct Lists {             // target entries
   const int32_t* cnt;      // distillation: by original row
   const int32_t* ids;
   const float* p;
-  int64_t K;
+  int64_t Kp;
 };
 
 // ---- distillation: a teacher row's probabilities, sorted by id, duplicates joined --------
@@ -122,9 +122,13 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
     __syncthreads();
     if (head) {
       at += __popc(w & lanemask_lt());
-      s.ids[t * K + at] = int32_t(k >> 32);
-      s.p[t * K + at] = q;
+      s.ids[t * s.Kp + at] = int32_t(k >> 32);
+      s.p[t * s.Kp + at] = q;
     }
+  }
+  for (int64_t i = n + tid; i < s.Kp; i += kSortThreads) {
+    s.ids[t * s.Kp + i] = kNoId;
+    s.p[t * s.Kp + i] = 0.0f;
   }
   ent = reduce(ent, false);
   if (tid == 0) {
@@ -134,51 +138,84 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
   }
 }
 
-// Walks a row's ascending entries as the tiles pass.
+// Walks a row's ascending entries as the tiles pass.  Entries come four at a time, and the
+// next four are on their way while these are used: a load per entry would cost its latency on
+// the spot.
 struct Cursor {
-  const int32_t* ids;
-  const float* p;
-  int32_t left;      // entries not passed
-  int32_t next;      // id of the next one (INT_MAX: none)
+  const int4* ids;      // the four after the next
+  const float4* ps;
+  int4 id, id2;         // shifted down as they are used; the next four
+  float4 p, p2;
+  int32_t left;         // of the four in id
   __device__ void start(const Lists& l, int64_t orig, bool live, int32_t v0) {
-    left = 0;
-    next = 0x7FFFFFFF;
+    left = 4;
+    id = id2 = make_int4(kNoId, kNoId, kNoId, kNoId);
+    p = p2 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    ids = nullptr;
     if (!live) return;
-    ids = l.ids + orig * l.K;
-    p = l.p + orig * l.K;
-    left = l.cnt[orig];
-    int32_t lo = 0, hi = left;       // first entry with id >= v0
+    const int32_t* row = l.ids + orig * l.Kp;
+    int32_t lo = 0, hi = l.cnt[orig];       // first entry with id >= v0
     while (lo < hi) {
       const int32_t mid = (lo + hi) >> 1;
-      if (ids[mid] < v0) lo = mid + 1;
+      if (row[mid] < v0) lo = mid + 1;
       else hi = mid;
     }
-    ids += lo;
-    p += lo;
-    left -= lo;
-    if (left > 0) next = *ids;
+    lo &= ~3;
+    if (lo >= l.cnt[orig]) return;
+    end = reinterpret_cast<const int4*>(row + l.Kp);
+    ids = reinterpret_cast<const int4*>(row + lo);
+    ps = reinterpret_cast<const float4*>(l.p + orig * l.Kp + lo);
+    id = *ids;
+    p = *ps;
+    fetch();
+    skip_to(v0);
+  }
+  __device__ void fetch() {
+    ++ids;
+    ++ps;
+    if (ids < end) {
+      id2 = *ids;
+      p2 = *ps;
+    } else {
+      id2.x = kNoId;
+    }
+  }
+  __device__ int32_t next() const { return id.x; }
+  __device__ float prob() const { return p.x; }
+  __device__ void step() {
+    id.x = id.y, id.y = id.z, id.z = id.w;
+    p.x = p.y, p.y = p.z, p.z = p.w;
+    if (--left == 0) {
+      id = id2;
+      p = p2;
+      left = 4;
+      fetch();
+    }
   }
   __device__ void skip_to(int32_t v0) {      // entries of the other column half
-    while (next < v0) step();
+    while (next() < v0) step();
   }
-  __device__ void step() {
-    ++ids;
-    ++p;
-    --left;
-    next = left > 0 ? *ids : 0x7FFFFFFF;
-  }
+  const int4* end;
 };
 
-// z of 32 consecutive vocabulary rows
-__device__ __forceinline__ void to_z(float (&v)[32], float c, const float* bias2) {
-  const float4* b = reinterpret_cast<const float4*>(bias2);
+// This tile's share of bias2 for one warp: loaded by begin() while the products run (a float4
+// per lane, the 128 columns of a half), spread to all lanes through shared memory.
+struct BiasTile {
+  static constexpr int kBytes = mm::kBN / 2 * 4;
+  static __device__ void load(const float* bias2, unsigned char* smem, int lane) {
+    const float4 b = __ldg(reinterpret_cast<const float4*>(bias2) + lane);
+    __syncwarp();
+    reinterpret_cast<float4*>(smem)[lane] = b;
+    __syncwarp();
+  }
+};
+// z = c s + bias2 of 32 consecutive vocabulary rows
+__device__ __forceinline__ void to_z(const float (&v)[32], F2 c, const float* bias, F2 (&z)[16]) {
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
-    const float4 x = __ldg(b + q);
-    v[4 * q] = fmaf(v[4 * q], c, x.x);
-    v[4 * q + 1] = fmaf(v[4 * q + 1], c, x.y);
-    v[4 * q + 2] = fmaf(v[4 * q + 2], c, x.z);
-    v[4 * q + 3] = fmaf(v[4 * q + 3], c, x.w);
+    const float4 x = *reinterpret_cast<const float4*>(bias + 4 * q);
+    z[2 * q] = fma2(f2(v[4 * q], v[4 * q + 1]), c, f2(x.x, x.y));
+    z[2 * q + 1] = fma2(f2(v[4 * q + 2], v[4 * q + 3]), c, f2(x.z, x.w));
   }
 }
 
@@ -187,11 +224,12 @@ __device__ __forceinline__ void to_z(float (&v)[32], float c, const float* bias2
 // sum q z][kBM rows], at index share + row block (which no two of them have in common, since
 // along the list one of the two always grows).
 constexpr int kPart = 2 * 3 * mm::kBM;
+constexpr int kBiasScratch = mm::kEpiWarps * BiasTile::kBytes;
 constexpr int kListScratch = mm::kEpiWarps * 32 * 33 * 4;      // a padded 32 x 32 block per warp
 
 template <bool kList>
 struct LossJob {
-  static constexpr int kStages = kList ? 5 : 6, kScratch = kList ? kListScratch : 0;
+  static constexpr int kStages = kList ? 5 : 6, kScratch = kBiasScratch + (kList ? kListScratch : 0);
   CUtensorMap maps[2];      // H, W (K-major)
   int32_t wait_limit, bf16;
   const int32_t* head;
@@ -229,30 +267,39 @@ struct LossJob {
     float m, l, dot;
     int32_t tgt;
     Cursor cur;
-    __device__ void tile(const LossJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const int32_t n0 = t.y * mm::kBN;
+    __device__ float* bias(const mm::Acc& a) { return reinterpret_cast<float*>(a.scratch + a.warp * BiasTile::kBytes); }
+    __device__ void begin(const LossJob& j, const mm::Tile& t, const mm::Acc& a) {
+      const int32_t v0 = t.y * mm::kBN + a.c_lo;
+      BiasTile::load(j.bias2 + v0, reinterpret_cast<unsigned char*>(bias(a)), a.lane);
       if (t.flags & kFirst) {
         m = neg_inf();
         l = dot = 0.0f;
-        const int32_t r = a.row;
-        const bool live = r < j.head[0];
-        if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, n0 + a.c_lo);
-        else tgt = live ? j.lists.tgt[r] : -1;
+        const bool live = a.row < j.head[0];
+        if constexpr (kList) cur.start(j.lists, live ? j.map[a.row] : 0, live, v0);
+        else tgt = live ? j.lists.tgt[a.row] : -1;
       }
-      if constexpr (kList) cur.skip_to(n0 + a.c_lo);
+      if constexpr (kList) cur.skip_to(v0);
+    }
+    __device__ void tile(const LossJob& j, const mm::Tile& t, const mm::Acc& a) {
+      const float* b = bias(a) - a.c_lo;
+      const F2 c2 = f2(j.c, j.c);
+#pragma unroll 1
       for (int32_t c0 = a.c_lo; c0 < a.c_hi; c0 += 32) {
         float z[32];
         a.ld32(c0, z);
         if (c0 + 32 == a.c_hi) a.release();
-        const int32_t v0 = n0 + c0;
-        to_z(z, j.c, j.bias2 + v0);
+        F2 z2[16];
+        to_z(z, c2, b + c0, z2);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) split(z2[k], z[2 * k], z[2 * k + 1]);
+        const int32_t v0 = t.y * mm::kBN + c0;
         if constexpr (kList) {
-          if (__any_sync(FULL, cur.next < v0 + 32)) {
-            float* mine = reinterpret_cast<float*>(a.scratch) + (a.warp * 32 + a.lane) * 33;   // no other lane's
+          if (__any_sync(FULL, cur.next() < v0 + 32)) {
+            float* mine = reinterpret_cast<float*>(a.scratch + kBiasScratch) + (a.warp * 32 + a.lane) * 33;   // no other lane's
 #pragma unroll
             for (int k = 0; k < 32; ++k) mine[k] = z[k];
-            while (cur.next < v0 + 32) {
-              dot = fmaf(*cur.p, mine[cur.next - v0], dot);
+            while (cur.next() < v0 + 32) {
+              dot = fmaf(cur.prob(), mine[cur.next() - v0], dot);
               cur.step();
             }
           }
@@ -267,19 +314,26 @@ struct LossJob {
         }
         float x[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) x[k] = fmaxf(fmaxf(z[k], z[k + 8]), fmaxf(z[k + 16], z[k + 24]));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] = fmaxf(x[k], x[k + 4]);
-        const float cm = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+        for (int k = 0; k < 8; ++k) x[k] = max3(z[4 * k], z[4 * k + 1], fmaxf(z[4 * k + 2], z[4 * k + 3]));
+        const float cm = fmaxf(max3(x[0], x[1], x[2]), max3(x[3], x[4], max3(x[5], x[6], x[7])));
         if (cm > m) {
           l *= ex2(m - cm);
           m = cm;
         }
-        const float base = m == neg_inf() ? 0.0f : m;
-        float e[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float base = m == neg_inf() ? 0.0f : -m;
+        const F2 base2 = f2(base, base);
+        F2 e0 = f2(0.0f, 0.0f), e1 = e0;
 #pragma unroll
-        for (int k = 0; k < 32; ++k) e[k & 3] += ex2(z[k] - base);
-        l += (e[0] + e[1]) + (e[2] + e[3]);
+        for (int k = 0; k < 16; k += 2) {
+          float p, q;
+          split(add2(z2[k], base2), p, q);
+          e0 = add2(e0, f2(ex2(p), ex2(q)));
+          split(add2(z2[k + 1], base2), p, q);
+          e1 = add2(e1, f2(ex2(p), ex2(q)));
+        }
+        float p, q;
+        split(add2(e0, e1), p, q);
+        l += p + q;
       }
       if (t.flags & kLast) {
         float* o = j.part + (int64_t(blockIdx.x >> 1) + t.x) * kPart + a.half * 3 * mm::kBM + a.rank * mm::kRows + a.lane_row;
@@ -292,11 +346,10 @@ struct LossJob {
   __device__ Epi epi() const { return Epi{}; }
 };
 
-// Joins a row's partial results and sums the losses.  A block has 32 rows: each of its 8 warps
-// joins a run of consecutive shares (one row may have as many as there are pairs), the first
-// then joins the warps' results in order.  The blocks' sums are added by whichever block
-// finishes last, in block order.
-constexpr int kJoinRows = 32, kJoinWarps = 8;
+// Joins a row's partial results and sums the losses.  A warp per row, a lane per partial result
+// (a single row has two from every pair), joined in a fixed tree.  The blocks' sums are added by
+// whichever block finishes last, in block order.
+constexpr int kJoinRows = 8;
 struct RowSum {
   float m, l, dot;
   __device__ void add(float pm, float pl, float pd) {
@@ -306,61 +359,55 @@ struct RowSum {
     dot += pd;
   }
 };
-__global__ void __launch_bounds__(32 * kJoinWarps)
+__global__ void __launch_bounds__(32 * kJoinRows)
 join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, int32_t pairs, const float* ent, float tau2,
             int32_t reduction, float* lse2, double* sums, float* loss) {
-  __shared__ float got[3][kJoinWarps][kJoinRows];
-  __shared__ double red[kJoinWarps];
+  __shared__ double red[kJoinRows];
   __shared__ bool last;
   const int32_t n = head[0], wid = threadIdx.x >> 5, lane = lane_id();
-  const int32_t r = int32_t(blockIdx.x) * kJoinRows + lane, mb = r / mm::kBM;
-  const int32_t tot = (n + mm::kBM - 1) / mm::kBM * nt;
-  RowSum s{neg_inf(), 0.0f, 0.0f};
+  const int32_t r = int32_t(blockIdx.x) * kJoinRows + wid, mb = r / mm::kBM;
+  double mine = 0.0;
   if (r < n) {
-    const int32_t c0 = share_of(tot, pairs, mb * nt), c1 = share_of(tot, pairs, (mb + 1) * nt - 1) + 1;
-    const int32_t per = (c1 - c0 + kJoinWarps - 1) / kJoinWarps, lo = c0 + wid * per, hi = min(c1, lo + per);
-#pragma unroll 4
-    for (int32_t c = lo; c < hi; ++c) {
-      const float* o = part + int64_t(c + mb) * kPart + r % mm::kBM;
-      s.add(o[0], o[mm::kBM], o[2 * mm::kBM]);
-      o += 3 * mm::kBM;
+    const int32_t tot = (n + mm::kBM - 1) / mm::kBM * nt;
+    const int32_t c0 = share_of(tot, pairs, mb * nt), parts = 2 * (share_of(tot, pairs, (mb + 1) * nt - 1) + 1 - c0);
+    RowSum s{neg_inf(), 0.0f, 0.0f};
+    for (int32_t i = lane; i < parts; i += 32) {
+      const float* o = part + int64_t(c0 + (i >> 1) + mb) * kPart + (i & 1) * 3 * mm::kBM + r % mm::kBM;
       s.add(o[0], o[mm::kBM], o[2 * mm::kBM]);
     }
-  }
-  got[0][wid][lane] = s.m;
-  got[1][wid][lane] = s.l;
-  got[2][wid][lane] = s.dot;
-  __syncthreads();
-  if (wid == 0) {
-    double mine = 0.0;
-    if (r < n) {
-      for (int w = 1; w < kJoinWarps; ++w) s.add(got[0][w][lane], got[1][w][lane], got[2][w][lane]);
-      const float z = s.m + log2f(s.l);
-      lse2[r] = z;
-      const int32_t orig = map[r];
-      const float v = tau2 * fmaf(z - s.dot, kLn2, ent ? ent[orig] : 0.0f);
-      if (reduction == GSP_REDUCE_NONE) loss[orig] = v;
-      mine = double(v);
-    }
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(FULL, mine, o);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+      s.add(__shfl_xor_sync(FULL, s.m, o), __shfl_xor_sync(FULL, s.l, o), __shfl_xor_sync(FULL, s.dot, o));
+    const float z = s.m + log2f(s.l);
+    const int32_t orig = map[r];
+    const float v = tau2 * fmaf(z - s.dot, kLn2, ent ? ent[orig] : 0.0f);
     if (lane == 0) {
-      sums[blockIdx.x] = mine;
-      __threadfence();
-      last = atomicAdd(head + 1, 1) == int32_t(gridDim.x) - 1;
+      lse2[r] = z;
+      if (reduction == GSP_REDUCE_NONE) loss[orig] = v;
     }
+    mine = double(v);
   }
   if (reduction == GSP_REDUCE_NONE) return;
+  if (lane == 0) red[wid] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < kJoinRows; ++i) s += red[i];
+    sums[blockIdx.x] = s;
+    __threadfence();
+    last = atomicAdd(head + 1, 1) == int32_t(gridDim.x) - 1;
+  }
   __syncthreads();
   if (!last) return;
   __threadfence();
   double v = 0.0;
-  for (int32_t i = threadIdx.x; i < int32_t(gridDim.x); i += 32 * kJoinWarps) v += *reinterpret_cast<volatile double*>(sums + i);
+  for (int32_t i = threadIdx.x; i < int32_t(gridDim.x); i += 32 * kJoinRows) v += *reinterpret_cast<volatile double*>(sums + i);
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
   if (lane == 0) red[wid] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
     v = 0.0;
-    for (int i = 0; i < kJoinWarps; ++i) v += red[i];
+    for (int i = 0; i < kJoinRows; ++i) v += red[i];
     *loss = float(reduction == GSP_REDUCE_MEAN ? v / (n > 0 ? n : 1) : v);
   }
 }
@@ -405,8 +452,9 @@ grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, 
 
 template <bool kList>
 struct LogitGradJob {
-  static constexpr int kColBytes = 2 * 4 * mm::kBN * 4;      // column sums of 4 x 32 rows, two buffers
-  static constexpr int kStages = kList ? 5 : 6, kScratch = kColBytes + (kList ? kListScratch : 0);
+  // scratch: bias2 of the tile; a 32 x 32 block per warp; column sums of 4 x 32 rows (two buffers)
+  static constexpr int kBlockOff = kBiasScratch, kColOff = kBlockOff + mm::kEpiWarps * kBlockBytes;
+  static constexpr int kStages = 5, kScratch = kColOff + 2 * 4 * mm::kBN * 4;
   CUtensorMap maps[2];      // H, W (K-major)
   int32_t wait_limit, bf16;
   const int32_t* head;
@@ -419,13 +467,14 @@ struct LogitGradJob {
   int64_t pitch;
   float* colpart;           // [128-row blocks][pitch], or null
 
+  // the same shares along the vocabulary as the forward pass, so that a row's entries are found
+  // once per share
   struct Walk {
-    int32_t x, step, tot, nt, nk, v0;
+    int32_t lo, x, hi, nt, nk, v0;
     __device__ bool next(mm::Tile& t) {
-      if (x >= tot) return false;
+      if (x >= hi) return false;
       t.x = x / nt;
       t.y = x - t.x * nt;
-      x += step;
       t.a = 0, t.b = 1;
       t.a0 = t.x * mm::kBM;
       t.b0 = v0 + t.y * mm::kBN;
@@ -433,48 +482,76 @@ struct LogitGradJob {
       t.nk = nk;
       t.a_mn = t.b_mn = false;
       t.bn = mm::kBN;
-      t.flags = 0;
+      t.flags = x == lo || t.y == 0 ? kFirst : 0;
+      ++x;
       return true;
     }
   };
   __device__ Walk walk(int32_t pair, int32_t pairs) const {
-    return Walk{pair, pairs, (head[0] + mm::kBM - 1) / mm::kBM * nt, nt, nk, v0};
+    const int32_t tot = (head[0] + mm::kBM - 1) / mm::kBM * nt, lo = share_lo(tot, pairs, pair);
+    return Walk{lo, lo, share_lo(tot, pairs, pair + 1), nt, nk, v0};
   }
 
   struct Epi {
+    float lse, ga;
+    int32_t tgt;
+    bool live;
+    Cursor cur;
+    __device__ float* bias(const mm::Acc& a) { return reinterpret_cast<float*>(a.scratch + a.warp * BiasTile::kBytes); }
+    __device__ void begin(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
+      const int32_t v0 = t.b0 + a.c_lo;
+      BiasTile::load(j.bias2 + v0, reinterpret_cast<unsigned char*>(bias(a)), a.lane);
+      if (t.flags & kFirst) {
+        live = a.row < j.head[0];
+        lse = j.lse2[a.row];
+        ga = j.ga[a.row];
+        if constexpr (kList) cur.start(j.lists, live ? j.map[a.row] : 0, live, v0);
+        else tgt = live ? j.lists.tgt[a.row] : -1;
+      }
+      if constexpr (kList) cur.skip_to(v0);
+    }
     __device__ void tile(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const int32_t r = a.row;
-      const bool live = r < j.head[0];
-      const float lse = j.lse2[r], ga = j.ga[r];
-      Cursor cur;
-      int32_t tgt = -1;
-      if constexpr (kList) cur.start(j.lists, live ? j.map[r] : 0, live, t.b0 + a.c_lo);
-      else tgt = live ? j.lists.tgt[r] : -1;
-      uint16_t* row = j.P + int64_t(r) * j.pitch + t.y * mm::kBN;
-      float* cols = reinterpret_cast<float*>(a.scratch) + a.buf * 4 * mm::kBN;
+      uint16_t* row = j.P + int64_t(a.row) * j.pitch + t.y * mm::kBN;
+      const float* b = bias(a) - a.c_lo;
+      float* block = reinterpret_cast<float*>(a.scratch + kBlockOff + a.warp * kBlockBytes);
+      float* cols = reinterpret_cast<float*>(a.scratch + kColOff) + (a.buf * 4 + (a.warp & 3)) * mm::kBN;
+      const F2 c2 = f2(j.c, j.c), lse2 = f2(-lse, -lse), ga2 = f2(ga, ga);
+#pragma unroll 1
       for (int32_t c0 = a.c_lo; c0 < a.c_hi; c0 += 32) {
         float z[32];
         a.ld32(c0, z);
         if (c0 + 32 == a.c_hi) a.release();
         const int32_t v0 = t.b0 + c0;
-        to_z(z, j.c, j.bias2 + v0);
+        {
+          F2 z2[16];
+          to_z(z, c2, b + c0, z2);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) z[k] = ga * ex2(z[k] - lse);
+          for (int k = 0; k < 16; ++k) {
+            float p, q;
+            split(add2(z2[k], lse2), p, q);
+            split(mul2(f2(ex2(p), ex2(q)), ga2), z[2 * k], z[2 * k + 1]);
+          }
+        }
         if (!live) {        // padding rows: 0 whatever their hidden states hold
 #pragma unroll
           for (int k = 0; k < 32; ++k) z[k] = 0.0f;
         }
+        bool staged = false;
         if constexpr (kList) {
-          if (__any_sync(FULL, cur.next < v0 + 32)) {
-            float* mine = reinterpret_cast<float*>(a.scratch + kColBytes) + (a.warp * 32 + a.lane) * 33;
-#pragma unroll
-            for (int k = 0; k < 32; ++k) mine[k] = z[k];
-            while (cur.next < v0 + 32) {
-              mine[cur.next - v0] = fmaf(-ga, *cur.p, mine[cur.next - v0]);
+          if (__any_sync(FULL, cur.next() < v0 + 32)) {
+            __syncwarp();       // the column sums of the block before have been read
+            block_put(block, z, a.lane);
+            float* mine = block + a.lane * kBlockLd;
+            while (cur.next() < v0 + 32) {
+              mine[cur.next() - v0] = fmaf(-ga, cur.prob(), mine[cur.next() - v0]);
               cur.step();
             }
 #pragma unroll
-            for (int k = 0; k < 32; ++k) z[k] = mine[k];
+            for (int q = 0; q < 8; ++q) {
+              const float4 x = *reinterpret_cast<const float4*>(mine + 4 * q);
+              z[4 * q] = x.x, z[4 * q + 1] = x.y, z[4 * q + 2] = x.z, z[4 * q + 3] = x.w;
+            }
+            staged = true;
           }
         } else {
           const int32_t d = tgt - v0;
@@ -490,12 +567,20 @@ struct LogitGradJob {
         for (int k = 0; k < 16; ++k) w[k] = pack2(z[2 * k], z[2 * k + 1], j.bf16 != 0);
         st256(row + c0, w);
         st256(row + c0 + 16, w + 8);
-        if (j.colpart) cols[(a.warp & 3) * mm::kBN + c0 + a.lane] = warp_col_sums(z, a.lane);
+        if (j.colpart) {
+          if (!staged) {
+            __syncwarp();
+            block_put(block, z, a.lane);
+          }
+          __syncwarp();
+          const float4 s = block_col_sums(block, a.lane);
+          if (a.lane < 8) *reinterpret_cast<float4*>(cols + c0 + 4 * a.lane) = s;
+        }
       }
       if (j.colpart) {
         a.sync();
         const int c = a.warp * 32 + a.lane;
-        const float* q = cols + c;
+        const float* q = reinterpret_cast<const float*>(a.scratch + kColOff) + a.buf * 4 * mm::kBN + c;
         j.colpart[int64_t(t.x * 2 + a.rank) * j.pitch + t.y * mm::kBN + c] =
             (q[0] + q[mm::kBN]) + (q[2 * mm::kBN] + q[3 * mm::kBN]);
       }
@@ -594,7 +679,7 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Li
   j.part = f.part;
   if ((rc = mm::launch(j, st))) return rc;
   if (reduction == GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, size_t(vw->T) * sizeof(float), st));
-  join_kernel<<<unsigned((vw->T + kJoinRows - 1) / kJoinRows), 32 * kJoinWarps, 0, st>>>(
+  join_kernel<<<unsigned((vw->T + kJoinRows - 1) / kJoinRows), 32 * kJoinRows, 0, st>>>(
       s.head, s.map, f.part, j.nt, mm::pair_ctas() / 2, ent, tau * tau, reduction, s.lse2, f.sums, loss);
   GSP_CHECK_LAUNCH();
   return GSP_OK;
@@ -702,7 +787,7 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   l.cnt = s.cnt;
   l.ids = s.ids;
   l.p = s.p;
-  l.K = K;
+  l.Kp = s.Kp;
   return run_forward<true>(vw, s, f, l, tau, reduction, s.ent, loss, st);
 }
 
@@ -738,7 +823,7 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
     l.cnt = s.cnt;
     l.ids = s.ids;
     l.p = s.p;
-    l.K = K;
+    l.Kp = s.Kp;
     return run_backward<true>(vw, s, b, l, tau, d_hidden, d_weight, d_bias, st);
   }
   l.tgt = s.tgt;
