@@ -439,7 +439,7 @@ int run_head(const gsp_vocab_view* vw, const State& s, const Fwd& f, int32_t L, 
   const bool bf = is_bf16(vw);
   int rc;
   if ((rc = make_map(&j.maps[0], bf, w, vw->D, vw->V, ldw, mm::kRows))) return rc;
-  if ((rc = make_map(&j.maps[1], bf, s.h, s.Dp, s.Tp, s.Dp, bn / 2))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, s.h, s.Dp, vw->T, s.Dp, bn / 2))) return rc;
   return mm::launch(j, st);
 }
 
@@ -572,7 +572,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
     spread_kernel<<<dim3(unsigned((b.pitch / 8 + 255) / 256), unsigned(B + 1), unsigned(zs)), 256, 0, st>>>(p);
     GSP_CHECK_LAUNCH();
     const GradPiece pc{b.P, b.pitch, v0, p.cols, v0 == 0, v0 + p.cols >= vw->V};
-    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, b.scale, d_hidden, d_weight, st))) return rc;
+    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, BiasSums{}, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
 }

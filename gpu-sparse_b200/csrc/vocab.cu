@@ -46,6 +46,7 @@ __device__ __forceinline__ void copy_row(const uint16_t* src, uint16_t* dst, int
     for (int64_t i = lane; i < cols / 8; i += 32) d[i] = __ldg(s + i);
     for (int64_t i = cols + lane; i < pad; i += 32) dst[i] = 0;
   } else {
+#pragma unroll 8
     for (int64_t i = lane; i < pad; i += 32) dst[i] = i < cols ? src[i] : uint16_t(0);
   }
 }
@@ -328,13 +329,39 @@ struct GradJob {
   __device__ Epi epi() const { return Epi{}; }
 };
 
+// d_bias of a piece: the column sums of P that the logits' epilogue left for every 128 rows.  8
+// warps share the row blocks of 32 columns; their sums are added in order.
+__device__ void bias_grad(const BiasSums& b, int32_t n, int32_t cols, const float* scale, int64_t block) {
+  __shared__ float got[8][32];
+  const int wid = threadIdx.x >> 5, lane = lane_id();
+  const int64_t c = block * 32 + lane;
+  const int32_t blocks = (n + mm::kRows - 1) / mm::kRows;
+  float s = 0.0f;
+  if (c < cols) {
+#pragma unroll 4
+    for (int32_t i = wid; i < blocks; i += 8) s += b.part[int64_t(i) * b.pitch + c];
+  }
+  got[wid][lane] = s;
+  __syncthreads();
+  if (wid > 0 || c >= cols) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) s += got[w][lane];
+  b.out[c] = s * *scale;
+}
+
 // Finishes the tiles that a border between two shares cuts: the pair whose share holds a tile's
 // last step adds the fragments in list order.  Block (pair, CTA of the pair, 8 rows): a warp per
-// row, 8 columns per lane.
-__global__ void __launch_bounds__(256) frag_kernel(const __grid_constant__ GradJob j, int32_t pairs) {
+// row, 8 columns per lane.  The blocks past them finish d_bias.
+__global__ void __launch_bounds__(256)
+finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blocks, const BiasSums b) {
+  if (int32_t(blockIdx.x) >= frag_blocks) {
+    bias_grad(b, *j.n_rows, j.cols, j.scale, int64_t(blockIdx.x) - frag_blocks);
+    return;
+  }
   const GradList l = j.list();
   const int64_t tot = l.total();
-  const int32_t groups = j.groups(pairs, tot), pair = blockIdx.x;
+  const int32_t pair = blockIdx.x / (2 * mm::kRows / 8), sub = blockIdx.x % (2 * mm::kRows / 8);
+  const int32_t groups = j.groups(pairs, tot);
   const int32_t g = pair / j.nbs, nb = pair % j.nbs;
   if (g >= groups) return;
   const int64_t x0 = g * tot / groups, x1 = (g + 1) * tot / groups;
@@ -344,7 +371,7 @@ __global__ void __launch_bounds__(256) frag_kernel(const __grid_constant__ GradJ
   l.at(x0, &is_h, &blk, &start, &nk);
   if (x0 == start || x0 - start >= nk || x1 - start < nk) return;    // begins here, or ends elsewhere
   const int32_t first = int32_t(((start + 1) * groups - 1) / tot);   // the share that holds the tile's first step
-  const int32_t rank = blockIdx.y, row = blockIdx.z * 8 + (threadIdx.x >> 5), c = lane_id() * 8;
+  const int32_t rank = sub & 1, row = (sub >> 1) * 8 + (threadIdx.x >> 5), c = lane_id() * 8;
   const int32_t r = blk * mm::kBM + rank * mm::kRows + row;
   if (r >= (is_h ? *j.n_rows : j.cols) || nb * mm::kBN + c >= j.D) return;
   float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -485,15 +512,15 @@ GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t 
 }
 
 int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, int64_t ldw, const GradPiece& pc,
-                  const GradScratch& g, const float* scale, void* d_hidden, void* d_weight, cudaStream_t st) {
-  if (!d_hidden && !d_weight) return GSP_OK;
+                  const GradScratch& g, const BiasSums& bias, const float* scale, void* d_hidden, void* d_weight,
+                  cudaStream_t st) {
   GradJob j{};
   const bool bf = is_bf16(vw);
   int rc;
   if ((rc = make_map(&j.maps[0], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kRows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kBK))) return rc;
   if ((rc = make_map(&j.maps[2], bf, w, vw->D, vw->V, ldw, mm::kBK))) return rc;
-  if ((rc = make_map(&j.maps[3], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kBK))) return rc;
+  if ((rc = make_map(&j.maps[3], bf, s.h, s.Dp, vw->T, s.Dp, mm::kBK))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.n_rows = s.head;
@@ -515,10 +542,13 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.scale = scale;
   j.dh = static_cast<uint16_t*>(d_hidden);
   j.dw = static_cast<uint16_t*>(d_weight);
-  if ((rc = mm::launch(j, st))) return rc;
+  if ((d_hidden || d_weight) && (rc = mm::launch(j, st))) return rc;
   const int32_t pairs = mm::pair_ctas() / 2;
-  if (j.nbs > pairs) return GSP_OK;      // no tile is cut
-  frag_kernel<<<dim3(unsigned(pairs), 2, mm::kRows / 8), 256, 0, st>>>(j, pairs);
+  // with more D tiles than pairs no tile is cut
+  const int32_t frag_blocks = (d_hidden || d_weight) && j.nbs <= pairs ? pairs * (2 * mm::kRows / 8) : 0;
+  const int32_t blocks = frag_blocks + (bias.out ? int32_t((pc.cols + 31) / 32) : 0);
+  if (blocks == 0) return GSP_OK;
+  finish_kernel<<<unsigned(blocks), 256, 0, st>>>(j, pairs, frag_blocks, bias);
   GSP_CHECK_LAUNCH();
   return GSP_OK;
 }

@@ -63,8 +63,8 @@ inline int64_t pack_counts(int64_t T) { return (T + 255) / 256 + 1; }
 
 // Backward products over a piece of the vocabulary [v0, v0 + cols): P [Tp, pitch] is the
 // gradient of the piece's logits,
-//   dH (+)= P W[v0 : v0 + cols],   dW[v0 : v0 + cols] = P^T H,
-// in one launch.  Between pieces dH is carried in fp32.
+//   dH (+)= P W[v0 : v0 + cols],   dW[v0 : v0 + cols] = P^T H   (each where asked for),
+// in one launch, and a second that finishes them.  Between pieces dH is carried in fp32.
 struct GradPiece {
   const uint16_t* P;
   int64_t pitch, v0, cols;
@@ -75,8 +75,16 @@ struct GradScratch {
   float* frag;        // partial tiles
 };
 GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t pitch);
+// column sums of the piece's unrounded P for every 128 rows [row blocks][pitch], and where
+// their total goes (null: nowhere)
+struct BiasSums {
+  const float* part;
+  int64_t pitch;
+  float* out;
+};
 int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, int64_t ldw, const GradPiece& pc,
-                  const GradScratch& g, const float* scale, void* d_hidden, void* d_weight, cudaStream_t st);
+                  const GradScratch& g, const BiasSums& bias, const float* scale, void* d_hidden, void* d_weight,
+                  cudaStream_t st);
 // columns of one piece: P takes at most kPieceBytes
 constexpr int64_t kPieceBytes = int64_t(512) << 20;
 int64_t piece_cols(int64_t Tp, int64_t V);
@@ -86,6 +94,17 @@ __device__ __forceinline__ void zero_tail_rows(uint16_t* h, int64_t Dp, int32_t 
   const int64_t end = (int64_t(n) + 63) / 64 * 64;
   uint4* p = reinterpret_cast<uint4*>(h + int64_t(n) * Dp);
   for (int64_t i = threadIdx.x; i < (end - n) * Dp / 8; i += blockDim.x) p[i] = make_uint4(0, 0, 0, 0);
+}
+// Zeroes this block's share of d_hidden's rows: the products write only those that took part.
+__device__ __forceinline__ void zero_share(void* d, int64_t bytes, int64_t block, int64_t blocks) {
+  const int64_t head = min64((16 - int64_t(reinterpret_cast<uintptr_t>(d) & 15)) & 15, bytes), n = (bytes - head) / 16;
+  char* c = static_cast<char*>(d);
+  if (block == 0) {
+    for (int64_t i = threadIdx.x; i < head; i += blockDim.x) c[i] = 0;
+    for (int64_t i = head + n * 16 + threadIdx.x; i < bytes; i += blockDim.x) c[i] = 0;
+  }
+  uint4* p = reinterpret_cast<uint4*>(c + head);
+  for (int64_t i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) p[i] = make_uint4(0, 0, 0, 0);
 }
 
 // ---- device helpers ----------------------------------------------------------------------

@@ -39,7 +39,8 @@ struct Lists {             // target entries
 };
 
 // ---- distillation: a teacher row's probabilities, sorted by id, duplicates joined --------
-constexpr int kSortThreads = 128;
+// kSortThreads: half the entries, rounded up to a power of two (32 to 512)
+template <int kSortThreads>
 __global__ void __launch_bounds__(kSortThreads)
 teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_ids, int32_t K, int32_t pow2, int64_t V,
                float inv_tau, State s) {
@@ -371,9 +372,19 @@ join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, in
     const int32_t tot = (n + mm::kBM - 1) / mm::kBM * nt;
     const int32_t c0 = share_of(tot, pairs, mb * nt), parts = 2 * (share_of(tot, pairs, (mb + 1) * nt - 1) + 1 - c0);
     RowSum s{neg_inf(), 0.0f, 0.0f};
-    for (int32_t i = lane; i < parts; i += 32) {
-      const float* o = part + int64_t(c0 + (i >> 1) + mb) * kPart + (i & 1) * 3 * mm::kBM + r % mm::kBM;
-      s.add(o[0], o[mm::kBM], o[2 * mm::kBM]);
+    for (int32_t i0 = 0; i0 < parts; i0 += 160) {        // five loads of each kind in flight
+      float pm[5], pl[5], pd[5];
+#pragma unroll
+      for (int k = 0; k < 5; ++k) {
+        const int32_t i = i0 + 32 * k + lane;
+        const float* o = part + int64_t(c0 + (i >> 1) + mb) * kPart + (i & 1) * 3 * mm::kBM + r % mm::kBM;
+        const bool in = i < parts;
+        pm[k] = in ? o[0] : neg_inf();
+        pl[k] = in ? o[mm::kBM] : 0.0f;
+        pd[k] = in ? o[2 * mm::kBM] : 0.0f;
+      }
+#pragma unroll
+      for (int k = 0; k < 5; ++k) s.add(pm[k], pl[k], pd[k]);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
@@ -414,10 +425,16 @@ join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, in
 
 // ---- backward ----------------------------------------------------------------------------
 // Row coefficients of P: ga[r] = tau * grad_loss (divided by the rows of a mean) over their
-// largest finite size; lse2 of the padding rows +inf, so that their P is 0.  One CTA.
+// largest finite size; lse2 of the padding rows +inf, so that their P is 0.  One CTA; the others
+// zero d_hidden.
 __global__ void __launch_bounds__(1024)
-grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, int32_t bf16, float* ga, float* scale) {
+grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, int32_t bf16, float* ga, float* scale,
+                 void* d_hidden, int64_t hidden_bytes) {
   __shared__ float red[32];
+  if (blockIdx.x > 0) {
+    zero_share(d_hidden, hidden_bytes, int64_t(blockIdx.x) - 1, int64_t(gridDim.x) - 1);
+    return;
+  }
   const int32_t n = s.head[0];
   const int32_t np = (n + kRowPad - 1) / kRowPad * kRowPad;
   const float mul = tau / float(reduction == GSP_REDUCE_MEAN ? (n > 0 ? n : 1) : 1);
@@ -589,27 +606,6 @@ struct LogitGradJob {
   __device__ Epi epi() const { return Epi{}; }
 };
 
-// d_bias of a piece: the row blocks' column sums.  8 warps share the blocks of 32 columns; their
-// sums are added in order.
-__global__ void __launch_bounds__(256)
-bias_grad_kernel(const int32_t* head, const float* colpart, int64_t pitch, int64_t cols, const float* scale, float* d_bias) {
-  __shared__ float got[8][32];
-  const int wid = threadIdx.x >> 5, lane = lane_id();
-  const int64_t c = int64_t(blockIdx.x) * 32 + lane;
-  const int32_t blocks = (head[0] + mm::kRows - 1) / mm::kRows;
-  float s = 0.0f;
-  if (c < cols) {
-#pragma unroll 4
-    for (int32_t b = wid; b < blocks; b += 8) s += colpart[int64_t(b) * pitch + c];
-  }
-  got[wid][lane] = s;
-  __syncthreads();
-  if (wid > 0 || c >= cols) return;
-#pragma unroll
-  for (int w = 1; w < 8; ++w) s += got[w][lane];
-  d_bias[c] = s * *scale;
-}
-
 // ---- host --------------------------------------------------------------------------------
 struct Fwd {
   int32_t* counts;
@@ -665,7 +661,7 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Li
   if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
   LossJob<kList> j{};
   const bool bf = is_bf16(vw);
-  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kRows))) return rc;
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, vw->T, s.Dp, mm::kRows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
@@ -694,7 +690,7 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
   if ((rc = weight_rows(vw, b.wcopy, &w, &ldw, st))) return rc;
   LogitGradJob<kList> j{};
   const bool bf = is_bf16(vw);
-  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, mm::kRows))) return rc;
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, vw->T, s.Dp, mm::kRows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
@@ -714,12 +710,8 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
     j.v0 = int32_t(v0);
     j.nt = int32_t((cols + mm::kBN - 1) / mm::kBN);
     if ((rc = mm::launch(j, st))) return rc;
-    if (d_bias) {
-      bias_grad_kernel<<<unsigned((cols + 31) / 32), 256, 0, st>>>(s.head, b.colpart, b.pitch, cols, b.scale, d_bias + v0);
-      GSP_CHECK_LAUNCH();
-    }
     const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V};
-    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, b.scale, d_hidden, d_weight, st))) return rc;
+    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, BiasSums{b.colpart, b.pitch, d_bias ? d_bias + v0 : nullptr}, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
 }
@@ -780,7 +772,13 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   GSP_REQUIRE(scores && ids && vw->hidden && vw->weight, GSP_ERR_ARG, "topk_distillation: null input");
   int32_t pow2 = 2;
   while (pow2 < K) pow2 <<= 1;
-  teacher_kernel<<<unsigned(vw->T), kSortThreads, size_t(pow2) * 12, st>>>(scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, s);
+  const size_t sort_bytes = size_t(pow2) * 12;
+#define GSP_TEACHER(n) teacher_kernel<n><<<unsigned(vw->T), n, sort_bytes, st>>>(scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, s)
+  if (pow2 <= 64) GSP_TEACHER(32);
+  else if (pow2 <= 128) GSP_TEACHER(64);
+  else if (pow2 <= 512) GSP_TEACHER(256);
+  else GSP_TEACHER(512);
+#undef GSP_TEACHER
   GSP_CHECK_LAUNCH();
   if ((rc = pack_rows(vw, nullptr, 0, s.flag, kLog2e / tau, s, f.counts, st))) return rc;
   Lists l{};
@@ -814,9 +812,11 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
     return GSP_OK;
   }
   GSP_REQUIRE(grad_loss && vw->weight, GSP_ERR_ARG, "vocab loss backward: null input");
-  if (d_hidden) GSP_CUDA(cudaMemsetAsync(d_hidden, 0, size_t(vw->T) * size_t(vw->D) * 2, st));
   if (!list) tau = 1.0f;
-  grad_rows_kernel<<<1, 1024, 0, st>>>(s, grad_loss, reduction, tau, is_bf16(vw), b.ga, b.scale);
+  const int64_t hidden_bytes = vw->T * vw->D * 2;
+  const int64_t zero_blocks = d_hidden ? min64((hidden_bytes + 65535) / 65536, num_sms()) : 0;
+  grad_rows_kernel<<<unsigned(1 + zero_blocks), 1024, 0, st>>>(s, grad_loss, reduction, tau, is_bf16(vw), b.ga, b.scale,
+                                                              d_hidden, hidden_bytes);
   GSP_CHECK_LAUNCH();
   Lists l{};
   if (list) {

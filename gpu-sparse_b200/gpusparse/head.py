@@ -22,7 +22,9 @@ results' sizes depend on the data.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 from typing import Iterable, Optional, Tuple
 
 import torch
@@ -63,57 +65,81 @@ def _check(what: str, hidden, weight, bias):
 
 def _view(hidden, weight, bias) -> L.VocabView:
     """View of row tensors (see _rows); hidden may be (T, D) of a backward call without data."""
-    v = L.VocabView()
+    V, D = weight.shape
     if isinstance(hidden, torch.Tensor):
-        v.T, v.D = hidden.shape
-        v.ld_hidden = hidden.stride(0) if v.T > 1 else v.D
-        v.hidden = hidden.data_ptr()
+        T = hidden.shape[0]
+        ldh, ptr = hidden.stride(0) if T > 1 else D, hidden.data_ptr()
     else:
-        v.T, v.D = hidden
-        v.ld_hidden = v.D
-    v.V = weight.shape[0]
-    v.ld_weight = weight.stride(0) if v.V > 1 else v.D
-    v.weight = weight.data_ptr()
-    v.bias = bias.data_ptr() if bias is not None else None
-    v.dtype = _DTYPES[weight.dtype]
-    return v
+        T, ldh, ptr = hidden[0], D, None
+    return L.VocabView(T, V, D, ldh, weight.stride(0) if V > 1 else D, ptr, weight.data_ptr(),
+                       bias.data_ptr() if bias is not None else None, _DTYPES[weight.dtype], 0)
 
 
-def _buffers(v: L.VocabView, K: int, kind: int, dev):
+@functools.lru_cache(maxsize=1024)
+def _sizes(T, V, D, ld_weight, aligned, K, kind, backward, device_index):
+    """(state, workspace) bytes of a call: a function of its sizes alone (and of the device's
+    number of SMs)."""
     lib = L.lib()
-    sb = lib.gsp_vocab_state_bytes(v.T, v.V, v.D, K, kind)
-    wb = lib.gsp_vocab_ws_bytes(ctypes.byref(v), kind, 0)
+    v = L.VocabView(T, V, D, D, ld_weight, None, None if aligned else 2, None, L.W_BF16, 0)
+    sb = lib.gsp_vocab_state_bytes(T, V, D, K, kind)
+    wb = lib.gsp_vocab_ws_bytes(ctypes.byref(v), kind, int(backward))
     if sb < 0 or wb < 0:
         L.check(int(-min(sb, wb)), "vocabulary head")
-    return L.workspace(sb, dev), L.workspace(wb, dev)
+    return sb, wb
 
 
-def _backward_ws(v: L.VocabView, kind: int, dev) -> torch.Tensor:
-    wb = L.lib().gsp_vocab_ws_bytes(ctypes.byref(v), kind, 1)
-    if wb < 0:
-        L.check(int(-wb), "vocabulary head")
-    return L.workspace(wb, dev)
+def _bytes(v: L.VocabView, K: int, kind: int, backward: bool, dev):
+    return _sizes(v.T, v.V, v.D, v.ld_weight, v.weight % 16 == 0, K, kind, backward, dev.index)
+
+
+def _buffer(nbytes: int, dev) -> torch.Tensor:
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    """The device's context, or nothing to do where it is current already."""
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream(dev) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 # ---------------------------------------------------------------------------- losses
 def _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction):
     dev = hidden.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         v = _view(hidden, weight, bias)
         K = ids.shape[1] if kind == L.VOCAB_DISTILL else 0
-        state, ws = _buffers(v, K, kind, dev)
-        loss = torch.empty(v.T if reduction == 0 else (), dtype=torch.float32, device=dev)
+        sb, wb = _bytes(v, K, kind, False, dev)
+        state, ws = _buffer(sb, dev), _buffer(wb, dev)
+        loss = torch.empty((v.T,) if reduction == 0 else (), dtype=torch.float32, device=dev)
         if kind == L.VOCAB_CE:
             L.check(L.lib().gsp_vocab_ce(ctypes.byref(v), targets.data_ptr(), ignore_index, reduction,
-                                         loss.data_ptr(), state.data_ptr(), state.numel(),
-                                         ws.data_ptr(), ws.numel(), L.stream_of(dev)),
-                    "vocab_cross_entropy")
+                                         loss.data_ptr(), state.data_ptr(), sb, ws.data_ptr(), wb,
+                                         _stream(dev)), "vocab_cross_entropy")
         else:
             L.check(L.lib().gsp_vocab_distill(ctypes.byref(v), scores.data_ptr(), ids.data_ptr(), K,
-                                              tau, reduction, loss.data_ptr(), state.data_ptr(),
-                                              state.numel(), ws.data_ptr(), ws.numel(),
-                                              L.stream_of(dev)), "topk_distillation")
+                                              tau, reduction, loss.data_ptr(), state.data_ptr(), sb,
+                                              ws.data_ptr(), wb, _stream(dev)), "topk_distillation")
     return loss, state, K
+
+
+def _grad_buffers(ctx, T, weight):
+    """d_hidden, d_weight and d_bias as the backward pass needs them, else None."""
+    V, D = weight.shape
+    need_h, need_w, need_b = ctx.needs_input_grad[:3]
+    dev = weight.device
+    return (torch.empty((T, D), dtype=weight.dtype, device=dev) if need_h else None,
+            torch.empty((V, D), dtype=weight.dtype, device=dev) if need_w else None,
+            torch.empty(V, dtype=torch.float32, device=dev) if need_b else None)
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
 
 
 class _VocabLoss(torch.autograd.Function):
@@ -130,20 +156,18 @@ class _VocabLoss(torch.autograd.Function):
     def backward(ctx, grad):
         (weight,) = ctx.saved_tensors
         kind, K, tau, reduction = ctx.args
-        need_h, need_w, need_b = ctx.needs_input_grad[:3]
         dev = weight.device
-        with torch.cuda.device(dev):
-            v = _view((ctx.T, weight.shape[1]), weight, None)
+        with _on(dev):
+            v = _view((ctx.T, None), weight, None)
             grad = grad.to(torch.float32).contiguous()
-            ws = _backward_ws(v, kind, dev)
-            dh = torch.empty((v.T, v.D), dtype=weight.dtype, device=dev) if need_h else None
-            dw = torch.empty((v.V, v.D), dtype=weight.dtype, device=dev) if need_w else None
-            db = torch.empty(v.V, dtype=torch.float32, device=dev) if need_b else None
+            _, wb = _bytes(v, K, kind, True, dev)
+            ws = _buffer(wb, dev)
+            dh, dw, db = _grad_buffers(ctx, ctx.T, weight)
             L.check(L.lib().gsp_vocab_loss_backward(
-                ctypes.byref(v), kind, K, tau, reduction, grad.data_ptr(), L.ptr(dh), L.ptr(dw),
-                L.ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), ws.numel(),
-                L.stream_of(dev)), "vocab loss backward")
-        return (dh, dw, db) + (None,) * 7
+                ctypes.byref(v), kind, K, tau, reduction, grad.data_ptr(), _ptr(dh), _ptr(dw),
+                _ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), wb, _stream(dev)),
+                "vocab loss backward")
+        return dh, dw, db, None, None, None, None, None, None, None
 
 
 def _loss(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction):
@@ -227,15 +251,16 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_scores
 # ---------------------------------------------------------------------------- sparse head
 def _head_forward(hidden, weight, bias, mask, Lt: int, train: bool):
     dev = hidden.device
-    with torch.cuda.device(dev):
+    with _on(dev):
         v = _view(hidden, weight, bias)
         B = v.T // Lt
-        state, ws = _buffers(v, 0, L.VOCAB_HEAD, dev)
+        sb, wb = _bytes(v, 0, L.VOCAB_HEAD, False, dev)
+        state, ws = _buffer(sb, dev), _buffer(wb, dev)
         y = torch.empty((B, v.V), dtype=torch.float32, device=dev)
         win = torch.empty((B, v.V), dtype=torch.int32, device=dev) if train else None
-        L.check(L.lib().gsp_sparse_head(ctypes.byref(v), Lt, L.ptr(mask), y.data_ptr(), L.ptr(win),
-                                        state.data_ptr(), state.numel(), ws.data_ptr(), ws.numel(),
-                                        L.stream_of(dev)), "sparse_head")
+        L.check(L.lib().gsp_sparse_head(ctypes.byref(v), Lt, _ptr(mask), y.data_ptr(), _ptr(win),
+                                        state.data_ptr(), sb, ws.data_ptr(), wb, _stream(dev)),
+                "sparse_head")
     return y, win, state
 
 
@@ -251,19 +276,17 @@ class _SparseHead(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         weight, y = ctx.saved_tensors
-        need_h, need_w, need_b = ctx.needs_input_grad[:3]
         dev = weight.device
-        with torch.cuda.device(dev):
-            v = _view((ctx.T, weight.shape[1]), weight, None)
+        with _on(dev):
+            v = _view((ctx.T, None), weight, None)
             dy = dy.to(torch.float32).contiguous()
-            ws = _backward_ws(v, L.VOCAB_HEAD, dev)
-            dh = torch.empty((v.T, v.D), dtype=weight.dtype, device=dev) if need_h else None
-            dw = torch.empty((v.V, v.D), dtype=weight.dtype, device=dev) if need_w else None
-            db = torch.empty(v.V, dtype=torch.float32, device=dev) if need_b else None
+            _, wb = _bytes(v, 0, L.VOCAB_HEAD, True, dev)
+            ws = _buffer(wb, dev)
+            dh, dw, db = _grad_buffers(ctx, ctx.T, weight)
             L.check(L.lib().gsp_sparse_head_backward(
-                ctypes.byref(v), ctx.Lt, y.data_ptr(), ctx.win.data_ptr(), dy.data_ptr(), L.ptr(dh),
-                L.ptr(dw), L.ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(),
-                ws.numel(), L.stream_of(dev)), "sparse_head backward")
+                ctypes.byref(v), ctx.Lt, y.data_ptr(), ctx.win.data_ptr(), dy.data_ptr(), _ptr(dh),
+                _ptr(dw), _ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), wb,
+                _stream(dev)), "sparse_head backward")
         return dh, dw, db, None, None
 
 
