@@ -65,6 +65,7 @@ struct Tile {
   int32_t ak, bk;
   int32_t nk;            // 64-deep steps; 0: the product is zero
   bool a_mn, b_mn;       // operand is MN-major
+  bool a_stream;         // A passes through L2 (B, and else A, is kept there)
   int32_t bn;            // rows of B of this tile (a K-major B's map has boxes of half of it)
   int32_t x, y, flags;   // the job's own coordinates
 };
@@ -121,14 +122,38 @@ __device__ __forceinline__ void cluster_sync() {
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// L2 policies of an operand's reads: kept (weights and states, read over and over) or first to
+// go (a matrix that streams through)
+__device__ __forceinline__ uint64_t l2_policy(bool keep) {
+  uint64_t p;
+  if (keep) {
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  } else {
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  }
+  return p;
+}
 // this CTA's copy of a box, counted at the barrier `bar` (a cluster address, in either CTA)
-__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
-      "[%4];" ::"r"(su32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint [%0], "
+      "[%1, {%2, %3}], [%4], %5;" ::"r"(su32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(policy)
       : "memory");
 }
+// Stores a box of shared memory (128-byte swizzled rows) where the map says; the executing
+// thread owns the copy's group.
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(su32(src))
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_wait() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// this thread's shared-memory writes before it become visible to bulk copies after it
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // arrives once the products issued so far are done, at this CTA's barrier or at both CTAs'
@@ -259,10 +284,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
   if (wid == 0) {
     if (lane == 0) {
       auto walk = job.walk(pair, pairs);
+      const uint64_t keep = l2_policy(true), stream = l2_policy(false);
       Tile t;
       uint32_t it = 0;
       bool ok = true;
       while (ok && walk.next(t)) {
+        const uint64_t pol_a = t.a_stream ? stream : keep;
         const CUtensorMap* ma = &job.maps[t.a];
         const CUtensorMap* mb = &job.maps[t.b];
         const int32_t nb = t.bn / 2, a0 = t.a0 + rank * kRows, b0 = t.b0 + rank * nb;
@@ -276,14 +303,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
           const uint32_t bar = in_first_cta(full + s);
           if (rank == 0) bar_expect(full + s, bytes);
           if (!t.a_mn) {
-            tma_2d(as, ma, t.ak + k * kBK, a0, bar);
+            tma_2d(as, ma, t.ak + k * kBK, a0, bar, pol_a);
           } else {
-            for (int32_t j = 0; j < kRows / 64; ++j) tma_2d(as + j * 8192, ma, a0 + j * 64, t.ak + k * kBK, bar);
+            for (int32_t j = 0; j < kRows / 64; ++j) tma_2d(as + j * 8192, ma, a0 + j * 64, t.ak + k * kBK, bar, pol_a);
           }
           if (!t.b_mn) {
-            tma_2d(bs, mb, t.bk + k * kBK, b0, bar);
+            tma_2d(bs, mb, t.bk + k * kBK, b0, bar, keep);
           } else {
-            for (int32_t j = 0; j < nb / 64; ++j) tma_2d(bs + j * 8192, mb, b0 + j * 64, t.bk + k * kBK, bar);
+            for (int32_t j = 0; j < nb / 64; ++j) tma_2d(bs + j * 8192, mb, b0 + j * 64, t.bk + k * kBK, bar, keep);
           }
         }
       }

@@ -202,6 +202,7 @@ struct GradJob {
         t.a = is_h ? 0 : 1;
         t.b = is_h ? 2 : 3;
         t.a_mn = !is_h;
+        t.a_stream = true;
         t.bk = (is_h ? v0 : 0) + k0 * mm::kBK;
         t.nk = k1 - k0;
         t.x = blk;

@@ -252,7 +252,7 @@ struct LossJob {
       t.b0 = t.y * mm::kBN;
       t.ak = t.bk = 0;
       t.nk = nk;
-      t.a_mn = t.b_mn = false;
+      t.a_mn = t.b_mn = t.a_stream = false;
       t.bn = mm::kBN;
       t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == nt - 1 ? kLast : 0);
       ++x;
@@ -469,10 +469,12 @@ grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, 
 
 template <bool kList>
 struct LogitGradJob {
-  // scratch: bias2 of the tile; a 32 x 32 block per warp; column sums of 4 x 32 rows (two buffers)
-  static constexpr int kBlockOff = kBiasScratch, kColOff = kBlockOff + mm::kEpiWarps * kBlockBytes;
-  static constexpr int kStages = 5, kScratch = kColOff + 2 * 4 * mm::kBN * 4;
-  CUtensorMap maps[2];      // H, W (K-major)
+  // scratch: per warp 32 rows x 64 columns of P on their way out; bias2 of the tile; a 32 x 32
+  // block per warp; column sums of 4 x 32 rows (two buffers)
+  static constexpr int kOutBytes = 32 * 128, kBiasOff = mm::kEpiWarps * kOutBytes, kBlockOff = kBiasOff + kBiasScratch;
+  static constexpr int kColOff = kBlockOff + mm::kEpiWarps * kBlockBytes;
+  static constexpr int kStages = 4, kScratch = kColOff + 2 * 4 * mm::kBN * 4;
+  CUtensorMap maps[3];      // H, W (K-major); P as 32 x 64 boxes
   int32_t wait_limit, bf16;
   const int32_t* head;
   const int32_t* map;
@@ -480,8 +482,7 @@ struct LogitGradJob {
   float c;
   const float *bias2, *lse2, *ga;
   Lists lists;
-  uint16_t* P;
-  int64_t pitch;
+  int64_t pitch;            // of P and colpart
   float* colpart;           // [128-row blocks][pitch], or null
 
   // the same shares along the vocabulary as the forward pass, so that a row's entries are found
@@ -497,9 +498,9 @@ struct LogitGradJob {
       t.b0 = v0 + t.y * mm::kBN;
       t.ak = t.bk = 0;
       t.nk = nk;
-      t.a_mn = t.b_mn = false;
+      t.a_mn = t.b_mn = t.a_stream = false;
       t.bn = mm::kBN;
-      t.flags = x == lo || t.y == 0 ? kFirst : 0;
+      t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 ? kLast : 0);
       ++x;
       return true;
     }
@@ -514,7 +515,7 @@ struct LogitGradJob {
     int32_t tgt;
     bool live;
     Cursor cur;
-    __device__ float* bias(const mm::Acc& a) { return reinterpret_cast<float*>(a.scratch + a.warp * BiasTile::kBytes); }
+    __device__ float* bias(const mm::Acc& a) { return reinterpret_cast<float*>(a.scratch + kBiasOff + a.warp * BiasTile::kBytes); }
     __device__ void begin(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
       const int32_t v0 = t.b0 + a.c_lo;
       BiasTile::load(j.bias2 + v0, reinterpret_cast<unsigned char*>(bias(a)), a.lane);
@@ -528,7 +529,7 @@ struct LogitGradJob {
       if constexpr (kList) cur.skip_to(v0);
     }
     __device__ void tile(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
-      uint16_t* row = j.P + int64_t(a.row) * j.pitch + t.y * mm::kBN;
+      unsigned char* out = a.scratch + a.warp * kOutBytes;
       const float* b = bias(a) - a.c_lo;
       float* block = reinterpret_cast<float*>(a.scratch + kBlockOff + a.warp * kBlockBytes);
       float* cols = reinterpret_cast<float*>(a.scratch + kColOff) + (a.buf * 4 + (a.warp & 3)) * mm::kBN;
@@ -582,8 +583,20 @@ struct LogitGradJob {
         uint32_t w[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) w[k] = pack2(z[2 * k], z[2 * k + 1], j.bf16 != 0);
-        st256(row + c0, w);
-        st256(row + c0 + 16, w + 8);
+        // half a 128-byte row at a time, 16-byte pieces swizzled as the map wants them
+        if ((c0 & 32) == 0) {
+          if (a.lane == 0) mm::tma_store_wait_read();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          reinterpret_cast<uint4*>(out + a.lane * 128)[(((c0 & 32) >> 3) + q) ^ (a.lane & 7)] =
+              make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+        if (c0 & 32) {
+          mm::fence_async();
+          __syncwarp();
+          if (a.lane == 0) mm::tma_store_2d(&j.maps[2], out, t.y * mm::kBN + c0 - 32, a.row);
+        }
         if (j.colpart) {
           if (!staged) {
             __syncwarp();
@@ -594,6 +607,7 @@ struct LogitGradJob {
           if (a.lane < 8) *reinterpret_cast<float4*>(cols + c0 + 4 * a.lane) = s;
         }
       }
+      if ((t.flags & kLast) && a.lane == 0) mm::tma_store_wait();
       if (j.colpart) {
         a.sync();
         const int c = a.warp * 32 + a.lane;
@@ -702,7 +716,7 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
   j.lse2 = s.lse2;
   j.ga = b.ga;
   j.lists = lists;
-  j.P = b.P;
+  if ((rc = make_map(&j.maps[2], bf, b.P, b.pitch, s.Tp, b.pitch, 32))) return rc;
   j.pitch = b.pitch;
   j.colpart = d_bias ? b.colpart : nullptr;
   for (int64_t v0 = 0; v0 < vw->V; v0 += b.pitch) {
