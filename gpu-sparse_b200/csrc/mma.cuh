@@ -66,6 +66,8 @@ struct Tile {
   int32_t nk;            // 64-deep steps; 0: the product is zero
   bool a_mn, b_mn;       // operand is MN-major
   bool a_stream;         // A passes through L2 (B, and else A, is kept there)
+  int32_t a_rows;        // rows of a K-major A's boxes, at most kRows; fewer: A has no more, they
+                         // are the first CTA's, and the other rows of the tile are not read
   int32_t bn;            // rows of B of this tile (a K-major B's map has boxes of half of it)
   int32_t x, y, flags;   // the job's own coordinates
 };
@@ -119,8 +121,10 @@ __device__ __forceinline__ uint32_t cta_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// relaxed: what it orders is tensor memory (the tcgen05 fences do that); a release would wait for
+// all stores in flight, which measured 14 % of the logits' gradient
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 // L2 policies of an operand's reads: kept (weights and states, read over and over) or first to
 // go (a matrix that streams through)
@@ -293,7 +297,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
         const CUtensorMap* ma = &job.maps[t.a];
         const CUtensorMap* mb = &job.maps[t.b];
         const int32_t nb = t.bn / 2, a0 = t.a0 + rank * kRows, b0 = t.b0 + rank * nb;
-        const uint32_t bytes = 2 * uint32_t(kABytes + nb * kBK * 2);
+        const bool few = !t.a_mn && t.a_rows < kRows;
+        const uint32_t bytes = uint32_t((few ? t.a_rows : 2 * kRows) + 2 * nb) * (kBK * 2);
         for (int32_t k = 0; k < t.nk; ++k, ++it) {
           const uint32_t s = it % kStages, n = it / kStages;
           if (n > 0) ok = bar_wait(empty + s, (n - 1) & 1, limit, fault);
@@ -303,7 +308,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
           const uint32_t bar = in_first_cta(full + s);
           if (rank == 0) bar_expect(full + s, bytes);
           if (!t.a_mn) {
-            tma_2d(as, ma, t.ak + k * kBK, a0, bar, pol_a);
+            if (!few || rank == 0) tma_2d(as, ma, t.ak + k * kBK, a0, bar, pol_a);
           } else {
             for (int32_t j = 0; j < kRows / 64; ++j) tma_2d(as + j * 8192, ma, a0 + j * 64, t.ak + k * kBK, bar, pol_a);
           }

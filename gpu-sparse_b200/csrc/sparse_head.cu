@@ -53,6 +53,7 @@ struct HeadJob {
       t.nk = nk;
       t.a_mn = t.b_mn = t.a_stream = false;
       t.bn = bn;
+      t.a_rows = mm::kRows;
       t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == ntt - 1 ? kLast : 0) | (x == lo ? kBegin : 0) |
                 (x == hi - 1 ? kEnd : 0);
       ++x;
@@ -521,6 +522,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
                                         int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream) {
   int rc = check_texts(vw, L, "sparse_head backward");
   if (rc) return rc;
+  if ((rc = check_grads(vw, d_hidden, d_weight, "sparse_head backward"))) return rc;
   const State s = carve_state(state, vw->T, vw->V, vw->D, 0, false);
   const Bwd b = carve_bwd(ws, vw);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,

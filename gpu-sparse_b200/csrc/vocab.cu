@@ -124,8 +124,8 @@ __global__ void __launch_bounds__(256) copy_weight_kernel(const uint16_t* w, int
 // number of steps, and a tile cut by a border is finished from its fp32 fragments by
 // frag_kernel, in list order.  Pairs are dealt to the 256-wide tiles of D in turn, so that the
 // pairs that read the same rows of P run side by side.
-constexpr int kPadBytes = 32 * 33 * 4;      // a warp's 32 x 32 block
-constexpr int kTileCost = 3;      // steps an epilogue counts for in the cut
+constexpr int kOutBytes = 32 * 128;    // a warp's 32 rows x 64 columns of dW on their way out
+constexpr int kTileCost = 3;           // steps an epilogue counts for in the cut
 
 struct GradList {
   int32_t nh, nw, nkh, nkw;       // tiles of each kind along this D tile, steps of each
@@ -146,15 +146,16 @@ struct GradList {
 };
 
 struct GradJob {
-  static constexpr int kStages = 6, kScratch = mm::kEpiWarps * kPadBytes;
-  CUtensorMap maps[4];       // P K-major, P MN-major, W MN-major, H MN-major
+  static constexpr int kStages = 6, kScratch = mm::kEpiWarps * kOutBytes;
+  CUtensorMap maps[5];       // P K-major, P MN-major, W MN-major, H MN-major; dW as 32 x 64 boxes
   int32_t wait_limit, bf16;
   const int32_t* n_rows;
   const int32_t* map;
   int32_t D, nbs;            // 256-wide tiles of D
   int32_t v0, cols, V;
   int32_t first, last;
-  bool want_h, want_w, vec_h, vec_w;
+  bool want_h, want_w;
+  int64_t ld_out;            // of dh and dw
   float* dh_acc;
   int32_t ld_acc;
   float* frag;               // [pairs][2: begun elsewhere, ends elsewhere][2 CTAs][128][256]
@@ -172,7 +173,7 @@ struct GradJob {
     return frag + ((int64_t(pair) * 2 + ends_elsewhere) * 2 + rank) * mm::kRows * mm::kBN;
   }
 
-  static constexpr int kIsH = 1, kFrag = 2, kEndsElsewhere = 4;
+  static constexpr int kIsH = 1, kFrag = 2, kEndsElsewhere = 4, kEnd = 8;
   struct Walk {
     GradList l;
     int64_t x, x1;
@@ -198,6 +199,7 @@ struct GradJob {
         t.bn = D - t.b0 > 128 ? 256 : 128;
         t.a0 = blk * mm::kBM;
         t.ak = k0 * mm::kBK;
+        t.a_rows = mm::kRows;
         t.b_mn = true;
         t.a = is_h ? 0 : 1;
         t.b = is_h ? 2 : 3;
@@ -207,7 +209,8 @@ struct GradJob {
         t.nk = k1 - k0;
         t.x = blk;
         t.y = nb;
-        t.flags = (is_h ? kIsH : 0) | (k0 > 0 || k1 < nk ? kFrag : 0) | (k1 < nk && k0 == 0 ? kEndsElsewhere : 0);
+        t.flags = (is_h ? kIsH : 0) | (k0 > 0 || k1 < nk ? kFrag : 0) | (k1 < nk && k0 == 0 ? kEndsElsewhere : 0) |
+                  (x >= x1 && nb + nb_step >= nbs ? kEnd : 0);
         return true;
       }
     }
@@ -223,12 +226,9 @@ struct GradJob {
 
   // 8 columns from c of a finished row: r a packed row (dH) or a vocabulary row of the piece (dW)
   __device__ void finish8(bool is_h, int32_t r, int32_t c, float (&v)[8]) const {
-    if (c >= D) return;
     uint16_t* out;
-    bool vec;
     const float sc = scale ? *scale : 1.0f;
     if (is_h) {
-      if (r >= *n_rows) return;
       float* acc = dh_acc + int64_t(r) * ld_acc + c;
       if (!first) {
 #pragma unroll
@@ -239,92 +239,82 @@ struct GradJob {
         for (int k = 0; k < 8; ++k) acc[k] = v[k];
         return;
       }
-      out = dh + int64_t(map[r]) * D + c;
-      vec = vec_h;
+      out = dh + int64_t(map ? map[r] : r) * ld_out + c;
     } else {
-      if (r >= cols) return;
-      out = dw + int64_t(v0 + r) * D + c;
-      vec = vec_w;
+      out = dw + int64_t(v0 + r) * ld_out + c;
     }
     const bool bf = bf16 != 0;
-    uint4 o;
-    uint32_t* u = &o.x;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) u[k] = pack2(v[2 * k] * sc, v[2 * k + 1] * sc, bf);
-    if (vec) {
-      *reinterpret_cast<uint4*>(out) = o;
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        if (c + k < D) out[k] = uint16_t(u[k >> 1] >> (16 * (k & 1)));
-      }
-    }
+    *reinterpret_cast<uint4*>(out) = make_uint4(pack2(v[0] * sc, v[1] * sc, bf), pack2(v[2] * sc, v[3] * sc, bf),
+                                                pack2(v[4] * sc, v[5] * sc, bf), pack2(v[6] * sc, v[7] * sc, bf));
   }
 
   struct Epi {
     bool is_h, live;
-    uint16_t* row;
+    uint16_t* row;         // of dH
     float sc;
     __device__ void begin(const GradJob& j, const mm::Tile& t, const mm::Acc& a) {
       is_h = t.flags & kIsH;
       live = is_h ? a.row < *j.n_rows : a.row < j.cols;
       row = nullptr;
-      if (live) row = is_h ? j.dh + int64_t(j.map[a.row]) * j.D : j.dw + int64_t(j.v0 + a.row) * j.D;
+      if (live && is_h) row = j.dh + int64_t(j.map ? j.map[a.row] : a.row) * j.ld_out;
       sc = j.scale ? *j.scale : 1.0f;
     }
     __device__ void tile(const GradJob& j, const mm::Tile& t, const mm::Acc& a) {
-      const bool bf = j.bf16 != 0, vec = is_h ? j.vec_h : j.vec_w;
+      const bool bf = j.bf16 != 0;
       float* acc = j.dh_acc + int64_t(a.row) * j.ld_acc;
       float* frag = j.fragment(int32_t(blockIdx.x) >> 1, (t.flags & kEndsElsewhere) != 0, a.rank) + a.lane_row * mm::kBN;
+      unsigned char* out = a.scratch + a.warp * kOutBytes;
       for (int32_t c = a.c_lo; c < a.c_hi; c += 32) {
         float v[32];
         a.ld32(c, v);
         if (c + 32 == a.c_hi) a.release();
         uint32_t* u = reinterpret_cast<uint32_t*>(v);
         const int32_t d0 = t.b0 + c;
-        if (d0 >= j.D) continue;
         if (t.flags & kFrag) {
-          if (!live) continue;
+          if (live && d0 < j.D) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) st256(frag + c + 8 * q, u + 8 * q);
-          continue;
-        }
-        if (is_h && !j.first && live) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t o[8];
-            ld256(acc + d0 + 8 * q, o);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[8 * q + k] += __uint_as_float(o[k]);
+            for (int q = 0; q < 4; ++q) st256(frag + c + 8 * q, u + 8 * q);
           }
-        }
-        if (is_h && !j.last) {
-          if (!live) continue;
+        } else if (is_h) {
+          if (!live || d0 >= j.D) continue;
+          if (!j.first) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) st256(acc + d0 + 8 * q, u + 8 * q);
-          continue;
-        }
+            for (int q = 0; q < 4; ++q) {
+              uint32_t o[8];
+              ld256(acc + d0 + 8 * q, o);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] *= sc;
-        if (vec) {
-          if (live) store_row16(row, d0, j.D, v, bf);
+              for (int k = 0; k < 8; ++k) v[8 * q + k] += __uint_as_float(o[k]);
+            }
+          }
+          if (!j.last) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) st256(acc + d0 + 8 * q, u + 8 * q);
+            continue;
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] *= sc;
+          store_row16(row, d0, int32_t(j.ld_out), v, bf);
         } else {
-          // rows that start anywhere: the warp's block is turned in shared memory, so that a
-          // store has the 32 columns of one row and not one column of 32 rows
-          float* block = reinterpret_cast<float*>(a.scratch + a.warp * kPadBytes);
-          __syncwarp();
+          // half a 128-byte row at a time, 16-byte pieces swizzled as the map wants them; the
+          // map cuts off what lies past dW's rows and columns
+          if ((c & 32) == 0) {
+            if (a.lane == 0) mm::tma_store_wait_read();
+            __syncwarp();
+          }
 #pragma unroll
-          for (int k = 0; k < 32; ++k) block[a.lane * 33 + k] = v[k];
-          __syncwarp();
-          const uint64_t mine = reinterpret_cast<uint64_t>(row);
-#pragma unroll 4
-          for (int q = 0; q < 32; ++q) {
-            uint16_t* to = reinterpret_cast<uint16_t*>(__shfl_sync(FULL, mine, q));
-            const float x = block[q * 33 + a.lane];
-            if (to && d0 + a.lane < j.D) to[d0 + a.lane] = uint16_t(pack2(x, 0.0f, bf));
+          for (int q = 0; q < 4; ++q)
+            reinterpret_cast<uint4*>(out + a.lane * 128)[(((c & 32) >> 3) + q) ^ (a.lane & 7)] =
+                make_uint4(pack2(v[8 * q] * sc, v[8 * q + 1] * sc, bf), pack2(v[8 * q + 2] * sc, v[8 * q + 3] * sc, bf),
+                           pack2(v[8 * q + 4] * sc, v[8 * q + 5] * sc, bf), pack2(v[8 * q + 6] * sc, v[8 * q + 7] * sc, bf));
+          if (c & 32) {
+            mm::fence_async();
+            __syncwarp();
+            const int32_t x = d0 - 32, y = j.v0 + a.row;
+            if (a.lane == 0 && x < j.D && y < j.V) mm::tma_store_2d(&j.maps[4], out, x, y);
           }
         }
       }
+      if ((t.flags & kEnd) && a.lane == 0) mm::tma_store_wait();
     }
   };
   __device__ Epi epi() const { return Epi{}; }
@@ -374,7 +364,7 @@ finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blo
   const int32_t first = int32_t(((start + 1) * groups - 1) / tot);   // the share that holds the tile's first step
   const int32_t rank = sub & 1, row = (sub >> 1) * 8 + (threadIdx.x >> 5), c = lane_id() * 8;
   const int32_t r = blk * mm::kBM + rank * mm::kRows + row;
-  if (r >= (is_h ? *j.n_rows : j.cols) || nb * mm::kBN + c >= j.D) return;
+  if (r >= (is_h ? *j.n_rows : j.cols) || nb * mm::kBN + c >= j.D) return;      // (D up to ld_out is padding)
   float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (int32_t s = first; s <= g; ++s) {
@@ -505,11 +495,44 @@ int64_t piece_cols(int64_t Tp, int64_t V) {
   return up((all + pieces - 1) / pieces, kRowPad);
 }
 
+// Gradient rows are stored in whole 32-byte pieces; rows of any other width are made in a padded
+// copy, which one more kernel unpacks.
+int check_grads(const gsp_vocab_view* vw, const void* d_hidden, const void* d_weight, const char* what) {
+  GSP_REQUIRE(vw->D % 16 != 0 || ((reinterpret_cast<uintptr_t>(d_hidden) | reinterpret_cast<uintptr_t>(d_weight)) & 31) == 0,
+              GSP_ERR_ARG, "%s: d_hidden and d_weight must start on 32-byte boundaries", what);
+  return GSP_OK;
+}
+
 GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t pitch) {
   GradScratch g{};
+  const int64_t ld = up(vw->D, 16);
   g.dh_acc = c.take<float>(pitch < vw->V ? Tp * up(vw->D, 32) : 0);
   g.frag = c.take<float>(int64_t(mm::pair_ctas()) * 2 * mm::kRows * mm::kBN);
+  g.dh = c.take<uint16_t>(vw->D % 16 ? Tp * ld : 0);
+  g.dw = c.take<uint16_t>(vw->D % 16 ? vw->V * ld : 0);
   return g;
+}
+
+// rows of ld 16-bit values -> rows of D at out (map: where each row goes); a warp per row
+__global__ void __launch_bounds__(256)
+unpad_kernel(const uint16_t* dh, const int32_t* n_rows, const int32_t* map, uint16_t* out_h, int64_t h_blocks,
+             const uint16_t* dw, int64_t V, uint16_t* out_w, int64_t ld, int64_t D) {
+  const int lane = lane_id();
+  const int64_t warp = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const uint16_t* src;
+  uint16_t* dst;
+  if (blockIdx.x < h_blocks) {
+    if (warp >= *n_rows) return;
+    src = dh + warp * ld;
+    dst = out_h + int64_t(map[warp]) * D;
+  } else {
+    const int64_t r = warp - h_blocks * 8;
+    if (r >= V) return;
+    src = dw + r * ld;
+    dst = out_w + r * D;
+  }
+#pragma unroll 8
+  for (int64_t i = lane; i < D; i += 32) dst[i] = src[i];
 }
 
 int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, int64_t ldw, const GradPiece& pc,
@@ -518,6 +541,11 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   GradJob j{};
   const bool bf = is_bf16(vw);
   int rc;
+  const bool padded = vw->D % 16 != 0;
+  uint16_t* dh = padded && d_hidden ? g.dh : static_cast<uint16_t*>(d_hidden);
+  uint16_t* dw = padded && d_weight ? g.dw : static_cast<uint16_t*>(d_weight);
+  j.ld_out = up(vw->D, 16);
+  if (dw && (rc = make_map(&j.maps[4], bf, dw, j.ld_out, vw->V, j.ld_out, 32))) return rc;
   if ((rc = make_map(&j.maps[0], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kRows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kBK))) return rc;
   if ((rc = make_map(&j.maps[2], bf, w, vw->D, vw->V, ldw, mm::kBK))) return rc;
@@ -525,7 +553,7 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.n_rows = s.head;
-  j.map = s.map;
+  j.map = padded ? nullptr : s.map;
   j.D = int32_t(vw->D);
   j.nbs = int32_t((vw->D + mm::kBN - 1) / mm::kBN);
   j.v0 = int32_t(pc.v0);
@@ -535,22 +563,27 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.last = pc.last;
   j.want_h = d_hidden != nullptr;
   j.want_w = d_weight != nullptr;
-  j.vec_h = vw->D % 16 == 0 && (reinterpret_cast<uintptr_t>(d_hidden) & 31) == 0;
-  j.vec_w = vw->D % 16 == 0 && (reinterpret_cast<uintptr_t>(d_weight) & 31) == 0;
   j.dh_acc = g.dh_acc;
   j.ld_acc = int32_t(up(vw->D, 32));
   j.frag = g.frag;
   j.scale = scale;
-  j.dh = static_cast<uint16_t*>(d_hidden);
-  j.dw = static_cast<uint16_t*>(d_weight);
+  j.dh = dh;
+  j.dw = dw;
   if ((d_hidden || d_weight) && (rc = mm::launch(j, st))) return rc;
   const int32_t pairs = mm::pair_ctas() / 2;
   // with more D tiles than pairs no tile is cut
   const int32_t frag_blocks = (d_hidden || d_weight) && j.nbs <= pairs ? pairs * (2 * mm::kRows / 8) : 0;
   const int32_t blocks = frag_blocks + (bias.out ? int32_t((pc.cols + 31) / 32) : 0);
-  if (blocks == 0) return GSP_OK;
-  finish_kernel<<<unsigned(blocks), 256, 0, st>>>(j, pairs, frag_blocks, bias);
-  GSP_CHECK_LAUNCH();
+  if (blocks > 0) {
+    finish_kernel<<<unsigned(blocks), 256, 0, st>>>(j, pairs, frag_blocks, bias);
+    GSP_CHECK_LAUNCH();
+  }
+  if (padded && pc.last && (d_hidden || d_weight)) {
+    const int64_t hb = d_hidden ? (vw->T + 7) / 8 : 0, wb = d_weight ? (vw->V + 7) / 8 : 0;
+    unpad_kernel<<<unsigned(hb + wb), 256, 0, st>>>(dh, s.head, s.map, static_cast<uint16_t*>(d_hidden), hb, dw, vw->V,
+                                                   static_cast<uint16_t*>(d_weight), j.ld_out, vw->D);
+    GSP_CHECK_LAUNCH();
+  }
   return GSP_OK;
 }
 

@@ -45,6 +45,7 @@ constexpr int32_t kNoId = 0x7FFFFFFF;
 State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool loss);
 
 int check_view(const gsp_vocab_view* vw, const char* what);
+int check_grads(const gsp_vocab_view* vw, const void* d_hidden, const void* d_weight, const char* what);
 inline bool is_bf16(const gsp_vocab_view* vw) { return vw->dtype == GSP_W_BF16; }
 // bytes of the copy of W that a projection whose rows a TMA map cannot describe needs (else 0)
 int64_t weight_copy_bytes(const gsp_vocab_view* vw);
@@ -73,6 +74,7 @@ struct GradPiece {
 struct GradScratch {
   float* dh_acc;      // [Tp, up(D, 32)], or null when there is one piece
   float* frag;        // partial tiles
+  uint16_t *dh, *dw;  // gradient rows padded to 16 columns, when D is not a multiple of 16
 };
 GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t pitch);
 // column sums of the piece's unrounded P for every 128 rows [row blocks][pitch], and where
@@ -136,14 +138,14 @@ __device__ __forceinline__ void ld256(const void* p, uint32_t* r) {
                : "l"(p)
                : "memory");
 }
-// 32 accumulators of one row -> 16-bit, columns c0 .. min(c0 + 32, D); the row starts on a
-// 32-byte boundary and D is a multiple of 16
-__device__ __forceinline__ void store_row16(uint16_t* row, int32_t c0, int32_t D, const float (&v)[32], bool bf16) {
+// 32 accumulators of one row -> 16-bit, columns c0 .. min(c0 + 32, ld); the row starts on a
+// 32-byte boundary and ld is a multiple of 16
+__device__ __forceinline__ void store_row16(uint16_t* row, int32_t c0, int32_t ld, const float (&v)[32], bool bf16) {
   uint32_t w[16];
 #pragma unroll
   for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
   st256(row + c0, w);
-  if (c0 + 16 < D) st256(row + c0 + 16, w + 8);
+  if (c0 + 16 < ld) st256(row + c0 + 16, w + 8);
 }
 // two fp32 operations per instruction (sm_100a)
 struct F2 {

@@ -236,15 +236,17 @@ struct LossJob {
   const int32_t* head;
   const int32_t* map;
   int32_t nt, nk;           // tiles along the vocabulary, steps along D
+  int32_t a_rows;
   float c;
   const float* bias2;
   Lists lists;
   float* part;              // [pairs + row blocks][kPart]
 
   struct Walk {
-    int32_t lo, x, hi, nt, nk;
+    int32_t lo, x, hi, nt, nk, a_rows;
     __device__ bool next(mm::Tile& t) {
       if (x >= hi) return false;
+      t.a_rows = a_rows;
       t.x = x / nt;
       t.y = x - t.x * nt;
       t.a = 0, t.b = 1;
@@ -261,7 +263,7 @@ struct LossJob {
   };
   __device__ Walk walk(int32_t pair, int32_t pairs) const {
     const int32_t tot = (head[0] + mm::kBM - 1) / mm::kBM * nt, lo = share_lo(tot, pairs, pair);
-    return Walk{lo, lo, share_lo(tot, pairs, pair + 1), nt, nk};
+    return Walk{lo, lo, share_lo(tot, pairs, pair + 1), nt, nk, a_rows};
   }
 
   struct Epi {
@@ -479,6 +481,7 @@ struct LogitGradJob {
   const int32_t* head;
   const int32_t* map;
   int32_t nk, v0, nt;       // the piece's first vocabulary row and 256-wide tiles
+  int32_t a_rows;
   float c;
   const float *bias2, *lse2, *ga;
   Lists lists;
@@ -488,9 +491,10 @@ struct LogitGradJob {
   // the same shares along the vocabulary as the forward pass, so that a row's entries are found
   // once per share
   struct Walk {
-    int32_t lo, x, hi, nt, nk, v0;
+    int32_t lo, x, hi, nt, nk, v0, a_rows;
     __device__ bool next(mm::Tile& t) {
       if (x >= hi) return false;
+      t.a_rows = a_rows;
       t.x = x / nt;
       t.y = x - t.x * nt;
       t.a = 0, t.b = 1;
@@ -507,7 +511,7 @@ struct LogitGradJob {
   };
   __device__ Walk walk(int32_t pair, int32_t pairs) const {
     const int32_t tot = (head[0] + mm::kBM - 1) / mm::kBM * nt, lo = share_lo(tot, pairs, pair);
-    return Walk{lo, lo, share_lo(tot, pairs, pair + 1), nt, nk, v0};
+    return Walk{lo, lo, share_lo(tot, pairs, pair + 1), nt, nk, v0, a_rows};
   }
 
   struct Epi {
@@ -660,6 +664,10 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
   return b;
 }
 
+// Rows of a box of H: up to 128 tokens no more than there are (a single token's product would
+// else spend as long on rows of nothing as on the vocabulary)
+int32_t box_rows(int64_t T) { return int32_t(T >= mm::kRows ? mm::kRows : up(T, 8)); }
+
 int check_reduction(int32_t reduction, const char* what) {
   GSP_REQUIRE(reduction >= GSP_REDUCE_NONE && reduction <= GSP_REDUCE_MEAN, GSP_ERR_ARG, "%s: unknown reduction %d", what,
               reduction);
@@ -675,7 +683,8 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Li
   if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
   LossJob<kList> j{};
   const bool bf = is_bf16(vw);
-  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, vw->T, s.Dp, mm::kRows))) return rc;
+  j.a_rows = box_rows(vw->T);
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, j.a_rows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
@@ -704,7 +713,8 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
   if ((rc = weight_rows(vw, b.wcopy, &w, &ldw, st))) return rc;
   LogitGradJob<kList> j{};
   const bool bf = is_bf16(vw);
-  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, vw->T, s.Dp, mm::kRows))) return rc;
+  j.a_rows = box_rows(vw->T);
+  if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, j.a_rows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
@@ -810,6 +820,7 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   int rc = check_view(vw, "vocab loss backward");
   if (rc) return rc;
   if ((rc = check_reduction(reduction, "vocab loss backward"))) return rc;
+  if ((rc = check_grads(vw, d_hidden, d_weight, "vocab loss backward"))) return rc;
   GSP_REQUIRE(kind == GSP_VOCAB_CE || kind == GSP_VOCAB_DISTILL, GSP_ERR_ARG, "vocab loss backward: unknown kind %d", kind);
   const bool list = kind == GSP_VOCAB_DISTILL;
   GSP_REQUIRE(!list || (K >= 1 && K <= GSP_DISTILL_MAX_K && tau > 0.0f && tau < __builtin_inff()), GSP_ERR_ARG,

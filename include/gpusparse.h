@@ -398,9 +398,10 @@ int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, const int64
 /* Gradients of either loss from the state its forward call left (vw with the same sizes and
  * weight; hidden unused): d_hidden [T, D] and d_weight [V, D] in dtype, d_bias fp32 [V], each
  * contiguous and each optional (NULL).  grad_loss: fp32, one value, or [T] with
- * GSP_REDUCE_NONE.  K and tau are the forward call's, for GSP_VOCAB_DISTILL.  The softmax is computed again, for a piece of the vocabulary at a time
- * (at most 512 MiB of ws); its gradient is rounded to dtype as an operand of the two
- * products that follow. */
+ * GSP_REDUCE_NONE.  K and tau are the forward call's, for GSP_VOCAB_DISTILL.  d_hidden and
+ * d_weight start on 32-byte boundaries when D is a multiple of 16.  The softmax is computed
+ * again, for a piece of the vocabulary at a time (at most 512 MiB of ws); its gradient is
+ * rounded to dtype as an operand of the two products that follow. */
 int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, int64_t K, float tau, int32_t reduction,
                             const float* grad_loss, void* d_hidden, void* d_weight, float* d_bias,
                             void* state, int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream);

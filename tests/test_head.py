@@ -83,6 +83,9 @@ def test_bad_calls_are_refused_before_any_launch():
     assert lib.gsp_vocab_loss_backward(ref, L.VOCAB_HEAD, 0, 1.0, 2, fake, fake, fake, fake, fake, big, fake, big, None) == E
     assert lib.gsp_vocab_loss_backward(ref, L.VOCAB_CE, 0, 1.0, 2, fake, fake, fake, fake, fake, sb, fake, bb - 1, None) == E
     assert lib.gsp_vocab_loss_backward(ref, L.VOCAB_CE, 0, 1.0, 2, None, fake, fake, fake, fake, sb, fake, bb, None) == E
+    odd = ctypes.c_void_p(4096 + 16)                    # gradients that are not 32-byte aligned
+    assert lib.gsp_vocab_loss_backward(ref, L.VOCAB_CE, 0, 1.0, 2, fake, odd, fake, fake, fake, sb, fake, bb, None) == E
+    assert lib.gsp_sparse_head_backward(ref, 10, fake, fake, fake, fake, odd, fake, fake, big, fake, big, None) == E
     assert lib.gsp_sparse_head(ref, 0, None, fake, None, fake, big, fake, big, None) == E
     assert lib.gsp_sparse_head(ref, 33, None, fake, None, fake, big, fake, big, None) == E      # 100 tokens
     assert lib.gsp_sparse_head(ref, 10, None, None, None, fake, big, fake, big, None) == E
