@@ -458,7 +458,7 @@ int check_texts(const gsp_vocab_view* vw, int64_t L, const char* what) {
 int64_t head_ws_bytes(const gsp_vocab_view* vw, bool backward) {
   return backward ? carve_bwd(nullptr, vw).bytes : carve_fwd(nullptr, vw).bytes;
 }
-int64_t loss_ws_bytes(const gsp_vocab_view* vw, bool backward);
+int64_t loss_ws_bytes(const gsp_vocab_view* vw, int64_t K, bool backward);
 
 }  // namespace vocab
 }  // namespace gsp
@@ -466,14 +466,14 @@ int64_t loss_ws_bytes(const gsp_vocab_view* vw, bool backward);
 using namespace gsp;
 using namespace gsp::vocab;
 
-extern "C" int64_t gsp_vocab_ws_bytes(const gsp_vocab_view* vw, int32_t kind, int32_t backward) {
+extern "C" int64_t gsp_vocab_ws_bytes(const gsp_vocab_view* vw, int64_t K, int32_t kind, int32_t backward) {
   const int rc = check_view(vw, "gsp_vocab_ws_bytes");
   if (rc) return -rc;
-  if (kind < GSP_VOCAB_CE || kind > GSP_VOCAB_HEAD) {
-    set_error("gsp_vocab_ws_bytes: unknown kind %d", kind);
+  if (kind < GSP_VOCAB_CE || kind > GSP_VOCAB_HEAD || K < 0) {
+    set_error("gsp_vocab_ws_bytes: bad arguments");
     return -GSP_ERR_ARG;
   }
-  return kind == GSP_VOCAB_HEAD ? head_ws_bytes(vw, backward != 0) : loss_ws_bytes(vw, backward != 0);
+  return kind == GSP_VOCAB_HEAD ? head_ws_bytes(vw, backward != 0) : loss_ws_bytes(vw, kind == GSP_VOCAB_DISTILL ? K : 0, backward != 0);
 }
 
 extern "C" int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_t* mask, float* y, int32_t* win, void* state,

@@ -393,12 +393,13 @@ State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool l
     s.tgt = c.take<int32_t>(K > 0 ? 0 : s.Tp);
   }
   if (K > 0) {
-    s.cnt = c.take<int32_t>(T);
-    s.ent = c.take<float>(T);
-    s.Kp = up(K, 4);
-    s.ids = c.take<int32_t>(T * s.Kp + 4);      // a row is read four entries at a time, and one
-    s.p = c.take<float>(T * s.Kp + 4);          // four ahead
-    s.flag = c.take<uint8_t>(T);
+    s.K = K;
+    s.hit = c.take<int4>(s.Tp * K);
+    // half a tile per bucket, more where that would be more buckets than fit the sort
+    s.bucket_shift = 7;
+    while ((s.Vp >> s.bucket_shift) > 8192) ++s.bucket_shift;
+    s.buckets = (s.Vp + (int64_t(1) << s.bucket_shift) - 1) >> s.bucket_shift;
+    s.off = c.take<int32_t>(s.Tp / 32 * (s.buckets + 1));
   }
   s.bytes = c.off;
   return s;

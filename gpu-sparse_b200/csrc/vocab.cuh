@@ -34,12 +34,11 @@ struct State {
   float* bias2;       // [Vp] bias in units of the exponent's base 2, -inf past V (losses)
   float* lse2;        // [Tp] log2 of the softmax's denominator (losses)
   int32_t* tgt;       // [Tp] target of every packed row (cross entropy)
-  int32_t* cnt;       // [T] teacher entries of every row (distillation)
-  float* ent;         // [T] sum p log p (distillation)
-  int32_t* ids;       // [T, Kp] ascending, distinct, kNoId past a row's cnt (distillation)
-  float* p;           // [T, Kp] (distillation)
-  uint8_t* flag;      // [T] row takes part (distillation)
-  int64_t Tp, Dp, Vp, Kp, bytes;
+  int4* hit;          // a teacher's entries of every 32 packed rows by vocabulary bucket: (id, row
+                      // of the 32, probability's bits, entry of the row), 32 K a group
+  int32_t* off;       // [Tp / 32, buckets + 1] first hit of every bucket
+  int64_t Tp, Dp, Vp, K, buckets, bytes;
+  int32_t bucket_shift;      // log2 of a bucket's vocabulary rows
 };
 constexpr int32_t kNoId = 0x7FFFFFFF;
 State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool loss);

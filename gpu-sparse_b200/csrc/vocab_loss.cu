@@ -32,10 +32,22 @@ constexpr int kFirst = 1, kLast = 2;
 
 struct Lists {             // target entries
   const int32_t* tgt;      // cross entropy: one per packed row
-  const int32_t* cnt;      // distillation: by original row
-  const int32_t* ids;
-  const float* p;
-  int64_t Kp;
+  const int4* hit;         // distillation (see State)
+  const int32_t* off;
+  float* pz;               // distillation, forward (see Teacher)
+  int64_t K, buckets;
+  int32_t shift;
+};
+Lists lists_of(const State& s, bool list, float* pz) {
+  return list ? Lists{nullptr, s.hit, s.off, pz, s.K, s.buckets, s.bucket_shift} : Lists{s.tgt, nullptr, nullptr, nullptr, 0, 0, 0};
+}
+// A teacher's rows while the forward pass works on them (null for cross entropy).
+struct Teacher {
+  int32_t* cnt;       // [T] entries of every row
+  float* ent;         // [T] sum p log p
+  int2* entry;        // [T, K] (id, probability's bits), ids distinct
+  float* pz;          // [Tp, K] by packed row: probability x logit of every entry
+  uint8_t* flag;      // [T] row takes part
 };
 
 // ---- distillation: a teacher row's probabilities, sorted by id, duplicates joined --------
@@ -43,7 +55,7 @@ struct Lists {             // target entries
 template <int kSortThreads>
 __global__ void __launch_bounds__(kSortThreads)
 teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_ids, int32_t K, int32_t pow2, int64_t V,
-               float inv_tau, State s) {
+               float inv_tau, const Teacher s) {
   extern __shared__ uint64_t key[];              // [pow2] (id << 32 | entry), then p [pow2]
   float* p = reinterpret_cast<float*>(key + pow2);
   __shared__ float red[kSortThreads / 32];
@@ -123,13 +135,8 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
     __syncthreads();
     if (head) {
       at += __popc(w & lanemask_lt());
-      s.ids[t * s.Kp + at] = int32_t(k >> 32);
-      s.p[t * s.Kp + at] = q;
+      s.entry[t * K + at] = make_int2(int32_t(k >> 32), __float_as_int(q));
     }
-  }
-  for (int64_t i = n + tid; i < s.Kp; i += kSortThreads) {
-    s.ids[t * s.Kp + i] = kNoId;
-    s.p[t * s.Kp + i] = 0.0f;
   }
   ent = reduce(ent, false);
   if (tid == 0) {
@@ -139,64 +146,88 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
   }
 }
 
-// Walks a row's ascending entries as the tiles pass.  Entries come four at a time, and the
-// next four are on their way while these are used: a load per entry would cost its latency on
-// the spot.
-struct Cursor {
-  const int4* ids;      // the four after the next
-  const float4* ps;
-  int4 id, id2;         // shifted down as they are used; the next four
-  float4 p, p2;
-  int32_t left;         // of the four in id
-  __device__ void start(const Lists& l, int64_t orig, bool live, int32_t v0) {
-    left = 4;
-    id = id2 = make_int4(kNoId, kNoId, kNoId, kNoId);
-    p = p2 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    ids = nullptr;
-    if (!live) return;
-    const int32_t* row = l.ids + orig * l.Kp;
-    int32_t lo = 0, hi = l.cnt[orig];       // first entry with id >= v0
-    while (lo < hi) {
-      const int32_t mid = (lo + hi) >> 1;
-      if (row[mid] < v0) lo = mid + 1;
-      else hi = mid;
-    }
-    lo &= ~3;
-    if (lo >= l.cnt[orig]) return;
-    end = reinterpret_cast<const int4*>(row + l.Kp);
-    ids = reinterpret_cast<const int4*>(row + lo);
-    ps = reinterpret_cast<const float4*>(l.p + orig * l.Kp + lo);
-    id = *ids;
-    p = *ps;
-    fetch();
-    skip_to(v0);
+// The entries of 32 packed rows (one epilogue warp's) sorted into buckets of the vocabulary (half
+// a tile's columns), so that the warp finds those of its block side by side, however they are
+// spread over the rows.  A CTA per 32 rows.  The order inside a bucket is the atomics' and
+// shows nowhere: every entry has a place of its own in pz and in P.
+__global__ void __launch_bounds__(512) bucket_kernel(const State s, const Teacher tc) {
+  extern __shared__ int32_t count[];           // [buckets]
+  __shared__ int32_t part[16];
+  const int32_t n = s.head[0], r0 = int32_t(blockIdx.x) * 32, rows = min(32, n - r0);
+  if (rows <= 0) return;
+  const int32_t nb = int32_t(s.buckets), tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  for (int32_t b = tid; b < nb; b += 512) count[b] = 0;
+  __syncthreads();
+  for (int32_t r = wid; r < rows; r += 16) {
+    const int32_t orig = s.map[r0 + r], c = tc.cnt[orig];
+    for (int32_t i = lane; i < c; i += 32) atomicAdd(count + (tc.entry[orig * s.K + i].x >> s.bucket_shift), 1);
   }
-  __device__ void fetch() {
-    ++ids;
-    ++ps;
-    if (ids < end) {
-      id2 = *ids;
-      p2 = *ps;
-    } else {
-      id2.x = kNoId;
+  __syncthreads();
+  // exclusive scan, 512 buckets at a time
+  int32_t* off = s.off + int64_t(blockIdx.x) * (nb + 1);
+  int32_t base = 0;
+  for (int32_t b0 = 0; b0 < nb; b0 += 512) {
+    const int32_t b = b0 + tid;
+    const int32_t v = b < nb ? count[b] : 0;
+    int32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t u = __shfl_up_sync(FULL, x, o);
+      if (lane >= o) x += u;
     }
+    if (lane == 31) part[wid] = x;
+    __syncthreads();
+    int32_t before = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i < wid) before += part[i];
+      all += part[i];
+    }
+    if (b < nb) off[b] = count[b] = base + before + x - v;
+    base += all;
+    __syncthreads();
   }
-  __device__ int32_t next() const { return id.x; }
-  __device__ float prob() const { return p.x; }
-  __device__ void step() {
-    id.x = id.y, id.y = id.z, id.z = id.w;
-    p.x = p.y, p.y = p.z, p.z = p.w;
-    if (--left == 0) {
-      id = id2;
-      p = p2;
-      left = 4;
-      fetch();
+  if (tid == 0) off[nb] = base;
+  int4* hit = s.hit + int64_t(r0) * s.K;
+  for (int32_t r = wid; r < rows; r += 16) {
+    const int32_t orig = s.map[r0 + r], c = tc.cnt[orig];
+    for (int32_t i = lane; i < c; i += 32) {
+      const int2 e = tc.entry[orig * s.K + i];
+      hit[atomicAdd(count + (e.x >> s.bucket_shift), 1)] = make_int4(e.x, r, e.y, i);
     }
   }
-  __device__ void skip_to(int32_t v0) {      // entries of the other column half
-    while (next() < v0) step();
+}
+
+// The entries of a warp's 32 rows x half a tile; the first 32 (usually all) wait in registers,
+// one per lane, loaded while products run.
+struct Hits {
+  const int4* first;
+  int32_t n;
+  int4 e;
+  __device__ void load(const Lists& l, int32_t row0, int32_t rows, int32_t v0, int lane) {
+    n = 0;
+    e.x = kNoId;
+    if (row0 >= rows) return;
+    const int32_t* off = l.off + int64_t(row0 / 32) * (l.buckets + 1) + (v0 >> l.shift);
+    const int32_t h = off[0];
+    n = off[1] - h;
+    first = l.hit + int64_t(row0) * l.K + h;
+    if (lane < n) e = first[lane];
   }
-  const int4* end;
+  // f(entry, live) for every 32 entries of the bucket that have some in [v0, v0 + 32): every lane
+  // calls it
+  template <typename F>
+  __device__ void each(int32_t v0, int lane, F&& f) const {
+    for (int32_t i = 0; i < n; i += 32) {
+      int4 x = e;
+      if (i > 0) {
+        x.x = kNoId;
+        if (i + lane < n) x = first[i + lane];
+      }
+      const bool in = x.x >= v0 && x.x < v0 + 32;
+      if (__any_sync(FULL, in)) f(x, in);
+    }
+  }
 };
 
 // This tile's share of bias2 for one warp: loaded by begin() while the products run (a float4
@@ -226,7 +257,7 @@ __device__ __forceinline__ void to_z(const float (&v)[32], F2 c, const float* bi
 // along the list one of the two always grows).
 constexpr int kPart = 2 * 3 * mm::kBM;
 constexpr int kBiasScratch = mm::kEpiWarps * BiasTile::kBytes;
-constexpr int kListScratch = mm::kEpiWarps * 32 * 33 * 4;      // a padded 32 x 32 block per warp
+constexpr int kListScratch = mm::kEpiWarps * kBlockBytes;      // a 32 x 32 block per warp
 
 template <bool kList>
 struct LossJob {
@@ -269,7 +300,7 @@ struct LossJob {
   struct Epi {
     float m, l, dot;
     int32_t tgt;
-    Cursor cur;
+    Hits hits;
     __device__ float* bias(const mm::Acc& a) { return reinterpret_cast<float*>(a.scratch + a.warp * BiasTile::kBytes); }
     __device__ void begin(const LossJob& j, const mm::Tile& t, const mm::Acc& a) {
       const int32_t v0 = t.y * mm::kBN + a.c_lo;
@@ -277,11 +308,9 @@ struct LossJob {
       if (t.flags & kFirst) {
         m = neg_inf();
         l = dot = 0.0f;
-        const bool live = a.row < j.head[0];
-        if constexpr (kList) cur.start(j.lists, live ? j.map[a.row] : 0, live, v0);
-        else tgt = live ? j.lists.tgt[a.row] : -1;
+        if constexpr (!kList) tgt = a.row < j.head[0] ? j.lists.tgt[a.row] : -1;
       }
-      if constexpr (kList) cur.skip_to(v0);
+      if constexpr (kList) hits.load(j.lists, a.row - a.lane, j.head[0], v0, a.lane);
     }
     __device__ void tile(const LossJob& j, const mm::Tile& t, const mm::Acc& a) {
       const float* b = bias(a) - a.c_lo;
@@ -297,15 +326,18 @@ struct LossJob {
         for (int k = 0; k < 16; ++k) split(z2[k], z[2 * k], z[2 * k + 1]);
         const int32_t v0 = t.y * mm::kBN + c0;
         if constexpr (kList) {
-          if (__any_sync(FULL, cur.next() < v0 + 32)) {
-            float* mine = reinterpret_cast<float*>(a.scratch + kBiasScratch) + (a.warp * 32 + a.lane) * 33;   // no other lane's
-#pragma unroll
-            for (int k = 0; k < 32; ++k) mine[k] = z[k];
-            while (cur.next() < v0 + 32) {
-              dot = fmaf(cur.prob(), mine[cur.next() - v0], dot);
-              cur.step();
+          float* block = reinterpret_cast<float*>(a.scratch + kBiasScratch + a.warp * kBlockBytes);
+          float* pz = j.lists.pz + int64_t(a.row - a.lane) * j.lists.K;
+          bool put = false;
+          hits.each(v0, a.lane, [&](const int4& e, bool in) {
+            if (!put) {
+              __syncwarp();
+              block_put(block, z, a.lane);
+              __syncwarp();
+              put = true;
             }
-          }
+            if (in) pz[e.y * j.lists.K + e.w] = __int_as_float(e.z) * block[e.y * kBlockLd + e.x - v0];
+          });
         } else {
           const int32_t d = tgt - v0;
           if (d >= 0 && d < 32) {
@@ -363,8 +395,8 @@ struct RowSum {
   }
 };
 __global__ void __launch_bounds__(32 * kJoinRows)
-join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, int32_t pairs, const float* ent, float tau2,
-            int32_t reduction, float* lse2, double* sums, float* loss) {
+join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, int32_t pairs, const Teacher tc, int64_t K,
+            float tau2, int32_t reduction, float* lse2, double* sums, float* loss) {
   __shared__ double red[kJoinRows];
   __shared__ bool last;
   const int32_t n = head[0], wid = threadIdx.x >> 5, lane = lane_id();
@@ -373,7 +405,12 @@ join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, in
   if (r < n) {
     const int32_t tot = (n + mm::kBM - 1) / mm::kBM * nt;
     const int32_t c0 = share_of(tot, pairs, mb * nt), parts = 2 * (share_of(tot, pairs, (mb + 1) * nt - 1) + 1 - c0);
-    RowSum s{neg_inf(), 0.0f, 0.0f};
+    const int32_t orig = map[r];
+    RowSum t{neg_inf(), 0.0f, 0.0f};
+    if (tc.pz) {
+      const int32_t c = tc.cnt[orig];
+      for (int32_t i = lane; i < c; i += 32) t.dot += tc.pz[int64_t(r) * K + i];
+    }
     for (int32_t i0 = 0; i0 < parts; i0 += 160) {        // five loads of each kind in flight
       float pm[5], pl[5], pd[5];
 #pragma unroll
@@ -386,14 +423,13 @@ join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, in
         pd[k] = in ? o[2 * mm::kBM] : 0.0f;
       }
 #pragma unroll
-      for (int k = 0; k < 5; ++k) s.add(pm[k], pl[k], pd[k]);
+      for (int k = 0; k < 5; ++k) t.add(pm[k], pl[k], pd[k]);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1)
-      s.add(__shfl_xor_sync(FULL, s.m, o), __shfl_xor_sync(FULL, s.l, o), __shfl_xor_sync(FULL, s.dot, o));
-    const float z = s.m + log2f(s.l);
-    const int32_t orig = map[r];
-    const float v = tau2 * fmaf(z - s.dot, kLn2, ent ? ent[orig] : 0.0f);
+      t.add(__shfl_xor_sync(FULL, t.m, o), __shfl_xor_sync(FULL, t.l, o), __shfl_xor_sync(FULL, t.dot, o));
+    const float z = t.m + log2f(t.l);
+    const float v = tau2 * fmaf(z - t.dot, kLn2, tc.pz ? tc.ent[orig] : 0.0f);
     if (lane == 0) {
       lse2[r] = z;
       if (reduction == GSP_REDUCE_NONE) loss[orig] = v;
@@ -518,7 +554,7 @@ struct LogitGradJob {
     float lse, ga;
     int32_t tgt;
     bool live;
-    Cursor cur;
+    Hits hits;
     __device__ float* bias(const mm::Acc& a) { return reinterpret_cast<float*>(a.scratch + kBiasOff + a.warp * BiasTile::kBytes); }
     __device__ void begin(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
       const int32_t v0 = t.b0 + a.c_lo;
@@ -527,10 +563,9 @@ struct LogitGradJob {
         live = a.row < j.head[0];
         lse = j.lse2[a.row];
         ga = j.ga[a.row];
-        if constexpr (kList) cur.start(j.lists, live ? j.map[a.row] : 0, live, v0);
-        else tgt = live ? j.lists.tgt[a.row] : -1;
+        if constexpr (!kList) tgt = live ? j.lists.tgt[a.row] : -1;
       }
-      if constexpr (kList) cur.skip_to(v0);
+      if constexpr (kList) hits.load(j.lists, a.row - a.lane, j.head[0], v0, a.lane);
     }
     __device__ void tile(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
       unsigned char* out = a.scratch + a.warp * kOutBytes;
@@ -560,20 +595,25 @@ struct LogitGradJob {
         }
         bool staged = false;
         if constexpr (kList) {
-          if (__any_sync(FULL, cur.next() < v0 + 32)) {
-            __syncwarp();       // the column sums of the block before have been read
-            block_put(block, z, a.lane);
-            float* mine = block + a.lane * kBlockLd;
-            while (cur.next() < v0 + 32) {
-              mine[cur.next() - v0] = fmaf(-ga, cur.prob(), mine[cur.next() - v0]);
-              cur.step();
+          hits.each(v0, a.lane, [&](const int4& e, bool in) {
+            if (!staged) {
+              __syncwarp();       // the column sums of the block before have been read
+              block_put(block, z, a.lane);
+              staged = true;
             }
+            const float g = __shfl_sync(FULL, ga, e.y & 31);
+            __syncwarp();
+            float* at = block + (e.y & 31) * kBlockLd + (e.x - v0);
+            if (in) *at = fmaf(-g, __int_as_float(e.z), *at);
+          });
+          if (staged) {
+            __syncwarp();
+            const float* mine = block + a.lane * kBlockLd;
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
               const float4 x = *reinterpret_cast<const float4*>(mine + 4 * q);
               z[4 * q] = x.x, z[4 * q + 1] = x.y, z[4 * q + 2] = x.z, z[4 * q + 3] = x.w;
             }
-            staged = true;
           }
         } else {
           const int32_t d = tgt - v0;
@@ -629,15 +669,23 @@ struct Fwd {
   int32_t* counts;
   float* part;
   double* sums;
+  Teacher tc;
   void* wcopy;
   int64_t bytes;
 };
-Fwd carve_fwd(void* base, const gsp_vocab_view* vw) {
+Fwd carve_fwd(void* base, const gsp_vocab_view* vw, int64_t K) {
   Fwd f{};
   Carver c{static_cast<char*>(base)};
   f.counts = c.take<int32_t>(pack_counts(vw->T));
   f.part = c.take<float>((mm::pair_ctas() / 2 + pad_rows(vw->T) / mm::kBM) * kPart);
   f.sums = c.take<double>(pad_rows(vw->T) / kJoinRows);
+  if (K > 0) {
+    f.tc.cnt = c.take<int32_t>(vw->T);
+    f.tc.ent = c.take<float>(vw->T);
+    f.tc.entry = c.take<int2>(vw->T * K);
+    f.tc.pz = c.take<float>(pad_rows(vw->T) * K);
+    f.tc.flag = c.take<uint8_t>(vw->T);
+  }
   f.wcopy = c.take<char>(weight_copy_bytes(vw));
   f.bytes = c.off;
   return f;
@@ -675,8 +723,8 @@ int check_reduction(int32_t reduction, const char* what) {
 }
 
 template <bool kList>
-int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Lists& lists, float tau, int32_t reduction,
-                const float* ent, float* loss, cudaStream_t st) {
+int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, float tau, int32_t reduction, float* loss,
+                cudaStream_t st) {
   const uint16_t* w;
   int64_t ldw;
   int rc;
@@ -694,19 +742,19 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, const Li
   j.nk = int32_t((vw->D + mm::kBK - 1) / mm::kBK);
   j.c = kLog2e / tau;
   j.bias2 = s.bias2;
-  j.lists = lists;
+  j.lists = lists_of(s, kList, f.tc.pz);
   j.part = f.part;
   if ((rc = mm::launch(j, st))) return rc;
   if (reduction == GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, size_t(vw->T) * sizeof(float), st));
   join_kernel<<<unsigned((vw->T + kJoinRows - 1) / kJoinRows), 32 * kJoinRows, 0, st>>>(
-      s.head, s.map, f.part, j.nt, mm::pair_ctas() / 2, ent, tau * tau, reduction, s.lse2, f.sums, loss);
+      s.head, s.map, f.part, j.nt, mm::pair_ctas() / 2, f.tc, s.K, tau * tau, reduction, s.lse2, f.sums, loss);
   GSP_CHECK_LAUNCH();
   return GSP_OK;
 }
 
 template <bool kList>
-int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const Lists& lists, float tau, void* d_hidden,
-                 void* d_weight, float* d_bias, cudaStream_t st) {
+int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, float tau, void* d_hidden, void* d_weight,
+                 float* d_bias, cudaStream_t st) {
   const uint16_t* w;
   int64_t ldw;
   int rc;
@@ -725,7 +773,7 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
   j.bias2 = s.bias2;
   j.lse2 = s.lse2;
   j.ga = b.ga;
-  j.lists = lists;
+  j.lists = lists_of(s, kList, nullptr);
   if ((rc = make_map(&j.maps[2], bf, b.P, b.pitch, s.Tp, b.pitch, 32))) return rc;
   j.pitch = b.pitch;
   j.colpart = d_bias ? b.colpart : nullptr;
@@ -742,8 +790,8 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, const L
 
 }  // namespace
 
-int64_t loss_ws_bytes(const gsp_vocab_view* vw, bool backward) {
-  return backward ? carve_bwd(nullptr, vw).bytes : carve_fwd(nullptr, vw).bytes;
+int64_t loss_ws_bytes(const gsp_vocab_view* vw, int64_t K, bool backward) {
+  return backward ? carve_bwd(nullptr, vw).bytes : carve_fwd(nullptr, vw, K).bytes;
 }
 
 }  // namespace vocab
@@ -760,7 +808,7 @@ extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, in
   cudaStream_t st = as_stream(stream);
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "vocab_cross_entropy: null loss");
   const State s = carve_state(state, vw->T, vw->V, vw->D, 0, true);
-  const Fwd f = carve_fwd(ws, vw);
+  const Fwd f = carve_fwd(ws, vw, 0);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "vocab_cross_entropy: state or workspace too small");
   if (vw->T == 0) {
@@ -769,9 +817,7 @@ extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, in
   }
   GSP_REQUIRE(targets && vw->hidden && vw->weight, GSP_ERR_ARG, "vocab_cross_entropy: null input");
   if ((rc = pack_rows(vw, targets, ignore_index, nullptr, kLog2e, s, f.counts, st))) return rc;
-  Lists l{};
-  l.tgt = s.tgt;
-  return run_forward<false>(vw, s, f, l, 1.0f, reduction, nullptr, loss, st);
+  return run_forward<false>(vw, s, f, 1.0f, reduction, loss, st);
 }
 
 extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, const int64_t* ids, int64_t K, float tau,
@@ -786,7 +832,7 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   GSP_REQUIRE(tau > 0.0f && tau < __builtin_inff(), GSP_ERR_ARG, "topk_distillation: temperature must be positive");
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "topk_distillation: null loss");
   const State s = carve_state(state, vw->T, vw->V, vw->D, K, true);
-  const Fwd f = carve_fwd(ws, vw);
+  const Fwd f = carve_fwd(ws, vw, K);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "topk_distillation: state or workspace too small");
   if (vw->T == 0) {
@@ -797,20 +843,19 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   int32_t pow2 = 2;
   while (pow2 < K) pow2 <<= 1;
   const size_t sort_bytes = size_t(pow2) * 12;
-#define GSP_TEACHER(n) teacher_kernel<n><<<unsigned(vw->T), n, sort_bytes, st>>>(scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, s)
+#define GSP_TEACHER(n) teacher_kernel<n><<<unsigned(vw->T), n, sort_bytes, st>>>(scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, f.tc)
   if (pow2 <= 64) GSP_TEACHER(32);
   else if (pow2 <= 128) GSP_TEACHER(64);
   else if (pow2 <= 512) GSP_TEACHER(256);
   else GSP_TEACHER(512);
 #undef GSP_TEACHER
   GSP_CHECK_LAUNCH();
-  if ((rc = pack_rows(vw, nullptr, 0, s.flag, kLog2e / tau, s, f.counts, st))) return rc;
-  Lists l{};
-  l.cnt = s.cnt;
-  l.ids = s.ids;
-  l.p = s.p;
-  l.Kp = s.Kp;
-  return run_forward<true>(vw, s, f, l, tau, reduction, s.ent, loss, st);
+  if ((rc = pack_rows(vw, nullptr, 0, f.tc.flag, kLog2e / tau, s, f.counts, st))) return rc;
+  const int bucket_bytes = int(s.buckets * 4);
+  if ((rc = ensure_smem(reinterpret_cast<const void*>(&bucket_kernel), bucket_bytes))) return rc;
+  bucket_kernel<<<unsigned((vw->T + 31) / 32), 512, bucket_bytes, st>>>(s, f.tc);
+  GSP_CHECK_LAUNCH();
+  return run_forward<true>(vw, s, f, tau, reduction, loss, st);
 }
 
 extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, int64_t K, float tau, int32_t reduction,
@@ -843,14 +888,6 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   grad_rows_kernel<<<unsigned(1 + zero_blocks), 1024, 0, st>>>(s, grad_loss, reduction, tau, is_bf16(vw), b.ga, b.scale,
                                                               d_hidden, hidden_bytes);
   GSP_CHECK_LAUNCH();
-  Lists l{};
-  if (list) {
-    l.cnt = s.cnt;
-    l.ids = s.ids;
-    l.p = s.p;
-    l.Kp = s.Kp;
-    return run_backward<true>(vw, s, b, l, tau, d_hidden, d_weight, d_bias, st);
-  }
-  l.tgt = s.tgt;
-  return run_backward<false>(vw, s, b, l, tau, d_hidden, d_weight, d_bias, st);
+  return list ? run_backward<true>(vw, s, b, tau, d_hidden, d_weight, d_bias, st)
+              : run_backward<false>(vw, s, b, tau, d_hidden, d_weight, d_bias, st);
 }

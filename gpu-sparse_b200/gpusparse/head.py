@@ -82,7 +82,7 @@ def _sizes(T, V, D, ld_weight, aligned, K, kind, backward, device_index):
     lib = L.lib()
     v = L.VocabView(T, V, D, D, ld_weight, None, None if aligned else 2, None, L.W_BF16, 0)
     sb = lib.gsp_vocab_state_bytes(T, V, D, K, kind)
-    wb = lib.gsp_vocab_ws_bytes(ctypes.byref(v), kind, int(backward))
+    wb = lib.gsp_vocab_ws_bytes(ctypes.byref(v), K, kind, int(backward))
     if sb < 0 or wb < 0:
         L.check(int(-min(sb, wb)), "vocabulary head")
     return sb, wb

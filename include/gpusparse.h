@@ -372,14 +372,14 @@ typedef struct gsp_vocab_view {
 #define GSP_REDUCE_MEAN 2
 #define GSP_DISTILL_MAX_K 1024
 
-/* A forward call leaves in `state` (gsp_vocab_state_bytes; K = teacher entries per row, else
- * 0) what its backward call needs: the rows that took part, packed, their softmax
+/* A forward call leaves in `state` (gsp_vocab_state_bytes; K = teacher entries per row, 0 but
+ * for GSP_VOCAB_DISTILL) what its backward call needs: the rows that took part, packed, their softmax
  * denominators and the teacher's probabilities.  The caller's hidden and targets are not
  * read again.  ws is scratch of the one call (gsp_vocab_ws_bytes, backward 0 or 1); no call
  * allocates, synchronises or keeps anything else, so calls can be captured, and calls with
  * their own buffers can overlap.  Both functions return a negative status on error. */
 int64_t gsp_vocab_state_bytes(int64_t T, int64_t V, int64_t D, int64_t K, int32_t kind);
-int64_t gsp_vocab_ws_bytes(const gsp_vocab_view* vw, int32_t kind, int32_t backward);
+int64_t gsp_vocab_ws_bytes(const gsp_vocab_view* vw, int64_t K, int32_t kind, int32_t backward);
 
 /* Softmax cross entropy of every row whose target lies in [0, V) and is not ignore_index;
  * the other rows take no part (their hidden states are never used, whatever they hold).
