@@ -10,9 +10,15 @@
 // direction), and a text that a share's border cuts leaves its partial maxima for a joining
 // kernel.  Texts may so have any length, and no work is lost to their padding.
 //
-// Backward.  Each (text, term) with y > 0 sends ds = dy exp(-y) to its winning token; as a
-// matrix P [tokens, V] with one entry per (text, term) this is the shape of the losses'
-// gradient, and the same two products finish it.
+// Backward.  Each (text, term) with y > 0 sends ds = dy exp(-y) to its winning token:
+//   dH[win] += ds W[v],   dW[v] += ds H[win],   d_bias[v] += ds.
+// Term weights are sparse (a trained head keeps hundreds of 30522 terms), so these are sums of
+// few rows of W and H, gathered from L2 in a fixed order, fp32 throughout: dW takes a term's
+// texts one after the other, dH a list of the entries sorted by token (a counting sort that keeps
+// the order of the terms).  While a head is still dense over short texts (more than one entry in
+// kGatherWeight of tokens x vocabulary) the gathers would cost more than products: then P
+// [tokens, V] with one entry per (text, term) goes through the losses' two products.  The
+// entries are counted on the GPU and the kernels of the other way return at once.
 #include "vocab.cuh"
 
 namespace gsp {
@@ -253,55 +259,385 @@ __global__ void __launch_bounds__(mm::kBM) head_join_kernel(const JoinParams p) 
 }
 
 // ---- backward ----------------------------------------------------------------------------
-// largest finite |dy| (fp16: an upper bound of |ds|, which scales P)
-__global__ void __launch_bounds__(256) absmax_kernel(const float* dy, int64_t n, uint32_t* out) {
-  float m = 0.0f;
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
-    const float a = fabsf(dy[i]);
-    if (a < __uint_as_float(0x7F800000u)) m = fmaxf(m, a);
+struct Survey {
+  int64_t nnz;            // entries: (text, term) pairs with a gradient
+  uint32_t absmax;        // largest finite |dy| (an upper bound of |ds|, which scales fp16's P)
+  uint32_t pad_;
+};
+
+// ds of (text, term) pairs o[k] (negative: none) and their tokens' packed rows (-1: no gradient);
+// all loads are issued before the first is used
+template <int N>
+__device__ __forceinline__ void entry_grads(const float* y, const int32_t* win, const float* dy, const int64_t (&o)[N],
+                                            int32_t (&row)[N], float (&ds)[N]) {
+  float d[N], v[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    row[k] = o[k] >= 0 ? win[o[k]] : -1;
+    d[k] = o[k] >= 0 ? dy[o[k]] : 0.0f;
+    v[k] = o[k] >= 0 ? y[o[k]] : 0.0f;
   }
-  const uint32_t w = __reduce_max_sync(FULL, __float_as_uint(m));
-  if (lane_id() == 0 && w) atomicMax(out, w);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (d[k] == 0.0f) row[k] = -1;
+    ds[k] = row[k] >= 0 ? d[k] * expf(-v[k]) : 0.0f;
+  }
 }
 
-__global__ void __launch_bounds__(1024) tail_kernel(State s) { zero_tail_rows(s.h, s.Dp, s.head[0]); }
-
-struct SpreadParams {
-  const int32_t *head, *map;
+// The counting sort.  A warp takes one of kSegs runs of a text's terms and keeps a counter per
+// token of the text in shared memory; the counts [packed row][run] are scanned in that order, so
+// that a token's entries end up side by side in the order of their terms.
+constexpr int kSegs = 64;
+constexpr int kSortSmem = 48 * 1024;
+struct SortParams {
+  const int32_t *head, *text;
   const float *y, *dy;
   const int32_t* win;
-  const uint32_t* absmax;       // fp16 only
+  int64_t B, V;
+  int32_t L;               // counters per warp; 0: the survey alone
+  int32_t* count;          // [packed rows][kSegs]
+  const int64_t* offset;   // their exclusive scan
+  int2* list;              // (term, ds)
+  Sparse sparse;
+};
+inline int sort_warps(int64_t L) { return int(L * 4 * 8 <= kSortSmem ? 8 : kSortSmem / (L * 4)); }
+
+// Counts; also the survey, d_hidden's zeroes and the packed rows' tail.  (Survey and counts are
+// zeroed before.)
+__global__ void __launch_bounds__(256)
+survey_kernel(State s, const SortParams p, Survey* out, void* d_hidden, int64_t hidden_bytes) {
+  extern __shared__ int32_t counters[];
+  const int lane = lane_id(), wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int64_t job = int64_t(blockIdx.x) * warps + wid, b = job / kSegs;
+  const int32_t seg = int32_t(job % kSegs);
+  if (b < p.B) {
+    const int32_t first = p.text[b], len = p.text[b + 1] - first;
+    const bool sort = p.L > 0;
+    int32_t* mine = counters + wid * p.L;
+    if (sort) {
+      for (int32_t i = lane; i < len; i += 32) mine[i] = 0;
+      __syncwarp();
+    }
+    const int64_t per = (p.V + kSegs - 1) / kSegs, lo = seg * per, hi = min64(p.V, lo + per);
+    uint32_t c = 0;
+    float m = 0.0f;
+    for (int64_t t0 = lo; t0 < hi; t0 += 256) {
+      int32_t r[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int64_t t = t0 + 32 * k + lane;
+        r[k] = -1;
+        if (t < hi) {
+          const float d = p.dy[b * p.V + t], a = fabsf(d);
+          const int32_t w = p.win[b * p.V + t];
+          if (a < __uint_as_float(0x7F800000u)) m = fmaxf(m, a);
+          if (d != 0.0f) r[k] = w;
+        }
+        c += r[k] >= 0;
+      }
+      if (sort) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if (r[k] >= 0) atomicAdd(mine + (r[k] - first), 1);
+        }
+      }
+    }
+    if (sort) {
+      __syncwarp();
+      for (int32_t i = lane; i < len; i += 32) p.count[int64_t(first + i) * kSegs + seg] = mine[i];
+    }
+    c = __reduce_add_sync(FULL, c);
+    const uint32_t w = __reduce_max_sync(FULL, __float_as_uint(m));
+    if (lane == 0) {
+      if (c) atomicAdd(reinterpret_cast<unsigned long long*>(&out->nnz), static_cast<unsigned long long>(c));
+      if (w) atomicMax(&out->absmax, w);
+    }
+  }
+  if (d_hidden) zero_share(d_hidden, hidden_bytes, blockIdx.x, gridDim.x);
+  if (blockIdx.x == 0) zero_tail_rows(s.h, s.Dp, s.head[0]);
+}
+
+// The list: every warp places its run's entries where the scan says.
+__global__ void __launch_bounds__(256) place_kernel(const SortParams p) {
+  extern __shared__ int32_t counters[];
+  const int lane = lane_id(), wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int64_t job = int64_t(blockIdx.x) * warps + wid, b = job / kSegs;
+  const int32_t seg = int32_t(job % kSegs);
+  if (b >= p.B || !p.sparse.gather(p.head[0], p.V)) return;
+  const int32_t first = p.text[b], len = p.text[b + 1] - first;
+  int32_t* next = counters + wid * p.L;
+  for (int32_t i = lane; i < len; i += 32) next[i] = int32_t(p.offset[int64_t(first + i) * kSegs + seg]);
+  __syncwarp();
+  const int64_t per = (p.V + kSegs - 1) / kSegs, lo = seg * per, hi = min64(p.V, lo + per);
+  for (int64_t t0 = lo; t0 < hi; t0 += 256) {
+    int64_t o[8];
+    int32_t r[8];
+    float g[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) o[k] = t0 + 32 * k + lane < hi ? b * p.V + t0 + 32 * k + lane : -1;
+    entry_grads(p.y, p.win, p.dy, o, r, g);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (!__any_sync(FULL, r[k] >= 0)) continue;
+      const uint32_t same = __match_any_sync(FULL, r[k]);
+      int32_t at = 0;
+      if (r[k] >= 0) at = next[r[k] - first];
+      __syncwarp();
+      if (r[k] >= 0) {
+        p.list[at + __popc(same & lanemask_lt())] = make_int2(int32_t(t0 + 32 * k + lane), __float_as_int(g[k]));
+        if (lane == __ffs(same) - 1) next[r[k] - first] = at + __popc(same);
+      }
+      __syncwarp();
+    }
+  }
+}
+
+struct GatherParams {
+  const int32_t *head, *map;
+  Sparse sparse;
+  const int64_t* offset;   // of the list, by packed row x kSegs
+  const int2* list;
+  const float *y, *dy;
+  const int32_t* win;
+  const uint16_t *h, *w;
+  int64_t Dp, ldw, B, V, D;
+  int32_t bf16;
+  uint16_t *dh, *dw;
+  float* db;
+};
+__device__ __forceinline__ float2 unpack2(uint32_t x, bool bf16) {
+  if (bf16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
+  float2 r;
+  asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b; }" : "=f"(r.x), "=f"(r.y) : "r"(x));
+  return r;
+}
+
+// 8 columns of every 256 from d0 of a row, zeros from column `end` on; rows start on 16-byte
+// boundaries, and the 16 bytes that hold its last column belong to it or to nobody
+template <int kCols>
+__device__ __forceinline__ void load_row(const uint16_t* from, int64_t d0, int64_t end, int lane, uint4 (&x)[kCols]) {
+#pragma unroll
+  for (int q = 0; q < kCols; ++q) {
+    const int64_t c = d0 + q * 256 + lane * 8;
+    x[q] = c < end ? __ldg(reinterpret_cast<const uint4*>(from + c)) : make_uint4(0, 0, 0, 0);
+  }
+}
+// acc += g x
+template <int kCols>
+__device__ __forceinline__ void add_row(float (&acc)[kCols][8], const uint4 (&x)[kCols], float g, bool bf) {
+#pragma unroll
+  for (int q = 0; q < kCols; ++q) {
+    const uint32_t u[4] = {x[q].x, x[q].y, x[q].z, x[q].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = unpack2(u[k], bf);
+      acc[q][2 * k] = fmaf(g, f.x, acc[q][2 * k]);
+      acc[q][2 * k + 1] = fmaf(g, f.y, acc[q][2 * k + 1]);
+    }
+  }
+}
+// 8 columns (or the last n of a row) at any address
+__device__ __forceinline__ void store8(uint16_t* out, int n, const float (&v)[8], bool bf) {
+  uint32_t u[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) u[k] = pack2(v[2 * k], v[2 * k + 1], bf);
+  if (n == 8 && (reinterpret_cast<uintptr_t>(out) & 15) == 0) {
+    *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k < n) out[k] = uint16_t(u[k >> 1] >> (16 * (k & 1)));
+    }
+  }
+}
+
+// dW and d_bias: a warp per term, eight terms per CTA.  The warp takes the texts in order, 256 at
+// a time through shared memory (whose loads are then whole sectors), and adds the winners' rows;
+// a lane has 8 columns of every 256, up to 1024 columns at a time.
+constexpr int kTexts = 256;
+template <int kCols>
+__global__ void __launch_bounds__(256, 2) gather_weight_kernel(const GatherParams p) {
+  __shared__ int32_t row[kTexts][9];
+  __shared__ float grad[kTexts][9];
+  const bool gather = p.sparse.gather(p.head[0], p.V) && p.dw;
+  if (!gather && !p.db) return;
+  const int64_t v0 = int64_t(blockIdx.x) * 8, v = v0 + (threadIdx.x >> 5);
+  const int wid = threadIdx.x >> 5, lane = lane_id();
+  const bool bf = p.bf16 != 0;
+  float db = 0.0f;
+  for (int64_t d0 = 0; d0 < (gather ? p.D : 1); d0 += 256 * kCols) {
+    float acc[kCols][8];
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc[q][k] = 0.0f;
+    }
+    for (int64_t b0 = 0; b0 < p.B; b0 += kTexts) {
+      __syncthreads();
+      int64_t o[kTexts * 8 / 256];
+      int32_t r[kTexts * 8 / 256];
+      float g[kTexts * 8 / 256];
+#pragma unroll
+      for (int i = 0; i < kTexts * 8 / 256; ++i) {
+        const int e = i * 256 + threadIdx.x, b = e >> 3, c = e & 7;
+        o[i] = b0 + b < p.B && v0 + c < p.V ? (b0 + b) * p.V + v0 + c : -1;
+      }
+      entry_grads(p.y, p.win, p.dy, o, r, g);
+#pragma unroll
+      for (int i = 0; i < kTexts * 8 / 256; ++i) {
+        const int e = i * 256 + threadIdx.x;
+        row[e >> 3][e & 7] = r[i];
+        grad[e >> 3][e & 7] = g[i];
+      }
+      __syncthreads();
+      const int texts = int(min64(kTexts, p.B - b0));
+      for (int q32 = 0; q32 < texts; q32 += 32) {
+        const int32_t r = row[q32 + lane][wid];
+        const float g = grad[q32 + lane][wid];
+        if (d0 == 0) db += g;
+        uint32_t live = __ballot_sync(FULL, r >= 0);
+        if (!gather) continue;
+        while (live) {
+          uint4 x[4][kCols];         // four rows in flight
+          float gs[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const int src = live ? __ffs(live) - 1 : 0;
+            const int32_t rs = __shfl_sync(FULL, r, src);
+            gs[t] = live ? __shfl_sync(FULL, g, src) : 0.0f;
+            load_row(p.h + int64_t(live ? rs : 0) * p.Dp, d0, live ? p.Dp : 0, lane, x[t]);
+            live &= live - 1;
+          }
+#pragma unroll
+          for (int t = 0; t < 4; ++t) add_row(acc, x[t], gs[t], bf);
+        }
+      }
+    }
+    if (!gather || v >= p.V) continue;
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) {
+      const int64_t c = d0 + q * 256 + lane * 8;
+      if (c < p.D) store8(p.dw + v * p.D + c, int(min64(8, p.D - c)), acc[q], bf);
+    }
+  }
+  if (p.db) {
+    for (int o = 16; o > 0; o >>= 1) db += __shfl_xor_sync(FULL, db, o);
+    if (lane == 0 && v < p.V) p.db[v] = db;
+  }
+}
+
+// dH: a warp per packed row, eight rows per CTA; a lane has 8 columns of every 256 (up to 1024
+// columns; blockIdx.y goes on).  A row with more than kHeavy entries (a token may have won most
+// of the vocabulary) is shared by the CTA's warps afterwards, whose sums are added in order.
+constexpr int kHeavy = 256;
+template <int kCols>
+__device__ __forceinline__ void gather_run(const GatherParams& p, int32_t lo, int32_t hi, int64_t d0, int lane, bool bf,
+                                           float (&acc)[kCols][8]) {
+#pragma unroll
+  for (int q = 0; q < kCols; ++q) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[q][k] = 0.0f;
+  }
+  for (int32_t i0 = lo; i0 < hi; i0 += 32) {
+    int2 e = make_int2(0, 0);
+    if (i0 + lane < hi) e = p.list[i0 + lane];
+    const int32_t m = min(32, hi - i0);
+    for (int32_t i = 0; i < m; i += 4) {
+      uint4 x[4][kCols];
+      float g[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int32_t v = __shfl_sync(FULL, e.x, i + t);
+        g[t] = __int_as_float(__shfl_sync(FULL, e.y, i + t));      // 0 past the last entry
+        load_row(p.w + int64_t(v) * p.ldw, d0, i + t < m ? p.D : 0, lane, x[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) add_row(acc, x[t], g[t], bf);
+    }
+  }
+}
+template <int kCols>
+__global__ void __launch_bounds__(256, 2) gather_hidden_kernel(const GatherParams p) {
+  __shared__ float4 sums[7][2][32];
+  const int32_t n = p.head[0], r0 = blockIdx.x * 8;
+  if (r0 >= n || !p.sparse.gather(n, p.V)) return;
+  const int wid = threadIdx.x >> 5, lane = lane_id();
+  const bool bf = p.bf16 != 0;
+  const int64_t d0 = int64_t(blockIdx.y) * 256 * kCols;
+  float acc[kCols][8];
+  const int32_t r = r0 + wid;
+  int32_t e0 = 0, e1 = 0;
+  if (r < n) {
+    e0 = int32_t(p.offset[int64_t(r) * kSegs]);
+    e1 = int32_t(p.offset[int64_t(r + 1) * kSegs]);
+  }
+  if (e1 > e0 && e1 - e0 <= kHeavy) {              // (a row without entries is zero already)
+    gather_run(p, e0, e1, d0, lane, bf, acc);
+    uint16_t* out = p.dh + int64_t(p.map[r]) * p.D;
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) {
+      const int64_t c = d0 + q * 256 + lane * 8;
+      if (c < p.D) store8(out + c, int(min64(8, p.D - c)), acc[q], bf);
+    }
+  }
+  if (!__syncthreads_or(e1 - e0 > kHeavy)) return;
+  for (int32_t h = r0; h < min(n, r0 + 8); ++h) {
+    e0 = int32_t(p.offset[int64_t(h) * kSegs]);
+    e1 = int32_t(p.offset[int64_t(h + 1) * kSegs]);
+    if (e1 - e0 <= kHeavy) continue;
+    const int32_t per = (e1 - e0 + 7) / 8, lo = min(e0 + wid * per, e1);
+    gather_run(p, lo, min(lo + per, e1), d0, lane, bf, acc);
+#pragma unroll
+    for (int q = 0; q < kCols; ++q) {
+      const int64_t c0 = d0 + q * 256, c = c0 + lane * 8;
+      if (c0 >= p.D) break;
+      __syncthreads();
+      if (wid > 0) {
+        sums[wid - 1][0][lane] = make_float4(acc[q][0], acc[q][1], acc[q][2], acc[q][3]);
+        sums[wid - 1][1][lane] = make_float4(acc[q][4], acc[q][5], acc[q][6], acc[q][7]);
+      }
+      __syncthreads();
+      if (wid > 0 || c >= p.D) continue;
+#pragma unroll
+      for (int w = 0; w < 7; ++w) {
+        const float4 a = sums[w][0][lane], b = sums[w][1][lane];
+        acc[q][0] += a.x, acc[q][1] += a.y, acc[q][2] += a.z, acc[q][3] += a.w;
+        acc[q][4] += b.x, acc[q][5] += b.y, acc[q][6] += b.z, acc[q][7] += b.w;
+      }
+      store8(p.dh + int64_t(p.map[h]) * p.D + c, int(min64(8, p.D - c)), acc[q], bf);
+    }
+  }
+}
+
+struct SpreadParams {
+  const int32_t *head, *text;
+  const float *y, *dy;
+  const int32_t* win;
+  const Survey* survey;
+  Sparse sparse;
   float* scale;
   uint16_t* P;
   int64_t pitch, v0, cols, V, B;
   int32_t L, bf16;
 };
-__device__ __forceinline__ float p_scale(const uint32_t* absmax) {     // P = ds * this
-  const float m = absmax ? __uint_as_float(*absmax) : 0.0f;
+__device__ __forceinline__ float p_scale(const Survey* s, bool bf16) {     // P = ds * this
+  const float m = bf16 ? 0.0f : __uint_as_float(s->absmax);
   return m > 0.0f ? 16384.0f / m : 1.0f;
-}
-__device__ __forceinline__ int32_t lower_row(const int32_t* map, int32_t n, int64_t key) {
-  int32_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int32_t mid = (lo + hi) >> 1;
-    if (map[mid] < key) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
 }
 constexpr int kSpreadRows = 64;
 // P of a piece: a thread owns 8 columns of one text and writes them for up to kSpreadRows of
 // its rows; the blocks of text B zero the rows past the packed ones.
 __global__ void __launch_bounds__(256) spread_kernel(const SpreadParams p) {
   const int32_t n = p.head[0];
+  if (p.sparse.gather(n, p.V)) return;
   const int64_t c = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
   const int64_t b = blockIdx.y;
-  const float up_by = p_scale(p.absmax);
+  const float up_by = p_scale(p.survey, p.bf16 != 0);
   if (blockIdx.x == 0 && b == 0 && blockIdx.z == 0 && threadIdx.x == 0) *p.scale = 1.0f / up_by;
   int32_t r0, r1;
   if (b < p.B) {
-    r0 = lower_row(p.map, n, b * p.L) + blockIdx.z * kSpreadRows;
-    r1 = min(lower_row(p.map, n, (b + 1) * p.L), r0 + kSpreadRows);
+    r0 = p.text[b] + blockIdx.z * kSpreadRows;
+    r1 = min(p.text[b + 1], r0 + kSpreadRows);
   } else {
     r0 = n + blockIdx.z * kSpreadRows;
     r1 = min((n + mm::kBM - 1) / mm::kBM * mm::kBM, r0 + kSpreadRows);
@@ -327,17 +663,6 @@ __global__ void __launch_bounds__(256) spread_kernel(const SpreadParams p) {
       u[k] = pack2(w[2 * k] == r ? ds[2 * k] : 0.0f, w[2 * k + 1] == r ? ds[2 * k + 1] : 0.0f, p.bf16 != 0);
     *reinterpret_cast<uint4*>(p.P + int64_t(r) * p.pitch + c) = o;
   }
-}
-
-__global__ void __launch_bounds__(256) head_bias_kernel(const float* y, const int32_t* win, const float* dy, int64_t B, int64_t V,
-                                                        float* d_bias) {
-  const int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (v >= V) return;
-  float s = 0.0f;
-  for (int64_t b = 0; b < B; ++b) {
-    if (win[b * V + v] >= 0) s += dy[b * V + v] * expf(-y[b * V + v]);
-  }
-  d_bias[v] = s;
 }
 
 // ---- dense rows -> CSR -------------------------------------------------------------------
@@ -398,10 +723,14 @@ Fwd carve_fwd(void* base, const gsp_vocab_view* vw) {
   return f;
 }
 struct Bwd {
-  uint32_t* absmax;
+  Survey* survey;
+  int32_t* count;
+  int64_t* offset;
+  void* scan;
   float* scale;
   GradScratch grad;
-  uint16_t* P;
+  uint16_t* P;        // or the list
+  int64_t zeroed, scan_bytes, room;
   void* wcopy;
   int64_t pitch, bytes;
 };
@@ -410,10 +739,16 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
   Carver c{static_cast<char*>(base)};
   const int64_t Tp = pad_rows(vw->T);
   b.pitch = piece_cols(Tp, vw->V);
-  b.absmax = c.take<uint32_t>(1);
+  b.survey = c.take<Survey>(1);
+  b.count = c.take<int32_t>(vw->T * kSegs);
+  b.zeroed = c.off;
+  b.offset = c.take<int64_t>(vw->T * kSegs + 1);
+  b.scan_bytes = gsp_scan_ws_bytes(vw->T * kSegs);
+  b.scan = c.take<char>(b.scan_bytes);
   b.scale = c.take<float>(1);
   b.grad = carve_grad(c, vw, Tp, b.pitch);
   b.P = c.take<uint16_t>(Tp * b.pitch);
+  b.room = Tp * b.pitch * 2 / int64_t(sizeof(int2));
   b.wcopy = c.take<char>(weight_copy_bytes(vw));
   b.bytes = c.off;
   return b;
@@ -443,6 +778,9 @@ int run_head(const gsp_vocab_view* vw, const State& s, const Fwd& f, int32_t L, 
   if ((rc = make_map(&j.maps[1], bf, s.h, s.Dp, vw->T, s.Dp, bn / 2))) return rc;
   return mm::launch(j, st);
 }
+
+// blocks of 256 columns that a lane of the gathering kernels holds
+int gather_cols(int64_t D) { return D > 768 ? 4 : int((D + 255) / 256); }
 
 int check_texts(const gsp_vocab_view* vw, int64_t L, const char* what) {
   const int rc = check_view(vw, what);
@@ -480,14 +818,14 @@ extern "C" int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_
                                int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream) {
   int rc = check_texts(vw, L, "sparse_head");
   if (rc) return rc;
-  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, false);
+  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, vw->T > 0 ? vw->T : 1);
   const Fwd f = carve_fwd(ws, vw);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "sparse_head: state or workspace too small");
   if (vw->T == 0) return GSP_OK;
   GSP_REQUIRE(vw->hidden && vw->weight && y, GSP_ERR_ARG, "sparse_head: null input or output");
   cudaStream_t st = as_stream(stream);
-  if ((rc = pack_rows(vw, nullptr, 0, mask, 0.0f, s, f.counts, st))) return rc;
+  if ((rc = pack_rows(vw, nullptr, 0, mask, 0.0f, L, s, f.counts, st))) return rc;
   const uint16_t* w;
   int64_t ldw;
   if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
@@ -523,7 +861,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   int rc = check_texts(vw, L, "sparse_head backward");
   if (rc) return rc;
   if ((rc = check_grads(vw, d_hidden, d_weight, "sparse_head backward"))) return rc;
-  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, false);
+  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, vw->T > 0 ? vw->T : 1);
   const Bwd b = carve_bwd(ws, vw);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,
               "sparse_head backward: state or workspace too small");
@@ -535,30 +873,85 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   }
   GSP_REQUIRE(y && win && dy && vw->weight, GSP_ERR_ARG, "sparse_head backward: null input");
   const int64_t B = vw->T / L;
-  if (d_bias) {
-    head_bias_kernel<<<unsigned((vw->V + 255) / 256), 256, 0, st>>>(y, win, dy, B, vw->V, d_bias);
-    GSP_CHECK_LAUNCH();
-  }
-  if (!d_hidden && !d_weight) return GSP_OK;
-  if (d_hidden) GSP_CUDA(cudaMemsetAsync(d_hidden, 0, size_t(vw->T) * size_t(vw->D) * 2, st));
   const bool bf = is_bf16(vw);
-  if (!bf) {
-    GSP_CUDA(cudaMemsetAsync(b.absmax, 0, sizeof(uint32_t), st));
-    absmax_kernel<<<num_sms() * 4, 256, 0, st>>>(dy, B * vw->V, b.absmax);
-    GSP_CHECK_LAUNCH();
-  }
-  tail_kernel<<<1, 1024, 0, st>>>(s);
-  GSP_CHECK_LAUNCH();
   const uint16_t* w;
   int64_t ldw;
   if ((rc = weight_rows(vw, b.wcopy, &w, &ldw, st))) return rc;
+  // longer texts than the sort has counters for take the products
+  const bool sort = d_hidden && L * 4 <= kSortSmem, may = !d_hidden || sort;
+  GSP_CUDA(cudaMemsetAsync(b.survey, 0, size_t(sort ? b.zeroed : int64_t(sizeof(Survey))), st));
+  SortParams q{};
+  q.head = s.head;
+  q.text = s.text;
+  q.y = y;
+  q.dy = dy;
+  q.win = win;
+  q.B = B;
+  q.V = vw->V;
+  q.L = sort ? int32_t(L) : 0;
+  q.count = b.count;
+  q.offset = b.offset;
+  q.list = reinterpret_cast<int2*>(b.P);
+  q.sparse = Sparse{may ? &b.survey->nnz : nullptr, b.room};
+  const int warps = sort ? sort_warps(L) : 8;
+  const unsigned sort_blocks = unsigned((B * kSegs + warps - 1) / warps);
+  const size_t sort_bytes = sort ? size_t(warps) * size_t(L) * 4 : 0;
+  survey_kernel<<<sort_blocks, 32 * warps, sort_bytes, st>>>(s, q, b.survey, d_hidden, vw->T * vw->D * 2);
+  GSP_CHECK_LAUNCH();
+  if (sort) {
+    if ((rc = gsp_scan_i32(b.count, vw->T * kSegs, b.offset, b.scan, b.scan_bytes, stream))) return rc;
+    place_kernel<<<sort_blocks, 32 * warps, sort_bytes, st>>>(q);
+    GSP_CHECK_LAUNCH();
+  }
+  GatherParams g{};
+  g.head = s.head;
+  g.map = s.map;
+  g.sparse = q.sparse;
+  g.offset = b.offset;
+  g.list = q.list;
+  g.y = y;
+  g.dy = dy;
+  g.win = win;
+  g.h = s.h;
+  g.w = w;
+  g.Dp = s.Dp;
+  g.ldw = ldw;
+  g.B = B;
+  g.V = vw->V;
+  g.D = vw->D;
+  g.bf16 = bf;
+  g.dh = static_cast<uint16_t*>(d_hidden);
+  g.dw = static_cast<uint16_t*>(d_weight);
+  g.db = d_bias;
+  if (d_weight || d_bias) {
+    const unsigned blocks = unsigned((vw->V + 7) / 8);
+    switch (gather_cols(vw->D)) {
+      case 1: gather_weight_kernel<1><<<blocks, 256, 0, st>>>(g); break;
+      case 2: gather_weight_kernel<2><<<blocks, 256, 0, st>>>(g); break;
+      case 3: gather_weight_kernel<3><<<blocks, 256, 0, st>>>(g); break;
+      default: gather_weight_kernel<4><<<blocks, 256, 0, st>>>(g);
+    }
+    GSP_CHECK_LAUNCH();
+  }
+  if (sort) {
+    const dim3 blocks(unsigned((vw->T + 7) / 8), unsigned((vw->D + 1023) / 1024));
+    switch (gather_cols(vw->D)) {
+      case 1: gather_hidden_kernel<1><<<blocks, 256, 0, st>>>(g); break;
+      case 2: gather_hidden_kernel<2><<<blocks, 256, 0, st>>>(g); break;
+      case 3: gather_hidden_kernel<3><<<blocks, 256, 0, st>>>(g); break;
+      default: gather_hidden_kernel<4><<<blocks, 256, 0, st>>>(g);
+    }
+    GSP_CHECK_LAUNCH();
+  }
+  if (!d_hidden && !d_weight) return GSP_OK;
   SpreadParams p{};
   p.head = s.head;
-  p.map = s.map;
+  p.text = s.text;
   p.y = y;
   p.dy = dy;
   p.win = win;
-  p.absmax = bf ? nullptr : b.absmax;
+  p.survey = b.survey;
+  p.sparse = q.sparse;
   p.scale = b.scale;
   p.P = b.P;
   p.pitch = b.pitch;
@@ -573,7 +966,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
     p.cols = min64(b.pitch, vw->V - v0);
     spread_kernel<<<dim3(unsigned((b.pitch / 8 + 255) / 256), unsigned(B + 1), unsigned(zs)), 256, 0, st>>>(p);
     GSP_CHECK_LAUNCH();
-    const GradPiece pc{b.P, b.pitch, v0, p.cols, v0 == 0, v0 + p.cols >= vw->V};
+    const GradPiece pc{b.P, b.pitch, v0, p.cols, v0 == 0, v0 + p.cols >= vw->V, q.sparse};
     if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, BiasSums{}, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;

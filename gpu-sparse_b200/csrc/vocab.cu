@@ -62,7 +62,8 @@ struct PackParams {
   float bias_scale;         // 0: no bias2
   float* bias2;
   uint16_t* h;
-  int32_t *map, *head, *tgt;
+  int32_t *map, *head, *tgt, *text;
+  int32_t L;                // > 0: texts of L rows
 };
 
 // 32 rows per CTA: their packed position is the number of valid rows before them.
@@ -104,7 +105,12 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackParams p) {
       if (p.targets) p.tgt[d] = int32_t(p.targets[r0 + i]);
     }
   }
+  if (p.L > 0 && wid == 0) {
+    const int64_t r = r0 + lane;
+    if (r < p.T && r % p.L == 0) p.text[r / p.L] = base + __popc(w & lanemask_lt());
+  }
   if (r0 + 32 >= p.T && threadIdx.x == 0) {
+    if (p.L > 0) p.text[p.T / p.L] = base + __popc(w);
     p.head[0] = base + __popc(w);
     p.head[1] = 0;
   }
@@ -150,6 +156,7 @@ struct GradJob {
   CUtensorMap maps[5];       // P K-major, P MN-major, W MN-major, H MN-major; dW as 32 x 64 boxes
   int32_t wait_limit, bf16;
   const int32_t* n_rows;
+  Sparse sparse;             // see GradPiece
   const int32_t* map;
   int32_t D, nbs;            // 256-wide tiles of D
   int32_t v0, cols, V;
@@ -164,6 +171,7 @@ struct GradJob {
 
   __device__ GradList list() const {
     const int32_t n = *n_rows;
+    if (sparse.gather(n, V)) return GradList{0, 0, 0, 0};
     return GradList{want_h ? (n + mm::kBM - 1) / mm::kBM : 0, want_w ? (cols + mm::kBM - 1) / mm::kBM : 0, (cols + 63) / 64,
                     (n + 63) / 64};
   }
@@ -378,7 +386,7 @@ finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blo
 
 }  // namespace
 
-State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool loss) {
+State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, int64_t texts) {
   State s{};
   Carver c{static_cast<char*>(base)};
   s.Tp = pad_rows(T);
@@ -387,7 +395,9 @@ State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool l
   s.head = c.take<int32_t>(16);
   s.map = c.take<int32_t>(s.Tp);
   s.h = c.take<uint16_t>(s.Tp * s.Dp);
-  if (loss) {
+  if (texts > 0) {
+    s.text = c.take<int32_t>(texts + 1);
+  } else {
     s.bias2 = c.take<float>(s.Vp);
     s.lse2 = c.take<float>(s.Tp);
     s.tgt = c.take<int32_t>(K > 0 ? 0 : s.Tp);
@@ -453,7 +463,7 @@ int make_map(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t 
 }
 
 int pack_rows(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore, const uint8_t* flag, float bias_scale,
-              const State& s, int32_t* counts, cudaStream_t st) {
+              int64_t L, const State& s, int32_t* counts, cudaStream_t st) {
   const int64_t T = vw->T;
   // up to 2048 rows every CTA counts the rows before its own itself (at most 8 loads a
   // thread), which saves the launch of the counting pass
@@ -481,6 +491,8 @@ int pack_rows(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore, 
   p.map = s.map;
   p.head = s.head;
   p.tgt = s.tgt;
+  p.text = s.text;
+  p.L = int32_t(L);
   const int64_t blocks = (T + 31) / 32;
   pack_kernel<<<unsigned(blocks < 32 ? 32 : blocks), 256, 0, st>>>(p);
   GSP_CHECK_LAUNCH();
@@ -517,7 +529,8 @@ GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t 
 // rows of ld 16-bit values -> rows of D at out (map: where each row goes); a warp per row
 __global__ void __launch_bounds__(256)
 unpad_kernel(const uint16_t* dh, const int32_t* n_rows, const int32_t* map, uint16_t* out_h, int64_t h_blocks,
-             const uint16_t* dw, int64_t V, uint16_t* out_w, int64_t ld, int64_t D) {
+             const uint16_t* dw, int64_t V, uint16_t* out_w, int64_t ld, int64_t D, Sparse sparse) {
+  if (sparse.gather(*n_rows, V)) return;
   const int lane = lane_id();
   const int64_t warp = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
   const uint16_t* src;
@@ -554,6 +567,7 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.n_rows = s.head;
+  j.sparse = pc.sparse;
   j.map = padded ? nullptr : s.map;
   j.D = int32_t(vw->D);
   j.nbs = int32_t((vw->D + mm::kBN - 1) / mm::kBN);
@@ -582,7 +596,7 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   if (padded && pc.last && (d_hidden || d_weight)) {
     const int64_t hb = d_hidden ? (vw->T + 7) / 8 : 0, wb = d_weight ? (vw->V + 7) / 8 : 0;
     unpad_kernel<<<unsigned(hb + wb), 256, 0, st>>>(dh, s.head, s.map, static_cast<uint16_t*>(d_hidden), hb, dw, vw->V,
-                                                   static_cast<uint16_t*>(d_weight), j.ld_out, vw->D);
+                                                   static_cast<uint16_t*>(d_weight), j.ld_out, vw->D, pc.sparse);
     GSP_CHECK_LAUNCH();
   }
   return GSP_OK;
@@ -596,5 +610,7 @@ extern "C" int64_t gsp_vocab_state_bytes(int64_t T, int64_t V, int64_t D, int64_
     gsp::set_error("gsp_vocab_state_bytes: bad arguments");
     return -GSP_ERR_ARG;
   }
-  return gsp::vocab::carve_state(nullptr, T, V, D, kind == GSP_VOCAB_DISTILL ? K : 0, kind != GSP_VOCAB_HEAD).bytes;
+  // the sparse head's texts: at most one per token
+  return gsp::vocab::carve_state(nullptr, T, V, D, kind == GSP_VOCAB_DISTILL ? K : 0,
+                                 kind == GSP_VOCAB_HEAD ? (T > 0 ? T : 1) : 0).bytes;
 }

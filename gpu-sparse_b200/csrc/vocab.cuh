@@ -31,6 +31,7 @@ struct State {
   int32_t* head;      // [0] packed rows, [1] ticket of the reducing kernels
   int32_t* map;       // [Tp] original row of every packed row, ascending
   uint16_t* h;        // [Tp, Dp] packed hidden states
+  int32_t* text;      // [texts + 1] first packed row of every text (sparse head)
   float* bias2;       // [Vp] bias in units of the exponent's base 2, -inf past V (losses)
   float* lse2;        // [Tp] log2 of the softmax's denominator (losses)
   int32_t* tgt;       // [Tp] target of every packed row (cross entropy)
@@ -41,7 +42,8 @@ struct State {
   int32_t bucket_shift;      // log2 of a bucket's vocabulary rows
 };
 constexpr int32_t kNoId = 0x7FFFFFFF;
-State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, bool loss);
+// loss: texts is 0; sparse head: K is 0
+State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, int64_t texts);
 
 int check_view(const gsp_vocab_view* vw, const char* what);
 int check_grads(const gsp_vocab_view* vw, const void* d_hidden, const void* d_weight, const char* what);
@@ -57,9 +59,22 @@ int make_map(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t 
 
 // Packs the rows that take part (targets: id in [0, V) and != ignore; else flag != 0) to the
 // front of st.h, keeping their order, and writes st.map, st.head[0]; bias2 when scale != 0.
+// L > 0: rows are texts of L tokens, and st.text is written.
 int pack_rows(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore, const uint8_t* flag, float bias_scale,
-              const State& s, int32_t* counts, cudaStream_t st);
+              int64_t L, const State& s, int32_t* counts, cudaStream_t st);
 inline int64_t pack_counts(int64_t T) { return (T + 255) / 256 + 1; }
+
+// How sparse the gradient of the logits is: with so few of n x V entries nonzero that gathering
+// rows for them costs less than the products (and with room for a list of them), they are
+// gathered.
+constexpr int64_t kGatherWeight = 160;
+struct Sparse {
+  const int64_t* nnz;      // entries, or null: always the products
+  int64_t room;
+  __device__ __forceinline__ bool gather(int64_t n, int64_t V) const {
+    return nnz && *nnz <= room && *nnz * kGatherWeight <= n * V;
+  }
+};
 
 // Backward products over a piece of the vocabulary [v0, v0 + cols): P [Tp, pitch] is the
 // gradient of the piece's logits,
@@ -69,6 +84,7 @@ struct GradPiece {
   const uint16_t* P;
   int64_t pitch, v0, cols;
   bool first, last;
+  Sparse sparse;           // few enough entries in P and the call does nothing
 };
 struct GradScratch {
   float* dh_acc;      // [Tp, up(D, 32)], or null when there is one piece

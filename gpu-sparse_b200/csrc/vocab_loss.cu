@@ -782,7 +782,7 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, float t
     j.v0 = int32_t(v0);
     j.nt = int32_t((cols + mm::kBN - 1) / mm::kBN);
     if ((rc = mm::launch(j, st))) return rc;
-    const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V};
+    const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V, Sparse{}};
     if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, BiasSums{b.colpart, b.pitch, d_bias ? d_bias + v0 : nullptr}, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
@@ -807,7 +807,7 @@ extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, in
   if ((rc = check_reduction(reduction, "vocab_cross_entropy"))) return rc;
   cudaStream_t st = as_stream(stream);
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "vocab_cross_entropy: null loss");
-  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, true);
+  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, 0);
   const Fwd f = carve_fwd(ws, vw, 0);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "vocab_cross_entropy: state or workspace too small");
@@ -816,7 +816,7 @@ extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, in
     return GSP_OK;
   }
   GSP_REQUIRE(targets && vw->hidden && vw->weight, GSP_ERR_ARG, "vocab_cross_entropy: null input");
-  if ((rc = pack_rows(vw, targets, ignore_index, nullptr, kLog2e, s, f.counts, st))) return rc;
+  if ((rc = pack_rows(vw, targets, ignore_index, nullptr, kLog2e, 0, s, f.counts, st))) return rc;
   return run_forward<false>(vw, s, f, 1.0f, reduction, loss, st);
 }
 
@@ -831,7 +831,7 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
               (long long)K, GSP_DISTILL_MAX_K);
   GSP_REQUIRE(tau > 0.0f && tau < __builtin_inff(), GSP_ERR_ARG, "topk_distillation: temperature must be positive");
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "topk_distillation: null loss");
-  const State s = carve_state(state, vw->T, vw->V, vw->D, K, true);
+  const State s = carve_state(state, vw->T, vw->V, vw->D, K, 0);
   const Fwd f = carve_fwd(ws, vw, K);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "topk_distillation: state or workspace too small");
@@ -850,7 +850,7 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   else GSP_TEACHER(512);
 #undef GSP_TEACHER
   GSP_CHECK_LAUNCH();
-  if ((rc = pack_rows(vw, nullptr, 0, f.tc.flag, kLog2e / tau, s, f.counts, st))) return rc;
+  if ((rc = pack_rows(vw, nullptr, 0, f.tc.flag, kLog2e / tau, 0, s, f.counts, st))) return rc;
   const int bucket_bytes = int(s.buckets * 4);
   if ((rc = ensure_smem(reinterpret_cast<const void*>(&bucket_kernel), bucket_bytes))) return rc;
   bucket_kernel<<<unsigned((vw->T + 31) / 32), 512, bucket_bytes, st>>>(s, f.tc);
@@ -871,7 +871,7 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   GSP_REQUIRE(!list || (K >= 1 && K <= GSP_DISTILL_MAX_K && tau > 0.0f && tau < __builtin_inff()), GSP_ERR_ARG,
               "vocab loss backward: bad teacher entries or temperature");
   cudaStream_t st = as_stream(stream);
-  const State s = carve_state(state, vw->T, vw->V, vw->D, list ? K : 0, true);
+  const State s = carve_state(state, vw->T, vw->V, vw->D, list ? K : 0, 0);
   const Bwd b = carve_bwd(ws, vw);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,
               "vocab loss backward: state or workspace too small");

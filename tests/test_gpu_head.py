@@ -334,6 +334,10 @@ def check_head(h, w, b, mask, dy):
     (130, 33, 257, 64, HF),
     (5, 256, 4000, 128, BF),
     (2, 300, 128, 1000, BF),
+    (2, 400, 65, 1100, BF),         # more columns than one slice of the gathered sums
+    (3, 320, 500, 331, HF),
+    (200, 2, 700, 96, BF),          # more texts than one round of the gathered sums
+    (150, 300, 40, 96, HF),
 ])
 def test_sparse_head(B, Lt, V, D, dt):
     h, w, b, dy = head_inputs(B, Lt, V, D, dt, seed=B + Lt)
