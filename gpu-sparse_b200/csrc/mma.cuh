@@ -65,6 +65,8 @@ struct Tile {
   int32_t ak, bk;
   int32_t nk;            // 64-deep steps; 0: the product is zero
   bool a_mn, b_mn;       // operand is MN-major
+  bool b_cut;            // an MN-major B whose rows are no whole blocks of 64 (2D map, a copy per
+                         // block; else, and for A, a 3D map [block][k][64] and one copy)
   bool a_stream;         // A passes through L2 (B, and else A, is kept there)
   int32_t a_rows;        // rows of a K-major A's boxes, at most kRows; fewer: A has no more, they
                          // are the first CTA's, and the other rows of the tile are not read
@@ -143,6 +145,14 @@ __device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int32_
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint [%0], "
       "[%1, {%2, %3}], [%4], %5;" ::"r"(su32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "l"(policy)
+      : "memory");
+}
+__device__ __forceinline__ void tma_3d(void* dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t bar,
+                                       uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2.L2::cache_hint [%0], "
+      "[%1, {%2, %3, %4}], [%5], %6;" ::"r"(su32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
       : "memory");
 }
 // Stores a box of shared memory (128-byte swizzled rows) where the map says; the executing
@@ -298,7 +308,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
         const CUtensorMap* mb = &job.maps[t.b];
         const int32_t nb = t.bn / 2, a0 = t.a0 + rank * kRows, b0 = t.b0 + rank * nb;
         const bool few = !t.a_mn && t.a_rows < kRows;
-        const uint32_t bytes = uint32_t((few ? t.a_rows : 2 * kRows) + 2 * nb) * (kBK * 2);
+        // (an MN-major B is always read 128 rows wide: past D there are zeros)
+        const uint32_t bytes = uint32_t((few ? t.a_rows : 2 * kRows) + (t.b_mn ? kBN : 2 * nb)) * (kBK * 2);
         for (int32_t k = 0; k < t.nk; ++k, ++it) {
           const uint32_t s = it % kStages, n = it / kStages;
           if (n > 0) ok = bar_wait(empty + s, (n - 1) & 1, limit, fault);
@@ -310,12 +321,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
           if (!t.a_mn) {
             if (!few || rank == 0) tma_2d(as, ma, t.ak + k * kBK, a0, bar, pol_a);
           } else {
-            for (int32_t j = 0; j < kRows / 64; ++j) tma_2d(as + j * 8192, ma, a0 + j * 64, t.ak + k * kBK, bar, pol_a);
+            tma_3d(as, ma, 0, t.ak + k * kBK, a0 / 64, bar, pol_a);
           }
           if (!t.b_mn) {
             tma_2d(bs, mb, t.bk + k * kBK, b0, bar, keep);
+          } else if (!t.b_cut) {
+            tma_3d(bs, mb, 0, t.bk + k * kBK, b0 / 64, bar, keep);
           } else {
-            for (int32_t j = 0; j < nb / 64; ++j) tma_2d(bs + j * 8192, mb, b0 + j * 64, t.bk + k * kBK, bar, keep);
+            for (int32_t j = 0; j < kBN / 128; ++j) tma_2d(bs + j * 8192, mb, b0 + j * 64, t.bk + k * kBK, bar, keep);
           }
         }
       }

@@ -57,7 +57,7 @@ struct HeadJob {
       t.b0 = t.y * bn;
       t.ak = t.bk = 0;
       t.nk = nk;
-      t.a_mn = t.b_mn = t.a_stream = false;
+      t.a_mn = t.b_mn = t.b_cut = t.a_stream = false;
       t.bn = bn;
       t.a_rows = mm::kRows;
       t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == ntt - 1 ? kLast : 0) | (x == lo ? kBegin : 0) |

@@ -161,7 +161,7 @@ struct GradJob {
   int32_t D, nbs;            // 256-wide tiles of D
   int32_t v0, cols, V;
   int32_t first, last;
-  bool want_h, want_w;
+  bool want_h, want_w, w_cut;
   int64_t ld_out;            // of dh and dw
   float* dh_acc;
   int32_t ld_acc;
@@ -186,6 +186,7 @@ struct GradJob {
     GradList l;
     int64_t x, x1;
     int32_t nb, nb_step, nbs, D, v0;
+    bool w_cut;
     __device__ bool next(mm::Tile& t) {
       for (;;) {
         if (x >= x1) {             // with more D tiles than pairs a pair takes several, whole
@@ -209,6 +210,7 @@ struct GradJob {
         t.ak = k0 * mm::kBK;
         t.a_rows = mm::kRows;
         t.b_mn = true;
+        t.b_cut = is_h && w_cut;
         t.a = is_h ? 0 : 1;
         t.b = is_h ? 2 : 3;
         t.a_mn = !is_h;
@@ -226,10 +228,10 @@ struct GradJob {
   __device__ Walk walk(int32_t pair, int32_t pairs) const {
     const GradList l = list();
     const int64_t tot = l.total();
-    if (nbs > pairs) return Walk{l, tot > 0 ? 0 : 1, tot, pair, tot > 0 ? pairs : nbs, nbs, D, v0};
+    if (nbs > pairs) return Walk{l, tot > 0 ? 0 : 1, tot, pair, tot > 0 ? pairs : nbs, nbs, D, v0, w_cut};
     const int32_t groups = this->groups(pairs, tot), g = pair / nbs;
-    if (g >= groups) return Walk{l, 0, 0, 0, nbs, nbs, D, v0};
-    return Walk{l, g * tot / groups, (g + 1) * tot / groups, pair % nbs, nbs, nbs, D, v0};
+    if (g >= groups) return Walk{l, 0, 0, 0, nbs, nbs, D, v0, w_cut};
+    return Walk{l, g * tot / groups, (g + 1) * tot / groups, pair % nbs, nbs, nbs, D, v0, w_cut};
   }
 
   // 8 columns from c of a finished row: r a packed row (dH) or a vocabulary row of the piece (dW)
@@ -390,7 +392,7 @@ State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, int64_
   State s{};
   Carver c{static_cast<char*>(base)};
   s.Tp = pad_rows(T);
-  s.Dp = up(D, 8);
+  s.Dp = up(D, 64);
   s.Vp = up(V, kRowPad);
   s.head = c.take<int32_t>(16);
   s.map = c.take<int32_t>(s.Tp);
@@ -456,6 +458,20 @@ int make_map(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t 
   const cuuint32_t box[2] = {mm::kBK, cuuint32_t(box_rows)};
   const cuuint32_t es[2] = {1, 1};
   const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                         const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  GSP_REQUIRE(r == CUDA_SUCCESS, GSP_ERR_CUDA, "vocabulary head: tensor map failed (%d)", int(r));
+  return GSP_OK;
+}
+
+int make_map_mn(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tma_encoder();
+  GSP_REQUIRE(enc, GSP_ERR_CUDA, "vocabulary head: cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[3] = {64, cuuint64_t(rows), cuuint64_t(cols / 64)};
+  const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, 128};
+  const cuuint32_t box[3] = {64, mm::kBK, 2};
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                          const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   GSP_REQUIRE(r == CUDA_SUCCESS, GSP_ERR_CUDA, "vocabulary head: tensor map failed (%d)", int(r));
@@ -561,9 +577,12 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.ld_out = up(vw->D, 16);
   if (dw && (rc = make_map(&j.maps[4], bf, dw, j.ld_out, vw->V, j.ld_out, 32))) return rc;
   if ((rc = make_map(&j.maps[0], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kRows))) return rc;
-  if ((rc = make_map(&j.maps[1], bf, pc.P, pc.pitch, s.Tp, pc.pitch, mm::kBK))) return rc;
-  if ((rc = make_map(&j.maps[2], bf, w, vw->D, vw->V, ldw, mm::kBK))) return rc;
-  if ((rc = make_map(&j.maps[3], bf, s.h, s.Dp, vw->T, s.Dp, mm::kBK))) return rc;
+  if ((rc = make_map_mn(&j.maps[1], bf, pc.P, pc.pitch, s.Tp, pc.pitch))) return rc;
+  j.w_cut = vw->D % 64 != 0;
+  if ((rc = j.w_cut ? make_map(&j.maps[2], bf, w, vw->D, vw->V, ldw, mm::kBK)
+                    : make_map_mn(&j.maps[2], bf, w, vw->D, vw->V, ldw)))
+    return rc;
+  if ((rc = make_map_mn(&j.maps[3], bf, s.h, s.Dp, vw->T, s.Dp))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.n_rows = s.head;

@@ -56,6 +56,9 @@ int weight_rows(const gsp_vocab_view* vw, void* scratch, const uint16_t** w, int
 // 2D map of a row-major 16-bit matrix: boxes of 64 columns x box_rows rows, 128-byte swizzle,
 // zeros outside
 int make_map(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows);
+// The same matrix (cols a multiple of 64) as [cols / 64][rows][64] for an MN-major operand: boxes
+// of 2 x 64 x 64
+int make_map_mn(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld);
 
 // Packs the rows that take part (targets: id in [0, V) and != ignore; else flag != 0) to the
 // front of st.h, keeping their order, and writes st.map, st.head[0]; bias2 when scale != 0.

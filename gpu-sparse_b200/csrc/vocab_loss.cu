@@ -285,7 +285,7 @@ struct LossJob {
       t.b0 = t.y * mm::kBN;
       t.ak = t.bk = 0;
       t.nk = nk;
-      t.a_mn = t.b_mn = t.a_stream = false;
+      t.a_mn = t.b_mn = t.b_cut = t.a_stream = false;
       t.bn = mm::kBN;
       t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 || t.y == nt - 1 ? kLast : 0);
       ++x;
@@ -538,7 +538,7 @@ struct LogitGradJob {
       t.b0 = v0 + t.y * mm::kBN;
       t.ak = t.bk = 0;
       t.nk = nk;
-      t.a_mn = t.b_mn = t.a_stream = false;
+      t.a_mn = t.b_mn = t.b_cut = t.a_stream = false;
       t.bn = mm::kBN;
       t.flags = (x == lo || t.y == 0 ? kFirst : 0) | (x == hi - 1 ? kLast : 0);
       ++x;
