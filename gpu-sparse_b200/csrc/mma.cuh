@@ -75,6 +75,12 @@ struct Tile {
 };
 
 // ---- PTX ---------------------------------------------------------------------------------
+// Returns once the kernel before this one in the stream has finished and its writes are visible
+// (see launch() in vocab.cuh); only then may the kernel after this one be set up, so that no more
+// than two of a chain are in flight.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+}
 __device__ __forceinline__ uint32_t su32(const void* p) { return uint32_t(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void bar_init(uint64_t* b, uint32_t n) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(n));
@@ -293,6 +299,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
   __syncthreads();
   cluster_sync();
   fence_after();
+  after_previous();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
   if (wid == 0) {
@@ -419,16 +426,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
   }
 }
 
-// Launches a job on every pair of SMs.
+// CTAs of a launch: all pairs of SMs
 inline int pair_ctas() { return num_sms() & ~1; }
-template <class Job>
-int launch(const Job& job, cudaStream_t st) {
-  const int rc = ensure_smem(reinterpret_cast<const void*>(&mma_kernel<Job>), smem_bytes<Job>());
-  if (rc) return rc;
-  mma_kernel<Job><<<pair_ctas(), kThreads, smem_bytes<Job>(), st>>>(job);
-  GSP_CHECK_LAUNCH();
-  return GSP_OK;
-}
 
 }  // namespace mm
 }  // namespace gsp

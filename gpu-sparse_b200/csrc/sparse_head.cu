@@ -203,9 +203,8 @@ struct HeadJob {
 
 struct JoinParams {
   const int32_t *head, *map;
-  const uint8_t* mask;
   int32_t L, bn, pairs, nvt;
-  int64_t B, V;
+  int64_t V;
   const float* bias;
   const float* part_m;
   const int32_t* part_i;
@@ -213,21 +212,11 @@ struct JoinParams {
   int32_t* win;
 };
 
-// Blocks [0, pairs): a text that began in an earlier share and ends in this one is joined from
-// the shares it crosses, in order.  Blocks past them: texts without tokens get zero rows.
+// A block per share: a text that began in an earlier share and ends in this one is joined from
+// the shares it crosses, in order.
 __global__ void __launch_bounds__(mm::kBM) head_join_kernel(const JoinParams p) {
+  mm::after_previous();
   const int32_t n = p.head[0];
-  if (int32_t(blockIdx.x) >= p.pairs) {
-    const int64_t b = int64_t(blockIdx.x) - p.pairs;
-    bool any = false;
-    for (int64_t t = threadIdx.x; t < p.L; t += mm::kBM) any |= p.mask[b * p.L + t] != 0;
-    if (__syncthreads_or(any)) return;
-    for (int64_t v = threadIdx.x; v < p.V; v += mm::kBM) {
-      p.y[b * p.V + v] = 0.0f;
-      if (p.win) p.win[b * p.V + v] = -1;
-    }
-    return;
-  }
   const int32_t ntt = (n + p.bn - 1) / p.bn, tot = ntt * p.nvt, c = blockIdx.x;
   const int32_t lo = share_lo(tot, p.pairs, c), hi = share_lo(tot, p.pairs, c + 1);
   if (lo >= hi) return;
@@ -306,6 +295,7 @@ inline int sort_warps(int64_t L) { return int(L * 4 * 8 <= kSortSmem ? 8 : kSort
 // zeroed before.)
 __global__ void __launch_bounds__(256)
 survey_kernel(State s, const SortParams p, Survey* out, void* d_hidden, int64_t hidden_bytes) {
+  mm::after_previous();
   extern __shared__ int32_t counters[];
   const int lane = lane_id(), wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int64_t job = int64_t(blockIdx.x) * warps + wid, b = job / kSegs;
@@ -359,6 +349,7 @@ survey_kernel(State s, const SortParams p, Survey* out, void* d_hidden, int64_t 
 
 // The list: every warp places its run's entries where the scan says.
 __global__ void __launch_bounds__(256) place_kernel(const SortParams p) {
+  mm::after_previous();
   extern __shared__ int32_t counters[];
   const int lane = lane_id(), wid = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int64_t job = int64_t(blockIdx.x) * warps + wid, b = job / kSegs;
@@ -457,6 +448,7 @@ __device__ __forceinline__ void store8(uint16_t* out, int n, const float (&v)[8]
 constexpr int kTexts = 256;
 template <int kCols>
 __global__ void __launch_bounds__(256, 2) gather_weight_kernel(const GatherParams p) {
+  mm::after_previous();
   __shared__ int32_t row[kTexts][9];
   __shared__ float grad[kTexts][9];
   const bool gather = p.sparse.gather(p.head[0], p.V) && p.dw;
@@ -558,6 +550,7 @@ __device__ __forceinline__ void gather_run(const GatherParams& p, int32_t lo, in
 }
 template <int kCols>
 __global__ void __launch_bounds__(256, 2) gather_hidden_kernel(const GatherParams p) {
+  mm::after_previous();
   __shared__ float4 sums[7][2][32];
   const int32_t n = p.head[0], r0 = blockIdx.x * 8;
   if (r0 >= n || !p.sparse.gather(n, p.V)) return;
@@ -628,6 +621,7 @@ constexpr int kSpreadRows = 64;
 // P of a piece: a thread owns 8 columns of one text and writes them for up to kSpreadRows of
 // its rows; the blocks of text B zero the rows past the packed ones.
 __global__ void __launch_bounds__(256) spread_kernel(const SpreadParams p) {
+  mm::after_previous();
   const int32_t n = p.head[0];
   if (p.sparse.gather(n, p.V)) return;
   const int64_t c = (int64_t(blockIdx.x) * 256 + threadIdx.x) * 8;
@@ -667,6 +661,7 @@ __global__ void __launch_bounds__(256) spread_kernel(const SpreadParams p) {
 
 // ---- dense rows -> CSR -------------------------------------------------------------------
 __global__ void __launch_bounds__(1024) rows_count_kernel(const float* y, int64_t V, float min_weight, int32_t* nnz) {
+  mm::after_previous();
   __shared__ int32_t part[32];
   const float* row = y + int64_t(blockIdx.x) * V;
   int32_t n = 0;
@@ -681,6 +676,7 @@ __global__ void __launch_bounds__(1024) rows_count_kernel(const float* y, int64_
 }
 __global__ void __launch_bounds__(1024)
 rows_fill_kernel(const float* y, int64_t V, float min_weight, const int64_t* indptr, int32_t* indices, float* data) {
+  mm::after_previous();
   __shared__ int32_t part[32];
   const float* row = y + int64_t(blockIdx.x) * V;
   const int wid = threadIdx.x >> 5, lane = lane_id();
@@ -709,7 +705,6 @@ rows_fill_kernel(const float* y, int64_t V, float min_weight, const int64_t* ind
 struct Fwd {
   int32_t *counts, *part_i;
   float* part_m;
-  void* wcopy;
   int64_t bytes;
 };
 Fwd carve_fwd(void* base, const gsp_vocab_view* vw) {
@@ -718,7 +713,6 @@ Fwd carve_fwd(void* base, const gsp_vocab_view* vw) {
   f.counts = c.take<int32_t>(pack_counts(vw->T));
   f.part_m = c.take<float>(int64_t(mm::pair_ctas()) * mm::kBM);
   f.part_i = c.take<int32_t>(int64_t(mm::pair_ctas()) * mm::kBM);
-  f.wcopy = c.take<char>(weight_copy_bytes(vw));
   f.bytes = c.off;
   return f;
 }
@@ -731,7 +725,6 @@ struct Bwd {
   GradScratch grad;
   uint16_t* P;        // or the list
   int64_t zeroed, scan_bytes, room;
-  void* wcopy;
   int64_t pitch, bytes;
 };
 Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
@@ -749,14 +742,14 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
   b.grad = carve_grad(c, vw, Tp, b.pitch);
   b.P = c.take<uint16_t>(Tp * b.pitch);
   b.room = Tp * b.pitch * 2 / int64_t(sizeof(int2));
-  b.wcopy = c.take<char>(weight_copy_bytes(vw));
   b.bytes = c.off;
   return b;
 }
 
 template <bool kWin>
 int run_head(const gsp_vocab_view* vw, const State& s, const Fwd& f, int32_t L, int32_t bn, float* y, int32_t* win,
-             const uint16_t* w, int64_t ldw, cudaStream_t st) {
+             cudaStream_t st) {
+  const Weight w = weight_rows(vw, s);
   HeadJob<kWin> j{};
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = is_bf16(vw);
@@ -774,9 +767,9 @@ int run_head(const gsp_vocab_view* vw, const State& s, const Fwd& f, int32_t L, 
   j.part_i = f.part_i;
   const bool bf = is_bf16(vw);
   int rc;
-  if ((rc = make_map(&j.maps[0], bf, w, vw->D, vw->V, ldw, mm::kRows))) return rc;
+  if ((rc = make_map(&j.maps[0], bf, w.w, vw->D, vw->V, w.ld, mm::kRows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, s.h, s.Dp, vw->T, s.Dp, bn / 2))) return rc;
-  return mm::launch(j, st);
+  return launch_mma(j, st);
 }
 
 // blocks of 256 columns that a lane of the gathering kernels holds
@@ -818,31 +811,26 @@ extern "C" int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_
                                int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream) {
   int rc = check_texts(vw, L, "sparse_head");
   if (rc) return rc;
-  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, vw->T > 0 ? vw->T : 1);
+  const State s = carve_state(state, vw, 0, vw->T > 0 ? vw->T : 1);
   const Fwd f = carve_fwd(ws, vw);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "sparse_head: state or workspace too small");
   if (vw->T == 0) return GSP_OK;
   GSP_REQUIRE(vw->hidden && vw->weight && y, GSP_ERR_ARG, "sparse_head: null input or output");
   cudaStream_t st = as_stream(stream);
-  if ((rc = pack_rows(vw, nullptr, 0, mask, 0.0f, L, s, f.counts, st))) return rc;
-  const uint16_t* w;
-  int64_t ldw;
-  if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
+  if ((rc = pack_rows(vw, nullptr, 0, mask, 0.0f, Texts{L, y, win}, s, f.counts, st))) return rc;
   // columns of a tile: no more than the tokens need (a single query's product is then as short
   // as reading W allows)
   const int32_t bn = int32_t(vw->T >= mm::kBN ? mm::kBN : up(vw->T, 64));
-  rc = win ? run_head<true>(vw, s, f, int32_t(L), bn, y, win, w, ldw, st)
-           : run_head<false>(vw, s, f, int32_t(L), bn, y, win, w, ldw, st);
-  if (rc) return rc;
+  rc = win ? run_head<true>(vw, s, f, int32_t(L), bn, y, win, st)
+           : run_head<false>(vw, s, f, int32_t(L), bn, y, win, st);
+  if (rc || vw->T <= bn) return rc;      // one tile of tokens: no share cuts a text
   JoinParams p{};
   p.head = s.head;
   p.map = s.map;
-  p.mask = mask;
   p.L = int32_t(L);
   p.bn = bn;
   p.pairs = mm::pair_ctas() / 2;
-  p.B = vw->T / L;
   p.V = vw->V;
   p.nvt = int32_t((vw->V + mm::kBM - 1) / mm::kBM);
   p.bias = vw->bias;
@@ -850,9 +838,7 @@ extern "C" int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_
   p.part_i = f.part_i;
   p.y = y;
   p.win = win;
-  head_join_kernel<<<unsigned(p.pairs + (mask ? p.B : 0)), mm::kBM, 0, st>>>(p);
-  GSP_CHECK_LAUNCH();
-  return GSP_OK;
+  return launch(head_join_kernel, dim3(unsigned(p.pairs)), mm::kBM, 0, st, p);
 }
 
 extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, const float* y, const int32_t* win,
@@ -861,7 +847,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   int rc = check_texts(vw, L, "sparse_head backward");
   if (rc) return rc;
   if ((rc = check_grads(vw, d_hidden, d_weight, "sparse_head backward"))) return rc;
-  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, vw->T > 0 ? vw->T : 1);
+  const State s = carve_state(state, vw, 0, vw->T > 0 ? vw->T : 1);
   const Bwd b = carve_bwd(ws, vw);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,
               "sparse_head backward: state or workspace too small");
@@ -874,9 +860,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   GSP_REQUIRE(y && win && dy && vw->weight, GSP_ERR_ARG, "sparse_head backward: null input");
   const int64_t B = vw->T / L;
   const bool bf = is_bf16(vw);
-  const uint16_t* w;
-  int64_t ldw;
-  if ((rc = weight_rows(vw, b.wcopy, &w, &ldw, st))) return rc;
+  const Weight w = weight_rows(vw, s);
   // longer texts than the sort has counters for take the products
   const bool sort = d_hidden && L * 4 <= kSortSmem, may = !d_hidden || sort;
   GSP_CUDA(cudaMemsetAsync(b.survey, 0, size_t(sort ? b.zeroed : int64_t(sizeof(Survey))), st));
@@ -896,12 +880,11 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   const int warps = sort ? sort_warps(L) : 8;
   const unsigned sort_blocks = unsigned((B * kSegs + warps - 1) / warps);
   const size_t sort_bytes = sort ? size_t(warps) * size_t(L) * 4 : 0;
-  survey_kernel<<<sort_blocks, 32 * warps, sort_bytes, st>>>(s, q, b.survey, d_hidden, vw->T * vw->D * 2);
-  GSP_CHECK_LAUNCH();
+  rc = launch(survey_kernel, dim3(sort_blocks), 32 * warps, sort_bytes, st, s, q, b.survey, d_hidden, vw->T * vw->D * 2);
+  if (rc) return rc;
   if (sort) {
     if ((rc = gsp_scan_i32(b.count, vw->T * kSegs, b.offset, b.scan, b.scan_bytes, stream))) return rc;
-    place_kernel<<<sort_blocks, 32 * warps, sort_bytes, st>>>(q);
-    GSP_CHECK_LAUNCH();
+    if ((rc = launch(place_kernel, dim3(sort_blocks), 32 * warps, sort_bytes, st, q))) return rc;
   }
   GatherParams g{};
   g.head = s.head;
@@ -913,9 +896,9 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   g.dy = dy;
   g.win = win;
   g.h = s.h;
-  g.w = w;
+  g.w = w.w;
   g.Dp = s.Dp;
-  g.ldw = ldw;
+  g.ldw = w.ld;
   g.B = B;
   g.V = vw->V;
   g.D = vw->D;
@@ -925,23 +908,21 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   g.db = d_bias;
   if (d_weight || d_bias) {
     const unsigned blocks = unsigned((vw->V + 7) / 8);
-    switch (gather_cols(vw->D)) {
-      case 1: gather_weight_kernel<1><<<blocks, 256, 0, st>>>(g); break;
-      case 2: gather_weight_kernel<2><<<blocks, 256, 0, st>>>(g); break;
-      case 3: gather_weight_kernel<3><<<blocks, 256, 0, st>>>(g); break;
-      default: gather_weight_kernel<4><<<blocks, 256, 0, st>>>(g);
-    }
-    GSP_CHECK_LAUNCH();
+    const int cols = gather_cols(vw->D);
+    const auto kernel = cols == 1   ? gather_weight_kernel<1>
+                        : cols == 2 ? gather_weight_kernel<2>
+                        : cols == 3 ? gather_weight_kernel<3>
+                                    : gather_weight_kernel<4>;
+    if ((rc = launch(kernel, dim3(blocks), 256, 0, st, g))) return rc;
   }
   if (sort) {
     const dim3 blocks(unsigned((vw->T + 7) / 8), unsigned((vw->D + 1023) / 1024));
-    switch (gather_cols(vw->D)) {
-      case 1: gather_hidden_kernel<1><<<blocks, 256, 0, st>>>(g); break;
-      case 2: gather_hidden_kernel<2><<<blocks, 256, 0, st>>>(g); break;
-      case 3: gather_hidden_kernel<3><<<blocks, 256, 0, st>>>(g); break;
-      default: gather_hidden_kernel<4><<<blocks, 256, 0, st>>>(g);
-    }
-    GSP_CHECK_LAUNCH();
+    const int cols = gather_cols(vw->D);
+    const auto kernel = cols == 1   ? gather_hidden_kernel<1>
+                        : cols == 2 ? gather_hidden_kernel<2>
+                        : cols == 3 ? gather_hidden_kernel<3>
+                                    : gather_hidden_kernel<4>;
+    if ((rc = launch(kernel, blocks, 256, 0, st, g))) return rc;
   }
   if (!d_hidden && !d_weight) return GSP_OK;
   SpreadParams p{};
@@ -964,10 +945,10 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   for (int64_t v0 = 0; v0 < vw->V; v0 += b.pitch) {
     p.v0 = v0;
     p.cols = min64(b.pitch, vw->V - v0);
-    spread_kernel<<<dim3(unsigned((b.pitch / 8 + 255) / 256), unsigned(B + 1), unsigned(zs)), 256, 0, st>>>(p);
-    GSP_CHECK_LAUNCH();
+    rc = launch(spread_kernel, dim3(unsigned((b.pitch / 8 + 255) / 256), unsigned(B + 1), unsigned(zs)), 256, 0, st, p);
+    if (rc) return rc;
     const GradPiece pc{b.P, b.pitch, v0, p.cols, v0 == 0, v0 + p.cols >= vw->V, q.sparse};
-    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, BiasSums{}, b.scale, d_hidden, d_weight, st))) return rc;
+    if ((rc = grad_products(vw, s, w.w, w.ld, pc, b.grad, BiasSums{}, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
 }
@@ -975,16 +956,12 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
 extern "C" int gsp_dense_rows_count(const float* y, int64_t B, int64_t V, float min_weight, int32_t* nnz, void* stream) {
   GSP_REQUIRE(B >= 0 && V >= 1 && (B == 0 || (y && nnz)), GSP_ERR_ARG, "gsp_dense_rows_count: bad arguments");
   if (B == 0) return GSP_OK;
-  rows_count_kernel<<<unsigned(B), 1024, 0, as_stream(stream)>>>(y, V, min_weight, nnz);
-  GSP_CHECK_LAUNCH();
-  return GSP_OK;
+  return launch(rows_count_kernel, dim3(unsigned(B)), 1024, 0, as_stream(stream), y, V, min_weight, nnz);
 }
 
 extern "C" int gsp_dense_rows_fill(const float* y, int64_t B, int64_t V, float min_weight, const int64_t* indptr,
                                    int32_t* indices, float* data, void* stream) {
   GSP_REQUIRE(B >= 0 && V >= 1 && (B == 0 || (y && indptr)), GSP_ERR_ARG, "gsp_dense_rows_fill: bad arguments");
   if (B == 0) return GSP_OK;
-  rows_fill_kernel<<<unsigned(B), 1024, 0, as_stream(stream)>>>(y, V, min_weight, indptr, indices, data);
-  GSP_CHECK_LAUNCH();
-  return GSP_OK;
+  return launch(rows_fill_kernel, dim3(unsigned(B)), 1024, 0, as_stream(stream), y, V, min_weight, indptr, indices, data);
 }

@@ -32,6 +32,7 @@ __device__ __forceinline__ bool row_valid(const int64_t* targets, int64_t ignore
 
 __global__ void __launch_bounds__(256) count_kernel(const int64_t* targets, int64_t ignore, const uint8_t* flag, int64_t V,
                                                     int64_t T, int32_t* counts) {
+  mm::after_previous();
   const int64_t r = int64_t(blockIdx.x) * 256 + threadIdx.x;
   const int n = __syncthreads_count(r < T && row_valid(targets, ignore, flag, V, r));
   if (threadIdx.x == 0) counts[blockIdx.x] = n;
@@ -64,16 +65,40 @@ struct PackParams {
   uint16_t* h;
   int32_t *map, *head, *tgt, *text;
   int32_t L;                // > 0: texts of L rows
+  float* y;
+  int32_t* win;
+  const uint16_t* weight;   // to copy, or null
+  int64_t ldw, Dw;
+  uint16_t* w;
+  int32_t per, pack_blocks, text_blocks;      // rows per block; blocks of each kind, W's copy last
 };
 
-// 32 rows per CTA: their packed position is the number of valid rows before them.
+// Blocks of p.per (at most 32) rows: their packed position is the number of valid rows before
+// them.  Then a block per text that may be empty, and blocks of 8 rows of W's copy.
 __global__ void __launch_bounds__(256) pack_kernel(const PackParams p) {
   __shared__ int32_t part[8];
   __shared__ uint32_t word;
-  const int64_t r0 = int64_t(blockIdx.x) * 32;
   const int wid = threadIdx.x >> 5, lane = lane_id();
+  mm::after_previous();
+  if (int32_t(blockIdx.x) >= p.pack_blocks) {
+    const int64_t b = int32_t(blockIdx.x) - p.pack_blocks;
+    if (b < p.text_blocks) {
+      bool any = false;
+      for (int64_t t = threadIdx.x; t < p.L; t += 256) any |= p.flag[b * p.L + t] != 0;
+      if (__syncthreads_or(any)) return;
+      for (int64_t v = threadIdx.x; v < p.V; v += 256) {
+        p.y[b * p.V + v] = 0.0f;
+        if (p.win) p.win[b * p.V + v] = -1;
+      }
+    } else {
+      const int64_t r = (b - p.text_blocks) * 8 + wid;
+      if (r < p.V) copy_row(p.weight + r * p.ldw, p.w + r * p.Dw, p.D, p.Dw, lane);
+    }
+    return;
+  }
+  const int64_t r0 = int64_t(blockIdx.x) * p.per;
   if (p.bias_scale != 0.0f) {
-    for (int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x; v < p.Vp; v += int64_t(gridDim.x) * 256)
+    for (int64_t v = int64_t(blockIdx.x) * 256 + threadIdx.x; v < p.Vp; v += int64_t(p.pack_blocks) * 256)
       p.bias2[v] = v < p.V ? (p.bias ? p.bias[v] * p.bias_scale : 0.0f) : neg_inf();
   }
   if (r0 >= p.T) return;
@@ -88,7 +113,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackParams p) {
   mine = __reduce_add_sync(FULL, mine);
   if (lane == 0) part[wid] = mine;
   if (wid == 0) {
-    const uint32_t w = __ballot_sync(FULL, r0 + lane < p.T && row_valid(p.targets, p.ignore, p.flag, p.V, r0 + lane));
+    const uint32_t w = __ballot_sync(FULL, lane < p.per && r0 + lane < p.T && row_valid(p.targets, p.ignore, p.flag, p.V, r0 + lane));
     if (lane == 0) word = w;
   }
   __syncthreads();
@@ -96,7 +121,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackParams p) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) base += part[i];
   const uint32_t w = word;
-  for (int i = wid; i < 32; i += 8) {
+  for (int i = wid; i < p.per; i += 8) {
     if (!((w >> i) & 1)) continue;
     const int32_t d = base + __popc(w & ((1u << i) - 1));
     copy_row(p.hidden + (r0 + i) * p.ldh, p.h + int64_t(d) * p.Dp, p.D, p.Dp, lane);
@@ -107,19 +132,13 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackParams p) {
   }
   if (p.L > 0 && wid == 0) {
     const int64_t r = r0 + lane;
-    if (r < p.T && r % p.L == 0) p.text[r / p.L] = base + __popc(w & lanemask_lt());
+    if (lane < p.per && r < p.T && r % p.L == 0) p.text[r / p.L] = base + __popc(w & lanemask_lt());
   }
-  if (r0 + 32 >= p.T && threadIdx.x == 0) {
+  if (r0 + p.per >= p.T && threadIdx.x == 0) {
     if (p.L > 0) p.text[p.T / p.L] = base + __popc(w);
     p.head[0] = base + __popc(w);
     p.head[1] = 0;
   }
-}
-
-__global__ void __launch_bounds__(256) copy_weight_kernel(const uint16_t* w, int64_t ldw, int64_t V, int64_t D, int64_t Dp,
-                                                          uint16_t* out) {
-  const int64_t r = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (r < V) copy_row(w + r * ldw, out + r * Dp, D, Dp, lane_id());
 }
 
 // ---- backward products -------------------------------------------------------------------
@@ -131,6 +150,7 @@ __global__ void __launch_bounds__(256) copy_weight_kernel(const uint16_t* w, int
 // frag_kernel, in list order.  Pairs are dealt to the 256-wide tiles of D in turn, so that the
 // pairs that read the same rows of P run side by side.
 constexpr int kOutBytes = 32 * 128;    // a warp's 32 rows x 64 columns of dW on their way out
+constexpr int kFinishRows = 16;
 constexpr int kTileCost = 3;           // steps an epilogue counts for in the cut
 
 struct GradList {
@@ -351,17 +371,18 @@ __device__ void bias_grad(const BiasSums& b, int32_t n, int32_t cols, const floa
 }
 
 // Finishes the tiles that a border between two shares cuts: the pair whose share holds a tile's
-// last step adds the fragments in list order.  Block (pair, CTA of the pair, 8 rows): a warp per
-// row, 8 columns per lane.  The blocks past them finish d_bias.
+// last step adds the fragments in list order.  Block (pair, CTA of the pair, 16 rows): two rows per
+// warp, 8 columns per lane.  The blocks past them finish d_bias.
 __global__ void __launch_bounds__(256)
 finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blocks, const BiasSums b) {
+  mm::after_previous();
   if (int32_t(blockIdx.x) >= frag_blocks) {
     bias_grad(b, *j.n_rows, j.cols, j.scale, int64_t(blockIdx.x) - frag_blocks);
     return;
   }
   const GradList l = j.list();
   const int64_t tot = l.total();
-  const int32_t pair = blockIdx.x / (2 * mm::kRows / 8), sub = blockIdx.x % (2 * mm::kRows / 8);
+  const int32_t pair = blockIdx.x / (2 * mm::kRows / kFinishRows), sub = blockIdx.x % (2 * mm::kRows / kFinishRows);
   const int32_t groups = j.groups(pairs, tot);
   const int32_t g = pair / j.nbs, nb = pair % j.nbs;
   if (g >= groups) return;
@@ -372,23 +393,28 @@ finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blo
   l.at(x0, &is_h, &blk, &start, &nk);
   if (x0 == start || x0 - start >= nk || x1 - start < nk) return;    // begins here, or ends elsewhere
   const int32_t first = int32_t(((start + 1) * groups - 1) / tot);   // the share that holds the tile's first step
-  const int32_t rank = sub & 1, row = (sub >> 1) * 8 + (threadIdx.x >> 5), c = lane_id() * 8;
-  const int32_t r = blk * mm::kBM + rank * mm::kRows + row;
-  if (r >= (is_h ? *j.n_rows : j.cols) || nb * mm::kBN + c >= j.D) return;      // (D up to ld_out is padding)
-  float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int32_t s = first; s <= g; ++s) {
-    uint32_t o[8];
-    ld256(j.fragment(s * j.nbs + nb, s == first, rank) + row * mm::kBN + c, o);
+  const int32_t rank = sub & 1, c = lane_id() * 8;
+  if (nb * mm::kBN + c >= j.D) return;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] += __uint_as_float(o[k]);
+  for (int i = 0; i < kFinishRows / 8; ++i) {
+    const int32_t row = (sub >> 1) * kFinishRows + i * 8 + (threadIdx.x >> 5), r = blk * mm::kBM + rank * mm::kRows + row;
+    if (r >= (is_h ? *j.n_rows : j.cols)) return;
+    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int32_t s = first; s <= g; ++s) {
+      uint32_t o[8];
+      ld256(j.fragment(s * j.nbs + nb, s == first, rank) + row * mm::kBN + c, o);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += __uint_as_float(o[k]);
+    }
+    j.finish8(is_h, r, nb * mm::kBN + c, v);
   }
-  j.finish8(is_h, r, nb * mm::kBN + c, v);
 }
 
 }  // namespace
 
-State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, int64_t texts) {
+State carve_state(void* base, const gsp_vocab_view* vw, int64_t K, int64_t texts) {
+  const int64_t T = vw->T, V = vw->V, D = vw->D;
   State s{};
   Carver c{static_cast<char*>(base)};
   s.Tp = pad_rows(T);
@@ -413,6 +439,7 @@ State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, int64_
     s.buckets = (s.Vp + (int64_t(1) << s.bucket_shift) - 1) >> s.bucket_shift;
     s.off = c.take<int32_t>(s.Tp / 32 * (s.buckets + 1));
   }
+  if (!weight_direct(vw)) s.w = c.take<uint16_t>(V * up(D, 8));
   s.bytes = c.off;
   return s;
 }
@@ -427,26 +454,6 @@ int check_view(const gsp_vocab_view* vw, const char* what) {
   GSP_REQUIRE(up256(vw->T) / 256 * (up256(vw->V) / 256) < (int64_t(1) << 31), GSP_ERR_ARG,
               "%s: %lld tokens x %lld vocabulary rows are too many for one call", what, (long long)vw->T, (long long)vw->V);
   GSP_REQUIRE(vw->ld_hidden >= vw->D && vw->ld_weight >= vw->D, GSP_ERR_ARG, "%s: row stride smaller than the width", what);
-  return GSP_OK;
-}
-
-int64_t weight_copy_bytes(const gsp_vocab_view* vw) {
-  const bool direct = vw->ld_weight % 8 == 0 && (reinterpret_cast<uintptr_t>(vw->weight) & 15) == 0 && vw->ld_weight < (int64_t(1) << 38);
-  return direct ? 0 : up256(vw->V * up(vw->D, 8) * 2);
-}
-
-int weight_rows(const gsp_vocab_view* vw, void* scratch, const uint16_t** w, int64_t* ld, cudaStream_t st) {
-  if (weight_copy_bytes(vw) == 0) {
-    *w = static_cast<const uint16_t*>(vw->weight);
-    *ld = vw->ld_weight;
-    return GSP_OK;
-  }
-  const int64_t Dp = up(vw->D, 8);
-  copy_weight_kernel<<<unsigned((vw->V + 7) / 8), 256, 0, st>>>(static_cast<const uint16_t*>(vw->weight), vw->ld_weight, vw->V,
-                                                              vw->D, Dp, static_cast<uint16_t*>(scratch));
-  GSP_CHECK_LAUNCH();
-  *w = static_cast<const uint16_t*>(scratch);
-  *ld = Dp;
   return GSP_OK;
 }
 
@@ -479,14 +486,15 @@ int make_map_mn(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64
 }
 
 int pack_rows(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore, const uint8_t* flag, float bias_scale,
-              int64_t L, const State& s, int32_t* counts, cudaStream_t st) {
+              const Texts& texts, const State& s, int32_t* counts, cudaStream_t st) {
   const int64_t T = vw->T;
+  int rc;
   // up to 2048 rows every CTA counts the rows before its own itself (at most 8 loads a
   // thread), which saves the launch of the counting pass
   const bool pre = T > 2048;
   if (pre) {
-    count_kernel<<<unsigned((T + 255) / 256), 256, 0, st>>>(targets, ignore, flag, vw->V, T, counts);
-    GSP_CHECK_LAUNCH();
+    rc = launch(count_kernel, dim3(unsigned((T + 255) / 256)), 256, 0, st, targets, ignore, flag, vw->V, T, counts);
+    if (rc) return rc;
   }
   PackParams p{};
   p.hidden = static_cast<const uint16_t*>(vw->hidden);
@@ -508,11 +516,19 @@ int pack_rows(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore, 
   p.head = s.head;
   p.tgt = s.tgt;
   p.text = s.text;
-  p.L = int32_t(L);
-  const int64_t blocks = (T + 31) / 32;
-  pack_kernel<<<unsigned(blocks < 32 ? 32 : blocks), 256, 0, st>>>(p);
-  GSP_CHECK_LAUNCH();
-  return GSP_OK;
+  p.L = int32_t(texts.L);
+  p.y = texts.y;
+  p.win = texts.win;
+  p.weight = static_cast<const uint16_t*>(vw->weight);
+  p.ldw = vw->ld_weight;
+  p.Dw = up(vw->D, 8);
+  p.w = s.w;
+  p.per = T <= 4096 ? 8 : 32;      // few rows: more CTAs, a row per warp
+  const int64_t blocks = (T + p.per - 1) / p.per;
+  p.pack_blocks = int32_t(blocks < 32 ? 32 : blocks);
+  p.text_blocks = int32_t(texts.L > 0 && flag ? T / texts.L : 0);
+  const int64_t copy_blocks = s.w ? (vw->V + 7) / 8 : 0;
+  return launch(pack_kernel, dim3(unsigned(p.pack_blocks + p.text_blocks + copy_blocks)), 256, 0, st, p);
 }
 
 int64_t piece_cols(int64_t Tp, int64_t V) {
@@ -546,6 +562,7 @@ GradScratch carve_grad(Carver& c, const gsp_vocab_view* vw, int64_t Tp, int64_t 
 __global__ void __launch_bounds__(256)
 unpad_kernel(const uint16_t* dh, const int32_t* n_rows, const int32_t* map, uint16_t* out_h, int64_t h_blocks,
              const uint16_t* dw, int64_t V, uint16_t* out_w, int64_t ld, int64_t D, Sparse sparse) {
+  mm::after_previous();
   if (sparse.gather(*n_rows, V)) return;
   const int lane = lane_id();
   const int64_t warp = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -603,20 +620,19 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.scale = scale;
   j.dh = dh;
   j.dw = dw;
-  if ((d_hidden || d_weight) && (rc = mm::launch(j, st))) return rc;
+  if ((d_hidden || d_weight) && (rc = launch_mma(j, st))) return rc;
   const int32_t pairs = mm::pair_ctas() / 2;
   // with more D tiles than pairs no tile is cut
-  const int32_t frag_blocks = (d_hidden || d_weight) && j.nbs <= pairs ? pairs * (2 * mm::kRows / 8) : 0;
+  const int32_t frag_blocks = (d_hidden || d_weight) && j.nbs <= pairs ? pairs * (2 * mm::kRows / kFinishRows) : 0;
   const int32_t blocks = frag_blocks + (bias.out ? int32_t((pc.cols + 31) / 32) : 0);
   if (blocks > 0) {
-    finish_kernel<<<unsigned(blocks), 256, 0, st>>>(j, pairs, frag_blocks, bias);
-    GSP_CHECK_LAUNCH();
+    if ((rc = launch(finish_kernel, dim3(unsigned(blocks)), 256, 0, st, j, pairs, frag_blocks, bias))) return rc;
   }
   if (padded && pc.last && (d_hidden || d_weight)) {
     const int64_t hb = d_hidden ? (vw->T + 7) / 8 : 0, wb = d_weight ? (vw->V + 7) / 8 : 0;
-    unpad_kernel<<<unsigned(hb + wb), 256, 0, st>>>(dh, s.head, s.map, static_cast<uint16_t*>(d_hidden), hb, dw, vw->V,
-                                                   static_cast<uint16_t*>(d_weight), j.ld_out, vw->D, pc.sparse);
-    GSP_CHECK_LAUNCH();
+    rc = launch(unpad_kernel, dim3(unsigned(hb + wb)), 256, 0, st, dh, s.head, s.map, static_cast<uint16_t*>(d_hidden), hb, dw,
+                vw->V, static_cast<uint16_t*>(d_weight), j.ld_out, vw->D, pc.sparse);
+    if (rc) return rc;
   }
   return GSP_OK;
 }
@@ -624,12 +640,14 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
 }  // namespace vocab
 }  // namespace gsp
 
-extern "C" int64_t gsp_vocab_state_bytes(int64_t T, int64_t V, int64_t D, int64_t K, int32_t kind) {
-  if (T < 0 || V < 1 || D < 1 || K < 0 || kind < GSP_VOCAB_CE || kind > GSP_VOCAB_HEAD) {
+extern "C" int64_t gsp_vocab_state_bytes(const gsp_vocab_view* vw, int64_t K, int32_t kind) {
+  const int rc = gsp::vocab::check_view(vw, "gsp_vocab_state_bytes");
+  if (rc) return -rc;
+  if (K < 0 || kind < GSP_VOCAB_CE || kind > GSP_VOCAB_HEAD) {
     gsp::set_error("gsp_vocab_state_bytes: bad arguments");
     return -GSP_ERR_ARG;
   }
   // the sparse head's texts: at most one per token
-  return gsp::vocab::carve_state(nullptr, T, V, D, kind == GSP_VOCAB_DISTILL ? K : 0,
-                                 kind == GSP_VOCAB_HEAD ? (T > 0 ? T : 1) : 0).bytes;
+  return gsp::vocab::carve_state(nullptr, vw, kind == GSP_VOCAB_DISTILL ? K : 0,
+                                 kind == GSP_VOCAB_HEAD ? (vw->T > 0 ? vw->T : 1) : 0).bytes;
 }

@@ -38,20 +38,30 @@ struct State {
   int4* hit;          // a teacher's entries of every 32 packed rows by vocabulary bucket: (id, row
                       // of the 32, probability's bits, entry of the row), 32 K a group
   int32_t* off;       // [Tp / 32, buckets + 1] first hit of every bucket
+  uint16_t* w;        // [V, up(D, 8)] copy of a projection whose rows a TMA map cannot describe
   int64_t Tp, Dp, Vp, K, buckets, bytes;
   int32_t bucket_shift;      // log2 of a bucket's vocabulary rows
 };
 constexpr int32_t kNoId = 0x7FFFFFFF;
 // loss: texts is 0; sparse head: K is 0
-State carve_state(void* base, int64_t T, int64_t V, int64_t D, int64_t K, int64_t texts);
+State carve_state(void* base, const gsp_vocab_view* vw, int64_t K, int64_t texts);
 
 int check_view(const gsp_vocab_view* vw, const char* what);
 int check_grads(const gsp_vocab_view* vw, const void* d_hidden, const void* d_weight, const char* what);
 inline bool is_bf16(const gsp_vocab_view* vw) { return vw->dtype == GSP_W_BF16; }
-// bytes of the copy of W that a projection whose rows a TMA map cannot describe needs (else 0)
-int64_t weight_copy_bytes(const gsp_vocab_view* vw);
-// W as a TMA map can describe it: the caller's, or a copy in `scratch`
-int weight_rows(const gsp_vocab_view* vw, void* scratch, const uint16_t** w, int64_t* ld, cudaStream_t st);
+// whether a TMA map can describe W's rows as they are (else the forward call copies them)
+inline bool weight_direct(const gsp_vocab_view* vw) {
+  return vw->ld_weight % 8 == 0 && (reinterpret_cast<uintptr_t>(vw->weight) & 15) == 0 && vw->ld_weight < (int64_t(1) << 38);
+}
+// W as a TMA map can describe it
+struct Weight {
+  const uint16_t* w;
+  int64_t ld;
+};
+inline Weight weight_rows(const gsp_vocab_view* vw, const State& s) {
+  if (s.w) return Weight{s.w, up(vw->D, 8)};
+  return Weight{static_cast<const uint16_t*>(vw->weight), vw->ld_weight};
+}
 
 // 2D map of a row-major 16-bit matrix: boxes of 64 columns x box_rows rows, 128-byte swizzle,
 // zeros outside
@@ -61,10 +71,16 @@ int make_map(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t 
 int make_map_mn(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld);
 
 // Packs the rows that take part (targets: id in [0, V) and != ignore; else flag != 0) to the
-// front of st.h, keeping their order, and writes st.map, st.head[0]; bias2 when scale != 0.
-// L > 0: rows are texts of L tokens, and st.text is written.
+// front of st.h, keeping their order, and writes st.map, st.head[0] and st.w; bias2 when
+// bias_scale != 0.  Texts (texts.L > 0): st.text, and zero rows of y (and -1 in win) for those
+// without tokens.
+struct Texts {
+  int64_t L;
+  float* y;
+  int32_t* win;
+};
 int pack_rows(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignore, const uint8_t* flag, float bias_scale,
-              int64_t L, const State& s, int32_t* counts, cudaStream_t st);
+              const Texts& texts, const State& s, int32_t* counts, cudaStream_t st);
 inline int64_t pack_counts(int64_t T) { return (T + 255) / 256 + 1; }
 
 // How sparse the gradient of the logits is: with so few of n x V entries nonzero that gathering
@@ -125,6 +141,33 @@ __device__ __forceinline__ void zero_share(void* d, int64_t bytes, int64_t block
   }
   uint4* p = reinterpret_cast<uint4*>(c + head);
   for (int64_t i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) p[i] = make_uint4(0, 0, 0, 0);
+}
+
+// ---- launches ----------------------------------------------------------------------------
+// Every kernel of a call is launched so that it may start while the one before it in the stream
+// still runs, and begins with after_previous(), which returns once that one has finished and its
+// writes are visible: what is hidden is the launch itself and, in the products, the set-up of
+// barriers and tensor memory.
+template <class... P, class... A>
+int launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3(unsigned(threads));
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  GSP_CUDA(cudaLaunchKernelEx(&c, kernel, P(args)...));
+  return GSP_OK;
+}
+template <class Job>
+int launch_mma(const Job& job, cudaStream_t st) {
+  const int rc = ensure_smem(reinterpret_cast<const void*>(&mm::mma_kernel<Job>), mm::smem_bytes<Job>());
+  if (rc) return rc;
+  return launch(mm::mma_kernel<Job>, dim3(unsigned(mm::pair_ctas())), mm::kThreads, size_t(mm::smem_bytes<Job>()), st, job);
 }
 
 // ---- device helpers ----------------------------------------------------------------------

@@ -56,6 +56,7 @@ template <int kSortThreads>
 __global__ void __launch_bounds__(kSortThreads)
 teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_ids, int32_t K, int32_t pow2, int64_t V,
                float inv_tau, const Teacher s) {
+  mm::after_previous();
   extern __shared__ uint64_t key[];              // [pow2] (id << 32 | entry), then p [pow2]
   float* p = reinterpret_cast<float*>(key + pow2);
   __shared__ float red[kSortThreads / 32];
@@ -151,6 +152,7 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
 // spread over the rows.  A CTA per 32 rows.  The order inside a bucket is the atomics' and
 // shows nowhere: every entry has a place of its own in pz and in P.
 __global__ void __launch_bounds__(512) bucket_kernel(const State s, const Teacher tc) {
+  mm::after_previous();
   extern __shared__ int32_t count[];           // [buckets]
   __shared__ int32_t part[16];
   const int32_t n = s.head[0], r0 = int32_t(blockIdx.x) * 32, rows = min(32, n - r0);
@@ -397,6 +399,7 @@ struct RowSum {
 __global__ void __launch_bounds__(32 * kJoinRows)
 join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, int32_t pairs, const Teacher tc, int64_t K,
             float tau2, int32_t reduction, float* lse2, double* sums, float* loss) {
+  mm::after_previous();
   __shared__ double red[kJoinRows];
   __shared__ bool last;
   const int32_t n = head[0], wid = threadIdx.x >> 5, lane = lane_id();
@@ -468,6 +471,7 @@ join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, in
 __global__ void __launch_bounds__(1024)
 grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, int32_t bf16, float* ga, float* scale,
                  void* d_hidden, int64_t hidden_bytes) {
+  mm::after_previous();
   __shared__ float red[32];
   if (blockIdx.x > 0) {
     zero_share(d_hidden, hidden_bytes, int64_t(blockIdx.x) - 1, int64_t(gridDim.x) - 1);
@@ -670,7 +674,6 @@ struct Fwd {
   float* part;
   double* sums;
   Teacher tc;
-  void* wcopy;
   int64_t bytes;
 };
 Fwd carve_fwd(void* base, const gsp_vocab_view* vw, int64_t K) {
@@ -686,7 +689,6 @@ Fwd carve_fwd(void* base, const gsp_vocab_view* vw, int64_t K) {
     f.tc.pz = c.take<float>(pad_rows(vw->T) * K);
     f.tc.flag = c.take<uint8_t>(vw->T);
   }
-  f.wcopy = c.take<char>(weight_copy_bytes(vw));
   f.bytes = c.off;
   return f;
 }
@@ -694,7 +696,6 @@ struct Bwd {
   float *ga, *scale, *colpart;
   GradScratch grad;
   uint16_t* P;
-  void* wcopy;
   int64_t pitch, bytes;
 };
 Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
@@ -707,7 +708,6 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
   b.colpart = c.take<float>(Tp / mm::kRows * b.pitch);
   b.grad = carve_grad(c, vw, Tp, b.pitch);
   b.P = c.take<uint16_t>(Tp * b.pitch);
-  b.wcopy = c.take<char>(weight_copy_bytes(vw));
   b.bytes = c.off;
   return b;
 }
@@ -725,15 +725,13 @@ int check_reduction(int32_t reduction, const char* what) {
 template <bool kList>
 int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, float tau, int32_t reduction, float* loss,
                 cudaStream_t st) {
-  const uint16_t* w;
-  int64_t ldw;
+  const Weight w = weight_rows(vw, s);
   int rc;
-  if ((rc = weight_rows(vw, f.wcopy, &w, &ldw, st))) return rc;
   LossJob<kList> j{};
   const bool bf = is_bf16(vw);
   j.a_rows = box_rows(vw->T);
   if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, j.a_rows))) return rc;
-  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, w.w, vw->D, vw->V, w.ld, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.head = s.head;
@@ -744,26 +742,22 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, float ta
   j.bias2 = s.bias2;
   j.lists = lists_of(s, kList, f.tc.pz);
   j.part = f.part;
-  if ((rc = mm::launch(j, st))) return rc;
+  if ((rc = launch_mma(j, st))) return rc;
   if (reduction == GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, size_t(vw->T) * sizeof(float), st));
-  join_kernel<<<unsigned((vw->T + kJoinRows - 1) / kJoinRows), 32 * kJoinRows, 0, st>>>(
-      s.head, s.map, f.part, j.nt, mm::pair_ctas() / 2, f.tc, s.K, tau * tau, reduction, s.lse2, f.sums, loss);
-  GSP_CHECK_LAUNCH();
-  return GSP_OK;
+  return launch(join_kernel, dim3(unsigned((vw->T + kJoinRows - 1) / kJoinRows)), 32 * kJoinRows, 0, st, s.head, s.map, f.part,
+                j.nt, mm::pair_ctas() / 2, f.tc, s.K, tau * tau, reduction, s.lse2, f.sums, loss);
 }
 
 template <bool kList>
 int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, float tau, void* d_hidden, void* d_weight,
                  float* d_bias, cudaStream_t st) {
-  const uint16_t* w;
-  int64_t ldw;
+  const Weight w = weight_rows(vw, s);
   int rc;
-  if ((rc = weight_rows(vw, b.wcopy, &w, &ldw, st))) return rc;
   LogitGradJob<kList> j{};
   const bool bf = is_bf16(vw);
   j.a_rows = box_rows(vw->T);
   if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, j.a_rows))) return rc;
-  if ((rc = make_map(&j.maps[1], bf, w, vw->D, vw->V, ldw, mm::kBN / 2))) return rc;
+  if ((rc = make_map(&j.maps[1], bf, w.w, vw->D, vw->V, w.ld, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.head = s.head;
@@ -781,9 +775,9 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, float t
     const int64_t cols = min64(b.pitch, vw->V - v0);
     j.v0 = int32_t(v0);
     j.nt = int32_t((cols + mm::kBN - 1) / mm::kBN);
-    if ((rc = mm::launch(j, st))) return rc;
+    if ((rc = launch_mma(j, st))) return rc;
     const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V, Sparse{}};
-    if ((rc = grad_products(vw, s, w, ldw, pc, b.grad, BiasSums{b.colpart, b.pitch, d_bias ? d_bias + v0 : nullptr}, b.scale, d_hidden, d_weight, st))) return rc;
+    if ((rc = grad_products(vw, s, w.w, w.ld, pc, b.grad, BiasSums{b.colpart, b.pitch, d_bias ? d_bias + v0 : nullptr}, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
 }
@@ -807,7 +801,7 @@ extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, in
   if ((rc = check_reduction(reduction, "vocab_cross_entropy"))) return rc;
   cudaStream_t st = as_stream(stream);
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "vocab_cross_entropy: null loss");
-  const State s = carve_state(state, vw->T, vw->V, vw->D, 0, 0);
+  const State s = carve_state(state, vw, 0, 0);
   const Fwd f = carve_fwd(ws, vw, 0);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "vocab_cross_entropy: state or workspace too small");
@@ -816,7 +810,7 @@ extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, in
     return GSP_OK;
   }
   GSP_REQUIRE(targets && vw->hidden && vw->weight, GSP_ERR_ARG, "vocab_cross_entropy: null input");
-  if ((rc = pack_rows(vw, targets, ignore_index, nullptr, kLog2e, 0, s, f.counts, st))) return rc;
+  if ((rc = pack_rows(vw, targets, ignore_index, nullptr, kLog2e, Texts{}, s, f.counts, st))) return rc;
   return run_forward<false>(vw, s, f, 1.0f, reduction, loss, st);
 }
 
@@ -831,7 +825,7 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
               (long long)K, GSP_DISTILL_MAX_K);
   GSP_REQUIRE(tau > 0.0f && tau < __builtin_inff(), GSP_ERR_ARG, "topk_distillation: temperature must be positive");
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "topk_distillation: null loss");
-  const State s = carve_state(state, vw->T, vw->V, vw->D, K, 0);
+  const State s = carve_state(state, vw, K, 0);
   const Fwd f = carve_fwd(ws, vw, K);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
               "topk_distillation: state or workspace too small");
@@ -843,18 +837,17 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   int32_t pow2 = 2;
   while (pow2 < K) pow2 <<= 1;
   const size_t sort_bytes = size_t(pow2) * 12;
-#define GSP_TEACHER(n) teacher_kernel<n><<<unsigned(vw->T), n, sort_bytes, st>>>(scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, f.tc)
-  if (pow2 <= 64) GSP_TEACHER(32);
-  else if (pow2 <= 128) GSP_TEACHER(64);
-  else if (pow2 <= 512) GSP_TEACHER(256);
-  else GSP_TEACHER(512);
-#undef GSP_TEACHER
-  GSP_CHECK_LAUNCH();
-  if ((rc = pack_rows(vw, nullptr, 0, f.tc.flag, kLog2e / tau, 0, s, f.counts, st))) return rc;
+  const auto teacher = pow2 <= 64    ? teacher_kernel<32>
+                       : pow2 <= 128 ? teacher_kernel<64>
+                       : pow2 <= 512 ? teacher_kernel<256>
+                                     : teacher_kernel<512>;
+  const int sort_threads = pow2 <= 64 ? 32 : pow2 <= 128 ? 64 : pow2 <= 512 ? 256 : 512;
+  rc = launch(teacher, dim3(unsigned(vw->T)), sort_threads, sort_bytes, st, scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, f.tc);
+  if (rc) return rc;
+  if ((rc = pack_rows(vw, nullptr, 0, f.tc.flag, kLog2e / tau, Texts{}, s, f.counts, st))) return rc;
   const int bucket_bytes = int(s.buckets * 4);
   if ((rc = ensure_smem(reinterpret_cast<const void*>(&bucket_kernel), bucket_bytes))) return rc;
-  bucket_kernel<<<unsigned((vw->T + 31) / 32), 512, bucket_bytes, st>>>(s, f.tc);
-  GSP_CHECK_LAUNCH();
+  if ((rc = launch(bucket_kernel, dim3(unsigned((vw->T + 31) / 32)), 512, size_t(bucket_bytes), st, s, f.tc))) return rc;
   return run_forward<true>(vw, s, f, tau, reduction, loss, st);
 }
 
@@ -871,7 +864,7 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   GSP_REQUIRE(!list || (K >= 1 && K <= GSP_DISTILL_MAX_K && tau > 0.0f && tau < __builtin_inff()), GSP_ERR_ARG,
               "vocab loss backward: bad teacher entries or temperature");
   cudaStream_t st = as_stream(stream);
-  const State s = carve_state(state, vw->T, vw->V, vw->D, list ? K : 0, 0);
+  const State s = carve_state(state, vw, list ? K : 0, 0);
   const Bwd b = carve_bwd(ws, vw);
   GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,
               "vocab loss backward: state or workspace too small");
@@ -885,9 +878,9 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   if (!list) tau = 1.0f;
   const int64_t hidden_bytes = vw->T * vw->D * 2;
   const int64_t zero_blocks = d_hidden ? min64((hidden_bytes + 65535) / 65536, num_sms()) : 0;
-  grad_rows_kernel<<<unsigned(1 + zero_blocks), 1024, 0, st>>>(s, grad_loss, reduction, tau, is_bf16(vw), b.ga, b.scale,
-                                                              d_hidden, hidden_bytes);
-  GSP_CHECK_LAUNCH();
+  rc = launch(grad_rows_kernel, dim3(unsigned(1 + zero_blocks)), 1024, 0, st, s, grad_loss, reduction, tau, int32_t(is_bf16(vw)),
+              b.ga, b.scale, d_hidden, hidden_bytes);
+  if (rc) return rc;
   return list ? run_backward<true>(vw, s, b, tau, d_hidden, d_weight, d_bias, st)
               : run_backward<false>(vw, s, b, tau, d_hidden, d_weight, d_bias, st);
 }

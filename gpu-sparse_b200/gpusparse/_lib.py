@@ -147,7 +147,7 @@ def lib() -> ctypes.CDLL:
             "gsp_compacted_ws_bytes": (i64, [i64, i64, i64, i64]),
             "gsp_compacted_topk": (ctypes.c_int, [p, i64, i64, i64, p, i64, i64, p, p, p, i64,
                                                   p]),
-            "gsp_vocab_state_bytes": (i64, [i64, i64, i64, i64, i32]),
+            "gsp_vocab_state_bytes": (i64, [ctypes.POINTER(VocabView), i64, i32]),
             "gsp_vocab_ws_bytes": (i64, [ctypes.POINTER(VocabView), i64, i32, i32]),
             "gsp_vocab_ce": (ctypes.c_int, [ctypes.POINTER(VocabView), p, i64, i32, p, p, i64, p,
                                             i64, p]),

@@ -43,6 +43,13 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
+def _as(x: torch.Tensor, dtype) -> torch.Tensor:
+    """x contiguous and of that type (x itself where it is)."""
+    if x.dtype != dtype:
+        x = x.to(dtype)
+    return x if x.is_contiguous() else x.contiguous()
+
+
 def _check(what: str, hidden, weight, bias):
     L.require_cuda(hidden, "hidden")
     L.require_cuda(weight, "weight")
@@ -81,7 +88,7 @@ def _sizes(T, V, D, ld_weight, aligned, K, kind, backward, device_index):
     number of SMs)."""
     lib = L.lib()
     v = L.VocabView(T, V, D, D, ld_weight, None, None if aligned else 2, None, L.W_BF16, 0)
-    sb = lib.gsp_vocab_state_bytes(T, V, D, K, kind)
+    sb = lib.gsp_vocab_state_bytes(ctypes.byref(v), K, kind)
     wb = lib.gsp_vocab_ws_bytes(ctypes.byref(v), K, kind, int(backward))
     if sb < 0 or wb < 0:
         L.check(int(-min(sb, wb)), "vocabulary head")
@@ -94,6 +101,18 @@ def _bytes(v: L.VocabView, K: int, kind: int, backward: bool, dev):
 
 def _buffer(nbytes: int, dev) -> torch.Tensor:
     return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+def _state_and_ws(sb: int, wb: int, train: bool, dev):
+    """(buffers, address of the state, address of the workspace): the first buffer is the state
+    to keep for the backward pass, or both in one when there is none to keep it for.  The caller
+    holds the buffers until the call has been issued."""
+    if train:
+        state, ws = _buffer(sb, dev), _buffer(wb, dev)
+        return (state, ws), state.data_ptr(), ws.data_ptr()
+    sb = (sb + 255) // 256 * 256
+    both = _buffer(sb + wb, dev)
+    return (both,), both.data_ptr(), both.data_ptr() + sb
 
 
 _HERE = contextlib.nullcontext()
@@ -109,23 +128,24 @@ def _stream(dev) -> int:
 
 
 # ---------------------------------------------------------------------------- losses
-def _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction):
+def _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction,
+                  train):
     dev = hidden.device
     with _on(dev):
         v = _view(hidden, weight, bias)
         K = ids.shape[1] if kind == L.VOCAB_DISTILL else 0
         sb, wb = _bytes(v, K, kind, False, dev)
-        state, ws = _buffer(sb, dev), _buffer(wb, dev)
+        held, sp, wp = _state_and_ws(sb, wb, train, dev)
         loss = torch.empty((v.T,) if reduction == 0 else (), dtype=torch.float32, device=dev)
         if kind == L.VOCAB_CE:
-            L.check(L.lib().gsp_vocab_ce(ctypes.byref(v), targets.data_ptr(), ignore_index, reduction,
-                                         loss.data_ptr(), state.data_ptr(), sb, ws.data_ptr(), wb,
-                                         _stream(dev)), "vocab_cross_entropy")
+            rc = L.lib().gsp_vocab_ce(ctypes.byref(v), targets.data_ptr(), ignore_index, reduction,
+                                      loss.data_ptr(), sp, sb, wp, wb, _stream(dev))
         else:
-            L.check(L.lib().gsp_vocab_distill(ctypes.byref(v), scores.data_ptr(), ids.data_ptr(), K,
-                                              tau, reduction, loss.data_ptr(), state.data_ptr(), sb,
-                                              ws.data_ptr(), wb, _stream(dev)), "topk_distillation")
-    return loss, state, K
+            rc = L.lib().gsp_vocab_distill(ctypes.byref(v), scores.data_ptr(), ids.data_ptr(), K, tau,
+                                           reduction, loss.data_ptr(), sp, sb, wp, wb, _stream(dev))
+        if rc:
+            L.check(rc, "vocab_cross_entropy" if kind == L.VOCAB_CE else "topk_distillation")
+    return loss, held[0], K
 
 
 def _grad_buffers(ctx, T, weight):
@@ -146,7 +166,7 @@ class _VocabLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, kind, targets, ignore_index, scores, ids, tau, reduction):
         loss, state, K = _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids,
-                                       tau, reduction)
+                                       tau, reduction, True)
         ctx.save_for_backward(weight)
         ctx.state, ctx.T, ctx.args = state, hidden.shape[0], (kind, K, tau, reduction)
         return loss
@@ -159,7 +179,7 @@ class _VocabLoss(torch.autograd.Function):
         dev = weight.device
         with _on(dev):
             v = _view((ctx.T, None), weight, None)
-            grad = grad.to(torch.float32).contiguous()
+            grad = _as(grad, torch.float32)
             _, wb = _bytes(v, K, kind, True, dev)
             ws = _buffer(wb, dev)
             dh, dw, db = _grad_buffers(ctx, ctx.T, weight)
@@ -172,17 +192,18 @@ class _VocabLoss(torch.autograd.Function):
 
 def _loss(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction):
     lead = hidden.shape[:-1]
-    hidden = _rows(hidden.reshape(-1, hidden.shape[-1]))
+    hidden = _rows(hidden if len(lead) == 1 else hidden.reshape(-1, hidden.shape[-1]))
     weight = _rows(weight)
     if bias is not None:
-        bias = bias.to(torch.float32).contiguous()
+        bias = _as(bias, torch.float32)
     red = L.REDUCE[reduction]
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or
                                     (bias is not None and bias.requires_grad)):
         loss = _VocabLoss.apply(hidden, weight, bias, kind, targets, ignore_index, scores, ids, tau, red)
     else:
-        loss = _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, red)[0]
-    return loss.reshape(lead) if red == 0 else loss
+        loss = _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, red,
+                             False)[0]
+    return loss.reshape(lead) if red == 0 and len(lead) > 1 else loss
 
 
 def _check_reduction(what: str, reduction: str) -> None:
@@ -208,7 +229,7 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: tor
                          f"{tuple(hidden.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
     if targets.device != hidden.device:
         raise ValueError(f"vocab_cross_entropy: targets must live on {hidden.device}")
-    targets = targets.reshape(-1).to(torch.int64).contiguous()
+    targets = _as(targets if targets.dim() == 1 else targets.reshape(-1), torch.int64)
     return _loss(L.VOCAB_CE, hidden, weight, bias, targets, int(ignore_index), None, None, 1.0,
                  reduction)
 
@@ -242,8 +263,8 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_scores
         raise ValueError(f"topk_distillation: {K} teacher entries, 1 to {L.DISTILL_MAX_K} are supported")
     if not 0.0 < temperature < float("inf"):
         raise ValueError("topk_distillation: temperature must be positive")
-    scores = teacher_scores.detach().reshape(-1, K).to(torch.float32).contiguous()
-    ids = teacher_ids.reshape(-1, K).to(torch.int64).contiguous()
+    scores = _as(teacher_scores.detach().reshape(-1, K), torch.float32)
+    ids = _as(teacher_ids.reshape(-1, K), torch.int64)
     return _loss(L.VOCAB_DISTILL, hidden, weight, bias, None, 0, scores, ids, float(temperature),
                  reduction)
 
@@ -255,13 +276,14 @@ def _head_forward(hidden, weight, bias, mask, Lt: int, train: bool):
         v = _view(hidden, weight, bias)
         B = v.T // Lt
         sb, wb = _bytes(v, 0, L.VOCAB_HEAD, False, dev)
-        state, ws = _buffer(sb, dev), _buffer(wb, dev)
+        held, sp, wp = _state_and_ws(sb, wb, train, dev)
         y = torch.empty((B, v.V), dtype=torch.float32, device=dev)
         win = torch.empty((B, v.V), dtype=torch.int32, device=dev) if train else None
-        L.check(L.lib().gsp_sparse_head(ctypes.byref(v), Lt, _ptr(mask), y.data_ptr(), _ptr(win),
-                                        state.data_ptr(), sb, ws.data_ptr(), wb, _stream(dev)),
-                "sparse_head")
-    return y, win, state
+        rc = L.lib().gsp_sparse_head(ctypes.byref(v), Lt, _ptr(mask), y.data_ptr(), _ptr(win), sp, sb, wp,
+                                     wb, _stream(dev))
+        if rc:
+            L.check(rc, "sparse_head")
+    return y, win, held[0]
 
 
 class _SparseHead(torch.autograd.Function):
@@ -279,7 +301,7 @@ class _SparseHead(torch.autograd.Function):
         dev = weight.device
         with _on(dev):
             v = _view((ctx.T, None), weight, None)
-            dy = dy.to(torch.float32).contiguous()
+            dy = _as(dy, torch.float32)
             _, wb = _bytes(v, 0, L.VOCAB_HEAD, True, dev)
             ws = _buffer(wb, dev)
             dh, dw, db = _grad_buffers(ctx, ctx.T, weight)
@@ -309,7 +331,7 @@ def sparse_head(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
             raise ValueError(f"sparse_head: mask must be {(B, Lt)}, got {tuple(mask.shape)}")
         if mask.device != hidden.device:
             raise ValueError(f"sparse_head: mask must live on {hidden.device}")
-        mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+        mask = _as(mask if mask.dtype == torch.bool else mask != 0, torch.bool)
     if Lt == 0:
         return torch.zeros((B, V), dtype=torch.float32, device=hidden.device)
     if B > 65534:
@@ -317,7 +339,7 @@ def sparse_head(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     rows = _rows(hidden.reshape(B * Lt, D))
     weight = _rows(weight)
     if bias is not None:
-        bias = bias.to(torch.float32).contiguous()
+        bias = _as(bias, torch.float32)
     if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or
                                     (bias is not None and bias.requires_grad)):
         return _SparseHead.apply(rows, weight, bias, mask, Lt)

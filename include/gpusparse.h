@@ -378,7 +378,7 @@ typedef struct gsp_vocab_view {
  * read again.  ws is scratch of the one call (gsp_vocab_ws_bytes, backward 0 or 1); no call
  * allocates, synchronises or keeps anything else, so calls can be captured, and calls with
  * their own buffers can overlap.  Both functions return a negative status on error. */
-int64_t gsp_vocab_state_bytes(int64_t T, int64_t V, int64_t D, int64_t K, int32_t kind);
+int64_t gsp_vocab_state_bytes(const gsp_vocab_view* vw, int64_t K, int32_t kind);
 int64_t gsp_vocab_ws_bytes(const gsp_vocab_view* vw, int64_t K, int32_t kind, int32_t backward);
 
 /* Softmax cross entropy of every row whose target lies in [0, V) and is not ignore_index;

@@ -39,14 +39,14 @@ def test_sizes():
     for T in (0, 1, 255, 256, 257, 16384):
         v = view(T=T, V=30522, D=768)
         for kind in (L.VOCAB_CE, L.VOCAB_DISTILL, L.VOCAB_HEAD):
-            assert lib.gsp_vocab_state_bytes(T, 30522, 768, 10, kind) > T * 768 * 2
+            assert lib.gsp_vocab_state_bytes(ctypes.byref(v), 10, kind) > T * 768 * 2
             assert lib.gsp_vocab_ws_bytes(ctypes.byref(v), 10, kind, 0) > 0
             back = lib.gsp_vocab_ws_bytes(ctypes.byref(v), 10, kind, 1)
             assert 0 < back < (700 << 20)         # a piece of at most 512 MiB, and dH in fp32
-    # rows a tensor map cannot describe are copied: the workspace holds the copy
-    a = lib.gsp_vocab_ws_bytes(ctypes.byref(view()), 0, L.VOCAB_CE, 0)
+    # rows a tensor map cannot describe are copied: the state holds the copy
+    a = lib.gsp_vocab_state_bytes(ctypes.byref(view()), 0, L.VOCAB_CE)
     for odd in (view(ldw=65), view(ptr=4098), view(D=63)):
-        assert lib.gsp_vocab_ws_bytes(ctypes.byref(odd), 0, L.VOCAB_CE, 0) >= a + 500 * 64 * 2
+        assert lib.gsp_vocab_state_bytes(ctypes.byref(odd), 0, L.VOCAB_CE) >= a + 500 * 64 * 2
 
 
 @pytest.mark.parametrize("bad", [
@@ -57,6 +57,7 @@ def test_bad_views_are_refused(bad):
     lib = L.lib()
     v = view(**bad)
     assert lib.gsp_vocab_ws_bytes(ctypes.byref(v), 0, L.VOCAB_CE, 0) == -L.GSP_ERR_ARG
+    assert lib.gsp_vocab_state_bytes(ctypes.byref(v), 0, L.VOCAB_CE) == -L.GSP_ERR_ARG
     fake = ctypes.c_void_p(4096)
     rc = lib.gsp_vocab_ce(ctypes.byref(v), fake, -100, 2, fake, fake, 1 << 40, fake, 1 << 40, None)
     assert rc == L.GSP_ERR_ARG and lib.gsp_last_error()
@@ -66,7 +67,7 @@ def test_bad_calls_are_refused_before_any_launch():
     lib = L.lib()
     v, fake, big = view(), ctypes.c_void_p(4096), 1 << 40
     ref = ctypes.byref(v)
-    sb = lib.gsp_vocab_state_bytes(100, 500, 64, 0, L.VOCAB_CE)
+    sb = lib.gsp_vocab_state_bytes(ref, 0, L.VOCAB_CE)
     wb = lib.gsp_vocab_ws_bytes(ref, 0, L.VOCAB_CE, 0)
     bb = lib.gsp_vocab_ws_bytes(ref, 0, L.VOCAB_CE, 1)
     E = L.GSP_ERR_ARG
