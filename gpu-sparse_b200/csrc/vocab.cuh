@@ -187,6 +187,16 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool bf16) {
   }
   return r;
 }
+// 32 of them (one branch on the type)
+__device__ __forceinline__ void pack32(const float (&v)[32], uint32_t (&w)[16], bool bf16) {
+  if (bf16) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) w[k] = pack2(v[2 * k], v[2 * k + 1], true);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) w[k] = pack2(v[2 * k], v[2 * k + 1], false);
+  }
+}
 // 32-byte accesses of global memory (sm_100a), p a multiple of 32 bytes
 __device__ __forceinline__ void st256(void* p, const uint32_t* r) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]),
@@ -203,8 +213,7 @@ __device__ __forceinline__ void ld256(const void* p, uint32_t* r) {
 // 32-byte boundary and ld is a multiple of 16
 __device__ __forceinline__ void store_row16(uint16_t* row, int32_t c0, int32_t ld, const float (&v)[32], bool bf16) {
   uint32_t w[16];
-#pragma unroll
-  for (int j = 0; j < 16; ++j) w[j] = pack2(v[2 * j], v[2 * j + 1], bf16);
+  pack32(v, w, bf16);
   st256(row + c0, w);
   if (c0 + 16 < ld) st256(row + c0 + 16, w + 8);
 }
@@ -247,27 +256,31 @@ __device__ __forceinline__ void block_put(float* block, const float (&v)[32], in
 #pragma unroll
   for (int q = 0; q < 8; ++q) o[q] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
-// Column sums of the block: lane l receives those of columns 4 (l % 8) .. + 3 over the rows
-// l / 8 + 4 i, then the four lanes with the same columns add theirs (in a fixed order).
-__device__ __forceinline__ float4 block_col_sums(const float* block, int lane) {
+// Column sums of the block in two steps, so that other work can stand between the loads and the
+// sums: lane l loads columns 4 (l % 8) .. + 3 of the rows l / 8 + 4 i; lanes 0-15 receive the sums
+// over those rows and the rows of lane l + 16 (two partial sums per column).
+struct ColLoads {
+  float4 x[8];
+};
+__device__ __forceinline__ void block_load(ColLoads& c, const float* block, int lane) {
   const float* p = block + (lane >> 3) * kBlockLd + (lane & 7) * 4;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c.x[i] = *reinterpret_cast<const float4*>(p + 4 * i * kBlockLd);
+}
+__device__ __forceinline__ float4 block_sums(const ColLoads& c) {
   F2 a = f2(0.0f, 0.0f), b = a;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float4 x = *reinterpret_cast<const float4*>(p + 4 * i * kBlockLd);
-    a = add2(a, f2(x.x, x.y));
-    b = add2(b, f2(x.z, x.w));
+    a = add2(a, f2(c.x[i].x, c.x[i].y));
+    b = add2(b, f2(c.x[i].z, c.x[i].w));
   }
   float4 s;
   split(a, s.x, s.y);
   split(b, s.z, s.w);
-#pragma unroll
-  for (int o = 8; o <= 16; o <<= 1) {
-    s.x += __shfl_xor_sync(FULL, s.x, o);
-    s.y += __shfl_xor_sync(FULL, s.y, o);
-    s.z += __shfl_xor_sync(FULL, s.z, o);
-    s.w += __shfl_xor_sync(FULL, s.w, o);
-  }
+  s.x += __shfl_xor_sync(FULL, s.x, 16);
+  s.y += __shfl_xor_sync(FULL, s.y, 16);
+  s.z += __shfl_xor_sync(FULL, s.z, 16);
+  s.w += __shfl_xor_sync(FULL, s.w, 16);
   return s;
 }
 

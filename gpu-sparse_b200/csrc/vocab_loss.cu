@@ -512,10 +512,10 @@ grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, 
 template <bool kList>
 struct LogitGradJob {
   // scratch: per warp 32 rows x 64 columns of P on their way out; bias2 of the tile; a 32 x 32
-  // block per warp; column sums of 4 x 32 rows (two buffers)
+  // block per warp; column sums of 8 x 16 rows (two buffers)
   static constexpr int kOutBytes = 32 * 128, kBiasOff = mm::kEpiWarps * kOutBytes, kBlockOff = kBiasOff + kBiasScratch;
   static constexpr int kColOff = kBlockOff + mm::kEpiWarps * kBlockBytes;
-  static constexpr int kStages = 4, kScratch = kColOff + 2 * 4 * mm::kBN * 4;
+  static constexpr int kStages = 4, kScratch = kColOff + 2 * 8 * mm::kBN * 4;
   CUtensorMap maps[3];      // H, W (K-major); P as 32 x 64 boxes
   int32_t wait_limit, bf16;
   const int32_t* head;
@@ -575,10 +575,16 @@ struct LogitGradJob {
       unsigned char* out = a.scratch + a.warp * kOutBytes;
       const float* b = bias(a) - a.c_lo;
       float* block = reinterpret_cast<float*>(a.scratch + kBlockOff + a.warp * kBlockBytes);
-      float* cols = reinterpret_cast<float*>(a.scratch + kColOff) + (a.buf * 4 + (a.warp & 3)) * mm::kBN;
+      // partial column sums: two rows per warp of 32 rows
+      float* cols = reinterpret_cast<float*>(a.scratch + kColOff) + (a.buf * 8 + (a.warp & 3) * 2 + ((a.lane >> 3) & 1)) * mm::kBN +
+                    4 * (a.lane & 7);
       const F2 c2 = f2(j.c, j.c), lse2 = f2(-lse, -lse), ga2 = f2(ga, ga);
 #pragma unroll 1
       for (int32_t c0 = a.c_lo; c0 < a.c_hi; c0 += 32) {
+        // the column sums of the block before this one: loaded here, added up after this block's
+        // arithmetic, which covers their latency
+        ColLoads before;
+        if (j.colpart && c0 > a.c_lo) block_load(before, block, a.lane);
         float z[32];
         a.ld32(c0, z);
         if (c0 + 32 == a.c_hi) a.release();
@@ -629,8 +635,7 @@ struct LogitGradJob {
           }
         }
         uint32_t w[16];
-#pragma unroll
-        for (int k = 0; k < 16; ++k) w[k] = pack2(z[2 * k], z[2 * k + 1], j.bf16 != 0);
+        pack32(z, w, j.bf16 != 0);
         // half a 128-byte row at a time, 16-byte pieces swizzled as the map wants them
         if ((c0 & 32) == 0) {
           if (a.lane == 0) mm::tma_store_wait_read();
@@ -646,22 +651,32 @@ struct LogitGradJob {
           if (a.lane == 0) mm::tma_store_2d(&j.maps[2], out, t.y * mm::kBN + c0 - 32, a.row);
         }
         if (j.colpart) {
+          if (c0 > a.c_lo) {
+            const float4 x = block_sums(before);
+            if (a.lane < 16) *reinterpret_cast<float4*>(cols + c0 - 32) = x;
+          }
           if (!staged) {
             __syncwarp();
             block_put(block, z, a.lane);
           }
           __syncwarp();
-          const float4 s = block_col_sums(block, a.lane);
-          if (a.lane < 8) *reinterpret_cast<float4*>(cols + c0 + 4 * a.lane) = s;
         }
+      }
+      if (j.colpart) {
+        ColLoads last;
+        block_load(last, block, a.lane);
+        const float4 x = block_sums(last);
+        if (a.lane < 16) *reinterpret_cast<float4*>(cols + a.c_hi - 32) = x;
       }
       if ((t.flags & kLast) && a.lane == 0) mm::tma_store_wait();
       if (j.colpart) {
         a.sync();
         const int c = a.warp * 32 + a.lane;
-        const float* q = reinterpret_cast<const float*>(a.scratch + kColOff) + a.buf * 4 * mm::kBN + c;
-        j.colpart[int64_t(t.x * 2 + a.rank) * j.pitch + t.y * mm::kBN + c] =
-            (q[0] + q[mm::kBN]) + (q[2 * mm::kBN] + q[3 * mm::kBN]);
+        const float* q = reinterpret_cast<const float*>(a.scratch + kColOff) + a.buf * 8 * mm::kBN + c;
+        float x = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x += q[i * mm::kBN];
+        j.colpart[int64_t(t.x * 2 + a.rank) * j.pitch + t.y * mm::kBN + c] = x;
       }
     }
   };
