@@ -50,19 +50,26 @@ struct Teacher {
   uint8_t* flag;      // [T] row takes part
 };
 
-// ---- distillation: a teacher row's probabilities, sorted by id, duplicates joined --------
-// kSortThreads: half the entries, rounded up to a power of two (32 to 512)
-template <int kSortThreads>
-__global__ void __launch_bounds__(kSortThreads)
-teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_ids, int32_t K, int32_t pow2, int64_t V,
+// ---- distillation: a teacher row's probabilities, ids listed twice joined -----------------
+// A CTA per row.  The ids go into a hash table in shared memory (linear probing, at most half
+// full); an id belongs to the first entry that lists it, which adds up the others' probabilities
+// in the order they are listed.
+constexpr int kTeacherThreads = 512;      // a thread per entry, if possible: the work is latency
+struct TeacherSlot {
+  int32_t id, first, times;
+};
+__global__ void __launch_bounds__(kTeacherThreads)
+teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_ids, int32_t K, int32_t log_slots, int64_t V,
                float inv_tau, const Teacher s) {
   mm::after_previous();
-  extern __shared__ uint64_t key[];              // [pow2] (id << 32 | entry), then p [pow2]
-  float* p = reinterpret_cast<float*>(key + pow2);
-  __shared__ float red[kSortThreads / 32];
-  __shared__ int32_t wcount[kSortThreads / 32];
+  extern __shared__ TeacherSlot slot[];          // [1 << log_slots], then ids [K], p [K]
+  const int32_t slots = 1 << log_slots;
+  int32_t* id = reinterpret_cast<int32_t*>(slot + slots);      // then the entry's slot; -1: left out
+  float* p = reinterpret_cast<float*>(id + K);
+  __shared__ float red[kTeacherThreads / 32];
+  __shared__ int32_t wcount[kTeacherThreads / 32];
   const int64_t t = blockIdx.x;
-  const int tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const int threads = blockDim.x, warps = threads >> 5, tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
   auto reduce = [&](float v, bool is_max) {
     for (int o = 16; o > 0; o >>= 1) {
       const float u = __shfl_xor_sync(FULL, v, o);
@@ -72,72 +79,66 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
     if (lane == 0) red[wid] = v;
     __syncthreads();
     v = red[0];
-    for (int i = 1; i < kSortThreads / 32; ++i) v = is_max ? fmaxf(v, red[i]) : v + red[i];
+    for (int i = 1; i < warps; ++i) v = is_max ? fmaxf(v, red[i]) : v + red[i];
     return v;
   };
+  for (int32_t i = tid; i < slots; i += threads) slot[i] = TeacherSlot{-1, kNoId, 0};
   float mx = neg_inf();
-  for (int32_t j = tid; j < pow2; j += kSortThreads) {
-    uint64_t k = ~0ull;
-    float x = neg_inf();
-    if (j < K) {
-      const int64_t id = in_ids[t * K + j];
-      x = scores[t * K + j];
-      if (id >= 0 && id < V && x != neg_inf()) k = (uint64_t(id) << 32) | uint32_t(j);
-      else x = neg_inf();
-    }
-    key[j] = k;
+  for (int32_t j = tid; j < K; j += threads) {
+    const int64_t v = in_ids[t * K + j];
+    const float x = scores[t * K + j];
+    const bool in = v >= 0 && v < V && x != neg_inf();
+    id[j] = in ? int32_t(v) : -1;
     p[j] = x;
-    mx = fmaxf(mx, x);
+    if (in) mx = fmaxf(mx, x);
   }
   mx = reduce(mx, true);
   float sum = 0.0f;
-  for (int32_t j = tid; j < pow2; j += kSortThreads) {
-    const float e = key[j] == ~0ull ? 0.0f : expf((p[j] - mx) * inv_tau);
+  for (int32_t j = tid; j < K; j += threads) {
+    if (id[j] < 0) continue;
+    const float e = expf((p[j] - mx) * inv_tau);
     p[j] = e;
     sum += e;
-  }
-  sum = reduce(sum, false);
-  // ascending (id, entry)
-  for (int32_t size = 2; size <= pow2; size <<= 1) {
-    for (int32_t step = size >> 1; step > 0; step >>= 1) {
-      __syncthreads();
-      for (int32_t i = tid; i < pow2 / 2; i += kSortThreads) {
-        const int32_t a = 2 * i - (i & (step - 1)), b = a + step;
-        const uint64_t x = key[a], y = key[b];
-        if ((x > y) == ((a & size) == 0)) {
-          key[a] = y;
-          key[b] = x;
-        }
-      }
+    uint32_t h = uint32_t(id[j]) * 2654435761u >> (32 - log_slots);
+    for (;;) {                           // ends: there are more slots than entries
+      const int32_t was = atomicCAS(&slot[h].id, -1, id[j]);
+      if (was == -1 || was == id[j]) break;
+      h = (h + 1) & (slots - 1);
     }
+    atomicMin(&slot[h].first, j);
+    atomicAdd(&slot[h].times, 1);
+    id[j] = int32_t(h);                  // from here on the slot, which has the id
   }
-  __syncthreads();
+  sum = reduce(sum, false);              // (also makes the table visible)
   int32_t n = 0;
   float ent = 0.0f;
-  for (int32_t j0 = 0; j0 < pow2; j0 += kSortThreads) {
+  for (int32_t j0 = 0; j0 < K; j0 += threads) {
     const int32_t j = j0 + tid;
-    const uint64_t k = j < pow2 ? key[j] : ~0ull;
-    bool head = k != ~0ull && (j == 0 || (key[j - 1] >> 32) != (k >> 32));
+    bool head = false;
     float q = 0.0f;
-    if (head) {
-      for (int32_t i = j; i < pow2 && (key[i] >> 32) == (k >> 32); ++i) q += p[uint32_t(key[i])];
-      q /= sum;
-      head = q != 0.0f;                     // an entry whose probability underflowed adds nothing
-      if (head) ent += q * logf(q);
+    if (j < K && id[j] >= 0) {
+      const TeacherSlot& own = slot[id[j]];
+      head = own.first == j;
+      if (head) {
+        q = p[j];
+        if (own.times > 1) {
+          for (int32_t i = j + 1; i < K; ++i) q += id[i] == id[j] ? p[i] : 0.0f;
+        }
+        q /= sum;
+        head = q != 0.0f;                // an entry whose probability underflowed adds nothing
+        if (head) ent += q * logf(q);
+      }
     }
     const uint32_t w = __ballot_sync(FULL, head);
     if (lane == 0) wcount[wid] = __popc(w);
     __syncthreads();
     int32_t at = n;
-    for (int i = 0; i < kSortThreads / 32; ++i) {
+    for (int i = 0; i < warps; ++i) {
       if (i < wid) at += wcount[i];
       n += wcount[i];
     }
     __syncthreads();
-    if (head) {
-      at += __popc(w & lanemask_lt());
-      s.entry[t * K + at] = make_int2(int32_t(k >> 32), __float_as_int(q));
-    }
+    if (head) s.entry[t * K + at + __popc(w & lanemask_lt())] = make_int2(slot[id[j]].id, __float_as_int(q));
   }
   ent = reduce(ent, false);
   if (tid == 0) {
@@ -151,24 +152,35 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
 // a tile's columns), so that the warp finds those of its block side by side, however they are
 // spread over the rows.  A CTA per 32 rows.  The order inside a bucket is the atomics' and
 // shows nowhere: every entry has a place of its own in pz and in P.
-__global__ void __launch_bounds__(512) bucket_kernel(const State s, const Teacher tc) {
+constexpr int kBucketThreads = 1024, kBucketAhead = 8;
+__global__ void __launch_bounds__(kBucketThreads) bucket_kernel(const State s, const Teacher tc) {
   mm::after_previous();
   extern __shared__ int32_t count[];           // [buckets]
-  __shared__ int32_t part[16];
-  const int32_t n = s.head[0], r0 = int32_t(blockIdx.x) * 32, rows = min(32, n - r0);
-  if (rows <= 0) return;
+  __shared__ int32_t part[32];
+  const int32_t n = s.head[0], r0 = int32_t(blockIdx.x) * 32;
+  if (r0 >= n) return;
   const int32_t nb = int32_t(s.buckets), tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
-  for (int32_t b = tid; b < nb; b += 512) count[b] = 0;
+  for (int32_t b = tid; b < nb; b += kBucketThreads) count[b] = 0;
   __syncthreads();
-  for (int32_t r = wid; r < rows; r += 16) {
-    const int32_t orig = s.map[r0 + r], c = tc.cnt[orig];
-    for (int32_t i = lane; i < c; i += 32) atomicAdd(count + (tc.entry[orig * s.K + i].x >> s.bucket_shift), 1);
+  // a warp per row, kBucketAhead entries per lane in flight
+  const bool live = r0 + wid < n;
+  const int64_t orig = live ? s.map[r0 + wid] : 0;
+  const int32_t c = live ? tc.cnt[orig] : 0;
+  const int2* entry = tc.entry + orig * s.K;
+  for (int32_t i0 = lane; i0 < c; i0 += 32 * kBucketAhead) {
+    int32_t id[kBucketAhead];
+#pragma unroll
+    for (int k = 0; k < kBucketAhead; ++k) id[k] = i0 + 32 * k < c ? entry[i0 + 32 * k].x : -1;
+#pragma unroll
+    for (int k = 0; k < kBucketAhead; ++k) {
+      if (id[k] >= 0) atomicAdd(count + (id[k] >> s.bucket_shift), 1);
+    }
   }
   __syncthreads();
-  // exclusive scan, 512 buckets at a time
+  // exclusive scan
   int32_t* off = s.off + int64_t(blockIdx.x) * (nb + 1);
   int32_t base = 0;
-  for (int32_t b0 = 0; b0 < nb; b0 += 512) {
+  for (int32_t b0 = 0; b0 < nb; b0 += kBucketThreads) {
     const int32_t b = b0 + tid;
     const int32_t v = b < nb ? count[b] : 0;
     int32_t x = v;
@@ -179,23 +191,21 @@ __global__ void __launch_bounds__(512) bucket_kernel(const State s, const Teache
     }
     if (lane == 31) part[wid] = x;
     __syncthreads();
-    int32_t before = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (i < wid) before += part[i];
-      all += part[i];
-    }
+    const int32_t w = part[lane];
+    const int32_t before = __reduce_add_sync(FULL, lane < wid ? w : 0), all = __reduce_add_sync(FULL, w);
     if (b < nb) off[b] = count[b] = base + before + x - v;
     base += all;
     __syncthreads();
   }
   if (tid == 0) off[nb] = base;
   int4* hit = s.hit + int64_t(r0) * s.K;
-  for (int32_t r = wid; r < rows; r += 16) {
-    const int32_t orig = s.map[r0 + r], c = tc.cnt[orig];
-    for (int32_t i = lane; i < c; i += 32) {
-      const int2 e = tc.entry[orig * s.K + i];
-      hit[atomicAdd(count + (e.x >> s.bucket_shift), 1)] = make_int4(e.x, r, e.y, i);
+  for (int32_t i0 = lane; i0 < c; i0 += 32 * kBucketAhead) {
+    int2 e[kBucketAhead];
+#pragma unroll
+    for (int k = 0; k < kBucketAhead; ++k) e[k] = i0 + 32 * k < c ? entry[i0 + 32 * k] : make_int2(-1, 0);
+#pragma unroll
+    for (int k = 0; k < kBucketAhead; ++k) {
+      if (e[k].x >= 0) hit[atomicAdd(count + (e[k].x >> s.bucket_shift), 1)] = make_int4(e[k].x, wid, e[k].y, i0 + 32 * k);
     }
   }
 }
@@ -849,20 +859,17 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
     return GSP_OK;
   }
   GSP_REQUIRE(scores && ids && vw->hidden && vw->weight, GSP_ERR_ARG, "topk_distillation: null input");
-  int32_t pow2 = 2;
-  while (pow2 < K) pow2 <<= 1;
-  const size_t sort_bytes = size_t(pow2) * 12;
-  const auto teacher = pow2 <= 64    ? teacher_kernel<32>
-                       : pow2 <= 128 ? teacher_kernel<64>
-                       : pow2 <= 512 ? teacher_kernel<256>
-                                     : teacher_kernel<512>;
-  const int sort_threads = pow2 <= 64 ? 32 : pow2 <= 128 ? 64 : pow2 <= 512 ? 256 : 512;
-  rc = launch(teacher, dim3(unsigned(vw->T)), sort_threads, sort_bytes, st, scores, ids, int32_t(K), pow2, vw->V, 1.0f / tau, f.tc);
+  int32_t log_slots = 5;
+  while ((1 << log_slots) < 2 * K) ++log_slots;
+  const size_t teacher_bytes = (size_t(1) << log_slots) * sizeof(TeacherSlot) + size_t(K) * 8;
+  const int threads = K >= kTeacherThreads ? kTeacherThreads : int(up(K, 32));
+  rc = launch(teacher_kernel, dim3(unsigned(vw->T)), threads, teacher_bytes, st, scores, ids, int32_t(K), log_slots, vw->V,
+              1.0f / tau, f.tc);
   if (rc) return rc;
   if ((rc = pack_rows(vw, nullptr, 0, f.tc.flag, kLog2e / tau, Texts{}, s, f.counts, st))) return rc;
   const int bucket_bytes = int(s.buckets * 4);
   if ((rc = ensure_smem(reinterpret_cast<const void*>(&bucket_kernel), bucket_bytes))) return rc;
-  if ((rc = launch(bucket_kernel, dim3(unsigned((vw->T + 31) / 32)), 512, size_t(bucket_bytes), st, s, f.tc))) return rc;
+  if ((rc = launch(bucket_kernel, dim3(unsigned((vw->T + 31) / 32)), kBucketThreads, size_t(bucket_bytes), st, s, f.tc))) return rc;
   return run_forward<true>(vw, s, f, tau, reduction, loss, st);
 }
 

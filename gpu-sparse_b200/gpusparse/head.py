@@ -50,6 +50,10 @@ def _as(x: torch.Tensor, dtype) -> torch.Tensor:
     return x if x.is_contiguous() else x.contiguous()
 
 
+def _is_integer(x: torch.Tensor) -> bool:
+    return not (x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool)
+
+
 def _check(what: str, hidden, weight, bias):
     L.require_cuda(hidden, "hidden")
     L.require_cuda(weight, "weight")
@@ -223,8 +227,7 @@ def vocab_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: tor
     """
     _check("vocab_cross_entropy", hidden, weight, bias)
     _check_reduction("vocab_cross_entropy", reduction)
-    if targets.shape != hidden.shape[:-1] or targets.dtype.is_floating_point or \
-            targets.dtype in (torch.bool, torch.complex64, torch.complex128):
+    if targets.shape != hidden.shape[:-1] or not _is_integer(targets):
         raise ValueError(f"vocab_cross_entropy: targets must be an integer tensor of shape "
                          f"{tuple(hidden.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
     if targets.device != hidden.device:
@@ -254,8 +257,9 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_scores
         raise ValueError(f"topk_distillation: teacher scores and ids must be "
                          f"{tuple(hidden.shape[:-1])} + [K], got {tuple(teacher_scores.shape)} and "
                          f"{tuple(teacher_ids.shape)}")
-    if teacher_ids.dtype.is_floating_point or teacher_ids.dtype == torch.bool:
-        raise ValueError("topk_distillation: teacher ids must be an integer tensor")
+    if not _is_integer(teacher_ids) or not teacher_scores.dtype.is_floating_point:
+        raise ValueError("topk_distillation: teacher ids must be an integer tensor and teacher scores "
+                         f"a floating one, got {teacher_ids.dtype} and {teacher_scores.dtype}")
     if teacher_scores.device != hidden.device or teacher_ids.device != hidden.device:
         raise ValueError(f"topk_distillation: teacher scores and ids must live on {hidden.device}")
     K = teacher_ids.shape[-1]

@@ -68,6 +68,8 @@ def check_ce(h, w, b, targets, ignore=-100, reduction="mean", grad=None):
     (64, 30522, 768, BF, 1.0, True),
     (5, 30522, 1024, HF, 1.0, False),
     (3000, 300, 128, BF, 0.15, True),
+    (20, 90, 19200, BF, 1.0, True),      # more 256-wide tiles of D than pairs of SMs
+    (600, 33000, 16, HF, 0.9, True),
 ])
 def test_cross_entropy(T, V, D, dt, frac, bias):
     h, w, b = make(T, V, D, dt, seed=T + V, bias=bias)
@@ -484,6 +486,57 @@ def test_backward_twice_and_changed_inputs():
         torch.autograd.grad(loss, (hl,))
 
 
+@pytest.mark.parametrize("which", ["h", "w", "b", "hb", "wb", "hw"])
+def test_gradients_asked_for_one_by_one(which):
+    """Any subset of the gradients equals the same ones of a full backward pass."""
+    import gpusparse
+    h, w, b = make(300, 700, 72, BF, seed=46)
+    targets = torch.arange(300, device=DEV) * 2
+    scores, ids = teacher(300, 700, 9, seed=2)
+    dy = torch.randn(3, 700, generator=torch.Generator().manual_seed(1)).to(DEV)
+    calls = [lambda a, c, d: gpusparse.vocab_cross_entropy(a, c, targets, bias=d),
+             lambda a, c, d: gpusparse.topk_distillation(a, c, scores, ids, bias=d),
+             lambda a, c, d: (gpusparse.sparse_head(a.reshape(3, 100, 72), c, bias=d) * dy).sum(),
+             lambda a, c, d: (gpusparse.sparse_head(a[:60].reshape(30, 2, 72), c, bias=d)[:3] * dy).sum()]
+    for call in calls:
+        full = [leaf(h), leaf(w), leaf(b)]
+        want = dict(zip("hwb", torch.autograd.grad(call(*full), full)))
+        some = [leaf(x) if n in which else x for n, x in zip("hwb", (h, w, b))]
+        got = torch.autograd.grad(call(*some), [x for n, x in zip("hwb", some) if n in which])
+        for n, x in zip([n for n in "hwb" if n in which], got):
+            assert torch.equal(x, want[n]), n
+
+
+def test_skewed_winners():
+    """One token of a long text wins nearly every term: its row of d_hidden sums thousands of
+    entries (shared by a CTA's warps), the others few."""
+    h, w, b, dy = head_inputs(2, 300, 3000, 96, BF, seed=47, bias_mean=0.0)
+    b += 8.0
+    h[:, 1:] = 0
+    h[:, 0] = (w.float().mean(0) * 0 + 0.03125).to(BF)
+    h[1, 7] = 0.0625
+    _, got = check_head(h, w, b, None, dy)
+    assert int((got[0][0].abs().sum(1) > 0).sum()) <= 300
+
+
+def test_overlapping_calls_on_two_streams():
+    """Calls in flight at the same time keep to their own buffers."""
+    import gpusparse
+    inputs = [step_inputs(48), step_inputs(49)]
+    want = [step(*x) for x in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(*inputs[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(x, y) for x, y in zip(out, want[i]))
+
+
 # ---------------------------------------------------------------------------- refusals
 def test_refusals():
     import gpusparse
@@ -496,7 +549,7 @@ def test_refusals():
                 lambda: ce(h, w, t, reduction="median"), lambda: ce(h, w[:0], t),
                 lambda: ce(h, w, t.cpu()), lambda: ce(h, w.cpu(), t.cpu()) if False else ce(h, w, t, bias=b.cpu()),
                 lambda: di(h, w, s, i[:, :3]), lambda: di(h, w, s, i, temperature=0.0),
-                lambda: di(h, w, s, i, temperature=float("inf")), lambda: di(h, w, s, s),
+                lambda: di(h, w, s, i, temperature=float("inf")), lambda: di(h, w, s, s), lambda: di(h, w, i, i),
                 lambda: di(h, w, torch.zeros(10, 1025, device=DEV), torch.zeros(10, 1025, dtype=torch.int64, device=DEV)),
                 lambda: di(h, w, s[:, :0], i[:, :0]), lambda: sh(h, w), lambda: sh(h[None], w, mask=t[None, :3]),
                 lambda: gpusparse.encode_queries(h[None], w, max_terms=0),
