@@ -132,8 +132,8 @@ def _stream(dev) -> int:
 
 
 # ---------------------------------------------------------------------------- losses
-def _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction,
-                  train):
+def _loss_forward(hidden, weight, bias, args, train):
+    kind, targets, ignore_index, scores, ids, tau, reduction = args
     dev = hidden.device
     with _on(dev):
         v = _view(hidden, weight, bias)
@@ -166,32 +166,40 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+def _loss_backward(ctx, grad):
+    (weight,) = ctx.saved_tensors
+    kind, K, tau, reduction, T, state = ctx.args
+    dev = weight.device
+    with _on(dev):
+        v = _view((T, None), weight, None)
+        grad = _as(grad, torch.float32)
+        _, wb = _bytes(v, K, kind, True, dev)
+        ws = _buffer(wb, dev)
+        dh, dw, db = _grad_buffers(ctx, T, weight)
+        rc = L.lib().gsp_vocab_loss_backward(
+            ctypes.byref(v), kind, K, tau, reduction, grad.data_ptr(), _ptr(dh), _ptr(dw), _ptr(db),
+            state.data_ptr(), state.numel(), ws.data_ptr(), wb, _stream(dev))
+        if rc:
+            L.check(rc, "vocab loss backward")
+    return dh, dw, db, None
+
+
+# The same for a caller that builds a graph of the gradients: differentiating them again raises.
+_loss_backward_once = torch.autograd.function.once_differentiable(_loss_backward)
+
+
 class _VocabLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, bias, kind, targets, ignore_index, scores, ids, tau, reduction):
-        loss, state, K = _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids,
-                                       tau, reduction, True)
+    def forward(ctx, hidden, weight, bias, args):
+        kind, tau, reduction = args[0], args[-2], args[-1]
+        loss, state, K = _loss_forward(hidden, weight, bias, args, True)
         ctx.save_for_backward(weight)
-        ctx.state, ctx.T, ctx.args = state, hidden.shape[0], (kind, K, tau, reduction)
+        ctx.args = (kind, K, tau, reduction, hidden.shape[0], state)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        (weight,) = ctx.saved_tensors
-        kind, K, tau, reduction = ctx.args
-        dev = weight.device
-        with _on(dev):
-            v = _view((ctx.T, None), weight, None)
-            grad = _as(grad, torch.float32)
-            _, wb = _bytes(v, K, kind, True, dev)
-            ws = _buffer(wb, dev)
-            dh, dw, db = _grad_buffers(ctx, ctx.T, weight)
-            L.check(L.lib().gsp_vocab_loss_backward(
-                ctypes.byref(v), kind, K, tau, reduction, grad.data_ptr(), _ptr(dh), _ptr(dw),
-                _ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), wb, _stream(dev)),
-                "vocab loss backward")
-        return dh, dw, db, None, None, None, None, None, None, None
+        return (_loss_backward_once if torch.is_grad_enabled() else _loss_backward)(ctx, grad)
 
 
 def _loss(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, reduction):
@@ -201,12 +209,12 @@ def _loss(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, r
     if bias is not None:
         bias = _as(bias, torch.float32)
     red = L.REDUCE[reduction]
+    args = (kind, targets, ignore_index, scores, ids, tau, red)
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or
                                     (bias is not None and bias.requires_grad)):
-        loss = _VocabLoss.apply(hidden, weight, bias, kind, targets, ignore_index, scores, ids, tau, red)
+        loss = _VocabLoss.apply(hidden, weight, bias, args)
     else:
-        loss = _loss_forward(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, red,
-                             False)[0]
+        loss = _loss_forward(hidden, weight, bias, args, False)[0]
     return loss.reshape(lead) if red == 0 and len(lead) > 1 else loss
 
 
@@ -290,30 +298,38 @@ def _head_forward(hidden, weight, bias, mask, Lt: int, train: bool):
     return y, win, held[0]
 
 
+def _head_backward(ctx, dy):
+    weight, y = ctx.saved_tensors
+    T, Lt, win, state = ctx.args
+    dev = weight.device
+    with _on(dev):
+        v = _view((T, None), weight, None)
+        dy = _as(dy, torch.float32)
+        _, wb = _bytes(v, 0, L.VOCAB_HEAD, True, dev)
+        ws = _buffer(wb, dev)
+        dh, dw, db = _grad_buffers(ctx, T, weight)
+        rc = L.lib().gsp_sparse_head_backward(
+            ctypes.byref(v), Lt, y.data_ptr(), win.data_ptr(), dy.data_ptr(), _ptr(dh), _ptr(dw), _ptr(db),
+            state.data_ptr(), state.numel(), ws.data_ptr(), wb, _stream(dev))
+        if rc:
+            L.check(rc, "sparse_head backward")
+    return dh, dw, db, None, None
+
+
+_head_backward_once = torch.autograd.function.once_differentiable(_head_backward)
+
+
 class _SparseHead(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, mask, Lt):
         y, win, state = _head_forward(hidden, weight, bias, mask, Lt, True)
         ctx.save_for_backward(weight, y)
-        ctx.win, ctx.state, ctx.T, ctx.Lt = win, state, hidden.shape[0], Lt
+        ctx.args = (hidden.shape[0], Lt, win, state)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        weight, y = ctx.saved_tensors
-        dev = weight.device
-        with _on(dev):
-            v = _view((ctx.T, None), weight, None)
-            dy = _as(dy, torch.float32)
-            _, wb = _bytes(v, 0, L.VOCAB_HEAD, True, dev)
-            ws = _buffer(wb, dev)
-            dh, dw, db = _grad_buffers(ctx, ctx.T, weight)
-            L.check(L.lib().gsp_sparse_head_backward(
-                ctypes.byref(v), ctx.Lt, y.data_ptr(), ctx.win.data_ptr(), dy.data_ptr(), _ptr(dh),
-                _ptr(dw), _ptr(db), ctx.state.data_ptr(), ctx.state.numel(), ws.data_ptr(), wb,
-                _stream(dev)), "sparse_head backward")
-        return dh, dw, db, None, None
+        return (_head_backward_once if torch.is_grad_enabled() else _head_backward)(ctx, dy)
 
 
 def sparse_head(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
