@@ -22,6 +22,12 @@
 // along m or n); both are read in place with 128-byte swizzled boxes, so no transposed copy
 // is ever made.
 //
+// What bounds it (B200, D = 768): with an epilogue that does nothing 4096 x 30522 logits take
+// 117 us, 1.64 PFLOP/s; the library's large products reach 1.67 in a burst.  In steps of
+// milliseconds the power limit takes the clock down (library: 1.39).  Operands come
+// from L2 at 10 TB/s; the logits of 16384 rows took 3.4 % less with half of A's loads left out and
+// 5.7 % less with all of them.
+//
 // Every wait is bounded.  A role whose wait runs out raises its CTA's fault flag and winds
 // down after its copies and products in flight have landed; the epilogue then sees NaN
 // accumulators for that and all later tiles of the CTA, so the results show it.

