@@ -167,8 +167,8 @@ def _ptr(t):
 
 
 def _loss_backward(ctx, grad):
-    (weight,) = ctx.saved_tensors
-    kind, K, tau, reduction, T, state = ctx.args
+    weight, state = ctx.saved_tensors
+    kind, K, tau, reduction, T = ctx.args
     dev = weight.device
     with _on(dev):
         v = _view((T, None), weight, None)
@@ -193,8 +193,8 @@ class _VocabLoss(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, args):
         kind, tau, reduction = args[0], args[-2], args[-1]
         loss, state, K = _loss_forward(hidden, weight, bias, args, True)
-        ctx.save_for_backward(weight)
-        ctx.args = (kind, K, tau, reduction, hidden.shape[0], state)
+        ctx.save_for_backward(weight, state)
+        ctx.args = (kind, K, tau, reduction, hidden.shape[0])
         return loss
 
     @staticmethod
@@ -299,8 +299,8 @@ def _head_forward(hidden, weight, bias, mask, Lt: int, train: bool):
 
 
 def _head_backward(ctx, dy):
-    weight, y = ctx.saved_tensors
-    T, Lt, win, state = ctx.args
+    weight, y, win, state = ctx.saved_tensors
+    T, Lt = ctx.args
     dev = weight.device
     with _on(dev):
         v = _view((T, None), weight, None)
@@ -323,8 +323,8 @@ class _SparseHead(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, mask, Lt):
         y, win, state = _head_forward(hidden, weight, bias, mask, Lt, True)
-        ctx.save_for_backward(weight, y)
-        ctx.args = (hidden.shape[0], Lt, win, state)
+        ctx.save_for_backward(weight, y, win, state)
+        ctx.args = (hidden.shape[0], Lt)
         return y
 
     @staticmethod

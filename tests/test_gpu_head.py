@@ -537,6 +537,32 @@ def test_overlapping_calls_on_two_streams():
             assert all(torch.equal(x, y) for x, y in zip(out, want[i]))
 
 
+def test_buffers_are_freed_with_the_backward_pass():
+    """A kept loss or kept weights hold none of the buffers of their backward pass once it has
+    run, and hooks on saved tensors see all of them."""
+    import gpusparse
+    h, w, b, targets, scores, ids = step_inputs(52)
+    calls = (lambda: gpusparse.vocab_cross_entropy(h, w, targets, bias=b),
+             lambda: gpusparse.topk_distillation(h, w, scores, ids, bias=b),
+             lambda: gpusparse.sparse_head(h[None], w, bias=b))
+    for call in calls:
+        want = torch.autograd.grad(call().sum(), (h, w, b))
+        del want
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = call()
+        torch.autograd.grad(out.sum(), (h, w, b))
+        torch.cuda.synchronize()
+        assert torch.cuda.memory_allocated() - before <= (out.numel() * 4 + 511) // 512 * 512
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(out.sum(), (h, w, b))
+        want = torch.autograd.grad(call().sum(), (h, w, b))
+        with torch.autograd.graph.save_on_cpu():
+            out = call()
+        got = torch.autograd.grad(out.sum(), (h, w, b))
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 # ---------------------------------------------------------------------------- refusals
 def test_refusals():
     import gpusparse
