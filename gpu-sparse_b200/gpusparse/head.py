@@ -345,17 +345,17 @@ def sparse_head(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     if hidden.dim() != 3:
         raise ValueError(f"sparse_head: hidden must be [B, L, D], got {tuple(hidden.shape)}")
     B, Lt, D = hidden.shape
-    V = weight.shape[0]
     if mask is not None:
         if mask.shape != (B, Lt):
             raise ValueError(f"sparse_head: mask must be {(B, Lt)}, got {tuple(mask.shape)}")
         if mask.device != hidden.device:
             raise ValueError(f"sparse_head: mask must live on {hidden.device}")
         mask = _as(mask if mask.dtype == torch.bool else mask != 0, torch.bool)
-    if Lt == 0:
-        return torch.zeros((B, V), dtype=torch.float32, device=hidden.device)
     if B > 65534:
         raise ValueError(f"sparse_head: {B} texts in one call, at most 65534 are supported")
+    if Lt == 0:          # texts of one token that takes no part
+        hidden, Lt = torch.nn.functional.pad(hidden, (0, 0, 0, 1)), 1
+        mask = torch.zeros((B, 1), dtype=torch.bool, device=hidden.device)
     rows = _rows(hidden.reshape(B * Lt, D))
     weight = _rows(weight)
     if bias is not None:

@@ -563,6 +563,17 @@ def test_buffers_are_freed_with_the_backward_pass():
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+def test_sparse_head_of_empty_texts_has_zero_gradients():
+    import gpusparse
+    h, w, b, _ = head_inputs(3, 4, 50, 16, BF, seed=35)
+    for some in (h[:, :0], h[:0], h[:0, :0]):
+        leaves = [leaf(some), leaf(w), leaf(b)]
+        y = gpusparse.sparse_head(leaves[0], leaves[1], bias=leaves[2])
+        assert y.shape == (some.shape[0], 50) and (y == 0).all()
+        got = torch.autograd.grad(y.sum(), leaves)
+        assert all(g.shape == x.shape and (g == 0).all() for g, x in zip(got, leaves))
+
+
 # ---------------------------------------------------------------------------- refusals
 def test_refusals():
     import gpusparse
