@@ -818,8 +818,7 @@ extern "C" int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_
   if (rc) return rc;
   const State s = carve_state(state, vw, 0, vw->T > 0 ? vw->T : 1);
   const Fwd f = carve_fwd(ws, vw);
-  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
-              "sparse_head: state or workspace too small");
+  if ((rc = check_buffers(state, state_bytes, s.bytes, ws, ws_bytes, f.bytes, "sparse_head"))) return rc;
   if (vw->T == 0) return GSP_OK;
   GSP_REQUIRE(vw->hidden && vw->weight && y, GSP_ERR_ARG, "sparse_head: null input or output");
   cudaStream_t st = as_stream(stream);
@@ -854,8 +853,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   if ((rc = check_grads(vw, d_hidden, d_weight, "sparse_head backward"))) return rc;
   const State s = carve_state(state, vw, 0, vw->T > 0 ? vw->T : 1);
   const Bwd b = carve_bwd(ws, vw);
-  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,
-              "sparse_head backward: state or workspace too small");
+  if ((rc = check_buffers(state, state_bytes, s.bytes, ws, ws_bytes, b.bytes, "sparse_head backward"))) return rc;
   cudaStream_t st = as_stream(stream);
   if (vw->T == 0) {
     if (d_weight) GSP_CUDA(cudaMemsetAsync(d_weight, 0, size_t(vw->V) * size_t(vw->D) * 2, st));

@@ -460,6 +460,15 @@ int check_view(const gsp_vocab_view* vw, const char* what) {
   return GSP_OK;
 }
 
+int check_buffers(const void* state, int64_t state_bytes, int64_t state_need, const void* ws, int64_t ws_bytes,
+                  int64_t ws_need, const char* what) {
+  GSP_REQUIRE(state && state_bytes >= state_need && ws && ws_bytes >= ws_need, GSP_ERR_ARG, "%s: state or workspace too small",
+              what);
+  GSP_REQUIRE(((reinterpret_cast<uintptr_t>(state) | reinterpret_cast<uintptr_t>(ws)) & 255) == 0, GSP_ERR_ARG,
+              "%s: state and workspace must start on 256-byte boundaries", what);
+  return GSP_OK;
+}
+
 int make_map(CUtensorMap* m, bool bf16, const void* base, int64_t cols, int64_t rows, int64_t ld, int box_rows) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tma_encoder();
   GSP_REQUIRE(enc, GSP_ERR_CUDA, "vocabulary head: cuTensorMapEncodeTiled is not available");

@@ -47,6 +47,9 @@ constexpr int32_t kNoId = 0x7FFFFFFF;
 State carve_state(void* base, const gsp_vocab_view* vw, int64_t K, int64_t texts);
 
 int check_view(const gsp_vocab_view* vw, const char* what);
+// state and workspace: large enough and on 256-byte boundaries, which all parts of them rely on
+int check_buffers(const void* state, int64_t state_bytes, int64_t state_need, const void* ws, int64_t ws_bytes,
+                  int64_t ws_need, const char* what);
 int check_grads(const gsp_vocab_view* vw, const void* d_hidden, const void* d_weight, const char* what);
 inline bool is_bf16(const gsp_vocab_view* vw) { return vw->dtype == GSP_W_BF16; }
 // whether a TMA map can describe W's rows as they are (else the forward call copies them)

@@ -833,8 +833,7 @@ extern "C" int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, in
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "vocab_cross_entropy: null loss");
   const State s = carve_state(state, vw, 0, 0);
   const Fwd f = carve_fwd(ws, vw, 0);
-  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
-              "vocab_cross_entropy: state or workspace too small");
+  if ((rc = check_buffers(state, state_bytes, s.bytes, ws, ws_bytes, f.bytes, "vocab_cross_entropy"))) return rc;
   if (vw->T == 0) {
     if (reduction != GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
     return GSP_OK;
@@ -857,8 +856,7 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "topk_distillation: null loss");
   const State s = carve_state(state, vw, K, 0);
   const Fwd f = carve_fwd(ws, vw, K);
-  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= f.bytes, GSP_ERR_ARG,
-              "topk_distillation: state or workspace too small");
+  if ((rc = check_buffers(state, state_bytes, s.bytes, ws, ws_bytes, f.bytes, "topk_distillation"))) return rc;
   if (vw->T == 0) {
     if (reduction != GSP_REDUCE_NONE) GSP_CUDA(cudaMemsetAsync(loss, 0, sizeof(float), st));
     return GSP_OK;
@@ -893,8 +891,7 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   cudaStream_t st = as_stream(stream);
   const State s = carve_state(state, vw, list ? K : 0, 0);
   const Bwd b = carve_bwd(ws, vw);
-  GSP_REQUIRE(state && state_bytes >= s.bytes && ws && ws_bytes >= b.bytes, GSP_ERR_ARG,
-              "vocab loss backward: state or workspace too small");
+  if ((rc = check_buffers(state, state_bytes, s.bytes, ws, ws_bytes, b.bytes, "vocab loss backward"))) return rc;
   const size_t VD = size_t(vw->V) * size_t(vw->D);
   if (vw->T == 0) {
     if (d_weight) GSP_CUDA(cudaMemsetAsync(d_weight, 0, VD * 2, st));

@@ -377,7 +377,8 @@ typedef struct gsp_vocab_view {
  * denominators and the teacher's probabilities.  The caller's hidden and targets are not
  * read again.  ws is scratch of the one call (gsp_vocab_ws_bytes, backward 0 or 1); no call
  * allocates, synchronises or keeps anything else, so calls can be captured, and calls with
- * their own buffers can overlap.  Both functions return a negative status on error. */
+ * their own buffers can overlap.  state and ws start on 256-byte boundaries.  Both functions
+ * return a negative status on error. */
 int64_t gsp_vocab_state_bytes(const gsp_vocab_view* vw, int64_t K, int32_t kind);
 int64_t gsp_vocab_ws_bytes(const gsp_vocab_view* vw, int64_t K, int32_t kind, int32_t backward);
 

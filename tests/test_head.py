@@ -97,6 +97,19 @@ def test_bad_calls_are_refused_before_any_launch():
     assert lib.gsp_dense_rows_fill(fake, 3, 0, 0.0, fake, fake, fake, None) == E
 
 
+@pytest.mark.parametrize("off", [2, 16, 128])
+def test_unaligned_buffers_are_refused(off):
+    lib = L.lib()
+    ref, fake, odd, big = ctypes.byref(view()), ctypes.c_void_p(4096), ctypes.c_void_p(4096 + off), 1 << 40
+    for st, ws in ((odd, fake), (fake, odd)):
+        for rc in (lib.gsp_vocab_ce(ref, fake, -100, 2, fake, st, big, ws, big, None),
+                   lib.gsp_vocab_distill(ref, fake, fake, 4, 1.0, 2, fake, st, big, ws, big, None),
+                   lib.gsp_vocab_loss_backward(ref, L.VOCAB_CE, 0, 1.0, 2, fake, fake, fake, fake, st, big, ws, big, None),
+                   lib.gsp_sparse_head(ref, 10, None, fake, None, st, big, ws, big, None),
+                   lib.gsp_sparse_head_backward(ref, 10, fake, fake, fake, fake, fake, fake, st, big, ws, big, None)):
+            assert rc == L.GSP_ERR_ARG and b"256" in lib.gsp_last_error()
+
+
 def test_host_tensors_are_refused():
     import gpusparse
     h, w = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(5, 8, dtype=torch.bfloat16)
