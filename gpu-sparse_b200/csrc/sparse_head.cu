@@ -746,7 +746,8 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
   b.scale = c.take<float>(1);
   b.grad = carve_grad(c, vw, Tp, b.pitch);
   b.P = c.take<uint16_t>(Tp * b.pitch);
-  b.room = Tp * b.pitch * 2 / int64_t(sizeof(int2));
+  // (positions in the list are 32-bit)
+  b.room = min64(Tp * b.pitch * 2 / int64_t(sizeof(int2)), (int64_t(1) << 31) - 64);
   b.bytes = c.off;
   return b;
 }

@@ -352,6 +352,14 @@ def test_sparse_head(B, Lt, V, D, dt):
     check_head(h, w, None, mask, dy)
 
 
+def test_sparse_head_of_texts_longer_than_the_sort_counts():
+    """Texts past 12288 tokens go through the products, however sparse their terms are."""
+    h, w, b, dy = head_inputs(2, 13000, 65, 16, BF, seed=36)
+    mask = torch.ones(2, 13000, dtype=torch.bool, device=DEV)
+    mask[1, 77:] = False
+    check_head(h, w, b, mask, dy)
+
+
 def test_sparse_head_masked_tokens_hold_anything():
     h, w, b, dy = head_inputs(6, 50, 500, 64, BF, seed=31)
     mask = torch.zeros(6, 50, dtype=torch.bool, device=DEV)
