@@ -58,7 +58,8 @@ struct Teacher {
 // ---- distillation: a teacher row's probabilities, ids listed twice joined -----------------
 // A CTA per row.  The ids go into a hash table in shared memory (linear probing, at most half
 // full); an id belongs to the first entry that lists it, which adds up the others' probabilities
-// in the order they are listed.
+// in the order they are listed.  Bound by latency: 4096 rows of 100 entries 25 us, 500 rows of
+// 1000 17 us.
 constexpr int kTeacherThreads = 512;      // a thread per entry, if possible: the work is latency
 struct TeacherSlot {
   int32_t id, first, times;
@@ -156,7 +157,8 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
 // The entries of 32 packed rows (one epilogue warp's) sorted into buckets of the vocabulary (half
 // a tile's columns), so that the warp finds those of its block side by side, however they are
 // spread over the rows.  A CTA per 32 rows.  The order inside a bucket is the atomics' and
-// shows nowhere: every entry has a place of its own in pz and in P.
+// shows nowhere: every entry has a place of its own in pz and in P.  4096 rows of 100 entries
+// take 7 us, 500 of 1000 22 us (16 CTAs of 32000 entries: atomics on shared memory).
 constexpr int kBucketThreads = 1024, kBucketAhead = 8;
 __global__ void __launch_bounds__(kBucketThreads) bucket_kernel(const State s, const Teacher tc) {
   mm::after_previous();

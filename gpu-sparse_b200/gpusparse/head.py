@@ -18,7 +18,9 @@ weight and bias; gradients come in the inputs' types, and equal inputs give equa
 Tokens that take no part (ignored targets, masked tokens, rows without teacher entries)
 are packed away on the GPU first: they cost nothing, and what they hold is never used.
 No call synchronises except ``encode_documents`` and ``build_index_from_hidden``, whose
-results' sizes depend on the data.
+results' sizes depend on the data; the others can be captured in a CUDA graph.  (As with any
+torch operator, a backward pass is captured only while no uncaptured graph of the same leaves is
+alive: that graph's accumulation nodes belong to another stream.)
 """
 from __future__ import annotations
 
