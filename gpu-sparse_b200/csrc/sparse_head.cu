@@ -401,12 +401,6 @@ struct GatherParams {
   uint16_t *dh, *dw;
   float* db;
 };
-__device__ __forceinline__ float2 unpack2(uint32_t x, bool bf16) {
-  if (bf16) return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
-  float2 r;
-  asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.f32.f16 %0, a; cvt.f32.f16 %1, b; }" : "=f"(r.x), "=f"(r.y) : "r"(x));
-  return r;
-}
 
 // 8 columns of every 256 from d0 of a row, zeros from column `end` on; rows start on 16-byte
 // boundaries, and the 16 bytes that hold its last column belong to it or to nobody

@@ -184,6 +184,7 @@ struct GradJob {
   int32_t D, nbs;            // 256-wide tiles of D
   int32_t v0, cols, V;
   int32_t first, last;
+  int32_t low;               // first row of P's low parts, or 0
   bool want_h, want_w, w_cut;
   int64_t ld_out;            // of dh and dw
   float* dh_acc;
@@ -192,8 +193,12 @@ struct GradJob {
   const float* scale;        // null: 1
   uint16_t *dh, *dw;
 
-  __device__ GradList list() const {
+  __device__ int32_t rows() const {       // of P, low parts among them
     const int32_t n = *n_rows;
+    return low && n > 0 ? low + n : n;
+  }
+  __device__ GradList list() const {
+    const int32_t n = rows();
     if (sparse.gather(n, V)) return GradList{0, 0, 0, 0};
     return GradList{want_h ? (n + mm::kBM - 1) / mm::kBM : 0, want_w ? (cols + mm::kBM - 1) / mm::kBM : 0, (cols + 63) / 64,
                     (n + 63) / 64};
@@ -209,7 +214,7 @@ struct GradJob {
     GradList l;
     int64_t x, x1;
     int32_t nb, nb_step, nbs, D, v0;
-    bool w_cut;
+    bool w_cut, low;
     __device__ bool next(mm::Tile& t) {
       for (;;) {
         if (x >= x1) {             // with more D tiles than pairs a pair takes several, whole
@@ -242,7 +247,7 @@ struct GradJob {
         t.nk = k1 - k0;
         t.x = blk;
         t.y = nb;
-        t.flags = (is_h ? kIsH : 0) | (k0 > 0 || k1 < nk ? kFrag : 0) | (k1 < nk && k0 == 0 ? kEndsElsewhere : 0) |
+        t.flags = (is_h ? kIsH : 0) | (k0 > 0 || k1 < nk || (is_h && low) ? kFrag : 0) | (k1 < nk && k0 == 0 ? kEndsElsewhere : 0) |
                   (x >= x1 && nb + nb_step >= nbs ? kEnd : 0);
         return true;
       }
@@ -251,10 +256,10 @@ struct GradJob {
   __device__ Walk walk(int32_t pair, int32_t pairs) const {
     const GradList l = list();
     const int64_t tot = l.total();
-    if (nbs > pairs) return Walk{l, tot > 0 ? 0 : 1, tot, pair, tot > 0 ? pairs : nbs, nbs, D, v0, w_cut};
+    if (nbs > pairs) return Walk{l, tot > 0 ? 0 : 1, tot, pair, tot > 0 ? pairs : nbs, nbs, D, v0, w_cut, false};
     const int32_t groups = this->groups(pairs, tot), g = pair / nbs;
-    if (g >= groups) return Walk{l, 0, 0, 0, nbs, nbs, D, v0, w_cut};
-    return Walk{l, g * tot / groups, (g + 1) * tot / groups, pair % nbs, nbs, nbs, D, v0, w_cut};
+    if (g >= groups) return Walk{l, 0, 0, 0, nbs, nbs, D, v0, w_cut, false};
+    return Walk{l, g * tot / groups, (g + 1) * tot / groups, pair % nbs, nbs, nbs, D, v0, w_cut, low > 0};
   }
 
   // 8 columns from c of a finished row: r a packed row (dH) or a vocabulary row of the piece (dW)
@@ -287,9 +292,9 @@ struct GradJob {
     float sc;
     __device__ void begin(const GradJob& j, const mm::Tile& t, const mm::Acc& a) {
       is_h = t.flags & kIsH;
-      live = is_h ? a.row < *j.n_rows : a.row < j.cols;
+      live = is_h ? a.row < j.rows() : a.row < j.cols;
       row = nullptr;
-      if (live && is_h) row = j.dh + int64_t(j.map ? j.map[a.row] : a.row) * j.ld_out;
+      if (live && is_h && !j.low) row = j.dh + int64_t(j.map ? j.map[a.row] : a.row) * j.ld_out;
       sc = j.scale ? *j.scale : 1.0f;
     }
     __device__ void tile(const GradJob& j, const mm::Tile& t, const mm::Acc& a) {
@@ -374,7 +379,8 @@ __device__ void bias_grad(const BiasSums& b, int32_t n, int32_t cols, const floa
 }
 
 // Finishes the tiles that a border between two shares cuts: the pair whose share holds a tile's
-// last step adds the fragments in list order.  Block (pair, CTA of the pair, 16 rows): two rows per
+// last step adds the fragments in list order.  With low parts it finishes dH's tile even uncut,
+// whose rows are then sums of two.  Block (pair, CTA of the pair, 16 rows): two rows per
 // warp, 8 columns per lane.  The blocks past them finish d_bias.
 __global__ void __launch_bounds__(256)
 finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blocks, const BiasSums b) {
@@ -394,7 +400,9 @@ finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blo
   int32_t blk, nk;
   int64_t start;
   l.at(x0, &is_h, &blk, &start, &nk);
-  if (x0 == start || x0 - start >= nk || x1 - start < nk) return;    // begins here, or ends elsewhere
+  const bool two = is_h && j.low > 0;
+  // begins here and is finished, or ends elsewhere
+  if ((x0 == start && !two) || x0 - start >= nk || x1 - start < nk) return;
   const int32_t first = int32_t(((start + 1) * groups - 1) / tot);   // the share that holds the tile's first step
   const int32_t rank = sub & 1, c = lane_id() * 8;
   if (nb * mm::kBN + c >= j.D) return;
@@ -403,12 +411,18 @@ finish_kernel(const __grid_constant__ GradJob j, int32_t pairs, int32_t frag_blo
     const int32_t row = (sub >> 1) * kFinishRows + i * 8 + (threadIdx.x >> 5), r = blk * mm::kBM + rank * mm::kRows + row;
     if (r >= (is_h ? *j.n_rows : j.cols)) return;
     float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int32_t s = first; s <= g; ++s) {
+    auto add = [&](int32_t s, int32_t in_tile) {
       uint32_t o[8];
-      ld256(j.fragment(s * j.nbs + nb, s == first, rank) + row * mm::kBN + c, o);
+      ld256(j.fragment(s * j.nbs + nb, s == first && s < g, in_tile / mm::kRows) + in_tile % mm::kRows * mm::kBN + c, o);
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += __uint_as_float(o[k]);
+    };
+    const int32_t in_tile = rank * mm::kRows + row;
+#pragma unroll 4
+    for (int32_t s = first; s <= g; ++s) add(s, in_tile);
+    if (two) {
+#pragma unroll 4
+      for (int32_t s = first; s <= g; ++s) add(s, in_tile + j.low);
     }
     j.finish8(is_h, r, nb * mm::kBN + c, v);
   }
@@ -611,7 +625,7 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   if ((rc = j.w_cut ? make_map(&j.maps[2], bf, w, vw->D, vw->V, ldw, mm::kBK)
                     : make_map_mn(&j.maps[2], bf, w, vw->D, vw->V, ldw)))
     return rc;
-  if ((rc = make_map_mn(&j.maps[3], bf, s.h, s.Dp, vw->T, s.Dp))) return rc;
+  if ((rc = make_map_mn(&j.maps[3], bf, s.h, s.Dp, pc.low ? s.Tp : vw->T, s.Dp))) return rc;
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.n_rows = s.head;
@@ -623,6 +637,7 @@ int grad_products(const gsp_vocab_view* vw, const State& s, const uint16_t* w, i
   j.cols = int32_t(pc.cols);
   j.V = int32_t(vw->V);
   j.first = pc.first;
+  j.low = pc.low;
   j.last = pc.last;
   j.want_h = d_hidden != nullptr;
   j.want_w = d_weight != nullptr;

@@ -25,6 +25,7 @@
 //   P is scaled so that the largest row coefficient is 1 in bf16, where a target's softmax - 1
 //   is then -1 or close and rounds to next to nothing, and 2^14 in fp16, whose range would lose
 //   gradients of 1e-8; the products' epilogue takes the scale out in fp32.
+//   For up to 128 rows P is held in two parts (see low_rows).
 #include "vocab.cuh"
 
 namespace gsp {
@@ -482,12 +483,22 @@ join_kernel(int32_t* head, const int32_t* map, const float* part, int32_t nt, in
 }
 
 // ---- backward ----------------------------------------------------------------------------
+// The packed rows a second time from row `low` on (see low_rows); the rows between and up to the
+// next 64, which the products read, zero.
+__device__ void low_parts(const State& s, int32_t low, int32_t n) {
+  const int32_t per = int32_t(s.Dp / 8), end = (low + n + 63) / 64 * 64;
+  uint4* h = reinterpret_cast<uint4*>(s.h);
+#pragma unroll 4
+  for (int32_t i = n * per + threadIdx.x; i < end * per; i += 1024)
+    h[i] = i >= low * per && i < (low + n) * per ? h[i - low * per] : make_uint4(0, 0, 0, 0);
+}
+
 // Row coefficients of P: ga[r] = tau * grad_loss (divided by the rows of a mean) over their
 // largest finite size; lse2 of the padding rows +inf, so that their P is 0.  One CTA; the others
 // zero d_hidden.
 __global__ void __launch_bounds__(1024)
-grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, int32_t bf16, float* ga, float* scale,
-                 void* d_hidden, int64_t hidden_bytes) {
+grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, int32_t bf16, int32_t low, float* ga,
+                 float* scale, void* d_hidden, int64_t hidden_bytes) {
   mm::after_previous();
   __shared__ float red[32];
   if (blockIdx.x > 0) {
@@ -495,6 +506,7 @@ grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, 
     return;
   }
   const int32_t n = s.head[0];
+  if (low > 0) low_parts(s, low, n);
   const int32_t np = (n + kRowPad - 1) / kRowPad * kRowPad;
   const float mul = tau / float(reduction == GSP_REDUCE_MEAN ? (n > 0 ? n : 1) : 1);
   float gmax = 0.0f;
@@ -523,7 +535,7 @@ grad_rows_kernel(State s, const float* grad_loss, int32_t reduction, float tau, 
       s.lse2[r] = __uint_as_float(0x7F800000u);
     }
   }
-  zero_tail_rows(s.h, s.Dp, n);
+  if (low == 0) zero_tail_rows(s.h, s.Dp, n);
 }
 
 template <bool kList>
@@ -539,6 +551,7 @@ struct LogitGradJob {
   const int32_t* map;
   int32_t nk, v0, nt;       // the piece's first vocabulary row and 256-wide tiles
   int32_t a_rows;
+  int32_t low;              // see low_rows
   float c;
   const float *bias2, *lse2, *ga;
   Lists lists;
@@ -574,19 +587,21 @@ struct LogitGradJob {
   struct Epi {
     float lse, ga;
     int32_t tgt;
-    bool live;
+    bool live, rest;        // rest: this warp's rows hold what the rounding of others left
     Hits hits;
     __device__ float* bias(const mm::Acc& a) { return reinterpret_cast<float*>(a.scratch + kBiasOff + a.warp * BiasTile::kBytes); }
     __device__ void begin(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
       const int32_t v0 = t.b0 + a.c_lo;
       BiasTile::load(j.bias2 + v0, reinterpret_cast<unsigned char*>(bias(a)), a.lane);
+      rest = j.low > 0 && a.row >= j.low;
+      const int32_t row = rest ? a.row - j.low : a.row;
       if (t.flags & kFirst) {
-        live = a.row < j.head[0];
-        lse = j.lse2[a.row];
-        ga = j.ga[a.row];
-        if constexpr (!kList) tgt = live ? j.lists.tgt[a.row] : -1;
+        live = row < j.head[0];
+        lse = j.lse2[row];
+        ga = j.ga[row];
+        if constexpr (!kList) tgt = live ? j.lists.tgt[row] : -1;
       }
-      if constexpr (kList) hits.load(j.lists, a.row - a.lane, j.head[0], v0, a.lane);
+      if constexpr (kList) hits.load(j.lists, row - a.lane, j.head[0], v0, a.lane);
     }
     __device__ void tile(const LogitGradJob& j, const mm::Tile& t, const mm::Acc& a) {
       unsigned char* out = a.scratch + a.warp * kOutBytes;
@@ -653,6 +668,14 @@ struct LogitGradJob {
         }
         uint32_t w[16];
         pack32(z, w, j.bf16 != 0);
+        if (rest) {
+          unpack_rest(z, w, j.bf16 != 0);
+          pack32(z, w, j.bf16 != 0);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) z[k] = 0.0f;      // no part of the column sums
+          __syncwarp();
+          staged = false;
+        }
         // half a 128-byte row at a time, 16-byte pieces swizzled as the map wants them
         if ((c0 & 32) == 0) {
           if (a.lane == 0) mm::tma_store_wait_read();
@@ -787,7 +810,8 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, float t
   int rc;
   LogitGradJob<kList> j{};
   const bool bf = is_bf16(vw);
-  j.a_rows = box_rows(vw->T);
+  j.low = low_rows(vw);
+  j.a_rows = box_rows(j.low + vw->T);
   if ((rc = make_map(&j.maps[0], bf, s.h, s.Dp, s.Tp, s.Dp, j.a_rows))) return rc;
   if ((rc = make_map(&j.maps[1], bf, w.w, vw->D, vw->V, w.ld, mm::kBN / 2))) return rc;
   j.wait_limit = gsp_get_wait_limit();
@@ -808,7 +832,7 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, float t
     j.v0 = int32_t(v0);
     j.nt = int32_t((cols + mm::kBN - 1) / mm::kBN);
     if ((rc = launch_mma(j, st))) return rc;
-    const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V, Sparse{}};
+    const GradPiece pc{b.P, b.pitch, v0, cols, v0 == 0, v0 + cols >= vw->V, Sparse{}, j.low};
     if ((rc = grad_products(vw, s, w.w, w.ld, pc, b.grad, BiasSums{b.colpart, b.pitch, d_bias ? d_bias + v0 : nullptr}, b.scale, d_hidden, d_weight, st))) return rc;
   }
   return GSP_OK;
@@ -905,7 +929,7 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   const int64_t hidden_bytes = vw->T * vw->D * 2;
   const int64_t zero_blocks = d_hidden ? min64((hidden_bytes + 65535) / 65536, num_sms()) : 0;
   rc = launch(grad_rows_kernel, dim3(unsigned(1 + zero_blocks)), 1024, 0, st, s, grad_loss, reduction, tau, int32_t(is_bf16(vw)),
-              b.ga, b.scale, d_hidden, hidden_bytes);
+              low_rows(vw), b.ga, b.scale, d_hidden, hidden_bytes);
   if (rc) return rc;
   return list ? run_backward<true>(vw, s, b, tau, d_hidden, d_weight, d_bias, st)
               : run_backward<false>(vw, s, b, tau, d_hidden, d_weight, d_bias, st);

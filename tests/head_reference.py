@@ -7,7 +7,9 @@ D (each of its additions may truncate, which is a whole unit of 2^-23, plus the 
   logit           E
   softmax value   a relative 2 E / tau + 2^-18 (its own logit and the denominator's; ex2, its
                   argument's rounding at |z| < 2^6 and the sum)
-  P               u |P| (its rounding) + the softmax value's error
+  P               u |P| (its rounding; u^2 |P| where up to 128 rows let it be held in two
+                  parts, whose products are then sums of twice as many terms) + the softmax
+                  value's error
   dH = P W, dW = P^T H   |dP| summed against |W|, |H|, fp32 sums of n terms (n 2^-23), and u
                   of the result
 fp16 adds the steps of its subnormal numbers: 2^-25 for a result, and for P (scaled so that
@@ -19,16 +21,16 @@ U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 SUB = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
 
 
-def _products(P, dP, h, w, dt, scale_floor):
+def _products(P, dP, h, w, dt, scale_floor, parts=1):
     """dH, dW, dbias and their bounds from P and its bound."""
     u, sub = U[dt], SUB[dt]
     T, V = P.shape
     aP = P.abs() + dP
-    dPr = dP + u * aP + scale_floor
+    dPr = dP + u ** parts * aP + scale_floor
     ah, aw = h.abs(), w.abs()
     dh, dw, db = P @ w, P.t() @ h, P.sum(0)
-    bh = dPr @ aw + (V + 64) * 2.0 ** -23 * (aP @ aw)
-    bw = dPr.t() @ ah + (T + 64) * 2.0 ** -23 * (aP.t() @ ah)
+    bh = dPr @ aw + (parts * V + 64) * 2.0 ** -23 * (aP @ aw)
+    bw = dPr.t() @ ah + (parts * T + 64) * 2.0 ** -23 * (aP.t() @ ah)
     bb = dP.sum(0) + (T + 64) * 2.0 ** -24 * aP.sum(0)
     return (dh, bh * (1 + u) + u * dh.abs() + sub), (dw, bw * (1 + u) + u * dw.abs() + sub), (db, bb)
 
@@ -61,7 +63,8 @@ def softmax_loss(h, w, b, q, live, tau, grads, dt):
     P = torch.where(live[:, None], P, 0.0)
     dP = ga.abs()[:, None] * (sm * e + 2.0 ** -22 * (sm + q))
     floor = SUB[dt] * float(ga.abs().max()) / 2.0 ** 14 if len(ga) else 0.0
-    return (loss, loss_b), _products(P, dP, h, w, dt, floor)
+    parts = 2 if len(h) <= 128 and D <= 74 * 256 else 1
+    return (loss, loss_b), _products(P, dP, h, w, dt, floor, parts)
 
 
 def sparse_head(h, w, b, mask, dy, dt, exact=True):

@@ -79,6 +79,22 @@ def test_cross_entropy(T, V, D, dt, frac, bias):
     check_ce(h, w, b, targets.to(DEV), grad=1.0 if dt == BF else 1024.0)
 
 
+@pytest.mark.parametrize("T", [1, 2, 33, 63, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("V,D,dt", [(200, 64, BF), (5000, 96, HF), (90, 331, HF), (3000, 520, BF)])
+def test_gradients_of_few_rows(T, V, D, dt):
+    """Up to 128 rows the gradients carry the output's rounding alone: losses of few entries a
+    row, whose roundings would show."""
+    h, w, b = make(T, V, D, dt, seed=T + V)
+    targets = torch.arange(T, device=DEV) * 7 % V
+    targets[T // 2:][::5] = -100
+    if T == 1:
+        targets[0] = V - 1
+    grad = torch.linspace(-2.0, 3.0, T, device=DEV) + 0.01
+    check_ce(h, w, b, targets, reduction="none", grad=grad)
+    scores, ids = teacher(T, V, 3, seed=T)
+    check_distill(leaf(h), leaf(w), b, scores, ids, 2.0)
+
+
 @pytest.mark.parametrize("reduction", ["sum", "none"])
 @pytest.mark.parametrize("dt", [BF, HF])
 def test_cross_entropy_reductions(reduction, dt):
