@@ -450,8 +450,9 @@ State carve_state(void* base, const gsp_vocab_view* vw, int64_t K, int64_t texts
   if (K > 0) {
     s.K = K;
     s.hit = c.take<int4>(s.Tp * K);
-    // half a tile per bucket, more where that would be more buckets than fit the sort
-    s.bucket_shift = 7;
+    // 32 columns (an epilogue's step) per bucket, more where that would be more buckets than the
+    // sort has counters for
+    s.bucket_shift = 5;
     while ((s.Vp >> s.bucket_shift) > 8192) ++s.bucket_shift;
     s.buckets = (s.Vp + (int64_t(1) << s.bucket_shift) - 1) >> s.bucket_shift;
     s.off = c.take<int32_t>(s.Tp / 32 * (s.buckets + 1));

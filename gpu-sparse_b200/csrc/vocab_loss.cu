@@ -155,19 +155,21 @@ teacher_kernel(const float* __restrict__ scores, const int64_t* __restrict__ in_
   }
 }
 
-// The entries of 32 packed rows (one epilogue warp's) sorted into buckets of the vocabulary (half
-// a tile's columns), so that the warp finds those of its block side by side, however they are
-// spread over the rows.  A CTA per 32 rows.  The order inside a bucket is the atomics' and
-// shows nowhere: every entry has a place of its own in pz and in P.  4096 rows of 100 entries
-// take 7 us, 500 of 1000 22 us (16 CTAs of 32000 entries: atomics on shared memory).
-constexpr int kBucketThreads = 1024, kBucketAhead = 8;
+// The entries of 32 packed rows (one epilogue warp's) sorted into buckets of the vocabulary (32
+// columns), so that the warp finds those of its block side by side, however they are spread over
+// the rows.  gridDim.y CTAs per 32 rows: each reads all entries, counts those before its share of
+// the buckets and places its own.  The order inside a bucket is the atomics' and shows nowhere:
+// every entry has a place of its own in pz and in P.  4096 rows of 100 entries take 8 us, 500 of
+// 1000 13 us (22 with one CTA per 32 rows).
+constexpr int kBucketThreads = 1024, kBucketAhead = 8, kBucketSplits = 8;
 __global__ void __launch_bounds__(kBucketThreads) bucket_kernel(const State s, const Teacher tc) {
   mm::after_previous();
-  extern __shared__ int32_t count[];           // [buckets]
+  extern __shared__ int32_t count[];           // [this CTA's buckets]
   __shared__ int32_t part[32];
   const int32_t n = s.head[0], r0 = int32_t(blockIdx.x) * 32;
   if (r0 >= n) return;
-  const int32_t nb = int32_t(s.buckets), tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const int32_t all_b = int32_t(s.buckets), tid = threadIdx.x, wid = tid >> 5, lane = tid & 31;
+  const int32_t b_lo = share_lo(all_b, gridDim.y, blockIdx.y), nb = share_lo(all_b, gridDim.y, blockIdx.y + 1) - b_lo;
   for (int32_t b = tid; b < nb; b += kBucketThreads) count[b] = 0;
   __syncthreads();
   // a warp per row, kBucketAhead entries per lane in flight
@@ -175,19 +177,25 @@ __global__ void __launch_bounds__(kBucketThreads) bucket_kernel(const State s, c
   const int64_t orig = live ? s.map[r0 + wid] : 0;
   const int32_t c = live ? tc.cnt[orig] : 0;
   const int2* entry = tc.entry + orig * s.K;
+  int32_t before_mine = 0;
   for (int32_t i0 = lane; i0 < c; i0 += 32 * kBucketAhead) {
     int32_t id[kBucketAhead];
 #pragma unroll
     for (int k = 0; k < kBucketAhead; ++k) id[k] = i0 + 32 * k < c ? entry[i0 + 32 * k].x : -1;
 #pragma unroll
     for (int k = 0; k < kBucketAhead; ++k) {
-      if (id[k] >= 0) atomicAdd(count + (id[k] >> s.bucket_shift), 1);
+      const int32_t b = (id[k] >> s.bucket_shift) - b_lo;
+      if (id[k] >= 0 && b < 0) ++before_mine;
+      if (id[k] >= 0 && b >= 0 && b < nb) atomicAdd(count + b, 1);
     }
   }
+  before_mine = __reduce_add_sync(FULL, before_mine);
+  if (lane == 0) part[wid] = before_mine;
+  __syncthreads();
+  int32_t base = __reduce_add_sync(FULL, part[lane]);
   __syncthreads();
   // exclusive scan
-  int32_t* off = s.off + int64_t(blockIdx.x) * (nb + 1);
-  int32_t base = 0;
+  int32_t* off = s.off + int64_t(blockIdx.x) * (all_b + 1) + b_lo;
   for (int32_t b0 = 0; b0 < nb; b0 += kBucketThreads) {
     const int32_t b = b0 + tid;
     const int32_t v = b < nb ? count[b] : 0;
@@ -205,7 +213,7 @@ __global__ void __launch_bounds__(kBucketThreads) bucket_kernel(const State s, c
     base += all;
     __syncthreads();
   }
-  if (tid == 0) off[nb] = base;
+  if (tid == 0 && blockIdx.y == gridDim.y - 1) off[nb] = base;
   int4* hit = s.hit + int64_t(r0) * s.K;
   for (int32_t i0 = lane; i0 < c; i0 += 32 * kBucketAhead) {
     int2 e[kBucketAhead];
@@ -213,39 +221,50 @@ __global__ void __launch_bounds__(kBucketThreads) bucket_kernel(const State s, c
     for (int k = 0; k < kBucketAhead; ++k) e[k] = i0 + 32 * k < c ? entry[i0 + 32 * k] : make_int2(-1, 0);
 #pragma unroll
     for (int k = 0; k < kBucketAhead; ++k) {
-      if (e[k].x >= 0) hit[atomicAdd(count + (e[k].x >> s.bucket_shift), 1)] = make_int4(e[k].x, wid, e[k].y, i0 + 32 * k);
+      const int32_t b = (e[k].x >> s.bucket_shift) - b_lo;
+      if (e[k].x >= 0 && b >= 0 && b < nb) hit[atomicAdd(count + b, 1)] = make_int4(e[k].x, wid, e[k].y, i0 + 32 * k);
     }
   }
 }
 
-// The entries of a warp's 32 rows x half a tile; the first 32 (usually all) wait in registers,
-// one per lane, loaded while products run.
+// The entries of a warp's 32 rows x half a tile, 32 at a time in registers, one per lane: the first
+// (usually all) loaded while products run, others when a block of 32 columns gets to them.  (With
+// one bucket per half tile, looked through for every 32 columns, the logits' gradient of 500 rows
+// of 1000 entries over 100000 words took 84 us instead of 75, their forward pass 64 instead of 54.)
 struct Hits {
   const int4* first;
-  int32_t n;
+  int32_t edge;         // lane i: where the half's i-th bucket begins
+  int32_t at;           // the 32 that e holds
+  int32_t v_half, shift;
   int4 e;
   __device__ void load(const Lists& l, int32_t row0, int32_t rows, int32_t v0, int lane) {
-    n = 0;
+    edge = at = 0;
+    v_half = v0;
+    shift = l.shift;
     e.x = kNoId;
     if (row0 >= rows) return;
-    const int32_t* off = l.off + int64_t(row0 / 32) * (l.buckets + 1) + (v0 >> l.shift);
-    const int32_t h = off[0];
-    n = off[1] - h;
-    first = l.hit + int64_t(row0) * l.K + h;
-    if (lane < n) e = first[lane];
+    const int32_t b = v0 >> l.shift;
+    if (lane < 5) edge = (l.off + int64_t(row0 / 32) * (l.buckets + 1))[min(b + lane, int32_t(l.buckets))];
+    const int32_t begin = __shfl_sync(FULL, edge, 0);
+    edge -= begin;
+    first = l.hit + int64_t(row0) * l.K + begin;
+    fetch(0, lane);
   }
-  // f(entry, live) for every 32 entries of the bucket that have some in [v0, v0 + 32): every lane
-  // calls it
+  __device__ void fetch(int32_t i, int lane) {
+    const int32_t n = __shfl_sync(FULL, edge, 4);
+    at = i;
+    e.x = kNoId;
+    if (i + lane < n) e = first[i + lane];
+  }
+  // f(entry, live) for every 32 entries that have some in [v0, v0 + 32): every lane calls it
   template <typename F>
-  __device__ void each(int32_t v0, int lane, F&& f) const {
-    for (int32_t i = 0; i < n; i += 32) {
-      int4 x = e;
-      if (i > 0) {
-        x.x = kNoId;
-        if (i + lane < n) x = first[i + lane];
-      }
-      const bool in = x.x >= v0 && x.x < v0 + 32;
-      if (__any_sync(FULL, in)) f(x, in);
+  __device__ void each(int32_t v0, int lane, F&& f) {
+    const int b = (v0 >> shift) - (v_half >> shift);
+    const int32_t lo = __shfl_sync(FULL, edge, b), hi = __shfl_sync(FULL, edge, b + 1);
+    for (int32_t i = lo & ~31; i < hi; i += 32) {
+      if (i != at) fetch(i, lane);
+      const bool in = e.x >= v0 && e.x < v0 + 32;
+      if (__any_sync(FULL, in)) f(e, in);
     }
   }
 };
@@ -896,9 +915,12 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
               1.0f / tau, f.tc);
   if (rc) return rc;
   if ((rc = pack_rows(vw, nullptr, 0, f.tc.flag, kLog2e / tau, Texts{}, s, f.counts, st))) return rc;
-  const int bucket_bytes = int(s.buckets * 4);
+  // few rows: several CTAs for each 32 of them
+  const int64_t groups = (vw->T + 31) / 32, wide = num_sms() / groups;
+  const unsigned splits = unsigned(wide < 1 ? 1 : min64(wide, kBucketSplits));
+  const int bucket_bytes = int((s.buckets + splits - 1) / splits * 4);
   if ((rc = ensure_smem(reinterpret_cast<const void*>(&bucket_kernel), bucket_bytes))) return rc;
-  if ((rc = launch(bucket_kernel, dim3(unsigned((vw->T + 31) / 32)), kBucketThreads, size_t(bucket_bytes), st, s, f.tc))) return rc;
+  if ((rc = launch(bucket_kernel, dim3(unsigned(groups), splits), kBucketThreads, size_t(bucket_bytes), st, s, f.tc))) return rc;
   return run_forward<true>(vw, s, f, tau, reduction, loss, st);
 }
 

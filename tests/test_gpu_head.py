@@ -283,6 +283,16 @@ def test_distillation(T, V, D, K, tau, dt, bias):
     check_distill(h, w, b, scores, ids, tau, grad=1.0 if dt == BF else 512.0)
 
 
+@pytest.mark.parametrize("T,V", [(40, 300000), (200, 600000), (40, 1200000)])
+def test_distillation_over_wide_vocabularies(T, V):
+    """Buckets of 64, 128 and 256 words; the widest in two pieces."""
+    h, w, b = make(T, V, 16, BF, seed=T)
+    scores, ids = teacher(T, V, 30, seed=T)
+    ids[:, :10] = ids[:1, :10] // 5000 * 5000 + torch.arange(10, device=DEV) * 37      # shared blocks
+    ids[:, 29] = V - 1 - torch.arange(T, device=DEV) % 3
+    check_distill(h, w, b, scores, ids, 1.0)
+
+
 def test_distillation_padding_duplicates_and_empty_rows():
     h, w, b = make(50, 400, 64, BF, seed=21)
     scores, ids = teacher(50, 400, 16, seed=3)
