@@ -133,6 +133,23 @@ def _stream(dev) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
+def _read_in_place(weight: torch.Tensor) -> bool:
+    """Whether tensor maps describe these rows; the state of a forward call holds a copy of
+    others."""
+    ld = weight.stride(0) if weight.shape[0] > 1 else weight.shape[1]
+    return ld % 8 == 0 and weight.data_ptr() % 16 == 0
+
+
+def _saved_weight(weight: torch.Tensor, in_place: bool) -> torch.Tensor:
+    """The forward call's weight as its state expects it: hooks on saved tensors may have given
+    its rows another layout."""
+    if not in_place or _read_in_place(weight):
+        return weight
+    V, D = weight.shape
+    rows = weight.new_empty((V, (D + 7) // 8 * 8))[:, :D]
+    return rows.copy_(weight)
+
+
 # ---------------------------------------------------------------------------- losses
 def _loss_forward(hidden, weight, bias, args, train):
     kind, targets, ignore_index, scores, ids, tau, reduction = args
@@ -170,9 +187,10 @@ def _ptr(t):
 
 def _loss_backward(ctx, grad):
     weight, state = ctx.saved_tensors
-    kind, K, tau, reduction, T = ctx.args
+    kind, K, tau, reduction, T, in_place = ctx.args
     dev = weight.device
     with _on(dev):
+        weight = _saved_weight(weight, in_place)
         v = _view((T, None), weight, None)
         grad = _as(grad, torch.float32)
         _, wb = _bytes(v, K, kind, True, dev)
@@ -196,7 +214,7 @@ class _VocabLoss(torch.autograd.Function):
         kind, tau, reduction = args[0], args[-2], args[-1]
         loss, state, K = _loss_forward(hidden, weight, bias, args, True)
         ctx.save_for_backward(weight, state)
-        ctx.args = (kind, K, tau, reduction, hidden.shape[0])
+        ctx.args = (kind, K, tau, reduction, hidden.shape[0], _read_in_place(weight))
         return loss
 
     @staticmethod
@@ -302,9 +320,10 @@ def _head_forward(hidden, weight, bias, mask, Lt: int, train: bool):
 
 def _head_backward(ctx, dy):
     weight, y, win, state = ctx.saved_tensors
-    T, Lt = ctx.args
+    T, Lt, in_place = ctx.args
     dev = weight.device
     with _on(dev):
+        weight = _saved_weight(weight, in_place)
         v = _view((T, None), weight, None)
         dy = _as(dy, torch.float32)
         _, wb = _bytes(v, 0, L.VOCAB_HEAD, True, dev)
@@ -326,7 +345,7 @@ class _SparseHead(torch.autograd.Function):
     def forward(ctx, hidden, weight, bias, mask, Lt):
         y, win, state = _head_forward(hidden, weight, bias, mask, Lt, True)
         ctx.save_for_backward(weight, y, win, state)
-        ctx.args = (hidden.shape[0], Lt)
+        ctx.args = (hidden.shape[0], Lt, _read_in_place(weight))
         return y
 
     @staticmethod

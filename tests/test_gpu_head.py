@@ -597,6 +597,24 @@ def test_buffers_are_freed_with_the_backward_pass():
         assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
+@pytest.mark.parametrize("D,ld", [(83, 88), (83, 83), (88, 96)])
+def test_hooks_may_change_the_layout_of_the_weight(D, ld):
+    import gpusparse
+    h, _, b = make(20, 300, D, BF, seed=53)
+    wide = (torch.randn(300, ld, generator=torch.Generator().manual_seed(54)) * 0.2).to(BF).to(DEV)
+    targets = torch.arange(20, device=DEV)
+    for call in (lambda h, w: gpusparse.vocab_cross_entropy(h, w, targets, bias=b),
+                 lambda h, w: gpusparse.sparse_head(h[None], w, bias=b)):
+        got = []
+        for hook in (False, True):
+            hl, wl = leaf(h), wide[:, :D].requires_grad_(True)
+            with torch.autograd.graph.saved_tensors_hooks(lambda x: x.clone(memory_format=torch.contiguous_format)
+                                                          if hook else x, lambda x: x):
+                out = call(hl, wl)
+            got.append(torch.autograd.grad(out.sum(), (hl, wl)))
+        assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
 def test_sparse_head_of_empty_texts_has_zero_gradients():
     import gpusparse
     h, w, b, _ = head_inputs(3, 4, 50, 16, BF, seed=35)
