@@ -28,9 +28,10 @@
 // from L2 at 10 TB/s; the logits of 16384 rows took 3.4 % less with half of A's loads left out and
 // 5.7 % less with all of them.
 //
-// Every wait is bounded.  A role whose wait runs out raises its CTA's fault flag and winds
-// down after its copies and products in flight have landed; the epilogue then sees NaN
-// accumulators for that and all later tiles of the CTA, so the results show it.
+// Every wait is bounded.  A role whose wait runs out raises its CTA's fault flag and stops; the
+// epilogue then sees NaN accumulators for that and all later tiles of the CTA, so the results
+// show it.  Before a pair ends, its CTAs tell each other how far they came, and whatever is still
+// on its way to one of them (copies, arrivals) is waited for there (wind_down).
 //
 // A job type provides
 //   kStages, kScratch            depth of the operand ring, bytes of epilogue scratch
@@ -58,6 +59,7 @@ constexpr int kABytes = kRows * kBK * 2;
 constexpr int kBBytes = kBN / 2 * kBK * 2;
 constexpr int kStageBytes = kABytes + kBBytes;
 constexpr int kTmemCols = 2 * kBN;
+constexpr int32_t kTailPolls = 1 << 24;  // of the waits for what has been issued already
 template <class Job>
 constexpr int smem_bytes() {
   return Job::kStages * kStageBytes + Job::kScratch + 256 + 1024;   // + barriers, alignment slack
@@ -113,19 +115,31 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, int32_t l
   }
   return false;
 }
-// copies and products already issued land before the CTA gives up its memory (a bound of its
-// own: the caller's limit may be 0)
+// waits for what is on its way already (a bound of its own: the caller's limit may be 0)
 __device__ __forceinline__ void bar_land(uint64_t* b, uint32_t parity) {
-  for (int32_t i = 0; i < (1 << 24); ++i) {
+  for (int32_t i = 0; i < kTailPolls; ++i) {
     if (bar_test(b, parity)) return;
     __nanosleep(32);
   }
 }
-// the address of the first CTA's copy of a shared-memory object of this CTA
-__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
+// the last `depth` of `count` phases of a ring of barriers (phase i is barrier i % depth's
+// (i / depth)-th)
+__device__ __forceinline__ void bars_land(uint64_t* ring, int32_t depth, int32_t count) {
+  for (int32_t i = count > depth ? count - depth : 0; i < count; ++i) bar_land(ring + i % depth, uint32_t(i / depth) & 1);
+}
+// counts bytes at a barrier that no copy brings
+__device__ __forceinline__ void bar_complete(uint64_t* b, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(su32(b)), "r"(bytes) : "memory");
+}
+// the address of a CTA's copy of a shared-memory object of this CTA
+__device__ __forceinline__ uint32_t in_cta(const void* p, int32_t rank) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(su32(p)));
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(su32(p)), "r"(rank));
   return r;
+}
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) { return in_cta(p, 0); }
+__device__ __forceinline__ void store_remote(uint32_t cluster_addr, int32_t v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
 }
 __device__ __forceinline__ uint32_t cta_rank() {
   uint32_t r;
@@ -264,6 +278,32 @@ struct Acc {
   }
 };
 
+// How far a CTA came: stages its producer asked for, stages and tiles whose products were issued
+// (the first CTA's; counted as they are issued: counters kept for the end of the loop cost it 2 %,
+// 628 instead of 613 us for 64 documents), and whether one of its waits ran out.
+struct Progress {
+  int32_t issued, fed, tiles, fault;
+};
+
+// After a wait has run out in either CTA, by one thread of each: returns once nothing is on its way
+// to this CTA's shared memory any more.  A stage is asked for only when the products have read what
+// its slot held, so the CTAs are at most kStages apart.  The copies of both count at the first CTA's
+// barriers: for a stage that only one of them asked for it makes up the other's part.
+template <int kStages>
+__device__ __noinline__ void wind_down(uint64_t* full, uint64_t* empty, uint64_t* acc_full, const Progress* progress, int32_t rank,
+                                       const Tile& t) {
+  const Progress own = progress[0], peer = progress[1], first = progress[rank];
+  if (rank == 0) {
+    // the second CTA's bytes of a stage: the same for all tiles of a job
+    const uint32_t second = uint32_t((!t.a_mn && t.a_rows < kRows ? 0 : kRows) + (t.b_mn ? kBN / 2 : t.bn / 2)) * (kBK * 2);
+    for (int32_t i = peer.issued; i < own.issued; ++i) bar_complete(full + i % kStages, second);
+    for (int32_t i = own.issued; i < peer.issued; ++i) bar_expect(full + i % kStages, second);
+    bars_land(full, kStages, own.issued > peer.issued ? own.issued : peer.issued);
+  }
+  bars_land(empty, kStages, first.fed);
+  bars_land(acc_full, 2, first.tiles);
+}
+
 template <class Job>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_kernel(const __grid_constant__ Job job) {
   constexpr int kStages = Job::kStages;
@@ -277,7 +317,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
   uint64_t* acc_empty = acc_full + 2;                                      // [2], used in the first CTA
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  volatile int32_t* fault = reinterpret_cast<volatile int32_t*>(tmem_slot + 1);
+  Progress* progress = reinterpret_cast<Progress*>(tmem_slot + 2);         // [2], own and the other CTA's
+  volatile int32_t *fault = &progress->fault, *fed = &progress->fed, *tiles = &progress->tiles;
   const int wid = threadIdx.x >> 5, lane = lane_id();
   const int32_t limit = job.wait_limit;
   const int32_t rank = int32_t(cta_rank());
@@ -293,7 +334,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
       bar_init(acc_empty + i, 2 * kEpiWarps);
     }
     bar_init(drain, 1);
-    *fault = 0;
+    progress[0] = Progress{0, 0, 0, 0};
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (wid == 2) {
@@ -345,18 +386,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
           }
         }
       }
+      progress->issued = int32_t(it);
+      // the last stages are handed back too: their copies have landed then, and the arrivals that
+      // say so find this CTA's barriers still there
+      for (uint32_t i = it > uint32_t(kStages) ? it - kStages : 0; ok && i < it; ++i)
+        ok = bar_wait(empty + i % kStages, (i / kStages) & 1, kTailPolls, fault);
       if (!ok) *fault = 1;
-      if (rank == 0) {
-        for (uint32_t i = 0; i < uint32_t(kStages) && i < it; ++i) {
-          const uint32_t j = it - 1 - i;
-          bar_land(full + j % kStages, (j / kStages) & 1);
-        }
-      } else if (!ok) {
-        // the second CTA's copies count at a barrier it cannot wait on: without a fault the
-        // products that read them have finished; with one, a millisecond is far more than any
-        // copy takes
-        for (int i = 0; i < 1024; ++i) __nanosleep(1000);
-      }
     }
   } else if (wid == 1) {
     if (lane == 0 && rank == 0) {
@@ -382,9 +417,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
 #pragma unroll
           for (int q = 0; q < kBK / 16; ++q) mma_f16(d, da + q * step_a, db + q * step_b, id, (k > 0 || q > 0) ? 1u : 0u);
           commit_both(empty + s);
+          *fed = int32_t(it) + 1;
         }
         if (!ok) break;
         commit_both(acc_full + buf);
+        *tiles = i + 1;
       }
       if (!ok) *fault = 1;
       commit_own(drain);          // every product issued has finished before the memory is given back
@@ -425,7 +462,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) mma_ker
   __syncwarp();
   fence_before();
   __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t to = in_cta(progress + 1, rank ^ 1);
+    store_remote(to, progress->issued);
+    store_remote(to + 4, progress->fed);
+    store_remote(to + 8, progress->tiles);
+    store_remote(to + 12, progress->fault);
+  }
   cluster_sync();         // neither CTA's memory goes away while the other may still use it
+  if (progress[0].fault | progress[1].fault) {      // both CTAs see both
+    if (threadIdx.x == 0) {
+      auto walk = job.walk(pair, pairs);
+      Tile t;
+      if (walk.next(t)) wind_down<kStages>(full, empty, acc_full, progress, rank, t);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   if (wid == 2) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));

@@ -680,3 +680,37 @@ def test_encode_index_search_and_distil(dt):
     # a student that scores the documents by dense vectors learns the ranking
     sq, sd = make(Q, N, D, dt, seed=63, bias=False)[:2]
     check_distill(sq, sd, None, scores, ids, 2.0, grad=1.0 if dt == BF else 256.0)
+
+
+# ---------------------------------------------------------------------------- waits that run out
+@pytest.mark.parametrize("limit", [0, 2])
+def test_wait_that_runs_out_in_the_backward_pass(limit):
+    """The logits' gradient and the products (whole tiles, cut ones, and P in two parts) under a
+    wait limit that some wait exceeds: NaN gradients, nothing hangs, and the next pass over the
+    same state is right again."""
+    import gpusparse
+    import gpusparse._lib as L
+    h, w, b = make(300, 900, 512, BF, seed=71)
+    targets = torch.arange(300, device=DEV) * 3
+    scores, ids = teacher(300, 900, 12, seed=71)
+    calls = [lambda a, c, d: gpusparse.vocab_cross_entropy(a, c, targets, bias=d),
+             lambda a, c, d: gpusparse.vocab_cross_entropy(a[:40], c, targets[:40], bias=d),
+             lambda a, c, d: gpusparse.topk_distillation(a, c, scores, ids, bias=d),
+             lambda a, c, d: gpusparse.sparse_head(a.reshape(150, 2, 512), c, bias=d).sum()]
+    lib = L.lib()
+    default = lib.gsp_get_wait_limit()
+    for call in calls:
+        leaves = [leaf(h), leaf(w), leaf(b)]
+        out = call(*leaves)
+        want = torch.autograd.grad(out, leaves, retain_graph=True)
+        torch.cuda.synchronize()
+        L.check(lib.gsp_set_wait_limit(limit), "wait limit")
+        try:
+            got = [torch.autograd.grad(out, leaves, retain_graph=True) for _ in range(3)]
+            torch.cuda.synchronize()
+        finally:
+            L.check(lib.gsp_set_wait_limit(default), "wait limit")
+        if limit == 0:
+            assert any(torch.isnan(g).any().item() for grads in got for g in grads)
+        after = torch.autograd.grad(out, leaves)
+        assert all(torch.equal(x, y) for x, y in zip(after, want))
