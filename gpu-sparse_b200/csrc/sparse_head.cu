@@ -13,7 +13,7 @@
 // short queries 342 us, 1.21 PFLOP/s, their ends costing the epilogue more; one query 13 us, of
 // which 7 are W's bytes.
 //
-// Backward.  Each (text, term) with y > 0 sends ds = dy exp(-y) to its winning token:
+// Backward.  Each (text, term) with y > 0 (or NaN) sends ds = dy exp(-y) to its winning token:
 //   dH[win] += ds W[v],   dW[v] += ds H[win],   d_bias[v] += ds.
 // Term weights are sparse (a trained head keeps hundreds of 30522 terms), so these are sums of
 // few rows of W and H, gathered from L2 in a fixed order, fp32 throughout: dW takes a term's
@@ -32,6 +32,11 @@ namespace {
 
 constexpr int kFirst = 1, kLast = 2;      // of a share along one row of tiles
 constexpr int kBegin = 4, kEnd = 8;       // of a share
+
+// Whether z takes the maximum over from m: it is larger, or the first NaN.  A NaN has a winner like
+// any other maximum, so that its gradient is NaN too.
+__device__ __forceinline__ bool takes(float z, float m) { return !(z <= m) && m == m; }
+__device__ __forceinline__ bool is_nan(float x) { return x != x; }
 
 template <bool kWin>
 struct HeadJob {
@@ -77,12 +82,13 @@ struct HeadJob {
   }
 
   struct Epi {
+    // (a NaN that no token won, -inf plus a bias of +inf, is given to the row)
     __device__ static void put(const HeadJob& j, int32_t row, int32_t v, float bias, float m, int32_t idx) {
       if (v >= j.V) return;
       const float x = m + bias;
       const int64_t o = int64_t(j.map[row] / j.L) * j.V + v;
-      j.y[o] = x > 0.0f ? log1pf(x) : (x != x ? x : 0.0f);
-      if (kWin) j.win[o] = x > 0.0f ? idx : -1;
+      j.y[o] = x > 0.0f ? log1pf(x) : (is_nan(x) ? x : 0.0f);
+      if (kWin) j.win[o] = x <= 0.0f ? -1 : (idx >= 0 ? idx : row);
     }
     __device__ static void part(const HeadJob& j, const mm::Acc& a, int which, float m, int32_t idx) {
       const int64_t o = (int64_t(blockIdx.x >> 1) * 2 + which) * mm::kBM + a.rank * mm::kRows + a.lane_row;
@@ -125,17 +131,22 @@ struct HeadJob {
           const int32_t rb = r0 + 16 * h;
           int32_t won = -1;
           if (bits == 0) {
+            const float before = m;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               if (kWin) won = z[16 * h + k] > m ? k : won;
               asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(z[16 * h + k]));
+            }
+            if (kWin && is_nan(m) && !is_nan(before)) {
+#pragma unroll
+              for (int k = 15; k >= 0; --k) won = is_nan(z[16 * h + k]) ? k : won;
             }
             if (kWin && won >= 0) idx = rb + won;
           } else {
             int32_t e = 0;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              if (kWin) idx = z[16 * h + k] > m ? rb + k : idx;
+              if (kWin) idx = takes(z[16 * h + k], m) ? rb + k : idx;
               asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(z[16 * h + k]));
               if ((bits >> k) & 1) {
                 slot_m[e * 32] = m;
@@ -182,13 +193,13 @@ struct HeadJob {
       float open_m = m;
       int32_t open_i = idx;
       if (head_row >= 0) {
-        const int32_t hi = kWin && head_m > cm ? head_i : ci;
+        const int32_t hi = kWin && takes(head_m, cm) ? head_i : ci;
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(head_m) : "f"(cm));
         if (cut) part(j, a, 0, head_m, hi);
         else put(j, head_row, v, bias, head_m, hi);
         cut = false;
       } else {
-        if (kWin) open_i = m > cm ? idx : ci;
+        if (kWin) open_i = takes(m, cm) ? idx : ci;
         asm("max.NaN.f32 %0, %0, %1;" : "+f"(open_m) : "f"(cm));
       }
       if ((t.flags & kLast) && a.half == 1) {
@@ -242,14 +253,14 @@ __global__ void __launch_bounds__(mm::kBM) head_join_kernel(const JoinParams p) 
   for (int32_t s = first; s <= c; ++s) {
     const int64_t o = (int64_t(s) * 2 + (s == c ? 0 : 1)) * mm::kBM + threadIdx.x;
     const float x = p.part_m[o];
-    if (p.win && x > m) idx = p.part_i[o];
+    if (p.win && takes(x, m)) idx = p.part_i[o];
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(x));
   }
   const int64_t v = int64_t(vt) * mm::kBM + threadIdx.x;
   if (v >= p.V) return;
   const float x = m + (p.bias ? p.bias[v] : 0.0f);
-  p.y[text * p.V + v] = x > 0.0f ? log1pf(x) : (x != x ? x : 0.0f);
-  if (p.win) p.win[text * p.V + v] = x > 0.0f ? idx : -1;
+  p.y[text * p.V + v] = x > 0.0f ? log1pf(x) : (is_nan(x) ? x : 0.0f);
+  if (p.win) p.win[text * p.V + v] = x <= 0.0f ? -1 : (idx >= 0 ? idx : r0);
 }
 
 // ---- backward ----------------------------------------------------------------------------
@@ -259,8 +270,8 @@ struct Survey {
   uint32_t pad_;
 };
 
-// ds of (text, term) pairs o[k] (negative: none) and their tokens' packed rows (-1: no gradient);
-// all loads are issued before the first is used
+// ds of (text, term) pairs o[k] (negative: none) and their tokens' packed rows (-1: no gradient; a
+// NaN weight has one, NaN, even where dy is 0); all loads are issued before the first is used
 template <int N>
 __device__ __forceinline__ void entry_grads(const float* y, const int32_t* win, const float* dy, const int64_t (&o)[N],
                                             int32_t (&row)[N], float (&ds)[N]) {
@@ -273,7 +284,7 @@ __device__ __forceinline__ void entry_grads(const float* y, const int32_t* win, 
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    if (d[k] == 0.0f) row[k] = -1;
+    if (d[k] == 0.0f && !is_nan(v[k])) row[k] = -1;
     ds[k] = row[k] >= 0 ? d[k] * expf(-v[k]) : 0.0f;
   }
 }
@@ -326,7 +337,7 @@ survey_kernel(State s, const SortParams p, Survey* out, void* d_hidden, int64_t 
           const float d = p.dy[b * p.V + t], a = fabsf(d);
           const int32_t w = p.win[b * p.V + t];
           if (a < __uint_as_float(0x7F800000u)) m = fmaxf(m, a);
-          if (d != 0.0f) r[k] = w;
+          if (w >= 0 && (d != 0.0f || is_nan(p.y[b * p.V + t]))) r[k] = w;
         }
         c += r[k] >= 0;
       }

@@ -360,7 +360,8 @@ def sparse_head(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
 
     hidden [B, L, D], weight [V, D], mask [B, L] (nonzero or True = the token takes part, in
     any pattern; None = all do).  A text without tokens has zero weights.  The gradient goes
-    to the token that won the maximum, the first one on ties.
+    to the token that won the maximum, the first one on ties; a NaN wins, and both the weight
+    and its gradients are NaN.
     """
     _check("sparse_head", hidden, weight, bias)
     if hidden.dim() != 3:

@@ -411,7 +411,8 @@ int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, int64_t K, f
  * no part, NULL = all do; any pattern),
  *   y[b, v] = log1p(max(0, max over the text's tokens of s[t, v]))     fp32 [B, V],
  * 0 for a text without tokens.  win (int32 [B, V], or NULL when no backward call follows) gets
- * the packed row of the token that won, the first on ties, or -1 where y is 0. */
+ * the packed row of the token that won, the first on ties, or -1 where y is 0.  A NaN logit
+ * of a token that takes part makes y NaN and wins, and the gradients that y sends are NaN. */
 int gsp_sparse_head(const gsp_vocab_view* vw, int64_t L, const uint8_t* mask, float* y, int32_t* win, void* state,
                     int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream);
 /* Its gradients from dy fp32 [B, V] and what the forward call left (vw with the same sizes and

@@ -714,3 +714,66 @@ def test_wait_that_runs_out_in_the_backward_pass(limit):
             assert any(torch.isnan(g).any().item() for grads in got for g in grads)
         after = torch.autograd.grad(out, leaves)
         assert all(torch.equal(x, y) for x, y in zip(after, want))
+
+
+# ---------------------------------------------------------------------------- NaN
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("zero", [False, True])
+@pytest.mark.parametrize("Lt,V", [(40, 300), (300, 300), (700, 300), (33, 2000)])
+def test_sparse_head_gradients_of_nan_weights(Lt, V, zero, dt):
+    """A token that takes part and holds NaN wins every term of its text: its row of d_hidden, and
+    all of d_weight and d_bias, are NaN (also where dy is 0, as 0 / (1 + NaN) is), whether rows are
+    gathered (long texts) or multiplied, and where shares cut the text.  The other texts' rows of
+    d_hidden are those they have without it."""
+    import gpusparse
+    h, w, b, dy = head_inputs(3, Lt, V, 64, dt, seed=81)
+    mask = torch.ones(3, Lt, dtype=torch.bool, device=DEV)
+    mask[1] = False
+    _, ((rh, bh), _, _) = R.sparse_head(h, w, b, mask, dy, dt)
+    h[1, 17] = float("nan")
+    h[1, 30] = float("nan")
+    if zero:
+        dy[1] = 0
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    y = gpusparse.sparse_head(leaves[0], leaves[1], bias=leaves[2])
+    assert torch.isnan(y[1]).all() and torch.isfinite(y[0]).all() and torch.isfinite(y[2]).all()
+    dh, dw, db = torch.autograd.grad(y, leaves, dy)
+    assert torch.isnan(dh[1, 17]).all() and torch.isnan(dw).all() and torch.isnan(db).all()
+    dh[1, 17] = 0
+    assert (dh[1] == 0).all()
+    R.assert_within(dh.reshape(3 * Lt, 64), (rh, bh), "dh")
+
+
+@pytest.mark.parametrize("Lt", [40, 300])
+def test_sparse_head_gradients_of_a_nan_bias(Lt):
+    import gpusparse
+    h, w, b, dy = head_inputs(3, Lt, 300, 64, BF, seed=82)
+    b[5] = float("nan")
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    y = gpusparse.sparse_head(leaves[0], leaves[1], bias=leaves[2])
+    assert torch.equal(torch.isnan(y), (torch.arange(300, device=DEV) == 5).expand(3, 300))
+    dh, dw, db = torch.autograd.grad(y, leaves, dy)
+    assert torch.isnan(db[5]) and torch.isnan(dw[5]).all()
+    assert int(torch.isnan(db).sum()) == 1 and int(torch.isnan(dw).any(1).sum()) == 1
+    assert (torch.isnan(dh).all(2).sum(1) == 1).all() and (torch.isnan(dh).any(2).sum(1) == 1).all()
+
+
+def test_sparse_head_gradients_of_a_wait_that_ran_out():
+    """NaN weights of a wait that ran out have NaN gradients, not those of the other terms."""
+    import gpusparse
+    import gpusparse._lib as L
+    h, w, b = make(300, 900, 512, BF, seed=83)
+    lib = L.lib()
+    default = lib.gsp_get_wait_limit()
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    L.check(lib.gsp_set_wait_limit(0), "wait limit")
+    try:
+        y = gpusparse.sparse_head(leaves[0].reshape(3, 100, 512), leaves[1], bias=leaves[2])
+        torch.cuda.synchronize()
+    finally:
+        L.check(lib.gsp_set_wait_limit(default), "wait limit")
+    bad = torch.isnan(y)
+    assert bad.any()
+    dh, dw, db = torch.autograd.grad(y.sum(), leaves)
+    terms = bad.any(0)
+    assert torch.isnan(db[terms]).all() and torch.isnan(dw[terms]).all() and torch.isnan(dh).any()
