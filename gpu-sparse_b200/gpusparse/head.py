@@ -393,7 +393,8 @@ def encode_documents(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[
                      mask: Optional[torch.Tensor] = None, min_weight: float = 0.0):
     """Documents as CSR rows for the index builders: ``(indptr int64 [B + 1], indices int32,
     data fp32)`` on the GPU, the terms of ``sparse_head`` with a weight above ``min_weight``
-    (>= 0) in ascending order.  Synchronises once for the number of terms."""
+    (>= 0) in ascending order.  Synchronises once for the number of terms.  Raises RuntimeError
+    where weights are NaN (hidden states that are, or a wait that ran out)."""
     if not min_weight >= 0.0:
         raise ValueError("encode_documents: min_weight must be >= 0")
     with torch.no_grad():
@@ -409,7 +410,12 @@ def encode_documents(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[
         L.check(lib.gsp_dense_rows_count(L.ptr(y), B, V, min_weight, L.ptr(nnz), st), "encode_documents")
         L.check(lib.gsp_scan_i32(L.ptr(nnz), B, L.ptr(indptr), L.ptr(ws), ws.numel(), st),
                 "encode_documents")
-        total = int(indptr[B].item())
+        # weights are >= 0: a sum is NaN where one of them is
+        total, bad = torch.stack((indptr[B], y.sum().isnan().to(torch.int64))).tolist()
+        if bad:
+            rows = torch.isnan(y.sum(dim=1)).nonzero().flatten()
+            raise RuntimeError(f"encode_documents: the weights of {rows.numel()} of {B} documents are NaN, "
+                               f"the first is document {int(rows[0])}")
         indices = torch.empty(total, dtype=torch.int32, device=dev)
         data = torch.empty(total, dtype=torch.float32, device=dev)
         L.check(lib.gsp_dense_rows_fill(L.ptr(y), B, V, min_weight, L.ptr(indptr), L.ptr(indices),
@@ -422,7 +428,8 @@ def encode_queries(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[to
                    ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Queries as the scorer takes them: term ids int32 and weights fp32, both [B, max_terms]
     (-1 / 0 padded), the ``max_terms`` strongest terms of ``sparse_head``, ties by ascending
-    term id."""
+    term id.  A query with a NaN weight (hidden states that are NaN, or a wait that ran out) has
+    NaN in all of its weights, and one term at least."""
     if max_terms < 1:
         raise ValueError("encode_queries: max_terms must be positive")
     with torch.no_grad():
@@ -436,6 +443,9 @@ def encode_queries(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[to
         if qi.shape[1] < max_terms:
             qi = torch.nn.functional.pad(qi, (0, max_terms - qi.shape[1]), value=-1)
             qs = torch.nn.functional.pad(qs, (0, max_terms - qs.shape[1]))
+        bad = y.sum(dim=1).isnan()
+        qs.masked_fill_(bad[:, None], float("nan"))
+        qi[:, 0] = torch.where(bad, qi[:, 0].clamp(min=0), qi[:, 0])
     return qi, qs
 
 

@@ -423,7 +423,8 @@ int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, const float* y
                              int64_t ws_bytes, void* stream);
 /* Rows of a dense [B, V] fp32 matrix (the sparse head's y) as CSR rows for the index builders:
  * nnz[b] = entries > min_weight, then (after a scan of nnz into indptr, gsp_scan_i32) their
- * columns and values in ascending column order. */
+ * columns and values in ascending column order.  A NaN is not above min_weight: the caller
+ * looks for NaN in y (encode_documents raises). */
 int gsp_dense_rows_count(const float* y, int64_t B, int64_t V, float min_weight, int32_t* nnz, void* stream);
 int gsp_dense_rows_fill(const float* y, int64_t B, int64_t V, float min_weight, const int64_t* indptr, int32_t* indices,
                         float* data, void* stream);

@@ -777,3 +777,48 @@ def test_sparse_head_gradients_of_a_wait_that_ran_out():
     dh, dw, db = torch.autograd.grad(y.sum(), leaves)
     terms = bad.any(0)
     assert torch.isnan(db[terms]).all() and torch.isnan(dw[terms]).all() and torch.isnan(dh).any()
+
+
+def test_encoding_shows_nan_weights():
+    """NaN weights of a document or query do not pass for missing terms: encode_documents and
+    build_index_from_hidden raise, encode_queries gives the query NaN weights."""
+    import gpusparse
+    h, w, b, _ = head_inputs(4, 20, 600, 64, BF, seed=84, bias_mean=-2.0)
+    qi, qs = gpusparse.encode_queries(h, w, bias=b, max_terms=50)
+    ip, ix, dtv = gpusparse.encode_documents(h, w, bias=b)
+    h[2, 5] = float("nan")
+    with pytest.raises(RuntimeError, match="NaN"):
+        gpusparse.encode_documents(h, w, bias=b)
+    with pytest.raises(RuntimeError, match="NaN"):
+        gpusparse.encode_documents(h, w, bias=b, min_weight=0.5)
+    with pytest.raises(RuntimeError, match="NaN"):
+        gpusparse.build_index_from_hidden([h[:2], h[2:]], w, bias=b)
+    mask = torch.ones(4, 20, dtype=torch.bool, device=DEV)
+    mask[2, 5] = False
+    gpusparse.encode_documents(h, w, bias=b, mask=mask)
+    qi2, qs2 = gpusparse.encode_queries(h, w, bias=b, max_terms=50)
+    others = torch.tensor([0, 1, 3], device=DEV)
+    assert torch.equal(qi2[others], qi[others]) and torch.equal(qs2[others], qs[others])
+    assert torch.isnan(qs2[2]).all() and int(qi2[2, 0]) >= 0
+    b[7] = float("nan")                                       # one term of every text
+    with pytest.raises(RuntimeError, match="NaN"):
+        gpusparse.encode_documents(h[:1], w, bias=b)
+    qi3, qs3 = gpusparse.encode_queries(h[:1], w, bias=b, max_terms=700)
+    assert torch.isnan(qs3).all() and qs3.shape == (1, 700) and int(qi3[0, 0]) >= 0
+
+
+def test_encoding_shows_a_wait_that_ran_out():
+    import gpusparse
+    import gpusparse._lib as L
+    h, w, b = make(300, 900, 512, BF, seed=85)
+    lib = L.lib()
+    default = lib.gsp_get_wait_limit()
+    L.check(lib.gsp_set_wait_limit(0), "wait limit")
+    try:
+        with pytest.raises(RuntimeError, match="NaN"):
+            gpusparse.encode_documents(h[None], w, bias=b)
+        qs = gpusparse.encode_queries(h[None], w, bias=b)[1]
+        torch.cuda.synchronize()
+    finally:
+        L.check(lib.gsp_set_wait_limit(default), "wait limit")
+    assert torch.isnan(qs).all()
