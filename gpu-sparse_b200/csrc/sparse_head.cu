@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(mm::kBM) head_join_kernel(const JoinParams p) 
 // ---- backward ----------------------------------------------------------------------------
 struct Survey {
   int64_t nnz;            // entries: (text, term) pairs with a gradient
-  uint32_t absmax;        // largest finite |dy| (an upper bound of |ds|, which scales fp16's P)
+  uint32_t absmax;        // largest finite |dy| of them (an upper bound of |ds|, which scales fp16's P)
   uint32_t pad_;
 };
 
@@ -336,7 +336,7 @@ survey_kernel(State s, const SortParams p, Survey* out, void* d_hidden, int64_t 
         if (t < hi) {
           const float d = p.dy[b * p.V + t], a = fabsf(d);
           const int32_t w = p.win[b * p.V + t];
-          if (a < __uint_as_float(0x7F800000u)) m = fmaxf(m, a);
+          if (w >= 0 && a < __uint_as_float(0x7F800000u)) m = fmaxf(m, a);
           if (w >= 0 && (d != 0.0f || is_nan(p.y[b * p.V + t]))) r[k] = w;
         }
         c += r[k] >= 0;
@@ -623,9 +623,11 @@ struct SpreadParams {
   int64_t pitch, v0, cols, V, B;
   int32_t L, bf16;
 };
-__device__ __forceinline__ float p_scale(const Survey* s, bool bf16) {     // P = ds * this
+// P = ds * this, at most 2^100: the quotient leaves fp32 for |dy| below 5e-35, and the gradients of
+// entries that 2^100 lifts to no more than 2^14 are far below fp16's smallest numbers anyway
+__device__ __forceinline__ float p_scale(const Survey* s, bool bf16) {
   const float m = bf16 ? 0.0f : __uint_as_float(s->absmax);
-  return m > 0.0f ? 16384.0f / m : 1.0f;
+  return m > 0.0f ? fminf(16384.0f / m, 0x1p100f) : 1.0f;
 }
 constexpr int kSpreadRows = 64;
 // P of a piece: a thread owns 8 columns of one text and writes them for up to kSpreadRows of

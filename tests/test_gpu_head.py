@@ -822,3 +822,24 @@ def test_encoding_shows_a_wait_that_ran_out():
     finally:
         L.check(lib.gsp_set_wait_limit(default), "wait limit")
     assert torch.isnan(qs).all()
+
+
+@pytest.mark.parametrize("case", ["tiny", "outlier"])
+def test_sparse_head_fp16_gradients_scale_with_the_entries_that_have_one(case):
+    """The products' 16-bit P is scaled by the largest dy of a term that has a weight: neither a
+    dy of 1e-36 (whose reciprocal leaves fp32) nor a huge dy of terms without weight costs the
+    others their gradient."""
+    import gpusparse
+    h, w, b, dy = head_inputs(30, 3, 700, 64, HF, seed=86)
+    ref, _ = R.sparse_head(h, w, b, torch.ones(30, 3, dtype=torch.bool, device=DEV), dy, HF)
+    live = ref[0] > 0
+    assert 0.1 < float(live.double().mean()) < 0.9
+    dy = dy * 1e-36 if case == "tiny" else torch.where(live, dy, 1e30)
+    _, (rh, rw, rb) = R.sparse_head(h, w, b, torch.ones(30, 3, dtype=torch.bool, device=DEV),
+                                    torch.where(live, dy, 0.0), HF)
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    got = torch.autograd.grad(gpusparse.sparse_head(leaves[0], leaves[1], bias=leaves[2]), leaves, dy)
+    R.assert_within(got[0].reshape(-1, 64), rh, "dh")
+    R.assert_within(got[1], rw, "dw")
+    # (fp32 results of 1e-36 have no subnormal parts to lose: 2^-126 is 1e-38)
+    R.assert_within(got[2], (rb[0], rb[1] + (2.0 ** -126 * 30 if case == "tiny" else 0.0)), "db")
