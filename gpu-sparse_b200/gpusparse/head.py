@@ -20,7 +20,8 @@ are packed away on the GPU first: they cost nothing, and what they hold is never
 No call synchronises except ``encode_documents`` and ``build_index_from_hidden``, whose
 results' sizes depend on the data; the others can be captured in a CUDA graph.  (As with any
 torch operator, a backward pass is captured only while no uncaptured graph of the same leaves is
-alive: that graph's accumulation nodes belong to another stream.)
+alive: that graph's accumulation nodes belong to another stream.)  Forward-mode derivatives and
+gradients of gradients raise.
 """
 from __future__ import annotations
 
@@ -30,6 +31,7 @@ import functools
 from typing import Iterable, Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib as L
 from .index import GPUInvertedIndex, build_from_csr_tensors
@@ -54,6 +56,16 @@ def _as(x: torch.Tensor, dtype) -> torch.Tensor:
 
 def _is_integer(x: torch.Tensor) -> bool:
     return not (x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool)
+
+
+def _differentiated(hidden, weight, bias) -> bool:
+    """Whether the call belongs in an autograd function: for a gradient, or for a forward-mode
+    tangent, which the function has no rule for and raises."""
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
+        return True
+    return forward_ad._current_level >= 0 and any(
+        x is not None and forward_ad.unpack_dual(x).tangent is not None for x in (hidden, weight, bias))
 
 
 def _check(what: str, hidden, weight, bias):
@@ -230,8 +242,7 @@ def _loss(kind, hidden, weight, bias, targets, ignore_index, scores, ids, tau, r
         bias = _as(bias, torch.float32)
     red = L.REDUCE[reduction]
     args = (kind, targets, ignore_index, scores, ids, tau, red)
-    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
+    if _differentiated(hidden, weight, bias):
         loss = _VocabLoss.apply(hidden, weight, bias, args)
     else:
         loss = _loss_forward(hidden, weight, bias, args, False)[0]
@@ -382,8 +393,7 @@ def sparse_head(hidden: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     weight = _rows(weight)
     if bias is not None:
         bias = _as(bias, torch.float32)
-    if torch.is_grad_enabled() and (rows.requires_grad or weight.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
+    if _differentiated(rows, weight, bias):
         return _SparseHead.apply(rows, weight, bias, mask, Lt)
     return _head_forward(rows, weight, bias, mask, Lt, False)[0]
 

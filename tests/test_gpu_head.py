@@ -843,3 +843,40 @@ def test_sparse_head_fp16_gradients_scale_with_the_entries_that_have_one(case):
     R.assert_within(got[1], rw, "dw")
     # (fp32 results of 1e-36 have no subnormal parts to lose: 2^-126 is 1e-38)
     R.assert_within(got[2], (rb[0], rb[1] + (2.0 ** -126 * 30 if case == "tiny" else 0.0)), "db")
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor needs no gradient, but its result without a tangent would be wrong."""
+    import torch.autograd.forward_ad as fwd
+    import gpusparse
+    h, w, b, targets, scores, ids = step_inputs(87)
+    h, w, b = h.detach(), w.detach(), b.detach()
+    for call in (lambda h, w, b: gpusparse.vocab_cross_entropy(h, w, targets, bias=b),
+                 lambda h, w, b: gpusparse.topk_distillation(h, w, scores, ids, bias=b),
+                 lambda h, w, b: gpusparse.sparse_head(h[None], w, bias=b),
+                 lambda h, w, b: gpusparse.encode_documents(h[None], w, bias=b)):
+        want = call(h, w, b)
+        for which in range(3):
+            with fwd.dual_level():
+                args = [h, w, b]
+                args[which] = fwd.make_dual(args[which], torch.ones_like(args[which]))
+                with pytest.raises(RuntimeError):
+                    call(*args)
+                with torch.no_grad(), pytest.raises(RuntimeError):
+                    call(*args)
+                got = call(h, w, b)                # no tangent: nothing to refuse
+        if isinstance(want, torch.Tensor):
+            assert torch.equal(got, want)
+
+
+def test_differentiating_a_gradient_again_is_refused():
+    import gpusparse
+    h, w, b, targets, scores, ids = step_inputs(88)
+    for call in (lambda: gpusparse.vocab_cross_entropy(h, w, targets, bias=b),
+                 lambda: gpusparse.topk_distillation(h, w, scores, ids, bias=b),
+                 lambda: gpusparse.sparse_head(h[None], w, bias=b).sum()):
+        want = torch.autograd.grad(call(), (h, w, b))
+        got = torch.autograd.grad(call(), (h, w, b), create_graph=True)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        with pytest.raises(RuntimeError):
+            got[0].float().sum().backward()

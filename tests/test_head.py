@@ -120,3 +120,18 @@ def test_host_tensors_are_refused():
         gpusparse.topk_distillation(h, w, torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int64))
     with pytest.raises(RuntimeError):
         gpusparse.sparse_head(h[None], w)
+
+
+def test_tangents_are_noticed():
+    """A dual tensor needs no gradient; its call still belongs in the autograd function, which
+    refuses it, and not in one that drops the tangent."""
+    import torch.autograd.forward_ad as fwd
+    from gpusparse import head
+    x, w, b = torch.ones(2, 3), torch.ones(4, 3), torch.ones(4)
+    assert not head._differentiated(x, w, b) and head._differentiated(x, w, torch.ones(4, requires_grad=True))
+    with fwd.dual_level():
+        assert not head._differentiated(x, w, None)
+        with torch.no_grad():
+            assert head._differentiated(fwd.make_dual(x, x), w, None)
+            assert head._differentiated(x, w, fwd.make_dual(b, b))
+            assert not head._differentiated(x, w, torch.ones(4, requires_grad=True))
