@@ -152,9 +152,21 @@ def _read_in_place(weight: torch.Tensor) -> bool:
     return ld % 8 == 0 and weight.data_ptr() % 16 == 0
 
 
+# Hooks on saved tensors may have given them another layout; the backward calls read them as the
+# forward calls left them: contiguous, the state on a 256-byte boundary.
+def _saved(x: torch.Tensor) -> torch.Tensor:
+    return x if x.is_contiguous() else x.contiguous()
+
+
+def _saved_state(state: torch.Tensor) -> torch.Tensor:
+    state = _saved(state)
+    return state if state.data_ptr() % 256 == 0 else state.clone()
+
+
 def _saved_weight(weight: torch.Tensor, in_place: bool) -> torch.Tensor:
-    """The forward call's weight as its state expects it: hooks on saved tensors may have given
-    its rows another layout."""
+    """The forward call's weight as its state expects it (which holds a copy of rows that are not
+    read in place)."""
+    weight = _rows(weight)
     if not in_place or _read_in_place(weight):
         return weight
     V, D = weight.shape
@@ -202,7 +214,7 @@ def _loss_backward(ctx, grad):
     kind, K, tau, reduction, T, in_place = ctx.args
     dev = weight.device
     with _on(dev):
-        weight = _saved_weight(weight, in_place)
+        weight, state = _saved_weight(weight, in_place), _saved_state(state)
         v = _view((T, None), weight, None)
         grad = _as(grad, torch.float32)
         _, wb = _bytes(v, K, kind, True, dev)
@@ -334,7 +346,8 @@ def _head_backward(ctx, dy):
     T, Lt, in_place = ctx.args
     dev = weight.device
     with _on(dev):
-        weight = _saved_weight(weight, in_place)
+        weight, state = _saved_weight(weight, in_place), _saved_state(state)
+        y, win = _saved(y), _saved(win)
         v = _view((T, None), weight, None)
         dy = _as(dy, torch.float32)
         _, wb = _bytes(v, 0, L.VOCAB_HEAD, True, dev)

@@ -880,3 +880,31 @@ def test_differentiating_a_gradient_again_is_refused():
         assert all(torch.equal(x, y) for x, y in zip(got, want))
         with pytest.raises(RuntimeError):
             got[0].float().sum().backward()
+
+
+@pytest.mark.parametrize("D", [83, 88])
+def test_hooks_may_change_the_layout_of_all_saved_tensors(D):
+    """Matrices saved column by column, and buffers (the state) off their boundaries."""
+    import gpusparse
+    h, w, b = make(60, 300, D, BF, seed=55)
+    targets = torch.arange(60, device=DEV)
+    scores, ids = teacher(60, 300, 5, seed=55)
+    dy = torch.randn(6, 300, generator=torch.Generator().manual_seed(1)).to(DEV)
+
+    def pack(x):
+        if x.dim() == 2:
+            return x.detach().t().contiguous()
+        return torch.cat((x.detach().new_zeros(8), x.detach()))
+
+    def unpack(x):
+        return x.t() if x.dim() == 2 else x[8:]
+    for call in (lambda h, w, b: gpusparse.vocab_cross_entropy(h, w, targets, bias=b),
+                 lambda h, w, b: gpusparse.topk_distillation(h, w, scores, ids, bias=b),
+                 lambda h, w, b: (gpusparse.sparse_head(h.reshape(6, 10, D), w, bias=b) * dy).sum()):
+        plain = [leaf(h), leaf(w), leaf(b)]
+        want = torch.autograd.grad(call(*plain), plain)
+        hooked = [leaf(h), leaf(w), leaf(b)]
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            out = call(*hooked)
+        got = torch.autograd.grad(out, hooked)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
