@@ -790,6 +790,14 @@ Bwd carve_bwd(void* base, const gsp_vocab_view* vw) {
 // else spend as long on rows of nothing as on the vocabulary)
 int32_t box_rows(int64_t T) { return int32_t(T >= mm::kRows ? mm::kRows : up(T, 8)); }
 
+// tau^2 scales the losses and 1 / tau the logits: both stay normal numbers
+int check_temperature(float tau, const char* what) {
+  const float t2 = tau * tau;
+  GSP_REQUIRE(tau > 0.0f && t2 >= 0x1p-126f && t2 < __builtin_inff(), GSP_ERR_ARG,
+              "%s: temperature must be positive, from 1.1e-19 to 1.8e19, got %g", what, double(tau));
+  return GSP_OK;
+}
+
 int check_reduction(int32_t reduction, const char* what) {
   GSP_REQUIRE(reduction >= GSP_REDUCE_NONE && reduction <= GSP_REDUCE_MEAN, GSP_ERR_ARG, "%s: unknown reduction %d", what,
               reduction);
@@ -897,7 +905,7 @@ extern "C" int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, 
   cudaStream_t st = as_stream(stream);
   GSP_REQUIRE(K >= 1 && K <= GSP_DISTILL_MAX_K, GSP_ERR_ARG, "topk_distillation: %lld teacher entries, 1 to %d are supported",
               (long long)K, GSP_DISTILL_MAX_K);
-  GSP_REQUIRE(tau > 0.0f && tau < __builtin_inff(), GSP_ERR_ARG, "topk_distillation: temperature must be positive");
+  if ((rc = check_temperature(tau, "topk_distillation"))) return rc;
   GSP_REQUIRE(loss || (vw->T == 0 && reduction == GSP_REDUCE_NONE), GSP_ERR_ARG, "topk_distillation: null loss");
   const State s = carve_state(state, vw, K, 0);
   const Fwd f = carve_fwd(ws, vw, K);
@@ -934,8 +942,8 @@ extern "C" int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, i
   if ((rc = check_grads(vw, d_hidden, d_weight, "vocab loss backward"))) return rc;
   GSP_REQUIRE(kind == GSP_VOCAB_CE || kind == GSP_VOCAB_DISTILL, GSP_ERR_ARG, "vocab loss backward: unknown kind %d", kind);
   const bool list = kind == GSP_VOCAB_DISTILL;
-  GSP_REQUIRE(!list || (K >= 1 && K <= GSP_DISTILL_MAX_K && tau > 0.0f && tau < __builtin_inff()), GSP_ERR_ARG,
-              "vocab loss backward: bad teacher entries or temperature");
+  GSP_REQUIRE(!list || (K >= 1 && K <= GSP_DISTILL_MAX_K), GSP_ERR_ARG, "vocab loss backward: bad teacher entries");
+  if (list && (rc = check_temperature(tau, "vocab loss backward"))) return rc;
   cudaStream_t st = as_stream(stream);
   const State s = carve_state(state, vw, list ? K : 0, 0);
   const Bwd b = carve_bwd(ws, vw);

@@ -299,7 +299,8 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_scores
     in any order (``score_topk`` and ``compacted_topk`` return this pair).  Entries with an
     id outside [0, V) or a score of -inf are left out, an id listed twice adds its
     probabilities, and a token without entries takes no part (as an ignored target in
-    ``vocab_cross_entropy``).  No gradient flows to the teacher's scores.
+    ``vocab_cross_entropy``).  No gradient flows to the teacher's scores.  The temperature's
+    square has to be a normal fp32 number (1.1e-19 to 1.8e19).
     """
     _check("topk_distillation", hidden, weight, bias)
     _check_reduction("topk_distillation", reduction)

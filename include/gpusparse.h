@@ -390,7 +390,7 @@ int gsp_vocab_ce(const gsp_vocab_view* vw, const int64_t* targets, int64_t ignor
                  void* state, int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream);
 /* Distillation from a teacher's top scores (scores fp32, ids int64, both [T, K], K <=
  * GSP_DISTILL_MAX_K): with p = softmax(scores / tau) over a row's entries, the loss of the
- * row is tau^2 KL(p || softmax(s / tau)).  Entries with an id outside [0, V) or a score of
+ * row is tau^2 KL(p || softmax(s / tau)), tau^2 a normal fp32 number.  Entries with an id outside [0, V) or a score of
  * -inf (the padding of gsp_score_topk and gsp_compacted_topk) are left out, an id listed
  * twice adds its probabilities, and a row without entries takes no part. */
 int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, const int64_t* ids, int64_t K, float tau,

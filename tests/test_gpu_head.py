@@ -908,3 +908,32 @@ def test_hooks_may_change_the_layout_of_all_saved_tensors(D):
             out = call(*hooked)
         got = torch.autograd.grad(out, hooked)
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("tau", [1.1e-19, 1e-6, 1e-2, 1e3, 1e6, 1.8e19])
+def test_distillation_at_extreme_temperatures(tau):
+    import gpusparse
+    h, w, b = make(40, 300, 64, BF, seed=56)
+    scores, ids = teacher(40, 300, 7, seed=56)
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    loss = gpusparse.topk_distillation(*leaves[:2], scores, ids, bias=leaves[2], temperature=tau)
+    grads = torch.autograd.grad(loss, leaves)
+    assert torch.isfinite(loss.detach()) or tau > 1e18          # (tau^2 ln(300 / 7) leaves fp32)
+    assert all(torch.isfinite(g).all() for g in grads)
+    if 1e-3 < tau < 1e7:
+        p = torch.softmax(scores.double() / tau, 1)
+        q = torch.zeros(40, 300, dtype=torch.float64, device=DEV).scatter_(1, ids, p)
+        rows = torch.full((40,), 1 / 40, device=DEV)
+        ref, refs = R.softmax_loss(h, w, b, q, torch.ones(40, dtype=torch.bool, device=DEV), tau, rows, BF)
+        R.assert_within(loss.detach(), (ref[0].mean(), ref[1].mean() + 2.0 ** -23 * ref[0].mean().abs()), "loss")
+        # at small temperatures softmax values pass below 2^-126, where they count as 0: P is off
+        # by 2^-126 of the row's coefficient tau / 40 there, its sums by that times the other
+        # operand (bf16's own subnormal steps are 2^-133 and with that less)
+        floor = 2.0 ** -126 * max(tau / 40, 1.0)
+        sums = (300 * float(w.abs().max()), 40 * float(h.abs().max()), 40)
+        for g, (value, bound), n, what in zip(grads, refs, sums, ("dh", "dw", "db")):
+            R.assert_within(g, (value, bound + n * floor), what)
+    with pytest.raises(ValueError):
+        gpusparse.topk_distillation(h, w, scores, ids, temperature=1e-25)
+    with pytest.raises(ValueError):
+        gpusparse.topk_distillation(h, w, scores, ids, temperature=1e25)

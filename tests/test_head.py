@@ -135,3 +135,18 @@ def test_tangents_are_noticed():
             assert head._differentiated(fwd.make_dual(x, x), w, None)
             assert head._differentiated(x, w, fwd.make_dual(b, b))
             assert not head._differentiated(x, w, torch.ones(4, requires_grad=True))
+
+
+def test_temperatures_that_leave_fp32_are_refused():
+    """The square or the reciprocal would be 0, infinite or short of bits, and the losses NaN."""
+    lib = L.lib()
+    ref, fake, big = ctypes.byref(view()), ctypes.c_void_p(4096), 1 << 40
+    for tau in (1e-45, 1e-39, 1e-30, 1.08e-19, 1.9e19, 1e30, -1.0, -1e-30):
+        assert lib.gsp_vocab_distill(ref, fake, fake, 4, tau, 2, fake, fake, big, fake, big, None) == L.GSP_ERR_ARG
+        assert b"temperature" in lib.gsp_last_error()
+        assert lib.gsp_vocab_loss_backward(ref, L.VOCAB_DISTILL, 4, tau, 2, fake, fake, fake, fake, fake, big, fake, big,
+                                           None) == L.GSP_ERR_ARG
+        assert b"temperature" in lib.gsp_last_error()
+    for tau in (1.1e-19, 1.8e19):         # accepted: the next check, of the buffers, is the one that refuses
+        assert lib.gsp_vocab_distill(ref, fake, fake, 4, tau, 2, fake, fake, 0, fake, big, None) == L.GSP_ERR_ARG
+        assert b"state" in lib.gsp_last_error()
