@@ -630,8 +630,9 @@ __device__ __forceinline__ float p_scale(const Survey* s, bool bf16) {
   return m > 0.0f ? fminf(16384.0f / m, 0x1p100f) : 1.0f;
 }
 constexpr int kSpreadRows = 64;
-// P of a piece: a thread owns 8 columns of one text and writes them for up to kSpreadRows of
-// its rows; the blocks of text B zero the rows past the packed ones.
+// P of a piece: a thread owns 8 columns of one text and writes them for kSpreadRows of its rows
+// (of every gridDim.z x kSpreadRows, for texts longer than a grid is deep); the blocks of text B
+// zero the rows past the packed ones.
 __global__ void __launch_bounds__(256) spread_kernel(const SpreadParams p) {
   mm::after_previous();
   const int32_t n = p.head[0];
@@ -640,15 +641,9 @@ __global__ void __launch_bounds__(256) spread_kernel(const SpreadParams p) {
   const int64_t b = blockIdx.y;
   const float up_by = p_scale(p.survey, p.bf16 != 0);
   if (blockIdx.x == 0 && b == 0 && blockIdx.z == 0 && threadIdx.x == 0) *p.scale = 1.0f / up_by;
-  int32_t r0, r1;
-  if (b < p.B) {
-    r0 = p.text[b] + blockIdx.z * kSpreadRows;
-    r1 = min(p.text[b + 1], r0 + kSpreadRows);
-  } else {
-    r0 = n + blockIdx.z * kSpreadRows;
-    r1 = min((n + mm::kBM - 1) / mm::kBM * mm::kBM, r0 + kSpreadRows);
-  }
-  if (r0 >= r1 || c >= p.pitch) return;
+  const int32_t r0 = (b < p.B ? p.text[b] : n) + blockIdx.z * kSpreadRows;
+  const int32_t end = b < p.B ? p.text[b + 1] : (n + mm::kBM - 1) / mm::kBM * mm::kBM;
+  if (r0 >= end || c >= p.pitch) return;
   int32_t w[8];
   float ds[8];
 #pragma unroll
@@ -661,13 +656,16 @@ __global__ void __launch_bounds__(256) spread_kernel(const SpreadParams p) {
       if (w[k] >= 0) ds[k] = p.dy[b * p.V + v] * expf(-p.y[b * p.V + v]) * up_by;
     }
   }
-  for (int32_t r = r0; r < r1; ++r) {
-    uint4 o;
-    uint32_t* u = &o.x;
+  for (int64_t rz = r0; rz < end; rz += int64_t(gridDim.z) * kSpreadRows) {
+    const int32_t r1 = int32_t(min64(end, rz + kSpreadRows));
+    for (int32_t r = int32_t(rz); r < r1; ++r) {
+      uint4 o;
+      uint32_t* u = &o.x;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      u[k] = pack2(w[2 * k] == r ? ds[2 * k] : 0.0f, w[2 * k + 1] == r ? ds[2 * k + 1] : 0.0f, p.bf16 != 0);
-    *reinterpret_cast<uint4*>(p.P + int64_t(r) * p.pitch + c) = o;
+      for (int k = 0; k < 4; ++k)
+        u[k] = pack2(w[2 * k] == r ? ds[2 * k] : 0.0f, w[2 * k + 1] == r ? ds[2 * k + 1] : 0.0f, p.bf16 != 0);
+      *reinterpret_cast<uint4*>(p.P + int64_t(r) * p.pitch + c) = o;
+    }
   }
 }
 
@@ -951,8 +949,7 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   p.B = B;
   p.L = int32_t(L);
   p.bf16 = bf;
-  const int64_t zs = ((L < mm::kBM ? mm::kBM : L) + kSpreadRows - 1) / kSpreadRows;
-  GSP_REQUIRE(zs <= 65535, GSP_ERR_ARG, "sparse_head backward: texts of %lld tokens are too long", (long long)L);
+  const int64_t zs = min64(((L < mm::kBM ? mm::kBM : L) + kSpreadRows - 1) / kSpreadRows, 65535);
   for (int64_t v0 = 0; v0 < vw->V; v0 += b.pitch) {
     p.v0 = v0;
     p.cols = min64(b.pitch, vw->V - v0);

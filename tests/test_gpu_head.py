@@ -937,3 +937,11 @@ def test_distillation_at_extreme_temperatures(tau):
         gpusparse.topk_distillation(h, w, scores, ids, temperature=1e-25)
     with pytest.raises(ValueError):
         gpusparse.topk_distillation(h, w, scores, ids, temperature=1e25)
+
+
+def test_sparse_head_of_a_text_longer_than_a_grid_is_deep():
+    """4.2 million tokens, more than 65535 blocks of 64 rows: the same winners and gradients as any."""
+    h, w, b, dy = head_inputs(1, 65535 * 64 + 100, 20, 8, BF, seed=57)
+    h[0, -50:] += 4.0           # the last rows, which only a second round reaches, win terms
+    _, got = check_head(h, w, b, None, dy)
+    assert (got[0][0, -50:] != 0).any()
