@@ -621,7 +621,7 @@ struct SpreadParams {
   float* scale;
   uint16_t* P;
   int64_t pitch, v0, cols, V, B;
-  int32_t L, bf16;
+  int32_t bf16;
 };
 // P = ds * this, at most 2^100: the quotient leaves fp32 for |dy| below 5e-35, and the gradients of
 // entries that 2^100 lifts to no more than 2^14 are far below fp16's smallest numbers anyway
@@ -947,7 +947,6 @@ extern "C" int gsp_sparse_head_backward(const gsp_vocab_view* vw, int64_t L, con
   p.pitch = b.pitch;
   p.V = vw->V;
   p.B = B;
-  p.L = int32_t(L);
   p.bf16 = bf;
   const int64_t zs = min64(((L < mm::kBM ? mm::kBM : L) + kSpreadRows - 1) / kSpreadRows, 65535);
   for (int64_t v0 = 0; v0 < vw->V; v0 += b.pitch) {

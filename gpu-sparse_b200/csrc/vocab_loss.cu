@@ -304,7 +304,6 @@ struct LossJob {
   CUtensorMap maps[2];      // H, W (K-major)
   int32_t wait_limit, bf16;
   const int32_t* head;
-  const int32_t* map;
   int32_t nt, nk;           // tiles along the vocabulary, steps along D
   int32_t a_rows;
   float c;
@@ -567,7 +566,6 @@ struct LogitGradJob {
   CUtensorMap maps[3];      // H, W (K-major); P as 32 x 64 boxes
   int32_t wait_limit, bf16;
   const int32_t* head;
-  const int32_t* map;
   int32_t nk, v0, nt;       // the piece's first vocabulary row and 256-wide tiles
   int32_t a_rows;
   int32_t low;              // see low_rows
@@ -817,7 +815,6 @@ int run_forward(const gsp_vocab_view* vw, const State& s, const Fwd& f, float ta
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.head = s.head;
-  j.map = s.map;
   j.nt = int32_t(s.Vp / mm::kBN);
   j.nk = int32_t((vw->D + mm::kBK - 1) / mm::kBK);
   j.c = kLog2e / tau;
@@ -844,7 +841,6 @@ int run_backward(const gsp_vocab_view* vw, const State& s, const Bwd& b, float t
   j.wait_limit = gsp_get_wait_limit();
   j.bf16 = bf;
   j.head = s.head;
-  j.map = s.map;
   j.nk = int32_t((vw->D + mm::kBK - 1) / mm::kBK);
   j.c = kLog2e / tau;
   j.bias2 = s.bias2;
