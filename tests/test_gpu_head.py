@@ -945,3 +945,41 @@ def test_sparse_head_of_a_text_longer_than_a_grid_is_deep():
     h[0, -50:] += 4.0           # the last rows, which only a second round reaches, win terms
     _, got = check_head(h, w, b, None, dy)
     assert (got[0][0, -50:] != 0).any()
+
+
+# ---------------------------------------------------------------------------- sizes and ways
+def test_winners_of_thousands_of_terms_are_gathered():
+    """The inputs of test_skewed_winners take the way they are meant for: few enough entries to be
+    gathered, and tokens with more of them than one warp sums alone (256)."""
+    h, w, b, dy = head_inputs(2, 300, 3000, 96, BF, seed=47, bias_mean=0.0)
+    b += 8.0
+    h[:, 1:] = 0
+    h[:, 0] = 0.03125
+    h[1, 7] = 0.0625
+    s = h.double() @ w.double().t() + b.double()
+    best, arg = s.max(dim=1)
+    assert (best > 0).all() and (dy != 0).all()
+    wins = torch.stack([torch.bincount(a, minlength=300) for a in arg])
+    assert (wins.max(dim=1).values > 256).all() and int((wins > 256).sum()) >= 3
+    assert dy.numel() * 160 <= 600 * 3000
+    check_head(h, w, b, None, dy)
+
+
+def test_weights_on_the_host_are_refused():
+    import gpusparse
+    h, w, b = make(10, 50, 16, BF, seed=51)
+    t = torch.zeros(10, dtype=torch.int64, device=DEV)
+    s, i = torch.zeros(10, 4, device=DEV), torch.zeros(10, 4, dtype=torch.int64, device=DEV)
+    for bad in (lambda: gpusparse.vocab_cross_entropy(h, w.cpu(), t),
+                lambda: gpusparse.topk_distillation(h, w.cpu(), s, i),
+                lambda: gpusparse.sparse_head(h[None], w.cpu()),
+                lambda: gpusparse.encode_documents(h[None], w.cpu()),
+                lambda: gpusparse.encode_queries(h[None], w.cpu())):
+        with pytest.raises(RuntimeError):
+            bad()
+    for bad in (lambda: gpusparse.topk_distillation(h, w, s.cpu(), i), lambda: gpusparse.topk_distillation(h, w, s, i.cpu()),
+                lambda: gpusparse.topk_distillation(h, w, s, i, bias=b.cpu()),
+                lambda: gpusparse.sparse_head(h[None], w, bias=b.cpu()),
+                lambda: gpusparse.sparse_head(h[None], w, mask=torch.ones(1, 10))):
+        with pytest.raises(ValueError):
+            bad()
