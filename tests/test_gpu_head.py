@@ -965,6 +965,188 @@ def test_winners_of_thousands_of_terms_are_gathered():
     check_head(h, w, b, None, dy)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_sparse_head_products_in_pieces(dt):
+    """Short texts with dense terms, more tokens x vocabulary than one piece of P holds: d_hidden is
+    carried over the pieces in fp32.  The reference is the definition, 250 texts at a time."""
+    import gpusparse
+    B, Lt, V, D = 2000, 10, 15000, 40
+    h, w, b, dy = head_inputs(B, Lt, V, D, dt, seed=91)
+    dy = dy.clamp_(-3.0, 3.0)
+    dy[:, 0] = 3.0                                   # every block of texts has the same largest dy
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    y = gpusparse.sparse_head(leaves[0], leaves[1], bias=leaves[2])
+    assert int((y > 0).sum()) * 160 > B * Lt * V and B * Lt * V * 2 > 512 << 20
+    dh, dw, db = torch.autograd.grad(y, leaves, dy)
+    rw = [torch.zeros(V, D, dtype=torch.float64, device=DEV) for _ in range(2)]
+    rb = [torch.zeros(V, dtype=torch.float64, device=DEV) for _ in range(2)]
+    all_in = torch.ones(250, Lt, dtype=torch.bool, device=DEV)
+    for lo in range(0, B, 250):
+        r = slice(lo, lo + 250)
+        ref, (qh, qw, qb) = R.sparse_head(h[r], w, b, all_in, dy[r], dt)
+        R.assert_within(y.detach()[r], ref, "y")
+        R.assert_within(dh[r].reshape(-1, D), qh, "dh")
+        for total, part in ((rw, qw), (rb, qb)):
+            total[0] += part[0]
+            total[1] += part[1]
+    # the blocks' bounds count sums of 2500 terms; the whole sum has 20000, each of at most the
+    # bound / u (the bound has u times every term)
+    rw[1] += B * Lt * 2.0 ** -23 * rw[1] / R.U[dt]
+    # d_bias: fp32 sums of 2000 terms of at most 3
+    rb[1] += B * 2.0 ** -24 * 3.0 * B
+    R.assert_within(dw, rw, "dw")
+    R.assert_within(db, rb, "db")
+
+
+def test_cross_entropy_offsets_past_32_bits():
+    """2.3e9 hidden values: rows are read, packed and written behind 2^31 elements."""
+    import gpusparse
+    T, V, D = 3_000_000, 300, 768
+    g = torch.Generator(device=DEV).manual_seed(92)
+    h = torch.randn(T, D, generator=g, device=DEV, dtype=BF)
+    w = (torch.randn(V, D, generator=g, device=DEV) * (2.0 / D ** 0.5)).to(BF)
+    targets = torch.randint(0, V, (T,), generator=g, device=DEV)
+    targets[torch.rand(T, generator=g, device=DEV) < 0.02] = -100
+    rows = torch.randn(T, generator=g, device=DEV)
+    hl, wl = h.requires_grad_(True), leaf(w)
+    loss = gpusparse.vocab_cross_entropy(hl, wl, targets, reduction="none")
+    dh, dw = torch.autograd.grad(loss, (hl, wl), rows)
+    loss, h = loss.detach(), h.detach()
+    want, off = torch.zeros(V, D, dtype=torch.float64, device=DEV), torch.zeros(V, D, dtype=torch.float64, device=DEV)
+    for lo in range(0, T, 100_000):
+        r = slice(lo, lo + 100_000)
+        live = targets[r] >= 0
+        ref, (rh, rw, _) = R.softmax_loss(h[r], w, None, one_hot(targets[r], V, live), live, 1.0, rows[r], BF)
+        assert ((loss[r].double() - ref[0]).abs() <= ref[1]).all()      # (compared on the GPU: 2.3e9 values)
+        assert ((dh[r].double() - rh[0]).abs() <= rh[1]).all()
+        want += rw[0]
+        off += rw[1]
+    # as above: sums of 3e6 terms instead of 1e5
+    R.assert_within(dw, (want, off + T * 2.0 ** -23 * off / R.U[BF]), "dw")
+
+
+def test_sparse_head_offsets_past_32_bits():
+    """60000 texts x 40000 terms, 2.4e9 weights; the gradient comes from the last texts."""
+    import gpusparse
+    B, V, D = 60_000, 40_000, 16
+    g = torch.Generator(device=DEV).manual_seed(93)
+
+    def grid(x, step):
+        return torch.round(x / step) * step
+    h = grid(torch.randn(B, 1, D, generator=g, device=DEV).clamp(-3.9, 3.9), 2.0 ** -5).to(BF)
+    w = grid((torch.randn(V, D, generator=g, device=DEV) / 4).clamp(-0.24, 0.24), 2.0 ** -10).to(BF)
+    b = grid(torch.randn(V, generator=g, device=DEV) * 0.5 - 1.0, 2.0 ** -10)
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    y = gpusparse.sparse_head(leaves[0], leaves[1], bias=leaves[2])
+    dy = torch.zeros(B, V, device=DEV)
+    dy[-40:] = torch.randn(40, V, generator=g, device=DEV)
+    dh, dw, db = torch.autograd.grad(y, leaves, dy)
+    one = torch.ones(40, 1, dtype=torch.bool, device=DEV)
+    for r in (slice(0, 40), slice(53_680, 53_720), slice(B - 40, B)):       # 53687 x 40000 > 2^31
+        ref, (rh, rw, rb) = R.sparse_head(h[r], w, b, one, dy[r], BF)
+        R.assert_within(y.detach()[r], ref, "y")
+        R.assert_within(dh[r].reshape(40, D), rh, "dh")
+    R.assert_within(dw, rw, "dw")
+    R.assert_within(db, rb, "db")
+    assert (dh[:-40] == 0).all()
+
+
+@pytest.mark.parametrize("T", [60, 300])
+def test_losses_of_rows_with_nan_or_infinities(T):
+    """A row that takes part and holds NaN or an infinity has a NaN loss and row of d_hidden, and
+    makes d_weight and d_bias NaN; the other rows' losses and gradients keep their bits."""
+    import gpusparse
+    h, w, b = make(T, 500, 64, BF, seed=94)
+    targets = torch.arange(T, device=DEV)
+    scores, ids = teacher(T, 500, 6, seed=94)
+    rows = torch.linspace(0.5, 2.0, T, device=DEV)
+    bad = [3, T - 1]
+    for call in (lambda x: gpusparse.vocab_cross_entropy(x[0], x[1], targets, bias=x[2], reduction="none"),
+                 lambda x: gpusparse.topk_distillation(x[0], x[1], scores, ids, bias=x[2], reduction="none")):
+        clean = [leaf(h), leaf(w), leaf(b)]
+        want = call(clean)
+        grads = torch.autograd.grad(want, clean, rows)
+        h2 = h.clone()
+        h2[3, 5], h2[T - 1, 60] = float("nan"), float("inf")
+        some = [leaf(h2), leaf(w), leaf(b)]
+        got = call(some)
+        dh, dw, db = torch.autograd.grad(got, some, rows)
+        others = torch.ones(T, dtype=torch.bool, device=DEV)
+        others[bad] = False
+        assert torch.isnan(got[bad]).all() and torch.equal(got[others], want[others])
+        assert torch.isnan(dh[bad]).all() and torch.equal(dh[others], grads[0][others])
+        assert torch.isnan(dw).all() and torch.isnan(db).all()
+
+
+def test_cross_entropy_of_a_target_outside_the_masked_vocabulary():
+    """A target whose bias is -inf: an infinite loss with the gradient softmax - one-hot."""
+    import gpusparse
+    h, w, b = make(50, 300, 64, BF, seed=95)
+    targets = torch.arange(50, device=DEV) * 5
+    b[20] = float("-inf")                       # row 4's target
+    leaves = [leaf(h), leaf(w), leaf(b)]
+    loss = gpusparse.vocab_cross_entropy(leaves[0], leaves[1], targets, bias=leaves[2], reduction="none")
+    rows = torch.ones(50, device=DEV)
+    live = torch.ones(50, dtype=torch.bool, device=DEV)
+    ref, (rh, rw, rb) = R.softmax_loss(h, w, b, one_hot(targets, 300, live), live, 1.0, rows, BF)
+    assert float(loss[4]) == float("inf") and float(ref[0][4]) == float("inf")
+    keep = torch.arange(50, device=DEV) != 4
+    R.assert_within(loss.detach()[keep], (ref[0][keep], ref[1][keep]), "loss")
+    for g, r, what in zip(torch.autograd.grad(loss, leaves, rows), (rh, rw, rb), ("dh", "dw", "db")):
+        R.assert_within(g, r, what)
+
+
+def test_encoding_of_nothing():
+    import gpusparse
+    h, w, b, _ = head_inputs(3, 4, 50, 16, BF, seed=96)
+    ip, ix, dtv = gpusparse.encode_documents(h[:0], w, bias=b)
+    assert ip.tolist() == [0] and ix.numel() == 0 and dtv.numel() == 0
+    ip, ix, dtv = gpusparse.encode_documents(h[:, :0], w, bias=b)
+    assert ip.tolist() == [0, 0, 0, 0] and ix.numel() == 0
+    qi, qs = gpusparse.encode_queries(h[:0], w, bias=b, max_terms=7)
+    assert qi.shape == (0, 7) and qs.shape == (0, 7)
+    qi, qs = gpusparse.encode_queries(h[:, :0], w, bias=b, max_terms=70)
+    assert qi.shape == (3, 70) and (qi == -1).all() and (qs == 0).all()
+
+
+# ---------------------------------------------------------------------------- threads, devices
+def test_calls_from_several_threads():
+    """Each thread on a stream of its own, forward and backward passes interleaved."""
+    import threading
+    inputs = [step_inputs(101 + i) for i in range(4)]
+    want = [step(*x) for x in inputs]
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in inputs], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(8):
+                    got[i].append(step(*inputs[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:              # noqa: BLE001 (shown by the main thread)
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(inputs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for outs, ref in zip(got, want):
+        assert len(outs) == 8 and all(torch.equal(x, y) for out in outs for x, y in zip(out, ref))
+
+
+def test_tensors_on_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    inputs = step_inputs(105)
+    want = step(*inputs)
+    there = [x.detach().to("cuda:1").requires_grad_(x.requires_grad) for x in inputs]
+    got = step(*there)
+    assert torch.cuda.current_device() == 0
+    assert all(y.device.index == 1 and torch.equal(x, y.to(x.device)) for x, y in zip(want, got))
+
+
 def test_weights_on_the_host_are_refused():
     import gpusparse
     h, w, b = make(10, 50, 16, BF, seed=51)
@@ -983,3 +1165,17 @@ def test_weights_on_the_host_are_refused():
                 lambda: gpusparse.sparse_head(h[None], w, mask=torch.ones(1, 10))):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_batched_transforms_are_refused():
+    import gpusparse
+    h, w, _ = make(12, 50, 16, BF, seed=51)
+    t = torch.zeros(4, dtype=torch.int64, device=DEV)
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda x: gpusparse.vocab_cross_entropy(x, w, t))(h.reshape(3, 4, 16))
+    with pytest.raises(RuntimeError):
+        torch.vmap(lambda x: gpusparse.sparse_head(x[None], w))(h.reshape(3, 4, 16))
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: gpusparse.vocab_cross_entropy(x, w, t))(h[:4])
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: gpusparse.sparse_head(x[None], w), (h[:4],), (h[4:8],))
