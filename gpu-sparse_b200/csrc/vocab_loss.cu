@@ -12,20 +12,24 @@
 // running maximum, sum and target dot product in registers along the share and write them once
 // per row block; a second kernel joins the partial results (in share order) and sums the losses.
 // Bound by the products (V = 30522, D = 768: 16384 rows 528 us, 1.45 PFLOP/s; one row 15 us, of
-// which 7 are W's bytes); with D = 64 the exponentials show, 64 us for 4096 rows.
+// which 7 are W's bytes).  With a small D it is the epilogue: 64 us for 4096 rows at D = 64, where
+// the exponentials alone are 27 (16 a cycle and SM); the rest is the latency of two epilogue warps
+// per scheduler.  The sums take ex2.approx (2^-22 relative), which leaves a loss off by 3e-7.
 //
 // Backward.  Per piece of the vocabulary: the logits' tiles again, whose epilogue turns them
 // into P = gradient of the logits, rounded once to 16 bits, then the two products of
 // vocab.cu.  A piece is as large as 512 MiB of P allow, since the products' tile lists want
-// to be long; P makes one trip through memory, which the products' arithmetic
-//   hides.  The logits' pass is bound by its epilogue: 624 us for 16384 rows (P leaves by TMA: 711
-//   instead of 771 us with plain stores at that step), and with D = 64 still 130 of the 164 us that
-//   4096 rows take with D = 768.
-//   d_bias sums the unrounded P (a butterfly over the warp's rows, then over row blocks).
-//   P is scaled so that the largest row coefficient is 1 in bf16, where a target's softmax - 1
-//   is then -1 or close and rounds to next to nothing, and 2^14 in fp16, whose range would lose
-//   gradients of 1e-8; the products' epilogue takes the scale out in fp32.
-//   For up to 128 rows P is held in two parts (see low_rows).
+// to be long; P makes one trip through memory, which the products' arithmetic hides.  The logits'
+// pass is bound by its epilogue: 624 us for 16384 rows (P leaves by TMA: 711 instead of 771 us
+// with plain stores at that step), and with D = 64 still 130 of the 164 us that 4096 rows take
+// with D = 768.  d_bias sums the unrounded P (a warp's 32 x 32 block through shared memory, then
+// the row blocks).
+//   P is scaled so that the largest row coefficient is 1 in bf16, where a target's softmax - 1 is
+// then -1 or close and rounds to next to nothing, and 2^14 in fp16, whose range would lose
+// gradients of 1e-8; the products' epilogue takes the scale out in fp32.  Rounding P to 16 bits is
+// what lets the products run at the 16-bit rate; gradients of 4096 distilled rows are off by 0.0023
+// of their norm in bf16 and those of 500 rows by 0.00029 in fp16, where rounding the exact ones
+// costs 0.0017 and 0.00021.  For up to 128 rows P is held in two parts (see low_rows).
 #include "vocab.cuh"
 
 namespace gsp {
@@ -575,8 +579,8 @@ struct LogitGradJob {
   int64_t pitch;            // of P and colpart
   float* colpart;           // [128-row blocks][pitch], or null
 
-  // the same shares along the vocabulary as the forward pass, so that a row's entries are found
-  // once per share
+  // shares along the vocabulary, as in the forward pass: a row's coefficients are read once per
+  // share (its entries are found by bucket, tile by tile)
   struct Walk {
     int32_t lo, x, hi, nt, nk, v0, a_rows;
     __device__ bool next(mm::Tile& t) {

@@ -2,7 +2,10 @@
 
 A learned-sparse encoder ends in a projection of its hidden states onto the vocabulary,
 s[t, v] = hidden[t] . weight[v] + bias[v].  The operators here run that projection on the
-tensor cores and reduce the logits where they are made, so none of them ever holds logits:
+tensor cores and reduce the logits where they are made, so none of them ever holds logits
+(backward passes write their gradient, in the inputs' type and for a piece of the vocabulary of
+512 MiB at a time; kept for them are the packed rows, 16 bytes per teacher entry, and the sparse
+head's weights and winners):
 
 * ``sparse_head``: term weights log1p(relu(max over a text's tokens of s)), [B, V];
   ``encode_documents`` / ``encode_queries`` turn them into what the index builders and the

@@ -350,7 +350,8 @@ int gsp_compacted_topk(const float* scores, int64_t B, int64_t L, int64_t stride
  * projection rows W [V, D] (both bf16 or both fp16), s[t, v] = H[t] . W[v] + bias[v] are the
  * logits.  No call stores them: products run on the tensor cores with fp32 accumulators and
  * are reduced where they are made.  Results do not depend on scheduling (no floating-point
- * atomics).  A bounded wait that runs out (gsp_set_wait_limit) gives NaN results. */
+ * atomics).  A bounded wait that runs out (gsp_set_wait_limit) gives NaN results, gradients among
+ * them. */
 typedef struct gsp_vocab_view {
     int64_t T;                 /* tokens (for the sparse head: texts x length) */
     int64_t V;
@@ -401,8 +402,11 @@ int gsp_vocab_distill(const gsp_vocab_view* vw, const float* scores, const int64
  * contiguous and each optional (NULL).  grad_loss: fp32, one value, or [T] with
  * GSP_REDUCE_NONE.  K and tau are the forward call's, for GSP_VOCAB_DISTILL.  d_hidden and
  * d_weight start on 32-byte boundaries when D is a multiple of 16.  The softmax is computed
- * again, for a piece of the vocabulary at a time (at most 512 MiB of ws); its gradient is
- * rounded to dtype as an operand of the two products that follow. */
+ * again, for a piece of the vocabulary at a time: 512 MiB of it, or 256 columns where they take
+ * more (past 2^20 rows).  ws holds such a piece, and next to it the fragments of cut tiles (39 MB),
+ * d_hidden in fp32 when there are several pieces, column sums, and padded copies of d_hidden and
+ * d_weight when D is not a multiple of 16.  The piece is rounded to dtype as an operand of the two
+ * products that follow. */
 int gsp_vocab_loss_backward(const gsp_vocab_view* vw, int32_t kind, int64_t K, float tau, int32_t reduction,
                             const float* grad_loss, void* d_hidden, void* d_weight, float* d_bias,
                             void* state, int64_t state_bytes, void* ws, int64_t ws_bytes, void* stream);
