@@ -1179,3 +1179,23 @@ def test_batched_transforms_are_refused():
         torch.func.grad(lambda x: gpusparse.vocab_cross_entropy(x, w, t))(h[:4])
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: gpusparse.sparse_head(x[None], w), (h[:4],), (h[4:8],))
+
+
+def test_compiled_callers():
+    """A compiled function around the calls keeps their results and gradients (the calls themselves
+    run as they are, between the compiled parts)."""
+    import gpusparse
+    h, w, b, targets, scores, ids = step_inputs(106)
+
+    def f(h, w, b):
+        return gpusparse.vocab_cross_entropy(h * 2, w, targets, bias=b) + \
+            gpusparse.topk_distillation(h, w, scores, ids, bias=b) + \
+            gpusparse.sparse_head(h[None], w, bias=b).mean()
+    want = f(h, w, b)
+    grads = torch.autograd.grad(want, (h, w, b))
+    compiled = torch.compile(f, backend="eager")
+    got = compiled(h, w, b)
+    assert torch.equal(got, want)
+    assert all(torch.equal(x, y) for x, y in zip(torch.autograd.grad(got, (h, w, b)), grads))
+    with torch.no_grad():
+        assert torch.equal(compiled(h, w, b), want)
